@@ -353,6 +353,33 @@ int32_t lumi_k_norm_add(uint64_t x, uint64_t o, uint64_t w, uint64_t y, uint64_t
  * out32 [rows][width] and / or hi (and lo) as bf16 halves (0: none).  width % 8 == 0, ld % 4 == 0, 16-byte aligned pointers. */
 int32_t lumi_k_gate_mul(uint64_t gu, int32_t ld, uint64_t out32, uint64_t hi, uint64_t lo, int32_t rows, int32_t width, uint64_t stream);
 
+/* ---- rows of 8-bit integers with a scale each, and their product -----------------------------
+ * A row t of numbers is held as integers q = rint(t * 127 / m) (ties to even), at most 127 in size, and one fp32 scale s = m / 127 with
+ * m = max(max |t|, 2^-100): t is about q * s.  A row that holds an infinity or a NaN gets q = 0 and s = NaN, so that all that is made from it is NaN.
+ * These calls have no counterpart in the reference.  All pointers are memory of the current device; what lies between a row's end and the next
+ * row (ld) is neither read nor written, rows begin on 16-byte boundaries.  Nothing is allocated and no workspace is shared: calls may overlap on any
+ * streams and be captured into graphs.  With no rows a call does nothing. */
+
+/* The norm in front of a projection: x[r] += o[r] (o = 0: x is left alone; the sum is rounded to x's type, and the norm sees the rounded row), then
+ * the rows x[r] / sqrt(mean(x[r]^2) + eps) * w over `width` elements as q[rows][ldq] and scale[rows].  w = 0: no norm, the rows of x as they are (a
+ * projection's weights [N][K] give q and w_scale of lumi_k_gemm_i8; eps is not looked at).  x_dtype, o_dtype: LUMI_DTYPE_*; w fp32, eps > 0.
+ * ldx and ldo are multiples of 4 (fp32) or 8 (bf16) elements, ldq of 16; x, o, w and q are 16-byte aligned. */
+int32_t lumi_k_norm_quant(uint64_t x, int32_t x_dtype, int32_t ldx, uint64_t o, int32_t o_dtype, int32_t ldo, uint64_t w, uint64_t q, int32_t ldq,
+                          uint64_t scale, int32_t rows, int32_t width, float eps, uint64_t stream);
+
+/* The gate of a feed-forward: rows of gu hold `width` gates and, from column `up` on, `width` ups; act(gate) * up as q and scale.  act: 0 sigmoid (the
+ * hybrid's, inference/src/model.rs:550-552), 1 silu.  up and ld are multiples of 4 (fp32) or 8 (bf16) elements, up >= width. */
+int32_t lumi_k_gate_quant(uint64_t gu, int32_t dtype, int32_t ld, int32_t up, int32_t act, uint64_t q, int32_t ldq, uint64_t scale, int32_t rows,
+                          int32_t width, uint64_t stream);
+
+/* D[m][n] = (sum over k of a[m][k] * w[n][k]) * a_scale[m] * w_scale[n] + bias[n] (+ D[m][n] if accumulate != 0); a [M][lda] and w [N][ldw] 8-bit
+ * integers (-128 is allowed), sums in 32-bit integers and so exact, the rest in fp32, rounded once to D's type (d_dtype LUMI_DTYPE_*, rows of ldd
+ * elements; no alignment beyond the element's).  bias may be 0.  K <= 131071 (LUMI_E_UNSUPPORTED beyond: the sums could overflow); lda and ldw are
+ * multiples of 16, a and w 16-byte aligned; D overlaps none of the operands.  status: a device int32 or 0; a bounded wait on the device that gave up
+ * sets the bit 4 of it and leaves NaN in the results that it cost. */
+int32_t lumi_k_gemm_i8(uint64_t a, int32_t lda, uint64_t a_scale, uint64_t w, int32_t ldw, uint64_t w_scale, uint64_t bias, uint64_t d, int32_t d_dtype,
+                       int32_t ldd, int32_t M, int32_t N, int32_t K, int32_t accumulate, uint64_t status, uint64_t stream);
+
 /* One Mamba block (RMSNorm -> in_proj -> state step -> out_proj + residual, inference/src/model.rs:296-375
  * in arithmetic) WITHOUT any allocation.  This entry point has no counterpart in the reference.
  *

@@ -1,0 +1,191 @@
+"""GPU: rows as 8-bit integers with a scale (lumi_k_norm_quant, lumi_k_gate_quant) against the definition in 64 bits.
+
+Tolerances, from the arithmetic (u = 2^-24, a rounding to fp32):
+* x + o: one rounding to fp32 (u), and for a bf16 stream one more (2^-8): compared with the same two roundings, which torch makes as well: equal.
+* scale without norm: m is exact, m / 127 one rounding: u.  With norm: the products x w round once (u), the quotient and the product with r once each, the sum
+  of squares over n elements is a tree of at most 64 serial additions per thread and 10 levels behind (each 1 u of a sum of positive terms, halved by the
+  root), its quotient, the sum with eps, root and reciprocal 1 u each: (74 / 2 + 8) u < 2^-18.
+* the gate: exp and the quotient are good to a few 2^-22 relative, times the size of the argument where the gate is far below zero: 2^-18 of |t| for
+  |gate| < 16, which is where the tests draw.
+* integers: t * 127 / m is off by at most 127 * (e + 2 u), e the relative error of t against m: an integer may differ from rint of the exact quotient only where that lies
+  that near a half.  So |q s - t| <= s (1 / 2 + that)."""
+import itertools
+
+import pytest
+import torch
+
+import lumi_b200
+
+pytestmark = pytest.mark.gpu
+LEAST = 2.0 ** -100
+SCALE_TOL = 2.0 ** -18
+EPS = 1e-5
+
+
+def call(name, *args):
+    lumi_b200.api.check(getattr(lumi_b200.lib(), name)(*args))
+
+
+def code(t):
+    return 1 if t.dtype == torch.bfloat16 else 0
+
+
+def rows_of(t, ld, dtype, fill=7.0):
+    """t in rows of ld elements; what lies between the rows holds `fill`."""
+    buf = torch.full((t.shape[0], ld), fill, device="cuda", dtype=dtype)
+    buf[:, :t.shape[1]] = t
+    return buf
+
+
+def norm(x, o, w, width, ldq, eps=EPS, stream=0):
+    q = torch.full((x.shape[0], ldq), 99, device="cuda", dtype=torch.int8)
+    s = torch.full((x.shape[0] + 1,), -1.0, device="cuda")
+    call("lumi_k_norm_quant", x.data_ptr(), code(x), x.stride(0), 0 if o is None else o.data_ptr(), 0 if o is None else code(o),
+         0 if o is None else o.stride(0), 0 if w is None else w.data_ptr(), q.data_ptr(), ldq, s.data_ptr(), x.shape[0], width, eps, stream)
+    torch.cuda.synchronize()
+    assert float(s[-1]) == -1.0 and bool((q[:, width:] == 99).all())      # what lies behind is left alone
+    return q[:, :width].double(), s[:-1].double()
+
+
+def check(q, s, t, factor, tol):
+    """q and s against rows t (64 bits), all times factor [rows, 1]."""
+    m = t.abs().amax(1).clamp(min=LEAST)
+    want = m / 127 * factor[:, 0]
+    assert float(((s - want).abs() / want).max()) <= SCALE_TOL
+    assert float(q.abs().max()) <= 127
+    steps = t / (m[:, None] / 127)
+    assert float((q - steps).abs().max()) <= 0.5 + 127 * (tol + 2.0 ** -22)
+    assert bool((q.abs().amax(1)[m > LEAST] == 127).all())
+
+
+WIDTHS = [1, 3, 8, 31, 100, 255, 256, 1000, 1024, 1031, 2048, 2816, 4100, 7360, 8192, 8200, 16384, 20001]
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("x_dtype,o_dtype", list(itertools.product([torch.float32, torch.bfloat16], [None, torch.float32, torch.bfloat16])))
+def test_norm(width, x_dtype, o_dtype):
+    g = torch.Generator(device="cuda").manual_seed(width)
+    for rows, pad, with_norm in ((1, 0, True), (5, 16, True), (5, 0, False), (613, 0, True)):
+        if rows * width > 3_000_000:
+            continue
+        ld = (width + 15) // 16 * 16 + pad
+        x0 = torch.randn(rows, width, generator=g, device="cuda") * 3
+        x = rows_of(x0, ld, x_dtype)
+        o = None if o_dtype is None else rows_of(torch.randn(rows, width, generator=g, device="cuda"), ld + 8, o_dtype, float("nan"))
+        w = torch.randn(width, generator=g, device="cuda") if with_norm else None
+        stream = x[:, :width].clone()
+        if o is not None:
+            stream = (stream.float() + o[:, :width].float()).to(x_dtype)
+        q, s = norm(x, o, w, width, ld)
+        assert torch.equal(x[:, :width], stream) and bool((x[:, width:] == 7).all())
+        t = stream.double()
+        factor = torch.ones(rows, 1, device="cuda", dtype=torch.float64)
+        if with_norm:
+            factor = 1 / torch.sqrt((t * t).mean(1, keepdim=True) + EPS)
+            t = t * w.double()
+        check(q, s, t, factor, 2.0 ** -24)
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", [0, 1])
+def test_gate(width, dtype, act):
+    g = torch.Generator(device="cuda").manual_seed(width + act)
+    for rows, pad in ((1, 0), (7, 16), (641, 0)):
+        if rows * width > 3_000_000:
+            continue
+        up = (width + 15) // 16 * 16 + pad
+        gate = (torch.randn(rows, width, generator=g, device="cuda") * 4).clamp(-15.9, 15.9)
+        ups = torch.randn(rows, width, generator=g, device="cuda")
+        gu = rows_of(gate, 2 * up + pad, dtype, float("nan"))
+        gu[:, up:up + width] = ups
+        z, u = gu[:, :width].double(), gu[:, up:up + width].double()
+        ldq = (width + 15) // 16 * 16
+        q = torch.full((rows, ldq), 99, device="cuda", dtype=torch.int8)
+        s = torch.full((rows + 1,), -1.0, device="cuda")
+        call("lumi_k_gate_quant", gu.data_ptr(), code(gu), gu.stride(0), up, act, q.data_ptr(), ldq, s.data_ptr(), rows, width, 0)
+        torch.cuda.synchronize()
+        assert float(s[-1]) == -1.0 and bool((q[:, width:] == 99).all())
+        t = torch.sigmoid(z) * u * (z if act else 1)
+        check(q[:, :width].double(), s[:-1].double(), t, torch.ones(rows, 1, device="cuda", dtype=torch.float64), 2.0 ** -18)
+
+
+@pytest.mark.parametrize("width", [5, 1024, 8192, 20001])
+def test_rows_of_zeros_small_and_large_numbers_and_of_none(width):
+    """Zeros give zeros; rows near the ends of fp32 keep their integers; an infinity or a NaN in a row gives NaN for that row alone."""
+    ld = (width + 15) // 16 * 16
+    g = torch.Generator(device="cuda").manual_seed(1)
+    base = torch.randn(8, width, generator=g, device="cuda")
+    base[0] = 0
+    base[1] *= 1e-29
+    base[2] *= 1e25
+    base[3, width // 2] = float("inf")
+    base[4, width - 1] = float("nan")
+    base[5, 0] = float("-inf")
+    base[6] = 0
+    base[6, width - 1] = -2.0                             # one number alone
+    x = rows_of(base, ld, torch.float32)
+    ones = torch.ones(width, device="cuda")
+    for w in (None, ones):
+        q, s = norm(x.clone(), None, w, width, ld)
+        assert bool(torch.isnan(s[3:6]).all()) and bool((q[3:6] == 0).all())
+        keep = [0, 1, 2, 6, 7]
+        t = base[keep].double()
+        factor = torch.ones(5, 1, device="cuda", dtype=torch.float64)
+        if w is not None:
+            factor = 1 / torch.sqrt((t * t).mean(1, keepdim=True) + EPS)
+        m = t.abs().amax(1).clamp(min=LEAST)
+        assert float(((s[keep] - m / 127 * factor[:, 0]).abs() / (m / 127 * factor[:, 0])).max()) <= SCALE_TOL
+        assert float((q[keep] - t / (m[:, None] / 127)).abs().max()) <= 0.5 + 127 * 2.0 ** -21
+        assert bool((q[0] == 0).all())
+    tiny = rows_of(torch.full((1, width), 1e-38, device="cuda"), ld, torch.float32)       # below 2^-100: held as zeros
+    q, s = norm(tiny, None, None, width, ld)
+    assert bool((q == 0).all()) and float(s[0]) == pytest.approx(LEAST / 127)
+
+
+def test_sums_of_squares_beyond_fp32():
+    """Squares that overflow, and squares that vanish beside a small eps, are taken again with the row scaled."""
+    width = 1024
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for size, eps in ((1e30, 1e-5), (1e20, 1e-5), (1e-25, 1e-37), (1e-21, 1e-30)):
+        for wide in (width, 20000):
+            t = torch.randn(3, wide, generator=g, device="cuda") * size
+            q, s = norm(rows_of(t, wide, torch.float32), None, torch.ones(wide, device="cuda"), wide, wide, eps)
+            t = t.double()
+            check(q, s, t, 1 / torch.sqrt((t * t).mean(1, keepdim=True) + float(torch.tensor(eps))), 2.0 ** -24)
+
+
+def test_same_bits_alone_and_among_others_and_again():
+    """A row's integers and scale do not depend on how many rows there are, nor on the run."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for width in (96, 1024, 2048, 5632):
+        x = torch.randn(1500, width, generator=g, device="cuda")
+        w = torch.randn(width, generator=g, device="cuda")
+        q, s = norm(x.clone(), None, w, width, width)
+        q2, s2 = norm(x.clone(), None, w, width, width)
+        assert torch.equal(q, q2) and torch.equal(s, s2)
+        for r in (0, 777, 1499):
+            q1, s1 = norm(x[r:r + 1].clone(), None, w, width, width)
+            assert torch.equal(q1[0], q[r]) and torch.equal(s1[0], s[r])
+
+
+def test_residual_onto_itself():
+    """o may be x: the rows are doubled."""
+    x = torch.randn(4, 1024, device="cuda", generator=torch.Generator(device="cuda").manual_seed(4))
+    want = x * 2
+    q, s = norm(x, x, None, 1024, 1024)
+    assert torch.equal(x, want)
+    check(q, s, want.double(), torch.ones(4, 1, device="cuda", dtype=torch.float64), 2.0 ** -24)
+
+
+def test_offsets_past_31_bits():
+    """Rows further than 2^31 elements from the first."""
+    width, ld, rows = 64, 1 << 20, 2100
+    x = torch.empty(rows * ld, device="cuda", dtype=torch.bfloat16)                  # 4.4 GB, 2.2e9 elements
+    v = x.view(rows, ld)[:, :width]
+    v.copy_(torch.randn(rows, width, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)))
+    q = torch.empty(rows * ld, device="cuda", dtype=torch.int8)
+    s = torch.empty(rows, device="cuda")
+    call("lumi_k_norm_quant", x.data_ptr(), 1, ld, 0, 0, 0, 0, q.data_ptr(), ld, s.data_ptr(), rows, width, 0.0, 0)
+    torch.cuda.synchronize()
+    check(q.view(rows, ld)[:, :width].double(), s.double(), v.double(), torch.ones(rows, 1, device="cuda", dtype=torch.float64), 2.0 ** -24)
