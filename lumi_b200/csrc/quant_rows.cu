@@ -7,6 +7,8 @@
 #include "device_args.h"
 #include "rows.cuh"
 
+#include <type_traits>
+
 namespace lumi {
 namespace {
 
@@ -20,6 +22,9 @@ struct QuantOut {
 };
 
 // ---- loads of four or eight numbers, as fp32
+// fast forms of the gate: relative error 2^-21 times the size of a negative gate
+__device__ __forceinline__ float fast_sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+
 template <int E>
 __device__ __forceinline__ void load_whole(const float* p, float (&v)[E]) {
 #pragma unroll
@@ -44,31 +49,49 @@ __device__ __forceinline__ void load_whole(const __nv_bfloat16* p, float (&v)[E]
         v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
     }
 }
+// Of the norm's weights, which no store of the kernel changes: loads that may pass the stores of x, but not the dependency wait.
+template <bool RAGGED>
+__device__ __forceinline__ void load_weights(const float* p, int n, float& a, float& b, float& c, float& d) {
+    a = b = c = d = 0.f;
+    if (RAGGED ? n >= 4 : n > 0) {
+        asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(a), "=f"(b), "=f"(c), "=f"(d) : "l"(p));
+    } else if (RAGGED) {
+        if (n > 0) a = p[0];
+        if (n > 1) b = p[1];
+        if (n > 2) c = p[2];
+    }
+}
 __device__ __forceinline__ float one(const float* p) { return *p; }
 __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-// n < E: the row ends within these numbers; what is behind it is neither read nor counted
-template <int E, typename T>
+// The row ends n numbers from here (n <= 0: before); what is behind it is neither read nor counted.  RAGGED: it may end within these E.
+template <bool RAGGED, int E, typename T>
 __device__ __forceinline__ void load_some(const T* p, int n, float (&v)[E]) {
-    if (n >= E) { load_whole<E>(p, v); return; }
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = i < n ? one(p + i) : 0.f;
+    for (int i = 0; i < E; ++i) v[i] = 0.f;
+    if (RAGGED ? n >= E : n > 0) {
+        load_whole<E>(p, v);
+    } else if (RAGGED) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) if (i < n) v[i] = one(p + i);
+    }
 }
 __device__ __forceinline__ float stored(float v, const float*) { return v; }
 __device__ __forceinline__ float stored(float v, const __nv_bfloat16*) { return __bfloat162float(__float2bfloat16_rn(v)); }
-template <int E>
+template <bool RAGGED, int E>
 __device__ __forceinline__ void store_some(float* p, int n, const float (&v)[E]) {
-    if (n >= E) {
+    if (RAGGED ? n >= E : n > 0) {
 #pragma unroll
         for (int i = 0; i < E / 4; ++i) *reinterpret_cast<float4*>(p + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         return;
     }
+    if (RAGGED)
 #pragma unroll
-    for (int i = 0; i < E; ++i) if (i < n) p[i] = v[i];
+        for (int i = 0; i < E; ++i) if (i < n) p[i] = v[i];
 }
-template <int E>
+template <bool RAGGED, int E>
 __device__ __forceinline__ void store_some(__nv_bfloat16* p, int n, const float (&v)[E]) {
     static_assert(E == 8, "");
-    if (n >= E) {
+    if (RAGGED ? n >= E : n > 0) {
         uint32_t u[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -78,14 +101,16 @@ __device__ __forceinline__ void store_some(__nv_bfloat16* p, int n, const float 
         *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
         return;
     }
+    if (RAGGED)
 #pragma unroll
-    for (int i = 0; i < E; ++i) if (i < n) p[i] = __float2bfloat16_rn(v[i]);
+        for (int i = 0; i < E; ++i) if (i < n) p[i] = __float2bfloat16_rn(v[i]);
 }
 
 // ---- sources of rows: load(): what memory holds of E numbers; values(): the numbers to be held in 8 bits, with the sum of squares
 // Norm, or rows as they are.  ADD: x += o first, rounded to x's type, so that the norm sees what later readers of x see.
-template <typename XT, typename OT, bool ADD, bool NORM>
+template <typename XT, typename OT, bool ADD, bool NORM, bool RAGGED>
 struct NormSource {
+    static constexpr bool kRagged = RAGGED;
     static constexpr int E = sizeof(XT) == 4 ? 4 : 8;
     static constexpr bool kNorm = NORM;
     XT* x; const OT* o; const float* w;
@@ -95,8 +120,8 @@ struct NormSource {
     struct Raw { float x[E], o[ADD ? E : 1]; };
     template <bool AGAIN>
     __device__ __forceinline__ void load(long row, int c, Raw& r) const {
-        load_some<E>(x + row * ldx + c, width - c, r.x);
-        if constexpr (ADD && !AGAIN) load_some<E>(o + row * ldo + c, width - c, r.o);
+        load_some<RAGGED, E>(x + row * ldx + c, width - c, r.x);
+        if constexpr (ADD && !AGAIN) load_some<RAGGED, E>(o + row * ldo + c, width - c, r.o);
     }
     // AGAIN: x has been added to already
     template <bool AGAIN>
@@ -104,10 +129,12 @@ struct NormSource {
         if constexpr (ADD && !AGAIN) {
 #pragma unroll
             for (int i = 0; i < E; ++i) r.x[i] = stored(r.x[i] + r.o[i], x);
-            store_some<E>(x + row * ldx + c, width - c, r.x);
+            store_some<RAGGED, E>(x + row * ldx + c, width - c, r.x);
         }
         float f[E];
-        if constexpr (NORM) load_some<E>(w + c, width - c, f);
+        if constexpr (NORM)
+#pragma unroll
+            for (int i = 0; i < E; i += 4) load_weights<RAGGED>(w + c + i, width - c - i, f[i], f[i + 1], f[i + 2], f[i + 3]);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             if constexpr (NORM) {
@@ -121,8 +148,9 @@ struct NormSource {
 };
 
 // Gate: rows hold gates, and from column `up` on as many ups.
-template <typename XT, bool SILU>
+template <typename XT, bool SILU, bool RAGGED>
 struct GateSource {
+    static constexpr bool kRagged = RAGGED;
     static constexpr int E = sizeof(XT) == 4 ? 4 : 8;
     static constexpr bool kNorm = false;
     const XT* gu;
@@ -131,13 +159,16 @@ struct GateSource {
     struct Raw { float g[E], u[E]; };
     template <bool AGAIN>
     __device__ __forceinline__ void load(long row, int c, Raw& r) const {
-        load_some<E>(gu + row * ld + c, width - c, r.g);
-        load_some<E>(gu + row * ld + up + c, width - c, r.u);
+        load_some<RAGGED, E>(gu + row * ld + c, width - c, r.g);
+        load_some<RAGGED, E>(gu + row * ld + up + c, width - c, r.u);
     }
     template <bool AGAIN>
     __device__ __forceinline__ void values(long, int, Raw& r, float (&t)[E], float&) const {
 #pragma unroll
-        for (int i = 0; i < E; ++i) t[i] = (SILU ? silu_f(r.g[i]) : sigmoid_f(r.g[i])) * r.u[i];
+        for (int i = 0; i < E; ++i) {
+            const float z = fast_sigmoid(r.g[i]);
+            t[i] = (SILU ? r.g[i] * z : z) * r.u[i];
+        }
     }
 };
 
@@ -148,12 +179,12 @@ __device__ __forceinline__ void largest(const float (&t)[E], uint32_t& m) {
 }
 
 // t * inv to the nearest integer, ties to even: added to 1.5 * 2^23, the integer is the sum's low byte.
-template <int E>
+template <bool RAGGED, int E>
 __device__ __forceinline__ void put(int8_t* q, int n, const float (&t)[E], float inv) {
     uint32_t b[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) b[i] = __float_as_uint(fmaf(t[i], inv, 12582912.f));
-    if (n >= E) {
+    if (RAGGED ? n >= E : n > 0) {
         uint32_t u[E / 4];
 #pragma unroll
         for (int i = 0; i < E / 4; ++i)
@@ -162,8 +193,9 @@ __device__ __forceinline__ void put(int8_t* q, int n, const float (&t)[E], float
         else *reinterpret_cast<uint32_t*>(q) = u[0];
         return;
     }
+    if (RAGGED)
 #pragma unroll
-    for (int i = 0; i < E; ++i) if (i < n) q[i] = (int8_t)b[i];
+        for (int i = 0; i < E; ++i) if (i < n) q[i] = (int8_t)b[i];
 }
 
 // Sum and maximum over the NT threads of a row (a whole warp, or the block).
@@ -236,15 +268,83 @@ __global__ void __launch_bounds__(NT) quant_wide_kernel(SRC src, QuantOut out) {
         if (!numbers)
 #pragma unroll
             for (int i = 0; i < E; ++i) t[i] = 0.f;
-        put<E>(out.q + row * out.ldq + c, src.width - c, t, inv);
+        put<SRC::kRagged, E>(out.q + row * out.ldq + c, src.width - c, t, inv);
     }
 }
 
+// The numbers of a row in the registers of NT threads (a warp, or the block), NC times E each: memory is read once, all of it asked for before the
+// first is used.
+template <typename SRC, int NT, int NC>
+__global__ void __launch_bounds__(NT == 32 ? 128 : NT) quant_rows_kernel(SRC src, QuantOut out, int rows) {
+    constexpr int E = SRC::E;
+    const long row = NT == 32 ? (long)blockIdx.x * 4 + (threadIdx.x >> 5) : (long)blockIdx.x;
+    const int tid = NT == 32 ? threadIdx.x & 31 : threadIdx.x;
+    pdl_release();
+    pdl_sync();
+    if (row >= rows) return;                              // whole warps, and only where a row is a warp's
+    typename SRC::Raw r[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) src.template load<false>(row, (i * NT + tid) * E, r[i]);
+    float sum = 0.f, t[NC][E];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        src.template values<false>(row, (i * NT + tid) * E, r[i], t[i], sum);
+        largest<E>(t[i], m);
+    }
+    reduce_row<NT>(sum, m);
+    const bool numbers = m < kInfBits;
+    float factor = 1.f;
+    if constexpr (SRC::kNorm)
+        factor = norm_factor(sum, src.width, src.eps, [&](float k) {
+            float part = 0.f;
+            uint32_t unused = 0;
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+#pragma unroll
+                for (int e = 0; e < E; ++e) part = fmaf(r[i].x[e] * k, r[i].x[e] * k, part);
+            reduce_row<NT>(part, unused);
+            return part;
+        });
+    const float top = fmaxf(__uint_as_float(m), kLeast), inv = numbers ? __fdiv_rn(127.f, top) : 0.f;
+    if (tid == 0) out.scale[row] = numbers ? __fdiv_rn(top, 127.f) * factor : __uint_as_float(0x7fffffffu);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int c = (i * NT + tid) * E;
+        if (!numbers)
+#pragma unroll
+            for (int e = 0; e < E; ++e) t[i][e] = 0.f;
+        put<SRC::kRagged, E>(out.q + row * out.ldq + c, src.width - c, t[i], inv);
+    }
+}
+
+template <typename SRC, int NT, int NC>
+int32_t launch_rows_of(const SRC& src, const QuantOut& out, int rows, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(NT == 32 ? (unsigned)(((long)rows + 3) / 4) : (unsigned)rows);
+    cfg.blockDim = dim3(NT == 32 ? 128 : NT);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // the launch itself overlaps the kernel in front
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if constexpr (NC > 0) LUMI_CUDA(cudaLaunchKernelEx(&cfg, quant_rows_kernel<SRC, NT, NC>, src, out, rows));
+    else LUMI_CUDA(cudaLaunchKernelEx(&cfg, quant_wide_kernel<SRC, NT>, src, out));
+    return LUMI_OK;
+}
+
+// The shape goes by the width alone, so that a row has the same bits alone and among others.
 template <typename SRC>
 int32_t launch(const SRC& src, const QuantOut& out, int rows, cudaStream_t st) {
-    quant_wide_kernel<SRC, 256><<<rows, 256, 0, st>>>(src, out);
-    LUMI_CUDA(cudaGetLastError());
-    return LUMI_OK;
+    constexpr int E = SRC::E, L = 8 / E;                  // L: a row's numbers are 2 L (4 L, 8 L) loads of a thread
+    if (src.width <= 32 * 8) return launch_rows_of<SRC, 32, L>(src, out, rows, st);
+    if (src.width <= 32 * 32) return launch_rows_of<SRC, 32, 4 * L>(src, out, rows, st);
+    if (src.width <= 256 * 8) return launch_rows_of<SRC, 256, L>(src, out, rows, st);
+    if (src.width <= 256 * 16) return launch_rows_of<SRC, 256, 2 * L>(src, out, rows, st);
+    if (src.width <= 256 * 32) return launch_rows_of<SRC, 256, 4 * L>(src, out, rows, st);
+    if (src.width <= 512 * 32) return launch_rows_of<SRC, 512, 4 * L>(src, out, rows, st);
+    return launch_rows_of<SRC, 1024, 0>(src, out, rows, st);
 }
 
 template <typename XT, typename OT>
@@ -254,8 +354,12 @@ int32_t launch_norm(uint64_t x, int ldx, uint64_t o, int ldo, uint64_t w, const 
         src.ldx = ldx; src.ldo = ldo; src.width = width; src.eps = eps;
         return launch(src, out, rows, st);
     };
-    if (o) return w ? go(NormSource<XT, OT, true, true>{}) : go(NormSource<XT, OT, true, false>{});
-    return w ? go(NormSource<XT, XT, false, true>{}) : go(NormSource<XT, XT, false, false>{});
+    auto ragged = [&](auto r) {
+        constexpr bool R = decltype(r)::value;
+        if (o) return w ? go(NormSource<XT, OT, true, true, R>{}) : go(NormSource<XT, OT, true, false, R>{});
+        return w ? go(NormSource<XT, XT, false, true, R>{}) : go(NormSource<XT, XT, false, false, R>{});
+    };
+    return width % NormSource<XT, OT, true, true, true>::E != 0 ? ragged(std::true_type{}) : ragged(std::false_type{});
 }
 
 bool aligned_rows(uint64_t p, int dtype, int ld) { return (p & 15) == 0 && ld % (dtype == LUMI_DTYPE_F32 ? 4 : 8) == 0; }
@@ -300,6 +404,10 @@ extern "C" int32_t lumi_k_gate_quant(uint64_t gu, int32_t dtype, int32_t ld, int
         src.ld = ld; src.up = up; src.width = width;
         return launch<SRC>(src, out, rows, st);
     };
-    if (dtype == LUMI_DTYPE_F32) return act ? go(GateSource<float, true>{}) : go(GateSource<float, false>{});
-    return act ? go(GateSource<__nv_bfloat16, true>{}) : go(GateSource<__nv_bfloat16, false>{});
+    auto ragged = [&](auto r) {
+        constexpr bool R = decltype(r)::value;
+        if (dtype == LUMI_DTYPE_F32) return act ? go(GateSource<float, true, R>{}) : go(GateSource<float, false, R>{});
+        return act ? go(GateSource<__nv_bfloat16, true, R>{}) : go(GateSource<__nv_bfloat16, false, R>{});
+    };
+    return width % (dtype == LUMI_DTYPE_F32 ? 4 : 8) != 0 ? ragged(std::true_type{}) : ragged(std::false_type{});
 }
