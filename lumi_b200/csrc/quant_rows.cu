@@ -1,5 +1,5 @@
 // Rows of numbers as 8-bit integers with a scale per row, for products in 8-bit integers: the norm in front of a projection (with the
-// residual's addition), weights on their way into 8 bits, the gate between a feed-forward's products.
+// residual's addition), weights on their way into 8 bits, the gate between a feed-forward's products; and such rows back as numbers.
 //
 // A row t is held as q = rint(t * 127 / m) and s = m / 127, m = max(max |t|, 2^-100).  The norm's factor r = 1 / sqrt(mean x^2 + eps) is the same for the
 // whole row and cancels out of q: t = x w without it, and s = m / 127 * r.  So the sum of squares and the maximum are reduced side by side, in one
@@ -7,6 +7,7 @@
 #include "device_args.h"
 #include "rows.cuh"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace lumi {
@@ -318,17 +319,23 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) quant_rows_kernel(SRC src
     }
 }
 
-template <typename SRC, int NT, int NC>
-int32_t launch_rows_of(const SRC& src, const QuantOut& out, int rows, cudaStream_t st) {
+// the launch itself overlaps the kernel in front
+cudaLaunchConfig_t dependent_launch(dim3 grid, int threads, cudaLaunchAttribute* attr, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(NT == 32 ? (unsigned)(((long)rows + 3) / 4) : (unsigned)rows);
-    cfg.blockDim = dim3(NT == 32 ? 128 : NT);
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // the launch itself overlaps the kernel in front
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    return cfg;
+}
+
+template <typename SRC, int NT, int NC>
+int32_t launch_rows_of(const SRC& src, const QuantOut& out, int rows, cudaStream_t st) {
+    cudaLaunchAttribute attr[1];
+    const cudaLaunchConfig_t cfg = dependent_launch(dim3(NT == 32 ? (unsigned)(((long)rows + 3) / 4) : (unsigned)rows), NT == 32 ? 128 : NT, attr, st);
     if constexpr (NC > 0) LUMI_CUDA(cudaLaunchKernelEx(&cfg, quant_rows_kernel<SRC, NT, NC>, src, out, rows));
     else LUMI_CUDA(cudaLaunchKernelEx(&cfg, quant_wide_kernel<SRC, NT>, src, out));
     return LUMI_OK;
@@ -360,6 +367,48 @@ int32_t launch_norm(uint64_t x, int ldx, uint64_t o, int ldo, uint64_t w, const 
         return w ? go(NormSource<XT, XT, false, true, R>{}) : go(NormSource<XT, XT, false, false, R>{});
     };
     return width % NormSource<XT, OT, true, true, true>::E != 0 ? ragged(std::true_type{}) : ragged(std::false_type{});
+}
+
+// ---- rows back as numbers: y = q s.  A warp takes up to 1024 numbers of a row, eight per lane at a time.
+template <typename YT, bool RAGGED>
+__global__ void __launch_bounds__(256) dequant_kernel(const int8_t* q, long ldq, const float* scale, YT* y, long ldy, int rows, int width) {
+    const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    pdl_release();
+    pdl_sync();
+    if (row >= rows) return;
+    const float s = scale[row];
+    q += row * ldq;
+    y += row * ldy;
+    for (int c0 = (int)blockIdx.y * 1024; c0 < width; c0 += (int)gridDim.y * 1024) {
+        uint2 u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = c0 + (i * 32 + lane) * 8;
+            if (RAGGED ? c + 8 <= width : c < width) {
+                asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(u[i].x), "=r"(u[i].y) : "l"(q + c));
+            } else {
+                uint8_t b[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (RAGGED)
+#pragma unroll
+                    for (int e = 0; e < 7; ++e) if (c + e < width) b[e] = (uint8_t)q[c + e];
+                u[i].x = b[0] | b[1] << 8 | b[2] << 16 | (uint32_t)b[3] << 24;
+                u[i].y = b[4] | b[5] << 8 | b[6] << 16 | (uint32_t)b[7] << 24;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = c0 + (i * 32 + lane) * 8;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                // a byte b + 128 under the exponent of 2^23 is the float 2^23 + 128 + b
+                const uint32_t w = (e < 4 ? u[i].x : u[i].y) ^ 0x80808080u;
+                v[e] = __fmul_rn(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540u | (uint32_t)(e & 3))) - 8388736.f, s);
+            }
+            store_some<RAGGED, 8>(y + c, width - c, v);
+        }
+    }
 }
 
 bool aligned_rows(uint64_t p, int dtype, int ld) { return (p & 15) == 0 && ld % (dtype == LUMI_DTYPE_F32 ? 4 : 8) == 0; }
@@ -410,4 +459,22 @@ extern "C" int32_t lumi_k_gate_quant(uint64_t gu, int32_t dtype, int32_t ld, int
         return act ? go(GateSource<__nv_bfloat16, true, R>{}) : go(GateSource<__nv_bfloat16, false, R>{});
     };
     return width % (dtype == LUMI_DTYPE_F32 ? 4 : 8) != 0 ? ragged(std::true_type{}) : ragged(std::false_type{});
+}
+
+extern "C" int32_t lumi_k_dequant_rows(uint64_t q, int32_t ldq, uint64_t scale, uint64_t y, int32_t y_dtype, int32_t ldy, int32_t rows, int32_t width,
+                                       uint64_t stream) {
+    if (!q || !scale || !y || !known(y_dtype) || rows < 0 || width <= 0 || ldq < width || ldy < width) return fail(LUMI_E_INVALID, "bad argument to lumi_k_dequant_rows");
+    if (!aligned_rows(y, y_dtype, ldy) || (q & 15) || ldq % 16 || (scale & 3))
+        return fail(LUMI_E_INVALID, "lumi_k_dequant_rows: rows have to begin on 16-byte boundaries");
+    if (rows == 0) return LUMI_OK;
+    LUMI_TRY(check_device_memory("lumi_k_dequant_rows", {q, scale, y}));
+    cudaLaunchAttribute attr[1];
+    const cudaLaunchConfig_t cfg = dependent_launch(dim3((unsigned)(((long)rows + 7) / 8), std::min(65535, (width + 1023) / 1024)), 256, attr, (cudaStream_t)stream);
+    auto go = [&](auto* to, auto r) {
+        using YT = std::remove_pointer_t<decltype(to)>;
+        return cudaLaunchKernelEx(&cfg, dequant_kernel<YT, decltype(r)::value>, (const int8_t*)q, (long)ldq, (const float*)scale, to, (long)ldy, rows, width);
+    };
+    if (y_dtype == LUMI_DTYPE_F32) LUMI_CUDA(width % 8 ? go((float*)y, std::true_type{}) : go((float*)y, std::false_type{}));
+    else LUMI_CUDA(width % 8 ? go((__nv_bfloat16*)y, std::true_type{}) : go((__nv_bfloat16*)y, std::false_type{}));
+    return LUMI_OK;
 }

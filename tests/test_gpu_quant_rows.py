@@ -1,4 +1,4 @@
-"""GPU: rows as 8-bit integers with a scale (lumi_k_norm_quant, lumi_k_gate_quant) against the definition in 64 bits.
+"""GPU: rows as 8-bit integers with a scale (lumi_k_norm_quant, lumi_k_gate_quant, lumi_k_dequant_rows) against the definition in 64 bits.
 
 Tolerances, from the arithmetic (u = 2^-24, a rounding to fp32):
 * x + o: one rounding to fp32 (u), and for a bf16 stream one more (2^-8): compared with the same two roundings, which torch makes as well: equal.
@@ -189,3 +189,21 @@ def test_offsets_past_31_bits():
     call("lumi_k_norm_quant", x.data_ptr(), 1, ld, 0, 0, 0, 0, q.data_ptr(), ld, s.data_ptr(), rows, width, 0.0, 0)
     torch.cuda.synchronize()
     check(q.view(rows, ld)[:, :width].double(), s.double(), v.double(), torch.ones(rows, 1, device="cuda", dtype=torch.float64), 2.0 ** -24)
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_back(width, dtype):
+    """One product in fp32, for bf16 rounded once more: torch's own is the same bits.  -128 is allowed; a NaN or infinite scale is its row's alone."""
+    g = torch.Generator(device="cuda").manual_seed(width)
+    for rows, pad in ((1, 0), (9, 16), (300, 0)):
+        ld = (width + 15) // 16 * 16 + pad
+        q = torch.randint(-128, 128, (rows, ld), generator=g, device="cuda", dtype=torch.int16).to(torch.int8)
+        s = torch.randn(rows + 1, generator=g, device="cuda")
+        if rows > 2:
+            s[1], s[2] = float("nan"), float("inf")
+        y = torch.full((rows, ld), 7.0, device="cuda", dtype=dtype)
+        call("lumi_k_dequant_rows", q.data_ptr(), ld, s.data_ptr(), y.data_ptr(), code(y), ld, rows, width, 0)
+        torch.cuda.synchronize()
+        assert bool((y[:, width:] == 7).all())
+        assert torch.equal((q[:, :width].float() * s[:rows, None]).to(dtype).nan_to_num(nan=1e30), y[:, :width].nan_to_num(nan=1e30))

@@ -19,6 +19,12 @@ def gate(**k):
     return lumi_b200.lib().lumi_k_gate_quant(*{**a, **k}.values())
 
 
+def dequant(**k):
+    a = dict(q=P, ldq=64, scale=P, y=P, y_dtype=0, ldy=64, rows=0, width=64, stream=0)
+    assert set(k) <= set(a)
+    return lumi_b200.lib().lumi_k_dequant_rows(*{**a, **k}.values())
+
+
 def gemm(**k):
     a = dict(a=P, lda=64, a_scale=P, w=P, ldw=64, w_scale=P, bias=0, d=P, d_dtype=0, ldd=64, M=0, N=64, K=64, accumulate=0, status=0, stream=0)
     assert set(k) <= set(a)
@@ -41,6 +47,13 @@ def test_gate_refuses(k):
     assert gate(**k) == INVALID
 
 
+@pytest.mark.parametrize("k", [
+    dict(q=0), dict(scale=0), dict(y=0), dict(y_dtype=2), dict(rows=-1), dict(width=0), dict(ldq=48), dict(ldq=72), dict(ldy=60), dict(ldy=66), dict(ldy=68, y_dtype=1),
+    dict(q=P + 8), dict(scale=P + 2), dict(y=P + 4)])
+def test_dequant_refuses(k):
+    assert dequant(**k) == INVALID
+
+
 @pytest.mark.parametrize("k,want", [
     (dict(a=0), INVALID), (dict(a_scale=0), INVALID), (dict(w=0), INVALID), (dict(w_scale=0), INVALID), (dict(d=0), INVALID), (dict(d_dtype=2), INVALID),
     (dict(M=-1), INVALID), (dict(N=-1), INVALID), (dict(K=0), INVALID), (dict(lda=48), INVALID), (dict(lda=72), INVALID), (dict(ldw=48), INVALID),
@@ -52,7 +65,7 @@ def test_gemm_refuses(k, want):
 
 
 def test_nothing_to_do():
-    assert norm() == 0 and norm(o=0, w=0, eps=0.0, ldo=0, o_dtype=9) == 0 and gate() == 0
+    assert norm() == 0 and norm(o=0, w=0, eps=0.0, ldo=0, o_dtype=9) == 0 and gate() == 0 and dequant() == 0
     assert gemm() == 0 and gemm(M=5, N=0, ldd=0) == 0 and gemm(K=131071, lda=131072, ldw=131072) == 0 and gemm(d=P + 2, d_dtype=1) == 0
 
 
@@ -64,5 +77,6 @@ def test_memory_that_is_not_the_devices_is_refused():
     k = dict(rows=1, x=p, o=0, w=p, q=p, scale=p)
     assert norm(**k) in (INVALID, CUDA)
     assert gate(rows=1, gu=p, q=p, scale=p) in (INVALID, CUDA)
+    assert dequant(rows=1, q=p, scale=p, y=p) in (INVALID, CUDA)
     assert gemm(M=1, a=p, a_scale=p, w=p, w_scale=p, d=p) in (INVALID, CUDA)
     assert len(lumi_b200.lib().lumi_last_error()) > 0
