@@ -372,8 +372,8 @@ int32_t lumi_k_norm_quant(uint64_t x, int32_t x_dtype, int32_t ldx, uint64_t o, 
 int32_t lumi_k_gate_quant(uint64_t gu, int32_t dtype, int32_t ld, int32_t up, int32_t act, uint64_t q, int32_t ldq, uint64_t scale, int32_t rows,
                           int32_t width, uint64_t stream);
 
-/* Rows of 8-bit integers back as numbers: y[r][i] = q[r][i] * scale[r], rounded once to y's type (y_dtype LUMI_DTYPE_*, rows of ldy elements, a multiple of
- * 4 (fp32) or 8 (bf16)). */
+/* Rows of 8-bit integers back as numbers: y[r][i] = q[r][i] * scale[r], rounded once to y's type (y_dtype LUMI_DTYPE_*, rows of ldy elements; no
+ * alignment beyond the element's, but rows on 16-byte boundaries and widths of whole eights go faster). */
 int32_t lumi_k_dequant_rows(uint64_t q, int32_t ldq, uint64_t scale, uint64_t y, int32_t y_dtype, int32_t ldy, int32_t rows, int32_t width, uint64_t stream);
 
 /* D[m][n] = (sum over k of a[m][k] * w[n][k]) * a_scale[m] * w_scale[n] + bias[n] (+ D[m][n] if accumulate != 0); a [M][lda] and w [N][ldw] 8-bit

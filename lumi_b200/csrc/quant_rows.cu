@@ -76,6 +76,8 @@ __device__ __forceinline__ void load_some(const T* p, int n, float (&v)[E]) {
         for (int i = 0; i < E; ++i) if (i < n) v[i] = one(p + i);
     }
 }
+__device__ __forceinline__ void put_one(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put_one(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ float stored(float v, const float*) { return v; }
 __device__ __forceinline__ float stored(float v, const __nv_bfloat16*) { return __bfloat162float(__float2bfloat16_rn(v)); }
 template <bool RAGGED, int E>
@@ -369,8 +371,9 @@ int32_t launch_norm(uint64_t x, int ldx, uint64_t o, int ldo, uint64_t w, const 
     return width % NormSource<XT, OT, true, true, true>::E != 0 ? ragged(std::true_type{}) : ragged(std::false_type{});
 }
 
-// ---- rows back as numbers: y = q s.  A warp takes up to 1024 numbers of a row, eight per lane at a time.
-template <typename YT, bool RAGGED>
+// ---- rows back as numbers: y = q s.  A warp takes up to 1024 numbers of a row: eight per lane at a time, or (ONE) one, for rows of y that begin
+// anywhere and widths that are no multiples of eight.
+template <typename YT, bool ONE>
 __global__ void __launch_bounds__(256) dequant_kernel(const int8_t* q, long ldq, const float* scale, YT* y, long ldy, int rows, int width) {
     const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
@@ -380,25 +383,23 @@ __global__ void __launch_bounds__(256) dequant_kernel(const int8_t* q, long ldq,
     const float s = scale[row];
     q += row * ldq;
     y += row * ldy;
-    for (int c0 = (int)blockIdx.y * 1024; c0 < width; c0 += (int)gridDim.y * 1024) {
+    for (long c0 = (long)blockIdx.y * 1024; c0 < width; c0 += (long)gridDim.y * 1024) {
+        if constexpr (ONE) {
+            const long end = min(c0 + 1024, (long)width);
+#pragma unroll 8
+            for (long c = c0 + lane; c < end; c += 32) put_one(y + c, __fmul_rn((float)q[c], s));
+            continue;
+        }
         uint2 u[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int c = c0 + (i * 32 + lane) * 8;
-            if (RAGGED ? c + 8 <= width : c < width) {
-                asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(u[i].x), "=r"(u[i].y) : "l"(q + c));
-            } else {
-                uint8_t b[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (RAGGED)
-#pragma unroll
-                    for (int e = 0; e < 7; ++e) if (c + e < width) b[e] = (uint8_t)q[c + e];
-                u[i].x = b[0] | b[1] << 8 | b[2] << 16 | (uint32_t)b[3] << 24;
-                u[i].y = b[4] | b[5] << 8 | b[6] << 16 | (uint32_t)b[7] << 24;
-            }
+            const long c = c0 + (i * 32 + lane) * 8;
+            u[i] = make_uint2(0, 0);
+            if (c < width) asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(u[i].x), "=r"(u[i].y) : "l"(q + c));
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int c = c0 + (i * 32 + lane) * 8;
+            const long c = c0 + (i * 32 + lane) * 8;
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(256) dequant_kernel(const int8_t* q, long ldq,
                 const uint32_t w = (e < 4 ? u[i].x : u[i].y) ^ 0x80808080u;
                 v[e] = __fmul_rn(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540u | (uint32_t)(e & 3))) - 8388736.f, s);
             }
-            store_some<RAGGED, 8>(y + c, width - c, v);
+            if (c < width) store_some<false, 8>(y + c, 8, v);
         }
     }
 }
@@ -464,17 +465,18 @@ extern "C" int32_t lumi_k_gate_quant(uint64_t gu, int32_t dtype, int32_t ld, int
 extern "C" int32_t lumi_k_dequant_rows(uint64_t q, int32_t ldq, uint64_t scale, uint64_t y, int32_t y_dtype, int32_t ldy, int32_t rows, int32_t width,
                                        uint64_t stream) {
     if (!q || !scale || !y || !known(y_dtype) || rows < 0 || width <= 0 || ldq < width || ldy < width) return fail(LUMI_E_INVALID, "bad argument to lumi_k_dequant_rows");
-    if (!aligned_rows(y, y_dtype, ldy) || (q & 15) || ldq % 16 || (scale & 3))
-        return fail(LUMI_E_INVALID, "lumi_k_dequant_rows: rows have to begin on 16-byte boundaries");
+    if ((q & 15) || ldq % 16 || (scale & 3) || (y & (y_dtype == LUMI_DTYPE_F32 ? 3 : 1)))
+        return fail(LUMI_E_INVALID, "lumi_k_dequant_rows: rows of q have to begin on 16-byte boundaries, numbers on their own");
     if (rows == 0) return LUMI_OK;
     LUMI_TRY(check_device_memory("lumi_k_dequant_rows", {q, scale, y}));
     cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = dependent_launch(dim3((unsigned)(((long)rows + 7) / 8), std::min(65535, (width + 1023) / 1024)), 256, attr, (cudaStream_t)stream);
-    auto go = [&](auto* to, auto r) {
+    const cudaLaunchConfig_t cfg = dependent_launch(dim3((unsigned)(((long)rows + 7) / 8), (unsigned)std::min(65535l, ((long)width + 1023) / 1024)), 256, attr, (cudaStream_t)stream);
+    auto go = [&](auto* to, auto one) {
         using YT = std::remove_pointer_t<decltype(to)>;
-        return cudaLaunchKernelEx(&cfg, dequant_kernel<YT, decltype(r)::value>, (const int8_t*)q, (long)ldq, (const float*)scale, to, (long)ldy, rows, width);
+        return cudaLaunchKernelEx(&cfg, dequant_kernel<YT, decltype(one)::value>, (const int8_t*)q, (long)ldq, (const float*)scale, to, (long)ldy, rows, width);
     };
-    if (y_dtype == LUMI_DTYPE_F32) LUMI_CUDA(width % 8 ? go((float*)y, std::true_type{}) : go((float*)y, std::false_type{}));
-    else LUMI_CUDA(width % 8 ? go((__nv_bfloat16*)y, std::true_type{}) : go((__nv_bfloat16*)y, std::false_type{}));
+    const bool one = width % 8 != 0 || !aligned_rows(y, y_dtype, ldy);
+    if (y_dtype == LUMI_DTYPE_F32) LUMI_CUDA(one ? go((float*)y, std::true_type{}) : go((float*)y, std::false_type{}));
+    else LUMI_CUDA(one ? go((__nv_bfloat16*)y, std::true_type{}) : go((__nv_bfloat16*)y, std::false_type{}));
     return LUMI_OK;
 }

@@ -202,8 +202,10 @@ def test_rows_back(width, dtype):
         s = torch.randn(rows + 1, generator=g, device="cuda")
         if rows > 2:
             s[1], s[2] = float("nan"), float("inf")
-        y = torch.full((rows, ld), 7.0, device="cuda", dtype=dtype)
-        call("lumi_k_dequant_rows", q.data_ptr(), ld, s.data_ptr(), y.data_ptr(), code(y), ld, rows, width, 0)
-        torch.cuda.synchronize()
-        assert bool((y[:, width:] == 7).all())
-        assert torch.equal((q[:, :width].float() * s[:rows, None]).to(dtype).nan_to_num(nan=1e30), y[:, :width].nan_to_num(nan=1e30))
+        for ldy, shift in ((ld, 0), (width, 0), (width + 1, 1)):
+            whole = torch.full((rows * ldy + 8,), 7.0, device="cuda", dtype=dtype)
+            y = whole[shift:shift + rows * ldy].view(rows, ldy)
+            call("lumi_k_dequant_rows", q.data_ptr(), ld, s.data_ptr(), y.data_ptr(), code(y), ldy, rows, width, 0)
+            torch.cuda.synchronize()
+            assert bool((y[:, width:] == 7).all()) and bool((whole[:shift] == 7).all()) and bool((whole[shift + rows * ldy:] == 7).all())
+            assert torch.equal((q[:, :width].float() * s[:rows, None]).to(dtype).nan_to_num(nan=1e30), y[:, :width].nan_to_num(nan=1e30))

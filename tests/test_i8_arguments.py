@@ -48,8 +48,8 @@ def test_gate_refuses(k):
 
 
 @pytest.mark.parametrize("k", [
-    dict(q=0), dict(scale=0), dict(y=0), dict(y_dtype=2), dict(rows=-1), dict(width=0), dict(ldq=48), dict(ldq=72), dict(ldy=60), dict(ldy=66), dict(ldy=68, y_dtype=1),
-    dict(q=P + 8), dict(scale=P + 2), dict(y=P + 4)])
+    dict(q=0), dict(scale=0), dict(y=0), dict(y_dtype=2), dict(rows=-1), dict(width=0), dict(ldq=48), dict(ldq=72), dict(ldy=60),
+    dict(q=P + 8), dict(scale=P + 2), dict(y=P + 2), dict(y=P + 1, y_dtype=1)])
 def test_dequant_refuses(k):
     assert dequant(**k) == INVALID
 
