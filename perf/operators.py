@@ -164,13 +164,13 @@ def _library(s):
         gu = s["gu"]
         check(lib.lumi_k_gate_quant(gu.data_ptr(), _dtype(gu), gu.stride(0), s["up"], 1 if s["act"] == "silu" else 0, q.data_ptr(), q.stride(0),
                                     scale.data_ptr(), s["rows"], s["width"], stream))
-        torch.mul(q, scale[:, None], out=y)      # the values that the integers stand for
+        check(lib.lumi_k_dequant_rows(q.data_ptr(), q.stride(0), scale.data_ptr(), y.data_ptr(), 1, y.stride(0), s["rows"], s["width"], stream))
         return {"y": y, "scale": scale}
     v, o, w = s["v"], s["add"], s["w"]
     check(lib.lumi_k_norm_quant(v.data_ptr(), _dtype(v), v.stride(0), 0 if o is None else o.data_ptr(), 0 if o is None else _dtype(o),
                                 0 if o is None else o.stride(0), 0 if w is None else w.data_ptr(), q.data_ptr(), q.stride(0), scale.data_ptr(),
                                 s["rows"], s["width"], EPS, stream))
-    torch.mul(q, scale[:, None], out=y)
+    check(lib.lumi_k_dequant_rows(q.data_ptr(), q.stride(0), scale.data_ptr(), y.data_ptr(), 1, y.stride(0), s["rows"], s["width"], stream))
     return {"y": y, "scale": scale, "x": v}
 
 
