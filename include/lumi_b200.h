@@ -358,7 +358,7 @@ int32_t lumi_k_gate_mul(uint64_t gu, int32_t ld, uint64_t out32, uint64_t hi, ui
  * m = max(max |t|, 2^-100): t is about q * s.  A row that holds an infinity or a NaN gets q = 0 and s = NaN, so that all that is made from it is NaN.
  * These calls have no counterpart in the reference.  All pointers are memory of the current device; what lies between a row's end and the next
  * row (ld) is neither read nor written, rows begin on 16-byte boundaries.  Nothing is allocated and no workspace is shared: calls may overlap on any
- * streams and be captured into graphs.  With no rows a call does nothing. */
+ * streams and be captured into graphs.  With no rows a call does nothing; rows of more than 2^30 numbers are LUMI_E_UNSUPPORTED. */
 
 /* The norm in front of a projection: x[r] += o[r] (o = 0: x is left alone; the sum is rounded to x's type, and the norm sees the rounded row), then
  * the rows x[r] / sqrt(mean(x[r]^2) + eps) * w over `width` elements as q[rows][ldq] and scale[rows].  w = 0: no norm, the rows of x as they are (a
@@ -378,11 +378,17 @@ int32_t lumi_k_dequant_rows(uint64_t q, int32_t ldq, uint64_t scale, uint64_t y,
 
 /* D[m][n] = (sum over k of a[m][k] * w[n][k]) * a_scale[m] * w_scale[n] + bias[n] (+ D[m][n] if accumulate != 0); a [M][lda] and w [N][ldw] 8-bit
  * integers (-128 is allowed), sums in 32-bit integers and so exact, the rest in fp32, rounded once to D's type (d_dtype LUMI_DTYPE_*, rows of ldd
- * elements; no alignment beyond the element's).  bias may be 0.  K <= 131071 (LUMI_E_UNSUPPORTED beyond: the sums could overflow); lda and ldw are
+ * elements; no alignment beyond the element's).  bias may be 0.  K <= 131071, M and N <= 2^30 (LUMI_E_UNSUPPORTED beyond; longer sums could overflow); lda and ldw are
  * multiples of 16, a and w 16-byte aligned; D overlaps none of the operands.  status: a device int32 or 0; a bounded wait on the device that gave up
  * sets the bit 4 of it and leaves NaN in the results that it cost. */
 int32_t lumi_k_gemm_i8(uint64_t a, int32_t lda, uint64_t a_scale, uint64_t w, int32_t ldw, uint64_t w_scale, uint64_t bias, uint64_t d, int32_t d_dtype,
                        int32_t ldd, int32_t M, int32_t N, int32_t K, int32_t accumulate, uint64_t status, uint64_t stream);
+
+/* Failure-path test hook of that product: waits limited to wait_limit_ns, the operands of tile skip_unit (-1: none; in launch order, a pair's second CTA's) never
+ * arrive.  status: a zeroed device int32.  Returns LUMI_E_TIMEOUT when a wait gave up; the kernel has then returned cleanly and further calls work.  (Up to eight
+ * rows may have kernels without waits.)  Synchronises the default stream. */
+int32_t lumi_debug_gemm_i8_wait_timeout(uint64_t a, int32_t lda, uint64_t a_scale, uint64_t w, int32_t ldw, uint64_t w_scale, uint64_t d, int32_t d_dtype,
+                                        int32_t ldd, int32_t M, int32_t N, int32_t K, int32_t accumulate, uint64_t wait_limit_ns, int32_t skip_unit, uint64_t status);
 
 /* One Mamba block (RMSNorm -> in_proj -> state step -> out_proj + residual, inference/src/model.rs:296-375
  * in arithmetic) WITHOUT any allocation.  This entry point has no counterpart in the reference.

@@ -26,7 +26,7 @@ EXPORTS = [
     "lumi_session_free", "lumi_session_set_option", "lumi_prefill", "lumi_prefill_ragged", "lumi_extend", "lumi_model_set_option", "lumi_decode_step", "lumi_generate",
     "lumi_decode_loop_device", "lumi_profile_step", "lumi_score", "lumi_session_read_state", "lumi_session_state_bytes", "lumi_session_save_state", "lumi_session_load_state", "lumi_debug_run_block", "lumi_k_gemm_bf16_tcgen05",
     "lumi_k_gemv", "lumi_k_row_gemm", "lumi_debug_row_gemm_wait_timeout", "lumi_debug_gemm_wait_timeout", "lumi_debug_gemm", "lumi_debug_fmod_near", "lumi_debug_gemm_plan", "lumi_k_ssm_step", "lumi_k_ssd_prefill", "lumi_k_delta_rule",
-    "lumi_k_window_attention", "lumi_k_norm_add", "lumi_k_gate_mul", "lumi_k_norm_quant", "lumi_k_gate_quant", "lumi_k_dequant_rows", "lumi_k_gemm_i8", "lumi_mamba_block_static",
+    "lumi_k_window_attention", "lumi_k_norm_add", "lumi_k_gate_mul", "lumi_k_norm_quant", "lumi_k_gate_quant", "lumi_k_dequant_rows", "lumi_k_gemm_i8", "lumi_debug_gemm_i8_wait_timeout", "lumi_mamba_block_static",
 ]
 
 
@@ -113,6 +113,7 @@ def lib():
         L.lumi_k_gate_quant.argtypes = [u64] + [i32] * 4 + [u64, i32, u64, i32, i32, u64]
         L.lumi_k_dequant_rows.argtypes = [u64, i32, u64, u64] + [i32] * 4 + [u64]
         L.lumi_k_gemm_i8.argtypes = [u64, i32, u64, u64, i32, u64, u64, u64] + [i32] * 6 + [u64, u64]
+        L.lumi_debug_gemm_i8_wait_timeout.argtypes = [u64, i32, u64, u64, i32, u64, u64] + [i32] * 6 + [u64, i32, u64]
         L.lumi_mamba_block_static.argtypes = [vp, i32, u64, u64, u64, u64, u64, i32, u64]
         _lib = L
     return _lib

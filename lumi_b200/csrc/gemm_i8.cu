@@ -1,10 +1,10 @@
 // Products in 8-bit integers: D[m][n] = (sum over k of A[m][k] W[n][k]) * a_scale[m] * w_scale[n] + bias[n] (+ D[m][n]).  The sums are 32-bit
 // integers and therefore exact in any order: the kernels below, and any share of K, give the same bits.
 //
-// Three kernels: vector_kernel for up to eight rows (multiply-adds of four bytes on the CUDA cores, bound by the stream of W), tile_kernel for a batch of rows
-// (tcgen05, one tile per CTA or, with K shared, per cluster), pair_kernel for many (tcgen05 by pairs of CTAs, persistent, two accumulators).  In both tensor-core kernels the
-// weights are on the MMA's 128-row side and the rows of A are its columns: an accumulator lane is a column of D, so that a warp's 32 lanes write
-// 32 neighbouring results of a row of D without any rearrangement, whatever D's alignment.
+// Four kernels: vector_kernel for one or two rows (multiply-adds of four bytes on the CUDA cores), few_kernel for up to eight and a small W (warp-level MMA),
+// tile_kernel for a batch of rows (tcgen05, one tile per CTA or, with K shared, per cluster) and pair_kernel for many (tcgen05 by pairs of CTAs, persistent, two
+// accumulators).  In both tcgen05 kernels the weights are on the MMA's 128-row side and the rows of A are its columns: an accumulator lane is a column
+// of D, so that a warp's 32 lanes write 32 neighbouring results of a row of D without any rearrangement, whatever D's alignment.
 #include "device_args.h"
 #include "rows.cuh"
 #include "tcgen05.cuh"
@@ -20,6 +20,8 @@ constexpr int kWRows = 128;                  // rows of W per CTA: the M of the 
 constexpr int kWBytes = kWRows * kBlockK;
 constexpr int kMaxCols = 256;                // rows of A per tile: the N of the MMA
 constexpr int kMaxStages = 8;
+constexpr int kMaxRows = 1 << 30;            // of A and of W: places of tiles are 32-bit numbers
+constexpr int kClusterCtas = 128;             // CTAs in clusters that run at once for certain
 
 struct I8Args {
     const int8_t *a, *w;
@@ -37,9 +39,9 @@ __device__ __forceinline__ float old_value(const __nv_bfloat16* p) { return __bf
 __device__ __forceinline__ void put_value(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put_value(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 // the sum's way to a result, the same operations in every kernel
-__device__ __forceinline__ float scaled(int sum, float sa, float sw, float bias) { return __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(sum), sa), sw), bias); }
+__device__ __forceinline__ float scaled(int sum, float sa, float sw, float bias) { return __fmaf_rn(__fmul_rn(__int2float_rn(sum), sa), sw, bias); }
 
-// ---- up to eight rows: a warp takes R rows of W and a share of K --------------------------------
+// ---- one or two rows: a warp takes two rows of W and a share of K --------------------------------
 __device__ __forceinline__ int4 bytes16(const int8_t* p, int n) {       // the first n bytes, n < 16, zeros behind
     uint32_t u[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -49,7 +51,7 @@ __device__ __forceinline__ int4 bytes16(const int8_t* p, int n) {       // the f
 // of W: read once, and only behind the dependency wait
 __device__ __forceinline__ int4 stream16(const int8_t* p) {
     int4 v;
-    asm volatile("ld.global.cs.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.global.L1::no_allocate.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
 __device__ __forceinline__ int dot16(const int4& a, const int4& b, int s) {
@@ -59,6 +61,7 @@ __device__ __forceinline__ int dot16(const int4& a, const int4& b, int s) {
 constexpr int kVecRows = 2;                  // rows of W per warp
 constexpr int kVecDeep = 4;                  // pieces of 512 bytes of each that are under way
 
+// MB rows of A
 template <int MB, typename DT>
 __global__ void __launch_bounds__(256) vector_kernel(I8Args g, int shares) {
     __shared__ int part[8][kVecRows * MB];
@@ -87,7 +90,6 @@ __global__ void __launch_bounds__(256) vector_kernel(I8Args g, int shares) {
             if (k0 + u * step >= whole) break;
 #pragma unroll
             for (int m = 0; m < MB; ++m) {
-                if (m >= g.M) break;
                 const int4 a = *reinterpret_cast<const int4*>(g.a + m * g.lda + k0 + u * step);
 #pragma unroll
                 for (int r = 0; r < kVecRows; ++r) sum[r][m] = dot16(a, v[u][r], sum[r][m]);
@@ -99,8 +101,7 @@ __global__ void __launch_bounds__(256) vector_kernel(I8Args g, int shares) {
         for (int r = 0; r < kVecRows; ++r) {
             const int4 v = bytes16(w[r] + whole, g.K - whole);
 #pragma unroll
-            for (int m = 0; m < MB; ++m)
-                if (m < g.M) sum[r][m] = dot16(bytes16(g.a + m * g.lda + whole, g.K - whole), v, sum[r][m]);
+            for (int m = 0; m < MB; ++m) sum[r][m] = dot16(bytes16(g.a + m * g.lda + whole, g.K - whole), v, sum[r][m]);
         }
     }
 #pragma unroll
@@ -114,10 +115,76 @@ __global__ void __launch_bounds__(256) vector_kernel(I8Args g, int shares) {
     if (share != 0) return;
     for (int i = lane; i < kVecRows * MB; i += 32) {
         const int n = n0 + i / MB, m = i % MB;
-        if (n >= g.N || m >= g.M) continue;
+        if (n >= g.N) continue;
         int t = part[warp][i];
         for (int s = 1; s < shares; ++s) t += part[warp + s][i];
         float v = scaled(t, g.a_scale[m], g.w_scale[n], g.bias != nullptr ? g.bias[n] : 0.f);
+        DT* d = (DT*)g.d + m * g.ldd + n;
+        if (g.accumulate) v = __fadd_rn(v, old_value(d));
+        put_value(d, v);
+    }
+}
+
+// ---- three to eight rows: a warp takes 16 rows of W and a share of K ------------------------------
+__device__ __forceinline__ void mma_i8(int (&c)[4], int a0, int a1, int a2, int a3, int b0, int b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+constexpr int kFewW = 16;                    // rows of W per warp: the M of the MMA; rows of A are its columns
+constexpr int kFewRows = 8, kFewK = 4096;    // and only while W is small: at 16 MB the tensor cores' tiles stream it as fast
+constexpr long kFewBytes = 16l << 20;
+constexpr int kFewDeep = 4;                  // steps of 64 bytes of each that are under way
+
+// Lane 4 g + t holds bytes 16 t to 16 t + 15 of a step of rows g and g + 8 of W and of row g of A.  An MMA wants bytes 4 t and 16 + 4 t of 32: which bytes of K
+// these are does not matter as long as they are the same of both operands, so it is given words 0 and 1, the next one words 2 and 3.
+template <typename DT>
+__global__ void __launch_bounds__(256) few_kernel(I8Args g, int shares) {
+    __shared__ int4 part[8][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, t = lane & 3;
+    const int share = warp % shares, n0 = (blockIdx.x * (8 / shares) + warp / shares) * kFewW;
+    pdl_release();
+    pdl_sync();
+    int sum[4] = {0, 0, 0, 0};
+    const int8_t *w0 = g.w + (long)min(n0 + row, g.N - 1) * g.ldw, *w1 = g.w + (long)min(n0 + row + 8, g.N - 1) * g.ldw;
+    const int whole = g.K & ~15, step = shares * 64;
+    const int8_t* a = g.a + min(row, g.M - 1) * g.lda;
+    auto multiply = [&](const int4& u, const int4& v, const int4& x) {
+        mma_i8(sum, u.x, v.x, u.y, v.y, x.x, x.y);
+        mma_i8(sum, u.z, v.z, u.w, v.w, x.z, x.w);
+    };
+    const int4 zero = make_int4(0, 0, 0, 0);
+    for (int k0 = share * 64 + t * 16; k0 - t * 16 < whole; k0 += kFewDeep * step) {      // (the same for a whole warp)
+        int4 u[kFewDeep], v[kFewDeep];
+#pragma unroll
+        for (int d = 0; d < kFewDeep; ++d) {
+            const bool in = k0 + d * step < whole;
+            u[d] = in ? stream16(w0 + k0 + d * step) : zero;
+            v[d] = in ? stream16(w1 + k0 + d * step) : zero;
+        }
+#pragma unroll
+        for (int d = 0; d < kFewDeep; ++d)
+            multiply(u[d], v[d], k0 + d * step < whole && row < g.M ? *reinterpret_cast<const int4*>(a + k0 + d * step) : zero);
+    }
+    if (whole < g.K && share == shares - 1) {             // the last bytes of a K that is no multiple of 16
+        const int n = t == 0 ? g.K - whole : 0;
+        multiply(bytes16(w0 + whole, n), bytes16(w1 + whole, n), bytes16(a + whole, row < g.M ? n : 0));
+    }
+    if (shares > 1) {
+        part[warp][lane] = make_int4(sum[0], sum[1], sum[2], sum[3]);
+        __syncthreads();
+        if (share != 0) return;
+        for (int s = 1; s < shares; ++s) {
+            const int4 p = part[warp + s][lane];
+            sum[0] += p.x; sum[1] += p.y; sum[2] += p.z; sum[3] += p.w;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int n = n0 + row + (e >> 1) * 8, m = 2 * t + (e & 1);
+        if (n >= g.N || m >= g.M) continue;
+        float v = scaled(sum[e], g.a_scale[m], g.w_scale[n], g.bias != nullptr ? g.bias[n] : 0.f);
         DT* d = (DT*)g.d + m * g.ldd + n;
         if (g.accumulate) v = __fadd_rn(v, old_value(d));
         put_value(d, v);
@@ -141,60 +208,95 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d, uint64_t a, uint64_t b,
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// signed bytes by signed bytes into 32-bit integers, `rows` x `cols`
-__device__ __forceinline__ uint32_t i8_idesc(int rows, int cols) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(rows >> 4) << 24); }
-__device__ __forceinline__ void st_cluster_s32(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
-
-// Results of one row of W (this lane's) for 32 rows of A from m0 on, of which `live` exist.  buf: 32 floats of shared memory of this warp's own.
-template <bool WHOLE, typename DT>
-__device__ __forceinline__ void finish_columns(const I8Args& g, const uint32_t (&sum)[32], const float* buf, DT* d, int live, bool in, float sw, float bias) {
-    constexpr int STEP = 16;                              // old values that are under way together
-#pragma unroll
-    for (int j0 = 0; j0 < 32; j0 += STEP) {
-        float old[STEP];
-        if (g.accumulate) {
-            const DT* p = d;
-#pragma unroll
-            for (int j = 0; j < STEP; ++j, p += g.ldd) old[j] = in && (WHOLE || j0 + j < live) ? old_value(p) : 0.f;
-        }
-#pragma unroll
-        for (int j4 = 0; j4 < STEP; j4 += 4) {
-            const float4 sa = *reinterpret_cast<const float4*>(buf + j0 + j4);
-            const float s[4] = {sa.x, sa.y, sa.z, sa.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e, d += g.ldd) {
-                float v = scaled((int)sum[j0 + j4 + e], s[e], sw, bias);
-                if (g.accumulate) v = __fadd_rn(v, old[j4 + e]);
-                if (in && (WHOLE || j0 + j4 + e < live)) put_value(d, v);
-            }
+// Bounded wait, as mbar_wait, but the clock is only looked at every so many tries: reading it takes about as long as a stage of the pipeline.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+    uint64_t t0 = 0;
+    for (uint32_t i = 1;; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 63) == 0) {
+            const uint64_t t = globaltimer_ns();
+            if (t0 == 0) t0 = t;
+            else if (t - t0 > limit_ns) return false;
         }
     }
 }
+// An arrival that orders nothing but itself: a release would wait for this thread's results to reach memory, while all that the barrier guards has been read.
+__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// An operand tile's descriptor changes in its low word alone, by 16 bytes per one: the issuing thread adds, since composing two of them per MMA takes it
+// longer than a narrow MMA.
+__device__ __forceinline__ uint64_t moved(uint64_t desc, uint32_t units) { return (desc & 0xffffffff00000000ull) | (uint32_t)((uint32_t)desc + units); }
+// signed bytes by signed bytes into 32-bit integers, `rows` x `cols`
+__device__ __forceinline__ uint32_t i8_idesc(int rows, int cols) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(rows >> 4) << 24); }
+__device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__device__ __forceinline__ void shared_load4(uint32_t at, float (&v)[32], int i) {
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[i]), "=f"(v[i + 1]), "=f"(v[i + 2]), "=f"(v[i + 3]) : "r"(at + 4 * i) : "memory");
+}
+__device__ __forceinline__ float shared_value(uint32_t at, const float*) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float shared_value(uint32_t at, const __nv_bfloat16*) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+    return __uint_as_float((uint32_t)v << 16);
+}
+__device__ __forceinline__ void shared_put(uint32_t at, float v, const float*) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
+__device__ __forceinline__ void shared_put(uint32_t at, float v, const __nv_bfloat16*) {
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(__bfloat16_as_ushort(__float2bfloat16_rn(v))) : "memory");
+}
+// Results of one row of W (this lane's) for 32 rows of A, of which `live` exist; a_scale: in shared memory.
+template <bool WHOLE, typename DT>
+__device__ __forceinline__ void finish_columns(const I8Args& g, const uint32_t (&sum)[32], const float* a_scale, DT* d, int live, bool in, float sw, float bias) {
+    // everything is read before anything is written: the compiler cannot tell results from scales, and would wait for each group of them
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) shared_load4(smem_u32(a_scale), v, j);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = scaled((int)sum[j], v[j], sw, bias);
+    constexpr int STEP = 16;                              // old values that are under way together
+#pragma unroll
+    for (int j0 = 0; j0 < 32; j0 += STEP) {
+        if (g.accumulate) {
+            float old[STEP];
+            const DT* p = d;
+#pragma unroll
+            for (int j = 0; j < STEP; ++j, p += g.ldd) old[j] = in && (WHOLE || j0 + j < live) ? old_value(p) : 0.f;
+#pragma unroll
+            for (int j = 0; j < STEP; ++j) v[j0 + j] = __fadd_rn(v[j0 + j], old[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < STEP; ++j, d += g.ldd)
+            if (in && (WHOLE || j0 + j < live)) put_value(d, v[j0 + j]);
+    }
+}
 template <typename DT>
-__device__ __forceinline__ void finish_strip(const I8Args& g, uint32_t acc, float* buf, int m0, int n, float sw, float bias, bool lost) {
-    const int lane = threadIdx.x & 31, live = min(32, g.M - m0);
+__device__ __forceinline__ void finish_strip(const I8Args& g, uint32_t acc, const float* a_scale, int m0, int n, float sw, float bias, bool lost) {
+    const int live = min(32, g.M - m0);
     const bool in = n < g.N;
     DT* d = (DT*)g.d + (long)m0 * g.ldd + n;
     if (lost) {
         for (int j = 0; j < live; ++j) if (in) put_value(d + j * g.ldd, __uint_as_float(0x7fffffffu));
         return;
     }
-    __syncwarp();                                         // the last strip's scales have been read
-    buf[lane] = lane < live ? g.a_scale[m0 + lane] : 0.f;
     uint32_t sum[32];
     tmem_ld32(acc, sum);
-    __syncwarp();
-    if (live == 32) finish_columns<true, DT>(g, sum, buf, d, live, in, sw, bias);
-    else finish_columns<false, DT>(g, sum, buf, d, live, in, sw, bias);
+    if (live == 32) finish_columns<true, DT>(g, sum, a_scale, d, live, in, sw, bias);
+    else finish_columns<false, DT>(g, sum, a_scale, d, live, in, sw, bias);
 }
 
 struct TileTail {
     uint64_t full[kMaxStages], empty[kMaxStages], done, drain;
     uint32_t tmem_slot;
     int lost;                                // a wait of this CTA, or of one that shares K with it, ran out
-    alignas(16) float scales[8][32];
+    alignas(16) float a_scale[kMaxCols];     // of the tile's rows of A
 };
-constexpr int kTailBytes = 1280;
+constexpr int kTailBytes = 1536;
 static_assert(sizeof(TileTail) <= kTailBytes, "tail of the shared memory");
 
 struct TileShape { int cols, stages, splits; };
@@ -206,7 +308,7 @@ __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUten
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int S = sh.stages, cols = sh.cols, splits = sh.splits, stage = kWBytes + cols * kBlockK;
-    int* part = reinterpret_cast<int*>(base + S * stage);               // splits > 1: [split][row of A][row of W]
+    int* part = reinterpret_cast<int*>(base + S * stage);               // splits > 1: [split][four rows of A][row of W][4]
     TileTail& tl = *reinterpret_cast<TileTail*>(base + S * stage + (splits > 1 ? cols * kWRows * 4 : 0));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)blockIdx.x % splits, n0 = (int)blockIdx.x / splits * kWRows, m0 = blockIdx.y * cols;
@@ -242,7 +344,7 @@ __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUten
             int s = 0, issued = 0;
             uint32_t ph = 0;
             for (int i = 0; i < nkb; ++i) {
-                if (!mbar_wait(&tl.empty[s], ph ^ 1u, g.wait_ns)) { timed_out = true; break; }
+                if (!wait_for(&tl.empty[s], ph ^ 1u, g.wait_ns)) { timed_out = true; break; }
                 mbar_expect_tx(&tl.full[s], (uint32_t)stage);
                 tma_load_2d(base + s * stage, &map_w, &tl.full[s], (kb0 + i) * kBlockK, n0);
                 tma_load_2d(base + s * stage + kWBytes, &map_a, &tl.full[s], (kb0 + i) * kBlockK, m0);
@@ -250,67 +352,81 @@ __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUten
                 if (++s == S) { s = 0; ph ^= 1u; }
             }
             if (timed_out)                                              // let the copies land (bounded) that nobody may consume
-                for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(&tl.full[i % S], (uint32_t)(i / S) & 1u, g.wait_ns);
+                for (int i = max(0, issued - S); i < issued; ++i) wait_for(&tl.full[i % S], (uint32_t)(i / S) & 1u, g.wait_ns);
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            const uint32_t idesc = i8_idesc(kWRows, cols);
+            const uint32_t idesc = i8_idesc(kWRows, cols), units = (uint32_t)stage >> 4;
+            const uint64_t w0 = make_smem_desc(smem_u32(base)), a0 = make_smem_desc(smem_u32(base) + kWBytes);
             int s = 0;
             uint32_t ph = 0;
+            bool here = nkb > 0 && mbar_try_wait(&tl.full[0], 0);
             for (int i = 0; i < nkb; ++i) {
-                if (!mbar_wait(&tl.full[s], ph, g.wait_ns)) { timed_out = true; break; }
+                if (!here && !wait_for(&tl.full[s], ph, g.wait_ns)) { timed_out = true; break; }
                 tc_fence_after();
-                const uint32_t w = smem_u32(base + s * stage);
+                const uint64_t w = moved(w0, (uint32_t)s * units), a = moved(a0, (uint32_t)s * units);
 #pragma unroll
-                for (int k = 0; k < kBlockK / 32; ++k)
-                    umma_i8(tmem, make_smem_desc(w + k * 32), make_smem_desc(w + kWBytes + k * 32), idesc, (i > 0 || k > 0) ? 1u : 0u);
+                for (int k = 0; k < kBlockK / 32; ++k) umma_i8(tmem, moved(w, 2 * k), moved(a, 2 * k), idesc, (i > 0 || k > 0) ? 1u : 0u);
                 umma_commit(&tl.empty[s]);
                 if (++s == S) { s = 0; ph ^= 1u; }
+                here = i + 1 < nkb && mbar_try_wait(&tl.full[s], ph);
             }
             if (!timed_out) {
                 umma_commit(&tl.done);
             } else {                                                    // let every MMA issued so far finish (bounded), then pass the word on
                 umma_commit(&tl.drain);
-                mbar_wait(&tl.drain, 0, g.wait_ns);
+                wait_for(&tl.drain, 0, g.wait_ns);
                 *reinterpret_cast<volatile int*>(&tl.lost) = 1;
                 mbar_arrive(&tl.done);
             }
         }
     }
+    else if (warp < 6) {
+        for (int i = threadIdx.x - 64; i < cols; i += 128) tl.a_scale[i] = m0 + i < g.M ? g.a_scale[m0 + i] : 0.f;
+    }
     __syncwarp();
     const int q = warp & 3, half = warp >> 2;                           // TMEM lane quarter this warp may read; its share of the columns
     const int n = n0 + q * 32 + lane;
     const float sw = n < g.N ? g.w_scale[n] : 0.f, bias = n < g.N && g.bias != nullptr ? g.bias[n] : 0.f;
-    if (splits > 1) cluster_wait();                                     // every CTA of the cluster runs
-    if (!mbar_wait(&tl.done, 0, g.wait_ns)) timed_out = true;
+    const int RB = cols / splits, mine = m0 + rank * RB;                // rows of A that each CTA of the cluster finishes, a multiple of four; this one's first
+    // groups of four of them go to this warp and the one with the same quarter in turn; old values of the first group are asked for ahead of the wait
+    DT* const d = (DT*)g.d + (long)mine * g.ldd + n;
+    auto old_of = [&](int r, float (&o)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = g.accumulate && n < g.N && r + e < RB && mine + r + e < g.M ? old_value(d + (r + e) * g.ldd) : 0.f;
+    };
+    float ahead[4] = {0.f, 0.f, 0.f, 0.f};
+    if (splits > 1) {
+        old_of(4 * half, ahead);
+        cluster_wait();                                                 // every CTA of the cluster runs
+    }
+    __syncthreads();                                                    // the rows' scales are there
+    if (!wait_for(&tl.done, 0, g.wait_ns)) timed_out = true;
     timed_out = __any_sync(0xffffffffu, timed_out);                     // tcgen05.ld below is warp-collective
     const bool lost = timed_out || *reinterpret_cast<volatile int*>(&tl.lost) != 0;
     tc_fence_after();
-    const int RB = cols / splits;                                       // rows of A that each CTA of the cluster finishes
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
     if (splits == 1) {
 #pragma unroll 1
         for (int cb = half; cb < cols / 32; cb += 2) {
             if (m0 + cb * 32 >= g.M) break;
-            finish_strip<DT>(g, lanes + (uint32_t)(cb * 32), tl.scales[warp], m0 + cb * 32, n, sw, bias, lost);
+            finish_strip<DT>(g, lanes + (uint32_t)(cb * 32), tl.a_scale + cb * 32, m0 + cb * 32, n, sw, bias, lost);
         }
     } else {
         if (lost) {
             if (lane == 0)
                 for (int c = 0; c < splits; ++c) st_cluster_u32(map_to_rank(smem_u32(&tl.lost), (uint32_t)c), 1u);
         } else {
-            const uint32_t slot = smem_u32(part) + (uint32_t)(rank * RB * kWRows + q * 32 + lane) * 4u;
+            const uint32_t slot = smem_u32(part) + (uint32_t)(rank * RB * kWRows + (q * 32 + lane) * 4) * 4u;
 #pragma unroll 1
             for (int cb = half; cb < cols / 32; cb += 2) {
                 if (m0 + cb * 32 >= g.M) break;
                 uint32_t r[32];
                 tmem_ld32(lanes + (uint32_t)(cb * 32), r);
 #pragma unroll
-                for (int j4 = 0; j4 < 32; j4 += 4) {                    // RB is a multiple of four
+                for (int j4 = 0; j4 < 32; j4 += 4) {
                     const int b = cb * 32 + j4, to = b / RB;
-                    const uint32_t at = map_to_rank(slot + (uint32_t)(b - to * RB) * (kWRows * 4u), (uint32_t)to);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) st_cluster_s32(at + (uint32_t)j * (kWRows * 4u), r[j4 + j]);
+                    st_cluster_v4(map_to_rank(slot + (uint32_t)(b - to * RB) * (kWRows * 4u), (uint32_t)to), r[j4], r[j4 + 1], r[j4 + 2], r[j4 + 3]);
                 }
             }
         }
@@ -325,18 +441,26 @@ __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUten
     if (timed_out && g.status != nullptr) atomicOr(g.status, STATUS_TIMEOUT);
     if (splits == 1) return;
 
-    // ---- the rows of A that this CTA finishes: a warp's quarter of the rows of W, every second row of A
+    // ---- the rows of A that this CTA finishes
     const bool any_lost = *reinterpret_cast<volatile int*>(&tl.lost) != 0;
     if (n >= g.N) return;
-    for (int r = half; r < RB; r += 2) {
-        const int m = m0 + rank * RB + r;
-        if (m >= g.M) break;
-        int sum = 0;
-        for (int c = 0; c < splits; ++c) sum += part[(c * RB + r) * kWRows + q * 32 + lane];
-        DT* d = (DT*)g.d + (long)m * g.ldd + n;
-        float v = scaled(sum, g.a_scale[m], sw, bias);
-        if (g.accumulate) v = __fadd_rn(v, old_value(d));
-        put_value(d, any_lost ? __uint_as_float(0x7fffffffu) : v);
+    for (int r = 4 * half; r < RB; r += 8) {
+        if (mine + r >= g.M) break;
+        float next[4];
+        old_of(r + 8, next);
+        const int4* from = reinterpret_cast<const int4*>(part) + (r / 4) * kWRows + q * 32 + lane;
+        int4 sum = from[0];
+        for (int c = 1; c < splits; ++c) {
+            const int4 t = from[c * (RB / 4) * kWRows];
+            sum.x += t.x; sum.y += t.y; sum.z += t.z; sum.w += t.w;
+        }
+        const float4 sa = *reinterpret_cast<const float4*>(tl.a_scale + rank * RB + r);
+        const float v[4] = {scaled(sum.x, sa.x, sw, bias), scaled(sum.y, sa.y, sw, bias), scaled(sum.z, sa.z, sw, bias), scaled(sum.w, sa.w, sw, bias)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (mine + r + e < g.M) put_value(d + (r + e) * g.ldd, any_lost ? __uint_as_float(0x7fffffffu) : (g.accumulate ? __fadd_rn(v[e], ahead[e]) : v[e]));
+            ahead[e] = next[e];
+        }
     }
 }
 
@@ -348,20 +472,34 @@ __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUten
 constexpr int kPairThreads = 320;
 struct PairTail {
     uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], drain;
+    uint64_t old[8][2];                      // old values of D have arrived in a warp's buffers
     uint32_t tmem_slot, gave_up, issued[2];
     alignas(16) float scales[8][32];
 };
 static_assert(sizeof(PairTail) <= kTailBytes, "tail of the shared memory");
 constexpr int kBlockTiles = 16;
 
-struct PairShape { int cols, stages, tiles_a, tiles; };
+// staged: results (and old values) travel by tensor-map copies, which want D's rows to begin and end on 16-byte boundaries
+struct PairShape { int cols, stages, tiles_a, tiles, staged; };
+template <typename DT>
+constexpr int kStripBytes = 32 * 32 * (int)sizeof(DT);                  // a warp's strip of results; it has two such buffers
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* smem, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smem_u32(smem)), "r"(x), "r"(y) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// all but the last N stores of this thread have been read from shared memory
+template <int N>
+__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
 
 template <typename DT>
-__global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, I8Args g, PairShape sh) {
+__global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                                                                   const __grid_constant__ CUtensorMap map_d, I8Args g, PairShape sh) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int S = sh.stages, cols = sh.cols, stage = kWBytes + cols / 2 * kBlockK;
-    PairTail& tl = *reinterpret_cast<PairTail*>(base + S * stage);
+    uint8_t* strips = base + S * stage;
+    PairTail& tl = *reinterpret_cast<PairTail*>(strips + 16 * kStripBytes<DT>);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)(blockIdx.x & 1), first = (int)(blockIdx.x >> 1), at_once = (int)(gridDim.x >> 1);
     const int num_kb = (g.K + kBlockK - 1) / kBlockK, tiles_w = sh.tiles / sh.tiles_a;
@@ -369,6 +507,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) { mbar_init(&tl.full[s], 1); mbar_init(&tl.empty[s], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&tl.acc_full[i], 1); mbar_init(&tl.acc_empty[i], 16); }
+        for (int i = 0; i < 16; ++i) mbar_init(&tl.old[i >> 1][i & 1], 1);
         mbar_init(&tl.drain, 1);
         tl.gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -406,7 +545,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
                 int m0, n0;
                 place(t, m0, n0);
                 for (int kb = 0; kb < num_kb; ++kb, ++kbg) {
-                    if (!mbar_wait(&tl.empty[s], ph ^ 1u, g.wait_ns)) { timed_out = true; break; }
+                    if (!wait_for(&tl.empty[s], ph ^ 1u, g.wait_ns)) { timed_out = true; break; }
                     const uint32_t bar = map_to_rank(smem_u32(&tl.full[s]), 0);      // both CTAs' copies complete on the first one's barrier
                     if (rank == 0) mbar_expect_tx(&tl.full[s], 2u * (uint32_t)stage);
                     tma_load_2d_pair(base + s * stage, &map_w, bar, kb * kBlockK, n0 + rank * kWRows);
@@ -418,20 +557,20 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
-            const uint32_t idesc = i8_idesc(2 * kWRows, cols);
+            const uint32_t idesc = i8_idesc(2 * kWRows, cols), units = (uint32_t)stage >> 4;
+            const uint64_t w0 = make_smem_desc(smem_u32(base)), a0 = make_smem_desc(smem_u32(base) + kWBytes);
             int s = 0;
             uint32_t ph = 0, it = 0;
             for (int t = first; t < sh.tiles && !timed_out; t += at_once, ++it) {
                 const uint32_t as = it & 1u, aph = (it >> 1) & 1u, acc = tmem + as * kMaxCols;
-                if (!mbar_wait(&tl.acc_empty[as], aph ^ 1u, g.wait_ns)) { timed_out = true; break; }      // this accumulator has been read
+                if (!wait_for(&tl.acc_empty[as], aph ^ 1u, g.wait_ns)) { timed_out = true; break; }      // this accumulator has been read
                 tc_fence_after();
                 for (int kb = 0; kb < num_kb; ++kb) {
-                    if (!mbar_wait(&tl.full[s], ph, g.wait_ns)) { timed_out = true; break; }
+                    if (!wait_for(&tl.full[s], ph, g.wait_ns)) { timed_out = true; break; }
                     tc_fence_after();
-                    const uint32_t w = smem_u32(base + s * stage);
+                    const uint64_t w = moved(w0, (uint32_t)s * units), a = moved(a0, (uint32_t)s * units);
 #pragma unroll
-                    for (int k = 0; k < kBlockK / 32; ++k)
-                        umma_i8_pair(acc, make_smem_desc(w + k * 32), make_smem_desc(w + kWBytes + k * 32), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                    for (int k = 0; k < kBlockK / 32; ++k) umma_i8_pair(acc, moved(w, 2 * k), moved(a, 2 * k), idesc, (kb > 0 || k > 0) ? 1u : 0u);
                     umma_commit_pair(&tl.empty[s]);
                     if (++s == S) { s = 0; ph ^= 1u; }
                 }
@@ -440,32 +579,138 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
             }
             if (timed_out) {                                            // let every MMA issued so far finish (bounded) before TMEM is freed
                 umma_commit_pair(&tl.drain);
-                mbar_wait(&tl.drain, 0, g.wait_ns);
+                wait_for(&tl.drain, 0, g.wait_ns);
             }
         }
     } else {
-        const int q = warp & 3, half = (warp - 2) >> 2;
-        uint32_t it = 0;
+        const int q = warp & 3, half = (warp - 2) >> 2, strips_here = (cols / 32 - half + 1) >> 1;
+        DT* const buf = reinterpret_cast<DT*>(strips + (warp - 2) * 2 * kStripBytes<DT>);
+        uint64_t* const old = tl.old[warp - 2];
+        float* const a_scale = tl.scales[warp - 2];
+        const bool add = g.accumulate != 0;
+        uint32_t it = 0, b = 0, arrivals = 0;                           // b: the buffer of the next strip; arrivals: parity of either buffer's old values
+        int waited = 0;                                                 // buffers with old values under way (bits)
+        // the old values of strip i of tile t into buffer `to`, which the strip before the last has left
+        auto request = [&](int t, int i, uint32_t to) {
+            if (t >= sh.tiles) return;
+            int m0, n0;
+            place(t, m0, n0);
+            const int m = m0 + (half + 2 * i) * 32, nw = n0 + rank * kWRows + q * 32;
+            if (m >= g.M || nw >= g.N) return;
+            waited |= 1 << to;
+            if (lane == 0) {
+                stores_read<0>();
+                mbar_expect_tx(&old[to], (uint32_t)kStripBytes<DT>);
+                tma_load_2d(buf + to * 1024, &map_d, &old[to], nw, m);
+            }
+        };
+        // scales and bias of a tile: this lane's row of W, and its rows of A in this warp's strips; asked for while the tile before is finished
+        float next_w = 0.f, next_b = 0.f, next_a[kMaxCols / 64];
+        auto ask = [&](int t) {
+            if (t >= sh.tiles) return;
+            int m0, n0;
+            place(t, m0, n0);
+            const int n = n0 + rank * kWRows + q * 32 + lane;
+            next_w = n < g.N ? g.w_scale[n] : 0.f;
+            next_b = n < g.N && g.bias != nullptr ? g.bias[n] : 0.f;
+#pragma unroll
+            for (int i = 0; i < kMaxCols / 64; ++i) {
+                const int m = m0 + (half + 2 * i) * 32 + lane;
+                next_a[i] = i < strips_here && m < g.M ? g.a_scale[m] : 0.f;
+            }
+        };
+        ask(first);
+        if (sh.staged && add) request(first, 0, 0);
         for (int t = first; t < sh.tiles; t += at_once, ++it) {
             const uint32_t as = it & 1u, aph = (it >> 1) & 1u;
             int m0, n0;
             place(t, m0, n0);
-            const int n = n0 + rank * kWRows + q * 32 + lane;
-            const float sw = n < g.N ? g.w_scale[n] : 0.f, bias = n < g.N && g.bias != nullptr ? g.bias[n] : 0.f;
+            const int nw = n0 + rank * kWRows + q * 32, n = nw + lane;
+            const float sw = next_w, bias = next_b;
+            float sa[kMaxCols / 64];
+#pragma unroll
+            for (int i = 0; i < kMaxCols / 64; ++i) sa[i] = next_a[i];
             // after a wait that ran out, this tile and all that follow are left as NaN
-            if (!timed_out && !mbar_wait(&tl.acc_full[as], aph, g.wait_ns)) timed_out = true;
+            if (!timed_out && !wait_for(&tl.acc_full[as], aph, g.wait_ns)) timed_out = true;
             timed_out = __any_sync(0xffffffffu, timed_out);             // tcgen05.ld is warp-collective
             tc_fence_after();
             const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + as * kMaxCols;
+            ask(t + at_once);
+            auto column = [&](int i) { return (uint32_t)(half + 2 * i) * 32u; };
+            auto release = [&]() {                                      // this warp has read its share of the accumulator
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_relaxed(map_to_rank(smem_u32(&tl.acc_empty[as]), 0));
+            };
+            auto set_scales = [&](int i) {
+                __syncwarp();                                           // the last strip's have been read
+                a_scale[lane] = i == 0 ? sa[0] : (i == 1 ? sa[1] : (i == 2 ? sa[2] : sa[3]));
+                __syncwarp();
+            };
+            auto finish = [&](const uint32_t (&sum)[32], int i) {
+                const int m = m0 + (int)column(i);
+                const bool some = m < g.M && nw < g.N;
+                set_scales(i);
+                if (!timed_out && add) request(i + 1 < strips_here ? t : t + at_once, i + 1 < strips_here ? i + 1 : 0, b ^ 1u);
+                else if (lane == 0) stores_read<1>();
+                if (some) {
+                    const uint32_t at = smem_u32(buf + b * 1024 + lane);
+                    if (add) {
+                        if (!timed_out && !wait_for(&old[b], (arrivals >> b) & 1u, g.wait_ns)) timed_out = true;
+                        timed_out = __any_sync(0xffffffffu, timed_out);
+                        if (timed_out) {                                // results of which the old value is missing
+                            finish_strip<DT>(g, 0, a_scale, m, n, sw, bias, true);
+                            return;
+                        }
+                        arrivals ^= 1u << b;
+                        waited &= ~(1 << b);
+                    } else {
+                        __syncwarp();                                   // the buffer's last store has been read
+                    }
+                    float v[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) shared_load4(smem_u32(a_scale), v, j);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = scaled((int)sum[j], v[j], sw, bias);
+                    if (add) {
+                        float o[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = shared_value(at + j * 32 * (uint32_t)sizeof(DT), (const DT*)nullptr);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = __fadd_rn(v[j], o[j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) shared_put(at + j * 32 * (uint32_t)sizeof(DT), v[j], (const DT*)nullptr);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) tma_store_2d(&map_d, buf + b * 1024, nw, m);
+                    b ^= 1u;
+                } else if (add) {
+                    b ^= 1u;                                            // its neighbour's old values are on their way into the other buffer
+                }
+            };
+            if (!sh.staged || timed_out) {
+                for (int i = 0; i < strips_here; ++i) {
+                    const int m = m0 + (int)column(i);
+                    set_scales(i);
+                    if (m < g.M && nw < g.N) finish_strip<DT>(g, lanes + column(i), a_scale, m, n, sw, bias, timed_out);
+                }
+                release();
+            } else {
 #pragma unroll 1
-            for (int cb = half; cb < cols / 32; cb += 2) {
-                if (m0 + cb * 32 >= g.M) break;
-                finish_strip<DT>(g, lanes + (uint32_t)(cb * 32), tl.scales[warp - 2], m0 + cb * 32, n, sw, bias, timed_out);
+                for (int i = 0; i < strips_here; ++i) {
+                    uint32_t sum[32];
+                    tmem_ld32(lanes + column(i), sum);
+                    if (i + 1 == strips_here) release();
+                    finish(sum, i);
+                }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_at(map_to_rank(smem_u32(&tl.acc_empty[as]), 0));
         }
+        if (lane == 0) {
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+            for (int i = 0; i < 2; ++i) if (waited >> i & 1) wait_for(&old[i], (arrivals >> i) & 1u, g.wait_ns);      // (after a lost wait) copies under way
+        }
+        __syncwarp();
     }
     if (timed_out && g.status != nullptr) atomicOr(g.status, STATUS_TIMEOUT);
     tc_fence_before();
@@ -483,7 +728,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
                 if (i0 > i1) mbar_complete_tx(&tl.full[k % S], (uint32_t)stage);
                 else mbar_expect_tx(&tl.full[k % S], (uint32_t)stage);
             }
-            for (uint32_t k = hi > (uint32_t)S ? hi - S : 0; k < hi; ++k) mbar_wait(&tl.full[k % S], (k / S) & 1u, g.wait_ns);
+            for (uint32_t k = hi > (uint32_t)S ? hi - S : 0; k < hi; ++k) wait_for(&tl.full[k % S], (k / S) & 1u, g.wait_ns);
         }
         __syncwarp();
         cluster_arrive();
@@ -499,8 +744,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                   CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// [rows][K] bytes in rows of ld, box of 128 bytes by box_rows, 128-byte swizzle, zeros behind K and behind the last row
-int32_t make_i8_map(CUtensorMap* map, const void* ptr, long ld, int rows, int K, int box_rows) {
+int32_t make_map(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, long row_bytes, int rows, int cols, int box_rows, int box_cols, CUtensorMapSwizzle swizzle) {
     static std::atomic<EncodeTiledFn> encode{nullptr};
     EncodeTiledFn fn = encode.load(std::memory_order_acquire);
     if (fn == nullptr) {
@@ -511,12 +755,22 @@ int32_t make_i8_map(CUtensorMap* map, const void* ptr, long ld, int rows, int K,
         fn = reinterpret_cast<EncodeTiledFn>(p);
         encode.store(fn, std::memory_order_release);
     }
-    cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
-    cuuint32_t box[2] = {(cuuint32_t)kBlockK, (cuuint32_t)box_rows}, estr[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(LUMI_E_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (%d rows of %d bytes)", (int)r, rows, K);
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)row_bytes};
+    cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    const CUresult r = fn(map, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(LUMI_E_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (%d rows of %d)", (int)r, rows, cols);
     return LUMI_OK;
+}
+// [rows][K] bytes in rows of ld, box of 128 bytes by box_rows, 128-byte swizzle, zeros behind K and behind the last row
+int32_t make_i8_map(CUtensorMap* map, const void* ptr, long ld, int rows, int K, int box_rows) {
+    return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, ptr, ld, rows, K, box_rows, kBlockK, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// D by strips of 32 x 32
+template <typename DT>
+int32_t make_result_map(CUtensorMap* map, const I8Args& g) {
+    return make_map(map, sizeof(DT) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g.d, g.ldd * (long)sizeof(DT), g.M, g.N, 32, 32,
+                    CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 // Lets a kernel have as much shared memory as there is, once per device.
@@ -547,33 +801,62 @@ struct Launch {
     }
 };
 
-template <int MB, typename DT>
-int32_t launch_vector(const I8Args& g, cudaStream_t st) {
-    int shares = 1;                          // warps that share K: until the GPU has about 16 warps per SM, as long as each has 512 bytes of a row
-    while (shares < 8 && (long)g.N / kVecRows * shares < 16l * sm_count() && g.K > 512 * shares) shares *= 2;
-    const int rows = 8 / shares * kVecRows;
-    Launch l(dim3((g.N + rows - 1) / rows), 256, 0, 1, st);
-    LUMI_CUDA(cudaLaunchKernelEx(&l.cfg, vector_kernel<MB, DT>, g, shares));
+// Warps that share K: until the GPU has about 16 warps per SM, as long as each has a piece of a row.
+int shares_of_k(long groups, int K, int piece) {
+    int shares = 1;
+    while (shares < 8 && groups * shares < 16l * sm_count() && K > piece * shares) shares *= 2;
+    return shares;
+}
+template <typename DT>
+int32_t launch_few(const I8Args& g, cudaStream_t st) {
+    const bool one_or_two = g.M <= 2;
+    const int per_warp = one_or_two ? kVecRows : kFewW, shares = shares_of_k(((long)g.N + per_warp - 1) / per_warp, g.K, one_or_two ? 512 : 64);
+    const long rows = 8 / shares * per_warp;
+    Launch l(dim3((unsigned)((g.N + rows - 1) / rows)), 256, 0, 1, st);
+    if (g.M == 1) LUMI_CUDA(cudaLaunchKernelEx(&l.cfg, vector_kernel<1, DT>, g, shares));
+    else if (one_or_two) LUMI_CUDA(cudaLaunchKernelEx(&l.cfg, vector_kernel<2, DT>, g, shares));
+    else LUMI_CUDA(cudaLaunchKernelEx(&l.cfg, few_kernel<DT>, g, shares));
     return LUMI_OK;
 }
 
-template <typename DT>
-int32_t launch_tile(const I8Args& g, cudaStream_t st) {
-    static std::atomic<uint64_t> ready{0};
+// Tile and shares of K for a product whose tiles fit on the GPU at once (cols 0: they do not).  The estimate, in microseconds behind what every launch
+// takes: 0.25 per k-block (one thread issues its four MMAs, whatever their width), and for the results, or for sums that cross the cluster's
+// shared memory, by the tile's width and the number of CTAs.  Measured, columns / shares (CTAs): 16 x 7360 x 1024 32/1 (58) 5.1, 32/2 (116) 6.0; 64 x 1024 x 2816 32/1 (16) 8.6,
+// 32/4 (64) 4.8, 64/4 (32) 6.0; 256 x 1024 x 2816 32/1 (64) 9.3, 64/4 (128) 7.0, 128/4 (64) 8.7; 512 x 259 x 8192 32/2 (96) 12.4, 64/4 (96) 9.5; a second round of CTAs costs
+// as much as the first: 256 x 7360 x 1024 128/1 (116) 6.5, 32/1 (464) 11.1, 128/2 (232) 20.5.
+TileShape tile_shape(const I8Args& g) {
     const int num_kb = (g.K + kBlockK - 1) / kBlockK;
-    TileShape sh;
-    sh.cols = g.M <= 32 ? 32 : (g.M <= 64 ? 64 : 128);
-    const long tiles = (long)((g.N + kWRows - 1) / kWRows), whole = tiles * ((g.M + sh.cols - 1) / sh.cols);
-    sh.splits = 1;
-    while (sh.splits < 8 && num_kb >= 4 * sh.splits && whole * 2 * sh.splits <= sm_count()) sh.splits *= 2;
-    const int stage = kWBytes + sh.cols * kBlockK, part = sh.splits > 1 ? sh.cols * kWRows * 4 : 0;
-    const int budget = (whole * sh.splits > sm_count() ? 112 : 220) * 1024 - part - kTailBytes - 1024;
-    sh.stages = std::max(2, std::min({kMaxStages, budget / stage, (num_kb + sh.splits - 1) / sh.splits}));
+    const long tiles = ((long)g.N + kWRows - 1) / kWRows;
+    TileShape best{0, 0, 1};
+    double least = 0;
+    for (int cols = 32; cols <= kMaxCols; cols *= 2) {
+        const long whole = tiles * ((g.M + cols - 1) / cols);
+        if (whole > sm_count()) continue;
+        for (int splits = 1; splits <= 8; splits *= 2) {
+            if (splits > 1 && (cols > 128 || splits > num_kb || whole * splits > kClusterCtas)) break;
+            const double cost = 0.25 * ((num_kb + splits - 1) / splits) + (splits > 1 ? 0.3 + 0.028 * cols + 0.006 * (double)(whole * splits) : 0.008 * cols);
+            if (best.cols == 0 || cost < least) { best.cols = cols; best.splits = splits; least = cost; }
+        }
+    }
+    if (best.cols == 0) return best;
+    const long ctas = tiles * ((g.M + best.cols - 1) / best.cols) * best.splits;
+    // clusters find room beside one another where a CTA leaves half an SM
+    const int stage = kWBytes + best.cols * kBlockK, part = best.splits > 1 ? best.cols * kWRows * 4 : 0;
+    const int budget = (best.splits > 1 && ctas > 64 ? 112 : 220) * 1024 - part - kTailBytes - 1024;
+    best.stages = std::max(2, std::min({kMaxStages, budget / stage, (num_kb + best.splits - 1) / best.splits}));
+    return best;
+}
+
+template <typename DT>
+int32_t launch_tile(const I8Args& g, const TileShape& sh, cudaStream_t st) {
+    static std::atomic<uint64_t> ready{0};
     CUtensorMap ma, mw;
     LUMI_TRY(make_i8_map(&ma, g.a, g.lda, g.M, g.K, sh.cols));
     LUMI_TRY(make_i8_map(&mw, g.w, g.ldw, g.N, g.K, kWRows));
     LUMI_TRY(allow_smem((const void*)tile_kernel<DT>, ready));
-    Launch l(dim3((unsigned)(tiles * sh.splits), (g.M + sh.cols - 1) / sh.cols), 256, sh.stages * stage + part + kTailBytes + 1024, sh.splits, st);
+    const int part = sh.splits > 1 ? sh.cols * kWRows * 4 : 0;
+    Launch l(dim3((unsigned)((g.N + kWRows - 1) / kWRows * sh.splits), (unsigned)((g.M + sh.cols - 1) / sh.cols)), 256,
+             sh.stages * (kWBytes + sh.cols * kBlockK) + part + kTailBytes + 1024, sh.splits, st);
     LUMI_CUDA(cudaLaunchKernelEx(&l.cfg, tile_kernel<DT>, ma, mw, g, sh));
     return LUMI_OK;
 }
@@ -586,21 +869,24 @@ int32_t launch_pair(const I8Args& g, int cols, cudaStream_t st) {
     sh.tiles_a = (g.M + cols - 1) / cols;
     sh.tiles = sh.tiles_a * ((g.N + 2 * kWRows - 1) / (2 * kWRows));
     const int stage = kWBytes + cols / 2 * kBlockK;
-    sh.stages = std::min(kMaxStages, (220 * 1024 - kTailBytes) / stage);
-    CUtensorMap ma, mw;
+    sh.stages = std::min(kMaxStages, (227 * 1024 - 1024 - kTailBytes - 16 * kStripBytes<DT>) / stage);
+    // (a store is cut at the end of a row by whole 16 bytes)
+    sh.staged = ((uintptr_t)g.d & 15) == 0 && g.ldd * sizeof(DT) % 16 == 0 && g.N * sizeof(DT) % 16 == 0;
+    CUtensorMap ma, mw, md{};
+    if (sh.staged) LUMI_TRY(make_result_map<DT>(&md, g));
     LUMI_TRY(make_i8_map(&ma, g.a, g.lda, g.M, g.K, cols / 2));
     LUMI_TRY(make_i8_map(&mw, g.w, g.ldw, g.N, g.K, kWRows));
     LUMI_TRY(allow_smem((const void*)pair_kernel<DT>, ready));
-    Launch l(dim3(2 * std::min(sh.tiles, sm_count() / 2)), kPairThreads, sh.stages * stage + kTailBytes + 1024, 2, st);
-    LUMI_CUDA(cudaLaunchKernelEx(&l.cfg, pair_kernel<DT>, ma, mw, g, sh));
+    Launch l(dim3(2 * std::min(sh.tiles, sm_count() / 2)), kPairThreads, sh.stages * stage + 16 * kStripBytes<DT> + kTailBytes + 1024, 2, st);
+    LUMI_CUDA(cudaLaunchKernelEx(&l.cfg, pair_kernel<DT>, ma, mw, md, g, sh));
     return LUMI_OK;
 }
 
 // Columns of the pairs' tiles: the GPU works in rounds of a tile per pair, a round costs about its tile's columns.
-int pair_cols(const I8Args& g, long& cost) {
+int pair_cols(const I8Args& g) {
     const long pairs = sm_count() / 2, tiles_w = (g.N + 2 * kWRows - 1) / (2 * kWRows);
     int best = 0;
-    cost = 0;
+    long cost = 0;
     for (int c = kMaxCols; c >= 64; c -= 32) {
         const long k = (tiles_w * ((g.M + c - 1) / c) + pairs - 1) / pairs * (c + 32);
         if (best == 0 || k < cost) { best = c; cost = k; }
@@ -610,13 +896,9 @@ int pair_cols(const I8Args& g, long& cost) {
 
 template <typename DT>
 int32_t launch_product(const I8Args& g, cudaStream_t st) {
-    if (g.M <= 1) return launch_vector<1, DT>(g, st);
-    if (g.M <= 2) return launch_vector<2, DT>(g, st);
-    if (g.M <= 4) return launch_vector<4, DT>(g, st);
-    if (g.M <= 8) return launch_vector<8, DT>(g, st);
-    long cost;
-    if (g.M > 1024) return launch_pair<DT>(g, pair_cols(g, cost), st);
-    return launch_tile<DT>(g, st);
+    if (g.M <= 2 || (g.M <= kFewRows && g.K <= kFewK && (long)g.N * g.K <= kFewBytes)) return launch_few<DT>(g, st);
+    const TileShape sh = tile_shape(g);
+    return sh.cols != 0 ? launch_tile<DT>(g, sh, st) : launch_pair<DT>(g, pair_cols(g), st);
 }
 
 }  // namespace
@@ -624,18 +906,36 @@ int32_t launch_product(const I8Args& g, cudaStream_t st) {
 
 using namespace lumi;
 
-extern "C" int32_t lumi_k_gemm_i8(uint64_t a, int32_t lda, uint64_t a_scale, uint64_t w, int32_t ldw, uint64_t w_scale, uint64_t bias, uint64_t d,
-                                  int32_t d_dtype, int32_t ldd, int32_t M, int32_t N, int32_t K, int32_t accumulate, uint64_t status, uint64_t stream) {
+static int32_t check_and_run(const char* name, uint64_t a, int32_t lda, uint64_t a_scale, uint64_t w, int32_t ldw, uint64_t w_scale, uint64_t bias, uint64_t d,
+                             int32_t d_dtype, int32_t ldd, int32_t M, int32_t N, int32_t K, int32_t accumulate, uint64_t status, uint64_t wait_ns, int skip_unit,
+                             cudaStream_t st) {
     if (!a || !a_scale || !w || !w_scale || !d || M < 0 || N < 0 || K <= 0 || lda < K || ldw < K || ldd < N ||
         (d_dtype != LUMI_DTYPE_F32 && d_dtype != LUMI_DTYPE_BF16))
-        return fail(LUMI_E_INVALID, "bad argument to lumi_k_gemm_i8");
+        return fail(LUMI_E_INVALID, "bad argument to %s", name);
     if ((a & 15) || (w & 15) || lda % 16 || ldw % 16 || ((a_scale | w_scale | bias | status) & 3) || (d & (d_dtype == LUMI_DTYPE_F32 ? 3 : 1)))
-        return fail(LUMI_E_INVALID, "lumi_k_gemm_i8: rows of A and W have to begin on 16-byte boundaries, numbers on their own");
+        return fail(LUMI_E_INVALID, "%s: rows of A and W have to begin on 16-byte boundaries, numbers on their own", name);
     // 131071 products of -128 and -128 are the most that a 32-bit sum holds
-    if (K > 131071) return fail(LUMI_E_UNSUPPORTED, "lumi_k_gemm_i8: K %d (at most 131071)", K);
+    if (K > 131071 || M > kMaxRows || N > kMaxRows) return fail(LUMI_E_UNSUPPORTED, "%s: M %d, N %d (at most %d), K %d (at most 131071)", name, M, N, kMaxRows, K);
     if (M == 0 || N == 0) return LUMI_OK;
-    LUMI_TRY(check_device_memory("lumi_k_gemm_i8", {a, a_scale, w, w_scale, bias, d, status}));
+    LUMI_TRY(check_device_memory(name, {a, a_scale, w, w_scale, bias, d, status}));
     const I8Args g{(const int8_t*)a, (const int8_t*)w, (const float*)a_scale, (const float*)w_scale, (const float*)bias, (void*)d, lda, ldw, ldd, M, N, K, accumulate,
-                   (int32_t*)status, kWaitLimitNs, -1};
-    return d_dtype == LUMI_DTYPE_F32 ? launch_product<float>(g, (cudaStream_t)stream) : launch_product<__nv_bfloat16>(g, (cudaStream_t)stream);
+                   (int32_t*)status, wait_ns, skip_unit};
+    return d_dtype == LUMI_DTYPE_F32 ? launch_product<float>(g, st) : launch_product<__nv_bfloat16>(g, st);
+}
+
+extern "C" int32_t lumi_k_gemm_i8(uint64_t a, int32_t lda, uint64_t a_scale, uint64_t w, int32_t ldw, uint64_t w_scale, uint64_t bias, uint64_t d,
+                                  int32_t d_dtype, int32_t ldd, int32_t M, int32_t N, int32_t K, int32_t accumulate, uint64_t status, uint64_t stream) {
+    return check_and_run("lumi_k_gemm_i8", a, lda, a_scale, w, ldw, w_scale, bias, d, d_dtype, ldd, M, N, K, accumulate, status, kWaitLimitNs, -1, (cudaStream_t)stream);
+}
+
+// Failure-path test hook: waits limited by the caller and a tile whose operands (a pair: the second CTA's) never arrive.
+extern "C" int32_t lumi_debug_gemm_i8_wait_timeout(uint64_t a, int32_t lda, uint64_t a_scale, uint64_t w, int32_t ldw, uint64_t w_scale, uint64_t d, int32_t d_dtype,
+                                                   int32_t ldd, int32_t M, int32_t N, int32_t K, int32_t accumulate, uint64_t wait_limit_ns, int32_t skip_unit,
+                                                   uint64_t status) {
+    if (!status || !wait_limit_ns) return fail(LUMI_E_INVALID, "bad argument to lumi_debug_gemm_i8_wait_timeout");
+    LUMI_TRY(check_and_run("lumi_debug_gemm_i8_wait_timeout", a, lda, a_scale, w, ldw, w_scale, 0, d, d_dtype, ldd, M, N, K, accumulate, status, wait_limit_ns,
+                           skip_unit, nullptr));
+    int32_t word = 0;
+    LUMI_CUDA(cudaMemcpy(&word, (const void*)status, sizeof(word), cudaMemcpyDeviceToHost));
+    return (word & STATUS_TIMEOUT) ? fail(LUMI_E_TIMEOUT, "a bounded wait of the 8-bit product ran out") : LUMI_OK;
 }

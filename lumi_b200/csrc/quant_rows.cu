@@ -14,6 +14,7 @@ namespace lumi {
 namespace {
 
 constexpr float kLeast = 7.888609052210118e-31f;           // 2^-100: keeps 127 / m finite
+constexpr int kMaxWidth = 1 << 30;                         // places within a row are 32-bit numbers
 constexpr uint32_t kInfBits = 0x7f800000u;
 
 struct QuantOut {
@@ -427,6 +428,7 @@ extern "C" int32_t lumi_k_norm_quant(uint64_t x, int32_t x_dtype, int32_t ldx, u
         return fail(LUMI_E_INVALID, "bad argument to lumi_k_norm_quant");
     if (!aligned_rows(x, x_dtype, ldx) || (o && !aligned_rows(o, o_dtype, ldo)) || (w & 15) || (q & 15) || ldq % 16 || (scale & 3))
         return fail(LUMI_E_INVALID, "lumi_k_norm_quant: rows have to begin on 16-byte boundaries");
+    if (width > kMaxWidth) return fail(LUMI_E_UNSUPPORTED, "lumi_k_norm_quant: width %d (at most %d)", width, kMaxWidth);
     if (rows == 0) return LUMI_OK;
     LUMI_TRY(check_device_memory("lumi_k_norm_quant", {x, o, w, q, scale}));
     const QuantOut out{(int8_t*)q, (float*)scale, ldq};

@@ -59,9 +59,15 @@ def test_dequant_refuses(k):
     (dict(M=-1), INVALID), (dict(N=-1), INVALID), (dict(K=0), INVALID), (dict(lda=48), INVALID), (dict(lda=72), INVALID), (dict(ldw=48), INVALID),
     (dict(ldw=72), INVALID), (dict(ldd=63), INVALID), (dict(a=P + 8), INVALID), (dict(w=P + 8), INVALID), (dict(a_scale=P + 2), INVALID),
     (dict(w_scale=P + 2), INVALID), (dict(bias=P + 2), INVALID), (dict(status=P + 2), INVALID), (dict(d=P + 2), INVALID), (dict(d=P + 1, d_dtype=1), INVALID),
-    (dict(K=131072, lda=131072, ldw=131072), UNSUPPORTED)])
+    (dict(K=131072, lda=131072, ldw=131072), UNSUPPORTED), (dict(M=2 ** 30 + 1), UNSUPPORTED), (dict(N=2 ** 30 + 1, ldd=2 ** 30 + 1), UNSUPPORTED)])
 def test_gemm_refuses(k, want):
     assert gemm(**k) == want
+
+
+def test_rows_that_are_too_long():
+    n = 2 ** 30 + 16
+    assert norm(width=n, ldx=n, ldo=n, ldq=n) == UNSUPPORTED
+    assert gate(width=n, up=n, ld=2 ** 31 - 64, ldq=n) == INVALID                  # two of them do not fit in a row
 
 
 def test_nothing_to_do():
