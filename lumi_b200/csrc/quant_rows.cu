@@ -8,6 +8,7 @@
 #include "rows.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace lumi {
@@ -23,32 +24,29 @@ struct QuantOut {
     int ldq;
 };
 
-// ---- loads of four or eight numbers, as fp32
-// fast forms of the gate: relative error 2^-21 times the size of a negative gate
-__device__ __forceinline__ float fast_sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+// e^-v and the quotient by the hardware's approximations: a relative error of 2^-21 and, where v is far below zero, of |v| 2^-23.  With the accurate forms
+// the arithmetic of a bf16 gate takes longer than its bytes.
+__device__ __forceinline__ float fast_sigmoid(float v) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return r;
+}
 
+// ---- E numbers of a row as memory holds them, four or eight
+template <typename T, int E>
+struct Words { uint32_t u[E * sizeof(T) / 4]; };
 template <int E>
-__device__ __forceinline__ void load_whole(const float* p, float (&v)[E]) {
+__device__ __forceinline__ void unpack(const Words<float, E>& w, float (&v)[E]) {
 #pragma unroll
-    for (int i = 0; i < E / 4; ++i) {
-        const float4 f = *reinterpret_cast<const float4*>(p + 4 * i);
-        v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
-    }
+    for (int i = 0; i < E; ++i) v[i] = __uint_as_float(w.u[i]);
 }
 template <int E>
-__device__ __forceinline__ void load_whole(const __nv_bfloat16* p, float (&v)[E]) {
-    uint32_t u[E / 2];
-    if constexpr (E == 8) {
-        const uint4 t = *reinterpret_cast<const uint4*>(p);
-        u[0] = t.x; u[1] = t.y; u[2] = t.z; u[3] = t.w;
-    } else {
-        const uint2 t = *reinterpret_cast<const uint2*>(p);
-        u[0] = t.x; u[1] = t.y;
-    }
+__device__ __forceinline__ void unpack(const Words<__nv_bfloat16, E>& w, float (&v)[E]) {
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) {
-        v[2 * i] = __uint_as_float(u[i] << 16);
-        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        v[2 * i] = __uint_as_float(w.u[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w.u[i] & 0xffff0000u);
     }
 }
 // Of the norm's weights, which no store of the kernel changes: loads that may pass the stores of x, but not the dependency wait.
@@ -63,18 +61,31 @@ __device__ __forceinline__ void load_weights(const float* p, int n, float& a, fl
         if (n > 2) c = p[2];
     }
 }
-__device__ __forceinline__ float one(const float* p) { return *p; }
-__device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 // The row ends n numbers from here (n <= 0: before); what is behind it is neither read nor counted.  RAGGED: it may end within these E.
-template <bool RAGGED, int E, typename T>
-__device__ __forceinline__ void load_some(const T* p, int n, float (&v)[E]) {
+template <bool RAGGED, typename T, int E>
+__device__ __forceinline__ void load_some(const T* p, int n, Words<T, E>& w) {
+    constexpr int N = E * (int)sizeof(T) / 4;
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = 0.f;
+    for (int i = 0; i < N; ++i) w.u[i] = 0;
     if (RAGGED ? n >= E : n > 0) {
-        load_whole<E>(p, v);
-    } else if (RAGGED) {
+        if constexpr (N == 2) {
+            const uint2 t = *reinterpret_cast<const uint2*>(p);
+            w.u[0] = t.x; w.u[1] = t.y;
+        } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) if (i < n) v[i] = one(p + i);
+            for (int i = 0; i < N / 4; ++i) {
+                const uint4 t = reinterpret_cast<const uint4*>(p)[i];
+                w.u[4 * i] = t.x; w.u[4 * i + 1] = t.y; w.u[4 * i + 2] = t.z; w.u[4 * i + 3] = t.w;
+            }
+        }
+    } else if (RAGGED && n > 0) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) if (i < n) w.u[i] = reinterpret_cast<const uint32_t*>(p)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; ++i) if (i < n) w.u[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
+        }
     }
 }
 __device__ __forceinline__ void put_one(float* p, float v) { *p = v; }
@@ -110,44 +121,57 @@ __device__ __forceinline__ void store_some(__nv_bfloat16* p, int n, const float 
         for (int i = 0; i < E; ++i) if (i < n) p[i] = __float2bfloat16_rn(v[i]);
 }
 
+// kStay: blocks stay for row after row.  kNarrow: the fewest eights of numbers that a thread of a block holds.  Measured ...
 // ---- sources of rows: load(): what memory holds of E numbers; values(): the numbers to be held in 8 bits, with the sum of squares
 // Norm, or rows as they are.  ADD: x += o first, rounded to x's type, so that the norm sees what later readers of x see.
 template <typename XT, typename OT, bool ADD, bool NORM, bool RAGGED>
 struct NormSource {
     static constexpr bool kRagged = RAGGED;
     static constexpr int E = sizeof(XT) == 4 ? 4 : 8;
-    static constexpr bool kNorm = NORM;
+    static constexpr bool kNorm = NORM, kStay = E == 8;
+    static constexpr int kNarrow = E == 8 ? 2 : 1;
     XT* x; const OT* o; const float* w;
     long ldx, ldo;
     int width;
     float eps;
-    struct Raw { float x[E], o[ADD ? E : 1]; };
+    struct None {};
+    struct Raw { Words<XT, E> x; std::conditional_t<ADD, Words<OT, E>, None> o; };
     template <bool AGAIN>
     __device__ __forceinline__ void load(long row, int c, Raw& r) const {
-        load_some<RAGGED, E>(x + row * ldx + c, width - c, r.x);
-        if constexpr (ADD && !AGAIN) load_some<RAGGED, E>(o + row * ldo + c, width - c, r.o);
+        load_some<RAGGED>(x + row * ldx + c, width - c, r.x);
+        if constexpr (ADD && !AGAIN) load_some<RAGGED>(o + row * ldo + c, width - c, r.o);
     }
     // AGAIN: x has been added to already
     template <bool AGAIN>
-    __device__ __forceinline__ void values(long row, int c, Raw& r, float (&t)[E], float& sum) const {
+    __device__ __forceinline__ void values(long row, int c, const Raw& r, float (&t)[E], float& sum) const {
+        unpack(r.x, t);
         if constexpr (ADD && !AGAIN) {
+            float add[E];
+            unpack(r.o, add);
 #pragma unroll
-            for (int i = 0; i < E; ++i) r.x[i] = stored(r.x[i] + r.o[i], x);
-            store_some<RAGGED, E>(x + row * ldx + c, width - c, r.x);
+            for (int i = 0; i < E; ++i) t[i] = stored(t[i] + add[i], x);
+            store_some<RAGGED, E>(x + row * ldx + c, width - c, t);
         }
-        float f[E];
-        if constexpr (NORM)
+        if constexpr (NORM) {
+            float f[E];
 #pragma unroll
             for (int i = 0; i < E; i += 4) load_weights<RAGGED>(w + c + i, width - c - i, f[i], f[i + 1], f[i + 2], f[i + 3]);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            if constexpr (NORM) {
-                sum = fmaf(r.x[i], r.x[i], sum);
-                t[i] = r.x[i] * f[i];
-            } else {
-                t[i] = r.x[i];
+            for (int i = 0; i < E; ++i) {
+                sum = fmaf(t[i], t[i], sum);
+                t[i] *= f[i];
             }
         }
+    }
+    // sum of squares of E numbers times k, from memory
+    __device__ __forceinline__ float squares(long row, int c, float k) const {
+        Raw r;
+        float v[E], part = 0.f;
+        load<true>(row, c, r);
+        unpack(r.x, v);
+#pragma unroll
+        for (int i = 0; i < E; ++i) part = fmaf(v[i] * k, v[i] * k, part);
+        return part;
     }
 };
 
@@ -156,22 +180,26 @@ template <typename XT, bool SILU, bool RAGGED>
 struct GateSource {
     static constexpr bool kRagged = RAGGED;
     static constexpr int E = sizeof(XT) == 4 ? 4 : 8;
-    static constexpr bool kNorm = false;
+    static constexpr bool kNorm = false, kStay = false;
+    static constexpr int kNarrow = E == 8 ? 4 : 1;
     const XT* gu;
     long ld;
     int up, width;
-    struct Raw { float g[E], u[E]; };
+    struct Raw { Words<XT, E> g, u; };
     template <bool AGAIN>
     __device__ __forceinline__ void load(long row, int c, Raw& r) const {
-        load_some<RAGGED, E>(gu + row * ld + c, width - c, r.g);
-        load_some<RAGGED, E>(gu + row * ld + up + c, width - c, r.u);
+        load_some<RAGGED>(gu + row * ld + c, width - c, r.g);
+        load_some<RAGGED>(gu + row * ld + up + c, width - c, r.u);
     }
     template <bool AGAIN>
-    __device__ __forceinline__ void values(long, int, Raw& r, float (&t)[E], float&) const {
+    __device__ __forceinline__ void values(long, int, const Raw& r, float (&t)[E], float&) const {
+        float u[E];
+        unpack(r.g, t);
+        unpack(r.u, u);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            const float z = fast_sigmoid(r.g[i]);
-            t[i] = (SILU ? r.g[i] * z : z) * r.u[i];
+            const float z = fast_sigmoid(t[i]);
+            t[i] = (SILU ? t[i] * z : z) * u[i];
         }
     }
 };
@@ -202,32 +230,46 @@ __device__ __forceinline__ void put(int8_t* q, int n, const float (&t)[E], float
         for (int i = 0; i < E; ++i) if (i < n) q[i] = (int8_t)b[i];
 }
 
-// Sum and maximum over the NT threads of a row (a whole warp, or the block).
-template <int NT>
-__device__ __forceinline__ void reduce_row(float& sum, uint32_t& m) {
-    sum = warp_total(sum);
+// Sum (SUM) and maximum over the threads of a row: a warp's, or the block's.  turn counts a block's reductions.
+template <bool WARP, bool SUM>
+__device__ __forceinline__ void reduce_row(float& sum, uint32_t& m, uint32_t& turn) {
+    if constexpr (SUM) sum = warp_total(sum);
     m = __reduce_max_sync(0xffffffffu, m);
-    if constexpr (NT > 32) {
-        __shared__ float ss[NT / 32];
-        __shared__ uint32_t sm[NT / 32];
-        const int warp = threadIdx.x >> 5;
-        __syncthreads();                              // an earlier reduction's values have been read
-        if ((threadIdx.x & 31) == 0) { ss[warp] = sum; sm[warp] = m; }
+    if constexpr (!WARP) {
+        __shared__ float ss[2][32];                   // in turn: nobody is two reductions ahead of anybody
+        __shared__ uint32_t sm[2][32];
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, b = turn++ & 1;
+        if (lane == 0) {
+            if constexpr (SUM) ss[b][warp] = sum;
+            sm[b][warp] = m;
+        }
         __syncthreads();
-        sum = 0.f; m = 0;
-#pragma unroll
-        for (int i = 0; i < NT / 32; ++i) { sum += ss[i]; m = max(m, sm[i]); }
+        if constexpr (SUM) sum = warp_total(lane < warps ? ss[b][lane] : 0.f);
+        m = __reduce_max_sync(0xffffffffu, lane < warps ? sm[b][lane] : 0u);
     }
 }
 
-// 1 / sqrt(sum / width + eps).  A sum of squares that has overflowed or vanished beside a small eps is taken again of numbers times k; again(k) gives it.
+// The norm's factor k / sqrt(sum / width + eps k^2), sum: of the squares of numbers times k.  k is 1, but a sum that has overflowed, or vanished beside a small
+// eps, is taken again with another; again(k) gives it, to every thread alike.
+struct Factor { float sum, k; };
 template <typename AGAIN>
-__device__ __forceinline__ float norm_factor(float sum, int width, float eps, AGAIN again) {
-    float k = 1.f;
-    if (!(sum < __uint_as_float(kInfBits))) k = 8.271806125530277e-25f;                          // 2^-80
-    else if (sum < kLeast && eps < 8.470329472543003e-22f) k = 1.152921504606847e18f;            // 2^-70; 2^60
-    if (k != 1.f) sum = again(k);
-    return __fmul_rn(k, __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)width), __fmul_rn(__fmul_rn(eps, k), k)))));
+__device__ __forceinline__ Factor norm_sum(float sum, float eps, AGAIN again) {
+    Factor f{sum, 1.f};
+    if (!(sum < __uint_as_float(kInfBits))) f.k = 8.271806125530277e-25f;                        // 2^-80
+    else if (sum < kLeast && eps < 8.470329472543003e-22f) f.k = 1.152921504606847e18f;          // 2^-70; 2^60
+    if (f.k != 1.f) f.sum = again(f.k);
+    return f;
+}
+__device__ __forceinline__ float norm_factor(const Factor& f, int width, float eps) {
+    return __fmul_rn(f.k, __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(f.sum, (float)width), __fmul_rn(__fmul_rn(eps, f.k), f.k)))));
+}
+
+template <typename SRC>
+__device__ __forceinline__ float row_scale(const SRC& src, const Factor& f, bool numbers, float top) {
+    if (!numbers) return __uint_as_float(0x7fffffffu);
+    float s = __fdiv_rn(top, 127.f);
+    if constexpr (SRC::kNorm) s = __fmul_rn(s, norm_factor(f, src.width, src.eps));
+    return s;
 }
 
 // Row per block of NT threads, the numbers read twice (the second time from L2): any width.
@@ -238,7 +280,7 @@ __global__ void __launch_bounds__(NT) quant_wide_kernel(SRC src, QuantOut out) {
     pdl_release();
     pdl_sync();
     float sum = 0.f;
-    uint32_t m = 0;
+    uint32_t m = 0, turn = 0;
     for (int c = threadIdx.x * E; c < src.width; c += NT * E) {
         typename SRC::Raw r;
         float t[E];
@@ -246,24 +288,19 @@ __global__ void __launch_bounds__(NT) quant_wide_kernel(SRC src, QuantOut out) {
         src.template values<false>(row, c, r, t, sum);
         largest<E>(t, m);
     }
-    reduce_row<NT>(sum, m);
+    reduce_row<false, SRC::kNorm>(sum, m, turn);
     const bool numbers = m < kInfBits;
-    float factor = 1.f;
+    Factor f{0.f, 1.f};
     if constexpr (SRC::kNorm)
-        factor = norm_factor(sum, src.width, src.eps, [&](float k) {
+        f = norm_sum(sum, src.eps, [&](float k) {
             float part = 0.f;
             uint32_t unused = 0;
-            for (int c = threadIdx.x * E; c < src.width; c += NT * E) {
-                typename SRC::Raw r;
-                src.template load<true>(row, c, r);
-#pragma unroll
-                for (int i = 0; i < E; ++i) part = fmaf(r.x[i] * k, r.x[i] * k, part);
-            }
-            reduce_row<NT>(part, unused);
+            for (int c = threadIdx.x * E; c < src.width; c += NT * E) part += src.squares(row, c, k);
+            reduce_row<false, true>(part, unused, turn);
             return part;
         });
     const float top = fmaxf(__uint_as_float(m), kLeast), inv = numbers ? __fdiv_rn(127.f, top) : 0.f;
-    if (threadIdx.x == 0) out.scale[row] = numbers ? __fdiv_rn(top, 127.f) * factor : __uint_as_float(0x7fffffffu);
+    if (threadIdx.x == 0) out.scale[row] = row_scale(src, f, numbers, top);
     for (int c = threadIdx.x * E; c < src.width; c += NT * E) {
         typename SRC::Raw r;
         float t[E], unused = 0.f;
@@ -276,49 +313,54 @@ __global__ void __launch_bounds__(NT) quant_wide_kernel(SRC src, QuantOut out) {
     }
 }
 
-// The numbers of a row in the registers of NT threads (a warp, or the block), NC times E each: memory is read once, all of it asked for before the
-// first is used.
-template <typename SRC, int NT, int NC>
-__global__ void __launch_bounds__(NT == 32 ? 128 : NT) quant_rows_kernel(SRC src, QuantOut out, int rows) {
+// The numbers of a row in the registers of a warp (WARP) or a block, NC times E for each thread: memory is read once, all of it asked for before the first is
+// used, and the next row's while this one is reduced and written.
+template <typename SRC, bool WARP, int NC>
+__global__ void __launch_bounds__(WARP ? 128 : 512, SRC::E == 8 && !WARP ? 2 : 1) quant_rows_kernel(SRC src, QuantOut out, int rows) {
     constexpr int E = SRC::E;
-    const long row = NT == 32 ? (long)blockIdx.x * 4 + (threadIdx.x >> 5) : (long)blockIdx.x;
-    const int tid = NT == 32 ? threadIdx.x & 31 : threadIdx.x;
+    const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, NT = WARP ? 32 : blockDim.x;
+    const long step = WARP ? 4l * gridDim.x : (long)gridDim.x;
+    long row = WARP ? (long)blockIdx.x * 4 + (threadIdx.x >> 5) : (long)blockIdx.x;
+    uint32_t turn = 0;
     pdl_release();
     pdl_sync();
     if (row >= rows) return;                              // whole warps, and only where a row is a warp's
     typename SRC::Raw r[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) src.template load<false>(row, (i * NT + tid) * E, r[i]);
-    float sum = 0.f, t[NC][E];
-    uint32_t m = 0;
+    for (; row < rows; row += step) {
+        float sum = 0.f, t[NC][E];
+        uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        src.template values<false>(row, (i * NT + tid) * E, r[i], t[i], sum);
-        largest<E>(t[i], m);
-    }
-    reduce_row<NT>(sum, m);
-    const bool numbers = m < kInfBits;
-    float factor = 1.f;
-    if constexpr (SRC::kNorm)
-        factor = norm_factor(sum, src.width, src.eps, [&](float k) {
-            float part = 0.f;
-            uint32_t unused = 0;
+        for (int i = 0; i < NC; ++i) {
+            src.template values<false>(row, (i * NT + tid) * E, r[i], t[i], sum);
+            largest<E>(t[i], m);
+        }
+        if (SRC::kStay && row + step < rows)
 #pragma unroll
-            for (int i = 0; i < NC; ++i)
+            for (int i = 0; i < NC; ++i) src.template load<false>(row + step, (i * NT + tid) * E, r[i]);
+        reduce_row<WARP, SRC::kNorm>(sum, m, turn);
+        const bool numbers = m < kInfBits;
+        Factor f{0.f, 1.f};
+        if constexpr (SRC::kNorm)
+            f = norm_sum(sum, src.eps, [&](float k) {
+                float part = 0.f;
+                uint32_t unused = 0;
+                for (int i = 0; i < NC; ++i) part += src.squares(row, (i * NT + tid) * E, k);
+                reduce_row<WARP, true>(part, unused, turn);
+                return part;
+            });
+        const float top = fmaxf(__uint_as_float(m), kLeast), inv = numbers ? __fdiv_rn(127.f, top) : 0.f;
 #pragma unroll
-                for (int e = 0; e < E; ++e) part = fmaf(r[i].x[e] * k, r[i].x[e] * k, part);
-            reduce_row<NT>(part, unused);
-            return part;
-        });
-    const float top = fmaxf(__uint_as_float(m), kLeast), inv = numbers ? __fdiv_rn(127.f, top) : 0.f;
-    if (tid == 0) out.scale[row] = numbers ? __fdiv_rn(top, 127.f) * factor : __uint_as_float(0x7fffffffu);
+        for (int i = 0; i < NC; ++i) {
+            const int c = (i * NT + tid) * E;
+            if (!numbers)
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        const int c = (i * NT + tid) * E;
-        if (!numbers)
-#pragma unroll
-            for (int e = 0; e < E; ++e) t[i][e] = 0.f;
-        put<SRC::kRagged, E>(out.q + row * out.ldq + c, src.width - c, t[i], inv);
+                for (int e = 0; e < E; ++e) t[i][e] = 0.f;
+            put<SRC::kRagged, E>(out.q + row * out.ldq + c, src.width - c, t[i], inv);
+        }
+        if (tid == 0) out.scale[row] = row_scale(src, f, numbers, top);      // by one thread: its divisions and root take longer than a row's numbers
+        if constexpr (!SRC::kStay) break;
     }
 }
 
@@ -335,26 +377,48 @@ cudaLaunchConfig_t dependent_launch(dim3 grid, int threads, cudaLaunchAttribute*
     return cfg;
 }
 
-template <typename SRC, int NT, int NC>
+template <typename SRC, bool WARP, int NC>
 int32_t launch_rows_of(const SRC& src, const QuantOut& out, int rows, cudaStream_t st) {
+    static std::atomic<int> registers{0};
+    int regs = registers.load(std::memory_order_relaxed);
+    if (regs == 0) {
+        cudaFuncAttributes at;
+        LUMI_CUDA(cudaFuncGetAttributes(&at, quant_rows_kernel<SRC, WARP, NC>));
+        regs = at.numRegs;
+        registers.store(regs, std::memory_order_relaxed);
+    }
+    const int chunks = (src.width + SRC::E - 1) / SRC::E, threads = WARP ? 128 : ((chunks + NC - 1) / NC + 31) / 32 * 32;
+    // as many blocks as run at once; registers are given out by eights per thread
+    const int per_sm = std::max(1, std::min({32, 2048 / threads, 65536 / ((regs + 7) / 8 * 8 * threads)}));
+    const long blocks = WARP ? ((long)rows + 3) / 4 : rows;
     cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = dependent_launch(dim3(NT == 32 ? (unsigned)(((long)rows + 3) / 4) : (unsigned)rows), NT == 32 ? 128 : NT, attr, st);
-    if constexpr (NC > 0) LUMI_CUDA(cudaLaunchKernelEx(&cfg, quant_rows_kernel<SRC, NT, NC>, src, out, rows));
-    else LUMI_CUDA(cudaLaunchKernelEx(&cfg, quant_wide_kernel<SRC, NT>, src, out));
+    const cudaLaunchConfig_t cfg = dependent_launch(dim3((unsigned)(SRC::kStay ? std::min(blocks, (long)per_sm * sm_count()) : blocks)), threads, attr, st);
+    LUMI_CUDA(cudaLaunchKernelEx(&cfg, quant_rows_kernel<SRC, WARP, NC>, src, out, rows));
     return LUMI_OK;
 }
 
 // The shape goes by the width alone, so that a row has the same bits alone and among others.
 template <typename SRC>
 int32_t launch(const SRC& src, const QuantOut& out, int rows, cudaStream_t st) {
-    constexpr int E = SRC::E, L = 8 / E;                  // L: a row's numbers are 2 L (4 L, 8 L) loads of a thread
-    if (src.width <= 32 * 8) return launch_rows_of<SRC, 32, L>(src, out, rows, st);
-    if (src.width <= 32 * 32) return launch_rows_of<SRC, 32, 4 * L>(src, out, rows, st);
-    if (src.width <= 256 * 8) return launch_rows_of<SRC, 256, L>(src, out, rows, st);
-    if (src.width <= 256 * 16) return launch_rows_of<SRC, 256, 2 * L>(src, out, rows, st);
-    if (src.width <= 256 * 32) return launch_rows_of<SRC, 256, 4 * L>(src, out, rows, st);
-    if (src.width <= 512 * 32) return launch_rows_of<SRC, 512, 4 * L>(src, out, rows, st);
-    return launch_rows_of<SRC, 1024, 0>(src, out, rows, st);
+    constexpr int L = 8 / SRC::E;                         // loads for eight numbers
+    const int width = src.width;
+    if (width <= 32 * 8) return launch_rows_of<SRC, true, L>(src, out, rows, st);
+    if (width <= 32 * 16) return launch_rows_of<SRC, true, 2 * L>(src, out, rows, st);
+    if constexpr (SRC::E == 8) {
+        if (width <= 32 * 24) return launch_rows_of<SRC, true, 3 * L>(src, out, rows, st);
+        if (width <= 32 * 32) return launch_rows_of<SRC, true, 4 * L>(src, out, rows, st);
+    }
+    if constexpr (SRC::kNarrow == 1) {
+        if (width <= 256 * 8) return launch_rows_of<SRC, false, L>(src, out, rows, st);
+    }
+    if constexpr (SRC::kNarrow <= 2) {
+        if (width <= 512 * 16) return launch_rows_of<SRC, false, 2 * L>(src, out, rows, st);
+    }
+    if (width <= 512 * 32) return launch_rows_of<SRC, false, 4 * L>(src, out, rows, st);
+    cudaLaunchAttribute attr[1];
+    const cudaLaunchConfig_t cfg = dependent_launch(dim3((unsigned)rows), 1024, attr, st);
+    LUMI_CUDA(cudaLaunchKernelEx(&cfg, quant_wide_kernel<SRC, 1024>, src, out));
+    return LUMI_OK;
 }
 
 template <typename XT, typename OT>
