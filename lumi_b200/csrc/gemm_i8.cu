@@ -829,7 +829,7 @@ TileShape tile_shape(const I8Args& g) {
     const long tiles = ((long)g.N + kWRows - 1) / kWRows;
     TileShape best{0, 0, 1};
     double least = 0;
-    for (int cols = 32; cols <= kMaxCols; cols *= 2) {
+    for (int cols = 32; cols <= kMaxCols; cols += 32) {
         const long whole = tiles * ((g.M + cols - 1) / cols);
         if (whole > sm_count()) continue;
         for (int splits = 1; splits <= 8; splits *= 2) {

@@ -3,7 +3,11 @@
 //
 // A row t is held as q = rint(t * 127 / m) and s = m / 127, m = max(max |t|, 2^-100).  The norm's factor r = 1 / sqrt(mean x^2 + eps) is the same for the
 // whole row and cancels out of q: t = x w without it, and s = m / 127 * r.  So the sum of squares and the maximum are reduced side by side, in one
-// pass over registers.  The maximum is taken over the bits of |t|, where infinities and NaN are largest: such a row gets q = 0 and s = NaN.
+// pass over registers.  The maximum keeps infinities and NaN: such a row gets q = 0 and s = NaN.  Sums, maxima and scales are fp32.
+//
+// What bounds them is memory: each number is read once and written once.  Arithmetic comes close where rows are bf16: the norm of 8192 x 4096 rows without a residual
+// (3 bytes per number, about 10 instructions) takes 21 us where DRAM takes 15.  Against rates that a plain copy reaches (6.55 TB/s): norm of 32768 x 1024 fp32 rows with a
+// residual 66 us, 101 %; gate of 32768 x 2816 bf16 rows 71 us, 99 %; these back as bf16 46 us, 93 %.  One row takes 1.7 us, which is its launch.
 #include "device_args.h"
 #include "rows.cuh"
 
@@ -121,15 +125,22 @@ __device__ __forceinline__ void store_some(__nv_bfloat16* p, int n, const float 
         for (int i = 0; i < E; ++i) if (i < n) p[i] = __float2bfloat16_rn(v[i]);
 }
 
-// kStay: blocks stay for row after row.  kNarrow: the fewest eights of numbers that a thread of a block holds.  Measured ...
 // ---- sources of rows: load(): what memory holds of E numbers; values(): the numbers to be held in 8 bits, with the sum of squares
+//
+// How a row is laid over threads goes by what a source reads (device time, us; DRAM's floor in brackets):
+// kWarp: up to this many numbers a row is a warp's, four warps per block.  fp32 without a residual 32768 x 1024: 26 (26), by blocks of 64 threads 35; with one, 74
+//   (65), by blocks of 128 threads 66: twice the bytes want more threads.
+// kEights: eights of numbers that each thread of a block holds, at least.  Gate of 32768 x 2816 bf16 rows: four 71 (70), two 81, one 117; norm of 16384 x 2048 fp32 rows with a
+//   residual: one 66 (66), four 68; of 8192 x 4096 bf16 rows with a residual: two 39 (36), one 42, four 60; without: four 21 (15), two 25.
+// kStay: as many blocks as run at once stay for row after row, the next one's loads ahead of this one's reduction.  It wins where a row is few bytes and has a residual's
+//   sum to write (bf16, 16384 x 2048: 41 against 59), and loses elsewhere: the registers cost more blocks (gate of 32768 x 2816 bf16 rows: 94 against 75).
 // Norm, or rows as they are.  ADD: x += o first, rounded to x's type, so that the norm sees what later readers of x see.
 template <typename XT, typename OT, bool ADD, bool NORM, bool RAGGED>
 struct NormSource {
     static constexpr bool kRagged = RAGGED;
     static constexpr int E = sizeof(XT) == 4 ? 4 : 8;
     static constexpr bool kNorm = NORM, kStay = E == 8 && ADD;
-    static constexpr int kNarrow = (E == 8 ? 2 : 1) * (ADD ? 1 : 2), kWarp = E == 8 || !ADD ? 1024 : 512;
+    static constexpr int kEights = ADD ? 1 : (E == 8 ? 4 : 2), kWarp = E == 8 || !ADD ? 1024 : 512;
     XT* x; const OT* o; const float* w;
     long ldx, ldo;
     int width;
@@ -181,7 +192,7 @@ struct GateSource {
     static constexpr bool kRagged = RAGGED;
     static constexpr int E = sizeof(XT) == 4 ? 4 : 8;
     static constexpr bool kNorm = false, kStay = false;
-    static constexpr int kNarrow = E == 8 ? 4 : 1, kWarp = E == 8 ? 1024 : 512;
+    static constexpr int kEights = E == 8 ? 4 : 1, kWarp = E == 8 ? 1024 : 512;
     const XT* gu;
     long ld;
     int up, width;
@@ -399,6 +410,14 @@ int32_t launch_rows_of(const SRC& src, const QuantOut& out, int rows, cudaStream
     return LUMI_OK;
 }
 
+// Two eights of numbers per thread instead of four, where whole warps then leave fewer threads without numbers: 1536 columns are 192 eights, 64 threads of four or 96 of
+// two.  Gate of 32768 x 1536 bf16 rows 42 -> 37 us, 16384 x 2400 35 -> 31; rows that end within an eight are slower so (32768 x 1111 50 -> 54).
+inline bool two_eights(int width) {
+    const int n = (width + 7) / 8;
+    auto slots = [&](int per) { return ((n + per - 1) / per + 31) / 32 * 32 * per; };
+    return 10 * slots(2) < 9 * slots(4);
+}
+
 // The shape goes by the width alone, so that a row has the same bits alone and among others.
 template <typename SRC>
 int32_t launch(const SRC& src, const QuantOut& out, int rows, cudaStream_t st) {
@@ -410,11 +429,11 @@ int32_t launch(const SRC& src, const QuantOut& out, int rows, cudaStream_t st) {
         if (width <= 32 * 24) return launch_rows_of<SRC, true, 3 * L>(src, out, rows, st);
         if (width <= 32 * 32) return launch_rows_of<SRC, true, 4 * L>(src, out, rows, st);
     }
-    if constexpr (SRC::kNarrow == 1) {
+    if constexpr (SRC::kEights == 1) {
         if (width <= 256 * 8) return launch_rows_of<SRC, false, L>(src, out, rows, st);
     }
-    if constexpr (SRC::kNarrow <= 2) {
-        if (width <= 512 * 16) return launch_rows_of<SRC, false, 2 * L>(src, out, rows, st);
+    if constexpr (SRC::kEights <= 2 || !SRC::kRagged) {
+        if (width <= 512 * 16 && (SRC::kEights <= 2 || two_eights(width))) return launch_rows_of<SRC, false, 2 * L>(src, out, rows, st);
     }
     if (width <= 512 * 32) return launch_rows_of<SRC, false, 4 * L>(src, out, rows, st);
     cudaLaunchAttribute attr[1];
