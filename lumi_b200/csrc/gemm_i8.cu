@@ -58,8 +58,10 @@ __device__ __forceinline__ int dot16(const int4& a, const int4& b, int s) {
     return __dp4a(a.w, b.w, __dp4a(a.z, b.z, __dp4a(a.y, b.y, __dp4a(a.x, b.x, s))));
 }
 
+// Bound by the stream of W, for small products by its latency.  Device time, us, 1 x 7360 x 1024 / 1 x 1024 x 8448 / 1 x 16384 x 4096 (67 MB, DRAM's floor 10.2): two rows of W per
+// warp and three pieces of each under way 3.0 / 3.5 / 12.4, four pieces 3.6 / 4.9 / 12.5, two 3.1 / 4.7 / 13.1; one row and four pieces 3.8 / 4.2 / 12.9.
 constexpr int kVecRows = 2;                  // rows of W per warp
-constexpr int kVecDeep = 4;                  // pieces of 512 bytes of each that are under way
+constexpr int kVecDeep = 3;                  // pieces of 512 bytes of each that are under way
 
 // MB rows of A
 template <int MB, typename DT>
@@ -132,10 +134,13 @@ __device__ __forceinline__ void mma_i8(int (&c)[4], int a0, int a1, int a2, int 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// A warp-level MMA needs neither TMEM nor tensor maps and no barrier to start, which is what a small product's time goes to; a large W streams better through the tiles
+// below.  Device time, us, this kernel / tile_kernel, 8 rows: 1024 x 1024 2.5 / 3.9, 7360 x 1024 4.1 / 5.0, 1024 x 2816 3.7 / 4.3, 1024 x 8448 13.9 / 6.2,
+// 32000 x 2048 16.6 / 15.4, 16384 x 4096 16.4 / 13.9; 16 rows 7360 x 1024 5.3 / 5.0.
 constexpr int kFewW = 16;                    // rows of W per warp: the M of the MMA; rows of A are its columns
-constexpr int kFewRows = 8, kFewK = 4096;    // and only while W is small: at 16 MB the tensor cores' tiles stream it as fast
-constexpr long kFewBytes = 16l << 20;
-constexpr int kFewDeep = 4;                  // steps of 64 bytes of each that are under way
+constexpr int kFewRows = 8, kFewK = 4096;
+constexpr long kFewBytes = 16l << 20;        // of W
+constexpr int kFewDeep = 3;                  // steps of 64 bytes of each that are under way
 
 // Lane 4 g + t holds bytes 16 t to 16 t + 15 of a step of rows g and g + 8 of W and of row g of A.  An MMA wants bytes 4 t and 16 + 4 t of 32: which bytes of K
 // these are does not matter as long as they are the same of both operands, so it is given words 0 and 1, the next one words 2 and 3.
@@ -302,7 +307,9 @@ static_assert(sizeof(TileTail) <= kTailBytes, "tail of the shared memory");
 struct TileShape { int cols, stages, splits; };
 
 // A tile of 128 rows of W and `cols` rows of A per cluster of `splits` CTAs, which share K; each of them finishes cols / splits rows of A.
-// Warp 0: copies.  Warp 1: TMEM and MMA.  All eight: accumulators (warp w reads the lanes of quarter w % 4, columns by halves).
+// Warp 0: copies.  Warp 1: TMEM and MMA.  All eight: accumulators (warp w reads the lanes of quarter w % 4, strips of 32 columns in turn).
+// What bounds it is a chain: launch and barriers, the first copies, 0.25 us per k-block (one thread waits, issues four MMAs and commits; copies by two threads or sums in turn in
+// four accumulators changed nothing, composing the descriptors anew took 0.29), the results.  203 x 2053 x 1111: 5.0 us, DRAM's floor 0.5.
 template <typename DT>
 __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, I8Args g, TileShape sh) {
     extern __shared__ uint8_t smem_raw[];
@@ -380,8 +387,7 @@ __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUten
                 mbar_arrive(&tl.done);
             }
         }
-    }
-    else if (warp < 6) {
+    } else if (warp < 6) {
         for (int i = threadIdx.x - 64; i < cols; i += 128) tl.a_scale[i] = m0 + i < g.M ? g.a_scale[m0 + i] : 0.f;
     }
     __syncwarp();
@@ -468,7 +474,13 @@ __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUten
 // Two CTAs of a cluster (two SMs) take tiles of 256 rows of W and `cols` rows of A (cta_group::2): each stages its 128 rows of W and half of the rows of A, the
 // first one issues the MMAs for both, each finishes its own rows of W.  Persistent, with two accumulators: a tile is finished while the next is multiplied.
 // Tiles go in blocks of 16 tiles of rows of A, rows of W by rows of W within a block, so that both operands come out of L2.
-// Warp 0: copies.  Warp 1: TMEM and MMA.  Warps 2 to 9: accumulators, two warps per quarter of the lanes, columns in turn.
+// Warp 0: copies.  Warp 1: TMEM and MMA.  Warps 2 to 9: accumulators, two warps per quarter of the lanes, strips of 32 columns in turn.
+//
+// Results go through shared memory to tensor-map stores where D's rows allow it, old values of D come the same way, asked for a strip ahead (4096 x 7360 x 1024 into fp32: 52 us; by
+// single loads 71).  The arrival that gives an accumulator back is relaxed: as a release it waited for the results to reach memory (4096 x 7360 x 1024 35 -> 29 us).
+//
+// What bounds it, 10^12 operations a second (twice the measured bf16 rate: 3342): 8192 x 8192 x 8192 3380, the tensor cores under their power limit; 8192 x 2048 x 8448 into an fp32
+// stream 2710; at short K the shared memory, which operands, their copies and the results share: 4096 x 7360 x 1024 2090, and 2950 with the results left out.
 constexpr int kPairThreads = 320;
 struct PairTail {
     uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], drain;
@@ -757,8 +769,17 @@ int32_t make_map(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, lo
     }
     cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)row_bytes};
     cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, estr[2] = {1, 1};
-    const CUresult r = fn(map, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto encode_map = [&] {
+        return fn(map, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode_map();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {                // a host thread that has launched nothing yet: its device is chosen, but the driver does not know
+        int dev = 0;
+        LUMI_CUDA(cudaGetDevice(&dev));
+        LUMI_CUDA(cudaSetDevice(dev));
+        r = encode_map();
+    }
     if (r != CUDA_SUCCESS) return fail(LUMI_E_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (%d rows of %d)", (int)r, rows, cols);
     return LUMI_OK;
 }
