@@ -363,7 +363,8 @@ int32_t lumi_k_gate_mul(uint64_t gu, int32_t ld, uint64_t out32, uint64_t hi, ui
 /* The norm in front of a projection: x[r] += o[r] (o = 0: x is left alone; the sum is rounded to x's type, and the norm sees the rounded row), then
  * the rows x[r] / sqrt(mean(x[r]^2) + eps) * w over `width` elements as q[rows][ldq] and scale[rows].  w = 0: no norm, the rows of x as they are (a
  * projection's weights [N][K] give q and w_scale of lumi_k_gemm_i8; eps is not looked at).  x_dtype, o_dtype: LUMI_DTYPE_*; w fp32, eps > 0.
- * ldx and ldo are multiples of 4 (fp32) or 8 (bf16) elements, ldq of 16; x, o, w and q are 16-byte aligned. */
+ * ldx and ldo are multiples of 4 (fp32) or 8 (bf16) elements, ldq of 16; x, o, w and q are 16-byte aligned.  o may be x itself; nothing else overlaps.
+ * A row for which x * w leaves fp32's range is one that holds an infinity.  Rows are independent: their results are the same bits alone and among others. */
 int32_t lumi_k_norm_quant(uint64_t x, int32_t x_dtype, int32_t ldx, uint64_t o, int32_t o_dtype, int32_t ldo, uint64_t w, uint64_t q, int32_t ldq,
                           uint64_t scale, int32_t rows, int32_t width, float eps, uint64_t stream);
 

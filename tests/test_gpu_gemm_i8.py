@@ -93,6 +93,37 @@ def test_large(d, bias, add):
     Case(300, 9000, 513, d, bias, add).run().check()
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 77, 200), (5, 77, 200), (30, 300, 1000), (30, 300, 3000), (5000, 520, 200)])
+@pytest.mark.parametrize("d", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_operands_that_begin_and_end_anywhere(M, N, K, d, shift):
+    """Bases 16 bytes behind a larger boundary, operands that end with their last number, results that begin at any element."""
+    g = torch.Generator(device="cuda").manual_seed(M + shift)
+    ld = up(K)
+
+    def rows(n):
+        buf = torch.full((16 + (n - 1) * ld + K,), 99, device="cuda", dtype=torch.int8)
+        t = buf[16:].as_strided((n, K), (ld, 1))
+        t.copy_(torch.randint(-128, 128, (n, K), generator=g, device="cuda", dtype=torch.int16).to(torch.int8))
+        return t
+
+    a, w = rows(M), rows(N)
+    sa, sw, b = (torch.rand(n + 1, generator=g, device="cuda")[1:] for n in (M, N, N))
+    old = torch.randn(M * N + shift + 1, generator=g, device="cuda").to(d)
+    for add in (0, 1):
+        whole = old.clone()
+        out = whole[shift:shift + M * N].view(M, N)
+        lumi_b200.api.check(lumi_b200.lib().lumi_k_gemm_i8(a.data_ptr(), ld, sa.data_ptr(), w.data_ptr(), ld, sw.data_ptr(), b.data_ptr(), out.data_ptr(),
+                                                           int(d == torch.bfloat16), N, M, N, K, add, 0, 0))
+        torch.cuda.synchronize()
+        p = (a.double() @ w.double().t()) * sa.double()[:, None] * sw.double()
+        q = p + b.double()
+        r = q + (old[shift:shift + M * N].view(M, N).double() if add else 0)
+        allowed = 3.01 * U * p.abs() + 1.01 * U * (q.abs() + r.abs()) + (1.01 * 2.0 ** -8 * r.abs() if d == torch.bfloat16 else 0)
+        assert float(((out.double() - r).abs() - allowed).max()) <= 0
+        assert torch.equal(whole[:shift], old[:shift]) and torch.equal(whole[shift + M * N:], old[shift + M * N:])
+
+
 @pytest.mark.parametrize("M,N", [(1, 7), (3, 40), (20, 130), (300, 300)])
 def test_largest_sums(M, N):
     """131071 products of -128 and -128: 2^31 - 2^14."""

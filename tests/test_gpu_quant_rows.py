@@ -209,3 +209,44 @@ def test_rows_back(width, dtype):
             torch.cuda.synchronize()
             assert bool((y[:, width:] == 7).all()) and bool((whole[:shift] == 7).all()) and bool((whole[shift + rows * ldy:] == 7).all())
             assert torch.equal((q[:, :width].float() * s[:rows, None]).to(dtype).nan_to_num(nan=1e30), y[:, :width].nan_to_num(nan=1e30))
+
+
+@pytest.mark.parametrize("width", [5, 260, 1001, 4100, 70001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_that_begin_on_16_bytes_and_no_more(width, dtype):
+    """Bases 16 bytes behind a larger boundary, rows that are whole 16 bytes long and no more, operands that end where they do."""
+    e = 128 // torch.finfo(dtype).bits
+    ld, ldq, rows = (width + e - 1) // e * e, (width + 15) // 16 * 16, 3
+    g = torch.Generator(device="cuda").manual_seed(width)
+
+    def rows_at(ld, dtype, step):
+        buf = torch.zeros(step + (rows - 1) * ld + width, device="cuda", dtype=dtype)      # the last row ends with its numbers
+        return buf, buf[step:].as_strided((rows, width), (ld, 1))
+
+    _, x = rows_at(ld, dtype, e)
+    _, o = rows_at(ld, dtype, e)
+    for t in (x, o):
+        t.copy_(torch.randn(rows, width, generator=g, device="cuda"))
+    w = torch.zeros(4 + width, device="cuda")[4:]
+    w.copy_(torch.randn(width, generator=g, device="cuda"))
+    whole, q = rows_at(ldq, torch.int8, 16)
+    s = torch.zeros(rows + 1, device="cuda")[1:]
+    want = (x.float() + o.float()).to(dtype)
+    call("lumi_k_norm_quant", x.data_ptr(), code(x), ld, o.data_ptr(), code(o), ld, w.data_ptr(), q.data_ptr(), ldq, s.data_ptr(), rows, width, EPS, 0)
+    torch.cuda.synchronize()
+    assert torch.equal(x, want) and bool((whole[:16] == 0).all())
+    t = want.double()
+    check(q.double(), s.double(), t * w.double(), 1 / torch.sqrt((t * t).mean(1, keepdim=True) + EPS), 2.0 ** -24)
+    up = ld
+    buf = torch.zeros(e + (rows - 1) * 2 * up + up + width, device="cuda", dtype=dtype)
+    gu = buf[e:]
+    gate, ups = gu.as_strided((rows, width), (2 * up, 1)), gu[up:].as_strided((rows, width), (2 * up, 1))
+    gate.copy_(x.clamp(-15, 15)), ups.copy_(o)
+    call("lumi_k_gate_quant", gu.data_ptr(), code(gu), 2 * up, up, 1, q.data_ptr(), ldq, s.data_ptr(), rows, width, 0)
+    torch.cuda.synchronize()
+    z = gate.double()
+    check(q.double(), s.double(), torch.sigmoid(z) * z * ups.double(), torch.ones(rows, 1, device="cuda", dtype=torch.float64), 2.0 ** -18)
+    y = torch.zeros(rows * width + 1, device="cuda", dtype=dtype)[1:].view(rows, width)
+    call("lumi_k_dequant_rows", q.data_ptr(), ldq, s.data_ptr(), y.data_ptr(), code(y), width, rows, width, 0)
+    torch.cuda.synchronize()
+    assert torch.equal(y, (q.float() * s[:, None]).to(dtype))
