@@ -232,6 +232,14 @@ __device__ __forceinline__ void mbar_arrive_relaxed(uint32_t cluster_addr) {
 // An operand tile's descriptor changes in its low word alone, by 16 bytes per one: the issuing thread adds, since composing two of them per MMA takes it
 // longer than a narrow MMA.
 __device__ __forceinline__ uint64_t moved(uint64_t desc, uint32_t units) { return (desc & 0xffffffff00000000ull) | (uint32_t)((uint32_t)desc + units); }
+// One lane of a warp that has not parted.  The warps that issue copies and MMAs run their loops whole, so that what these instructions want in uniform registers is computed there: by
+// one lane in a branch of its own, each MMA took its issuing thread four moves more.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+__device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
 // signed bytes by signed bytes into 32-bit integers, `rows` x `cols`
 __device__ __forceinline__ uint32_t i8_idesc(int rows, int cols) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(rows >> 4) << 24); }
 __device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -317,7 +325,7 @@ __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUten
     const int S = sh.stages, cols = sh.cols, splits = sh.splits, stage = kWBytes + cols * kBlockK;
     int* part = reinterpret_cast<int*>(base + S * stage);               // splits > 1: [split][four rows of A][row of W][4]
     TileTail& tl = *reinterpret_cast<TileTail*>(base + S * stage + (splits > 1 ? cols * kWRows * 4 : 0));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const int rank = (int)blockIdx.x % splits, n0 = (int)blockIdx.x / splits * kWRows, m0 = blockIdx.y * cols;
     const int num_kb = (g.K + kBlockK - 1) / kBlockK, kb0 = (int)((long)rank * num_kb / splits), nkb = (int)((long)(rank + 1) * num_kb / splits) - kb0;
     const uint32_t tmem_cols = cols <= 32 ? 32u : (cols <= 64 ? 64u : (cols <= 128 ? 128u : 256u));
@@ -347,14 +355,17 @@ __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUten
     pdl_sync();
 
     if (warp == 0) {
-        if (lane == 0 && (int)(blockIdx.y * gridDim.x + blockIdx.x) != g.skip_unit) {
+        if ((int)(blockIdx.y * gridDim.x + blockIdx.x) != g.skip_unit) {
             int s = 0, issued = 0;
             uint32_t ph = 0;
             for (int i = 0; i < nkb; ++i) {
-                if (!wait_for(&tl.empty[s], ph ^ 1u, g.wait_ns)) { timed_out = true; break; }
-                mbar_expect_tx(&tl.full[s], (uint32_t)stage);
-                tma_load_2d(base + s * stage, &map_w, &tl.full[s], (kb0 + i) * kBlockK, n0);
-                tma_load_2d(base + s * stage + kWBytes, &map_a, &tl.full[s], (kb0 + i) * kBlockK, m0);
+                if (!__all_sync(0xffffffffu, wait_for(&tl.empty[s], ph ^ 1u, g.wait_ns))) { timed_out = true; break; }
+                if (elect_one()) {
+                    mbar_expect_tx(&tl.full[s], (uint32_t)stage);
+                    tma_load_2d(base + s * stage, &map_w, &tl.full[s], (kb0 + i) * kBlockK, n0);
+                    tma_load_2d(base + s * stage + kWBytes, &map_a, &tl.full[s], (kb0 + i) * kBlockK, m0);
+                }
+                __syncwarp();
                 issued = i + 1;
                 if (++s == S) { s = 0; ph ^= 1u; }
             }
@@ -362,30 +373,28 @@ __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUten
                 for (int i = max(0, issued - S); i < issued; ++i) wait_for(&tl.full[i % S], (uint32_t)(i / S) & 1u, g.wait_ns);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = i8_idesc(kWRows, cols), units = (uint32_t)stage >> 4;
-            const uint64_t w0 = make_smem_desc(smem_u32(base)), a0 = make_smem_desc(smem_u32(base) + kWBytes);
-            int s = 0;
-            uint32_t ph = 0;
-            bool here = nkb > 0 && mbar_try_wait(&tl.full[0], 0);
-            for (int i = 0; i < nkb; ++i) {
-                if (!here && !wait_for(&tl.full[s], ph, g.wait_ns)) { timed_out = true; break; }
-                tc_fence_after();
+        const uint32_t idesc = i8_idesc(kWRows, cols), units = (uint32_t)stage >> 4;
+        const uint64_t w0 = make_smem_desc(smem_u32(base)), a0 = make_smem_desc(smem_u32(base) + kWBytes);
+        int s = 0;
+        uint32_t ph = 0;
+        for (int i = 0; i < nkb; ++i) {
+            if (!__all_sync(0xffffffffu, wait_for(&tl.full[s], ph, g.wait_ns))) { timed_out = true; break; }
+            tc_fence_after();
+            if (elect_one()) {
                 const uint64_t w = moved(w0, (uint32_t)s * units), a = moved(a0, (uint32_t)s * units);
 #pragma unroll
                 for (int k = 0; k < kBlockK / 32; ++k) umma_i8(tmem, moved(w, 2 * k), moved(a, 2 * k), idesc, (i > 0 || k > 0) ? 1u : 0u);
                 umma_commit(&tl.empty[s]);
-                if (++s == S) { s = 0; ph ^= 1u; }
-                here = i + 1 < nkb && mbar_try_wait(&tl.full[s], ph);
+                if (i + 1 == nkb) umma_commit(&tl.done);
             }
-            if (!timed_out) {
-                umma_commit(&tl.done);
-            } else {                                                    // let every MMA issued so far finish (bounded), then pass the word on
-                umma_commit(&tl.drain);
-                wait_for(&tl.drain, 0, g.wait_ns);
-                *reinterpret_cast<volatile int*>(&tl.lost) = 1;
-                mbar_arrive(&tl.done);
-            }
+            __syncwarp();
+            if (++s == S) { s = 0; ph ^= 1u; }
+        }
+        if (timed_out && elect_one()) {                                 // let every MMA issued so far finish (bounded), then pass the word on
+            umma_commit(&tl.drain);
+            wait_for(&tl.drain, 0, g.wait_ns);
+            *reinterpret_cast<volatile int*>(&tl.lost) = 1;
+            mbar_arrive(&tl.done);
         }
     } else if (warp < 6) {
         for (int i = threadIdx.x - 64; i < cols; i += 128) tl.a_scale[i] = m0 + i < g.M ? g.a_scale[m0 + i] : 0.f;
@@ -512,7 +521,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
     const int S = sh.stages, cols = sh.cols, stage = kWBytes + cols / 2 * kBlockK;
     uint8_t* strips = base + S * stage;
     PairTail& tl = *reinterpret_cast<PairTail*>(strips + 16 * kStripBytes<DT>);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const int rank = (int)(blockIdx.x & 1), first = (int)(blockIdx.x >> 1), at_once = (int)(gridDim.x >> 1);
     const int num_kb = (g.K + kBlockK - 1) / kBlockK, tiles_w = sh.tiles / sh.tiles_a;
 
@@ -548,51 +557,55 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
     pdl_sync();
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t kbg = 0;                                           // k-blocks issued so far, over all tiles
-            int s = 0;
-            uint32_t ph = 0;
-            for (int t = first; t < sh.tiles && !timed_out; t += at_once) {
-                if (t == g.skip_unit && rank == 1) break;
-                int m0, n0;
-                place(t, m0, n0);
-                for (int kb = 0; kb < num_kb; ++kb, ++kbg) {
-                    if (!wait_for(&tl.empty[s], ph ^ 1u, g.wait_ns)) { timed_out = true; break; }
+        uint32_t kbg = 0;                                               // k-blocks issued so far, over all tiles
+        int s = 0;
+        uint32_t ph = 0;
+        for (int t = first; t < sh.tiles && !timed_out; t += at_once) {
+            if (t == g.skip_unit && rank == 1) break;
+            int m0, n0;
+            place(t, m0, n0);
+            for (int kb = 0; kb < num_kb; ++kb, ++kbg) {
+                if (!__all_sync(0xffffffffu, wait_for(&tl.empty[s], ph ^ 1u, g.wait_ns))) { timed_out = true; break; }
+                if (elect_one()) {
                     const uint32_t bar = map_to_rank(smem_u32(&tl.full[s]), 0);      // both CTAs' copies complete on the first one's barrier
                     if (rank == 0) mbar_expect_tx(&tl.full[s], 2u * (uint32_t)stage);
                     tma_load_2d_pair(base + s * stage, &map_w, bar, kb * kBlockK, n0 + rank * kWRows);
                     tma_load_2d_pair(base + s * stage + kWBytes, &map_a, bar, kb * kBlockK, m0 + rank * (cols / 2));
-                    if (++s == S) { s = 0; ph ^= 1u; }
                 }
+                __syncwarp();
+                if (++s == S) { s = 0; ph ^= 1u; }
             }
-            st_cluster_u32(map_to_rank(smem_u32(&tl.issued[rank]), 0), kbg);
         }
+        if (lane == 0) st_cluster_u32(map_to_rank(smem_u32(&tl.issued[rank]), 0), kbg);
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             const uint32_t idesc = i8_idesc(2 * kWRows, cols), units = (uint32_t)stage >> 4;
             const uint64_t w0 = make_smem_desc(smem_u32(base)), a0 = make_smem_desc(smem_u32(base) + kWBytes);
             int s = 0;
             uint32_t ph = 0, it = 0;
             for (int t = first; t < sh.tiles && !timed_out; t += at_once, ++it) {
                 const uint32_t as = it & 1u, aph = (it >> 1) & 1u, acc = tmem + as * kMaxCols;
-                if (!wait_for(&tl.acc_empty[as], aph ^ 1u, g.wait_ns)) { timed_out = true; break; }      // this accumulator has been read
+                if (!__all_sync(0xffffffffu, wait_for(&tl.acc_empty[as], aph ^ 1u, g.wait_ns))) { timed_out = true; break; }      // this accumulator has been read
                 tc_fence_after();
                 for (int kb = 0; kb < num_kb; ++kb) {
-                    if (!wait_for(&tl.full[s], ph, g.wait_ns)) { timed_out = true; break; }
+                    if (!__all_sync(0xffffffffu, wait_for(&tl.full[s], ph, g.wait_ns))) { timed_out = true; break; }
                     tc_fence_after();
-                    const uint64_t w = moved(w0, (uint32_t)s * units), a = moved(a0, (uint32_t)s * units);
+                    if (elect_one()) {
+                        const uint64_t w = moved(w0, (uint32_t)s * units), a = moved(a0, (uint32_t)s * units);
 #pragma unroll
-                    for (int k = 0; k < kBlockK / 32; ++k) umma_i8_pair(acc, moved(w, 2 * k), moved(a, 2 * k), idesc, (kb > 0 || k > 0) ? 1u : 0u);
-                    umma_commit_pair(&tl.empty[s]);
+                        for (int k = 0; k < kBlockK / 32; ++k) umma_i8_pair(acc, moved(w, 2 * k), moved(a, 2 * k), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                        umma_commit_pair(&tl.empty[s]);
+                        if (kb + 1 == num_kb) umma_commit_pair(&tl.acc_full[as]);
+                    }
+                    __syncwarp();
                     if (++s == S) { s = 0; ph ^= 1u; }
                 }
-                if (timed_out) break;
-                umma_commit_pair(&tl.acc_full[as]);
             }
-            if (timed_out) {                                            // let every MMA issued so far finish (bounded) before TMEM is freed
+            if (timed_out && elect_one()) {                             // let every MMA issued so far finish (bounded) before TMEM is freed
                 umma_commit_pair(&tl.drain);
                 wait_for(&tl.drain, 0, g.wait_ns);
             }
+            __syncwarp();
         }
     } else {
         const int q = warp & 3, half = (warp - 2) >> 2, strips_here = (cols / 32 - half + 1) >> 1;
