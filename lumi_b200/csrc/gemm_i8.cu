@@ -135,11 +135,11 @@ __device__ __forceinline__ void mma_i8(int (&c)[4], int a0, int a1, int a2, int 
 }
 
 // A warp-level MMA needs neither TMEM nor tensor maps and no barrier to start, which is what a small product's time goes to; a large W streams better through the tiles
-// below.  Device time, us, this kernel / tile_kernel, 8 rows: 1024 x 1024 2.5 / 3.9, 7360 x 1024 4.1 / 5.0, 1024 x 2816 3.7 / 4.3, 1024 x 8448 13.9 / 6.2,
-// 32000 x 2048 16.6 / 15.4, 16384 x 4096 16.4 / 13.9; 16 rows 7360 x 1024 5.3 / 5.0.
+// below.  Device time, us, this kernel / tile_kernel, 8 rows: 1024 x 1024 2.4 / 3.6, 7360 x 1024 4.0 / 4.4, 1024 x 2048 3.2 / 3.9, 5632 x 2048 5.8 / 6.1, 16384 x 1024 6.0 / 5.9,
+// 1024 x 2816 4.5 / 4.0, 1024 x 4096 7.1 / 4.3; with two such tiles for 16 rows 7360 x 1024 5.3 / 4.4.
 constexpr int kFewW = 16;                    // rows of W per warp: the M of the MMA; rows of A are its columns
-constexpr int kFewRows = 8, kFewK = 4096;
-constexpr long kFewBytes = 16l << 20;        // of W
+constexpr int kFewRows = 8, kFewK = 2048;
+constexpr long kFewBytes = 12l << 20;        // of W
 constexpr int kFewDeep = 3;                  // steps of 64 bytes of each that are under way
 
 // Lane 4 g + t holds bytes 16 t to 16 t + 15 of a step of rows g and g + 8 of W and of row g of A.  An MMA wants bytes 4 t and 16 + 4 t of 32: which bytes of K
@@ -249,19 +249,65 @@ __device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint32_t a, uint32_
 __device__ __forceinline__ void shared_load4(uint32_t at, float (&v)[32], int i) {
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[i]), "=f"(v[i + 1]), "=f"(v[i + 2]), "=f"(v[i + 3]) : "r"(at + 4 * i) : "memory");
 }
-__device__ __forceinline__ float shared_value(uint32_t at, const float*) {
+__device__ __forceinline__ float shared_value(uint32_t at) {
     float v;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
     return v;
 }
-__device__ __forceinline__ float shared_value(uint32_t at, const __nv_bfloat16*) {
-    uint16_t v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
-    return __uint_as_float((uint32_t)v << 16);
+__device__ __forceinline__ void shared_put(uint32_t at, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
+// bf16 strips cross shared memory as 8 x 8 matrices, transposed on their way: a quarter of the accesses that results one by one take.  A strip holds rows of A, 64 bytes each, whose
+// 16-byte pieces are XOR-ed with the row's place (the 64-byte swizzle of tensor maps), so that the eight rows of a matrix meet eight different banks.
+// Lane 4 r + c of a warp has columns 2 c and 2 c + 1 (rows of A) of rows r and r + 8 (of W) of 16 x 8 accumulators.
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
 }
-__device__ __forceinline__ void shared_put(uint32_t at, float v, const float*) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
-__device__ __forceinline__ void shared_put(uint32_t at, float v, const __nv_bfloat16*) {
-    asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(__bfloat16_as_ushort(__float2bfloat16_rn(v))) : "memory");
+__device__ __forceinline__ void tmem_arrived(uint32_t (&a)[16], uint32_t (&b)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]),
+                   "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]), "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15]),
+                   "+r"(b[0]), "+r"(b[1]), "+r"(b[2]), "+r"(b[3]), "+r"(b[4]), "+r"(b[5]), "+r"(b[6]), "+r"(b[7]),
+                   "+r"(b[8]), "+r"(b[9]), "+r"(b[10]), "+r"(b[11]), "+r"(b[12]), "+r"(b[13]), "+r"(b[14]), "+r"(b[15])
+                 :: "memory");
+}
+__device__ __forceinline__ uint32_t strip_piece(uint32_t strip, int b, int lane) {       // where lane points for the matrices of rows 8 b to 8 b + 7 of A
+    const int row = 8 * b + (lane & 7);
+    return strip + (uint32_t)(row * 64 + (((lane >> 3) ^ ((row >> 1) & 3)) << 4));
+}
+__device__ __forceinline__ void put_matrices(uint32_t at, const uint32_t (&m)[4]) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3]) : "memory");
+}
+__device__ __forceinline__ void get_matrices(uint32_t at, uint32_t (&m)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(m[0]), "=r"(m[1]), "=r"(m[2]), "=r"(m[3]) : "r"(at) : "memory");
+}
+// sums[g]: rows 16 g to 16 g + 15 of W, 32 rows of A; sw, bias: of rows lane / 4 + 8 k of W.
+__device__ __forceinline__ void finish_matrices(const uint32_t (&lo)[16], const uint32_t (&hi)[16], const float* a_scale, const float (&sw)[4], const float (&bias)[4], bool add,
+                                                uint32_t strip, int lane) {
+    float2 sa[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(sa[b].x), "=f"(sa[b].y) : "r"(smem_u32(a_scale) + (uint32_t)(8 * b + 2 * (lane & 3)) * 4u) : "memory");
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const uint32_t at = strip_piece(strip, b, lane);
+        uint32_t old[4], out[4];
+        if (add) get_matrices(at, old);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t s0 = k < 2 ? lo[4 * b + 2 * k] : hi[4 * b + 2 * (k - 2)], s1 = k < 2 ? lo[4 * b + 2 * k + 1] : hi[4 * b + 2 * (k - 2) + 1];
+            float v0 = scaled((int)s0, sa[b].x, sw[k], bias[k]), v1 = scaled((int)s1, sa[b].y, sw[k], bias[k]);
+            if (add) {
+                v0 = __fadd_rn(v0, __uint_as_float(old[k] << 16));
+                v1 = __fadd_rn(v1, __uint_as_float(old[k] & 0xffff0000u));
+            }
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v0, v1);
+            out[k] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        put_matrices(at, out);
+    }
 }
 // Results of one row of W (this lane's) for 32 rows of A, of which `live` exist; a_scale: in shared memory.
 template <bool WHOLE, typename DT>
@@ -316,8 +362,8 @@ struct TileShape { int cols, stages, splits; };
 
 // A tile of 128 rows of W and `cols` rows of A per cluster of `splits` CTAs, which share K; each of them finishes cols / splits rows of A.
 // Warp 0: copies.  Warp 1: TMEM and MMA.  All eight: accumulators (warp w reads the lanes of quarter w % 4, strips of 32 columns in turn).
-// What bounds it is a chain: launch and barriers, the first copies, 0.25 us per k-block (one thread waits, issues four MMAs and commits; copies by two threads or sums in turn in
-// four accumulators changed nothing, composing the descriptors anew took 0.29), the results.  203 x 2053 x 1111: 5.0 us, DRAM's floor 0.5.
+// What bounds it is a chain: launch and barriers, the first copies, 0.19 us per k-block (a wait, four MMAs, a commit; issued by one lane in a branch of its own it took 0.25, with
+// descriptors composed anew 0.29; copies by two threads or sums in turn in four accumulators changed nothing), the results.  203 x 2053 x 1111: 4.3 us, DRAM's floor 0.5.
 template <typename DT>
 __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, I8Args g, TileShape sh) {
     extern __shared__ uint8_t smem_raw[];
@@ -485,11 +531,13 @@ __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUten
 // Tiles go in blocks of 16 tiles of rows of A, rows of W by rows of W within a block, so that both operands come out of L2.
 // Warp 0: copies.  Warp 1: TMEM and MMA.  Warps 2 to 9: accumulators, two warps per quarter of the lanes, strips of 32 columns in turn.
 //
-// Results go through shared memory to tensor-map stores where D's rows allow it, old values of D come the same way, asked for a strip ahead (4096 x 7360 x 1024 into fp32: 52 us; by
-// single loads 71).  The arrival that gives an accumulator back is relaxed: as a release it waited for the results to reach memory (4096 x 7360 x 1024 35 -> 29 us).
+// Results go through shared memory to tensor-map stores where D's rows allow it, old values of D come the same way, asked for a strip ahead (4096 x 7360 x 1024 into fp32: 51 us; by
+// single loads 71).  The arrival that gives an accumulator back is relaxed: as a release it waited for the results to reach memory (4096 x 7360 x 1024 35 -> 29 us).  Copies and MMAs are issued
+// by whole warps with one lane elected (29 -> 28 us; 8192 x 8192 x 8192 325 -> 316).
 //
-// What bounds it, 10^12 operations a second (twice the measured bf16 rate: 3342): 8192 x 8192 x 8192 3380, the tensor cores under their power limit; 8192 x 2048 x 8448 into an fp32
-// stream 2710; at short K the shared memory, which operands, their copies and the results share: 4096 x 7360 x 1024 2090, and 2950 with the results left out.
+// What bounds it, 10^12 operations a second (twice the measured bf16 rate: 3342): 8192 x 8192 x 8192 3520, the tensor cores; 8192 x 2048 x 8448 into an fp32 stream 2890; at short K the
+// shared memory, which operands, their copies and the results share: 4096 x 7360 x 1024 2360 (26 us; 28 with the results of a bf16 strip put one by one), and 2950 with the results left
+// out.  Called back to back for a second, the power limit takes the clock from 1.97 to 1.55 GHz there (32 us) and to 1.3 GHz at long K (8192 x 2048 x 8448: 98 -> 117 us).
 constexpr int kPairThreads = 320;
 struct PairTail {
     uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], drain;
@@ -672,14 +720,20 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
                 a_scale[lane] = i == 0 ? sa[0] : (i == 1 ? sa[1] : (i == 2 ? sa[2] : sa[3]));
                 __syncwarp();
             };
-            auto finish = [&](const uint32_t (&sum)[32], int i) {
+            float sw4[4], bias4[4];                                     // bf16: of the rows of W that this lane has in matrices
+            if constexpr (sizeof(DT) == 2)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    sw4[k] = __shfl_sync(0xffffffffu, sw, (lane >> 2) + 8 * k);
+                    bias4[k] = __shfl_sync(0xffffffffu, bias, (lane >> 2) + 8 * k);
+                }
+            auto finish = [&](const auto& sum, const auto& high, int i) {
                 const int m = m0 + (int)column(i);
                 const bool some = m < g.M && nw < g.N;
                 set_scales(i);
                 if (!timed_out && add) request(i + 1 < strips_here ? t : t + at_once, i + 1 < strips_here ? i + 1 : 0, b ^ 1u);
                 else if (lane == 0) stores_read<1>();
                 if (some) {
-                    const uint32_t at = smem_u32(buf + b * 1024 + lane);
                     if (add) {
                         if (!timed_out && !wait_for(&old[b], (arrivals >> b) & 1u, g.wait_ns)) timed_out = true;
                         timed_out = __any_sync(0xffffffffu, timed_out);
@@ -692,20 +746,25 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
                     } else {
                         __syncwarp();                                   // the buffer's last store has been read
                     }
-                    float v[32];
+                    if constexpr (sizeof(DT) == 2) {
+                        finish_matrices(sum, high, a_scale, sw4, bias4, add, smem_u32(buf + b * 1024), lane);
+                    } else {
+                        const uint32_t at = smem_u32(buf + b * 1024 + lane);
+                        float v[32];
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) shared_load4(smem_u32(a_scale), v, j);
+                        for (int j = 0; j < 32; j += 4) shared_load4(smem_u32(a_scale), v, j);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = scaled((int)sum[j], v[j], sw, bias);
-                    if (add) {
-                        float o[32];
+                        for (int j = 0; j < 32; ++j) v[j] = scaled((int)sum[j], v[j], sw, bias);
+                        if (add) {
+                            float o[32];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = shared_value(at + j * 32 * (uint32_t)sizeof(DT), (const DT*)nullptr);
+                            for (int j = 0; j < 32; ++j) o[j] = shared_value(at + j * 128u);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = __fadd_rn(v[j], o[j]);
+                            for (int j = 0; j < 32; ++j) v[j] = __fadd_rn(v[j], o[j]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) shared_put(at + j * 128u, v[j]);
                     }
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) shared_put(at + j * 32 * (uint32_t)sizeof(DT), v[j], (const DT*)nullptr);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) tma_store_2d(&map_d, buf + b * 1024, nw, m);
@@ -724,10 +783,19 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
             } else {
 #pragma unroll 1
                 for (int i = 0; i < strips_here; ++i) {
-                    uint32_t sum[32];
-                    tmem_ld32(lanes + column(i), sum);
-                    if (i + 1 == strips_here) release();
-                    finish(sum, i);
+                    if constexpr (sizeof(DT) == 2) {
+                        uint32_t lo[16], hi[16];
+                        tmem_ld_16x32(lanes + column(i), lo);
+                        tmem_ld_16x32(lanes + (16u << 16) + column(i), hi);
+                        tmem_arrived(lo, hi);
+                        if (i + 1 == strips_here) release();
+                        finish(lo, hi, i);
+                    } else {
+                        uint32_t sum[32];
+                        tmem_ld32(lanes + column(i), sum);
+                        if (i + 1 == strips_here) release();
+                        finish(sum, sum, i);
+                    }
                 }
             }
         }
@@ -804,7 +872,7 @@ int32_t make_i8_map(CUtensorMap* map, const void* ptr, long ld, int rows, int K,
 template <typename DT>
 int32_t make_result_map(CUtensorMap* map, const I8Args& g) {
     return make_map(map, sizeof(DT) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g.d, g.ldd * (long)sizeof(DT), g.M, g.N, 32, 32,
-                    CU_TENSOR_MAP_SWIZZLE_NONE);
+                    sizeof(DT) == 4 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 // Lets a kernel have as much shared memory as there is, once per device.
@@ -854,10 +922,10 @@ int32_t launch_few(const I8Args& g, cudaStream_t st) {
 }
 
 // Tile and shares of K for a product whose tiles fit on the GPU at once (cols 0: they do not).  The estimate, in microseconds behind what every launch
-// takes: 0.25 per k-block (one thread issues its four MMAs, whatever their width), and for the results, or for sums that cross the cluster's
-// shared memory, by the tile's width and the number of CTAs.  Measured, columns / shares (CTAs): 16 x 7360 x 1024 32/1 (58) 5.1, 32/2 (116) 6.0; 64 x 1024 x 2816 32/1 (16) 8.6,
-// 32/4 (64) 4.8, 64/4 (32) 6.0; 256 x 1024 x 2816 32/1 (64) 9.3, 64/4 (128) 7.0, 128/4 (64) 8.7; 512 x 259 x 8192 32/2 (96) 12.4, 64/4 (96) 9.5; a second round of CTAs costs
-// as much as the first: 256 x 7360 x 1024 128/1 (116) 6.5, 32/1 (464) 11.1, 128/2 (232) 20.5.
+// takes: 0.19 per k-block, and for the results, or for sums that cross the cluster's shared memory, by the tile's width and the number of CTAs.  Measured, columns /
+// shares (CTAs): 16 x 7360 x 1024 32/1 (58) 4.4, 32/2 (116) 5.8; 64 x 1024 x 2816 32/2 (32) 5.4, 32/4 (64) 4.3, 32/8 (128) 4.6, 64/4 (32) 5.4; 512 x 1024 x 2816 32/1 (128) 6.8, 64/2 (128)
+// 9.4; 512 x 259 x 8192 32/2 (96) 12.0, 64/4 (96) 10.1; 512 x 5632 x 2048 192/1 (132) 8.8, 256/1 (88) 10.4.  A second round of CTAs costs as much as the first: 256 x 7360 x 1024 128/1
+// (116) 6.5, 32/1 (464) 11.1, 128/2 (232) 20.5 (with a slower issue).
 TileShape tile_shape(const I8Args& g) {
     const int num_kb = (g.K + kBlockK - 1) / kBlockK;
     const long tiles = ((long)g.N + kWRows - 1) / kWRows;
@@ -868,7 +936,7 @@ TileShape tile_shape(const I8Args& g) {
         if (whole > sm_count()) continue;
         for (int splits = 1; splits <= 8; splits *= 2) {
             if (splits > 1 && (cols > 128 || splits > num_kb || whole * splits > kClusterCtas)) break;
-            const double cost = 0.25 * ((num_kb + splits - 1) / splits) + (splits > 1 ? 0.3 + 0.028 * cols + 0.006 * (double)(whole * splits) : 0.008 * cols);
+            const double cost = 0.19 * ((num_kb + splits - 1) / splits) + (splits > 1 ? 0.2 + 0.025 * cols + 0.012 * (double)(whole * splits) : 0.008 * cols);
             if (best.cols == 0 || cost < least) { best.cols = cols; best.splits = splits; least = cost; }
         }
     }
