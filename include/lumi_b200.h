@@ -354,7 +354,7 @@ int32_t lumi_k_norm_add(uint64_t x, uint64_t o, uint64_t w, uint64_t y, uint64_t
 int32_t lumi_k_gate_mul(uint64_t gu, int32_t ld, uint64_t out32, uint64_t hi, uint64_t lo, int32_t rows, int32_t width, uint64_t stream);
 
 /* ---- rows of 8-bit integers with a scale each, and their product -----------------------------
- * A row t of numbers is held as integers q = rint(t * 127 / m) (ties to even), at most 127 in size, and one fp32 scale s = m / 127 with
+ * A row t of numbers is held as integers q = rint(t * (127 / m)) (fp32 quotient and product, ties to even), at most 127 in size, and one fp32 scale s = m / 127 with
  * m = max(max |t|, 2^-100): t is about q * s.  A row that holds an infinity or a NaN gets q = 0 and s = NaN, so that all that is made from it is NaN.
  * These calls have no counterpart in the reference.  All pointers are memory of the current device; what lies between a row's end and the next
  * row (ld) is neither read nor written, rows begin on 16-byte boundaries.  Nothing is allocated and no workspace is shared: calls may overlap on any

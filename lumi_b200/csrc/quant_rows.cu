@@ -1,7 +1,7 @@
 // Rows of numbers as 8-bit integers with a scale per row, for products in 8-bit integers: the norm in front of a projection (with the
 // residual's addition), weights on their way into 8 bits, the gate between a feed-forward's products; and such rows back as numbers.
 //
-// A row t is held as q = rint(t * 127 / m) and s = m / 127, m = max(max |t|, 2^-100).  The norm's factor r = 1 / sqrt(mean x^2 + eps) is the same for the
+// A row t is held as q = rint(t * (127 / m)) and s = m / 127, m = max(max |t|, 2^-100).  The norm's factor r = 1 / sqrt(mean x^2 + eps) is the same for the
 // whole row and cancels out of q: t = x w without it, and s = m / 127 * r.  So the sum of squares and the maximum are reduced side by side, in one
 // pass over registers.  The maximum keeps infinities and NaN: such a row gets q = 0 and s = NaN.  Sums, maxima and scales are fp32.
 //
@@ -222,13 +222,14 @@ __device__ __forceinline__ void largest(const float (&t)[E], float& m) {
     for (int i = 0; i < E; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(t[i])));
 }
 
-// t * inv to the nearest integer, ties to even: added to 1.5 * 2^23, the integer is the sum's low byte.  Zeros where the row is not all numbers.
+// t * inv, rounded to fp32, to the nearest integer, ties to even: added to 1.5 * 2^23, the integer is the sum's low byte.  (Without the first rounding a quotient that lies on a half
+// falls to the side that the reciprocal's error points to.)  Zeros where the row is not all numbers.
 template <bool RAGGED, int E>
 __device__ __forceinline__ void put(int8_t* q, int n, const float (&t)[E], float inv, bool numbers) {
     uint32_t b[E];
     if (numbers) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) b[i] = __float_as_uint(fmaf(t[i], inv, 12582912.f));
+        for (int i = 0; i < E; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(t[i], inv), 12582912.f));
     } else {
 #pragma unroll
         for (int i = 0; i < E; ++i) b[i] = 0;

@@ -250,3 +250,26 @@ def test_rows_that_begin_on_16_bytes_and_no_more(width, dtype):
     call("lumi_k_dequant_rows", q.data_ptr(), ldq, s.data_ptr(), y.data_ptr(), code(y), width, rows, width, 0)
     torch.cuda.synchronize()
     assert torch.equal(y, (q.float() * s[:, None]).to(dtype))
+
+
+@pytest.mark.parametrize("width", [33, 256, 1000, 2048, 8192, 20001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_definitions_own_bits(width, dtype):
+    """q = rint(t * (127 / m)), every operation in fp32, also of numbers that lie on halves of a step; and scales without a norm are m / 127.  The quotients are taken in 64
+    bits and rounded, which is their fp32 rounding (53 >= 2 * 24 + 2); torch's own divisions by and of a number multiply by a reciprocal instead."""
+    g = torch.Generator(device="cuda").manual_seed(width)
+    x = torch.randn(40, width, generator=g, device="cuda")
+    x[20:] = torch.randint(-508, 509, (20, width), generator=g, device="cuda") / 4          # quarters of steps, where the largest is 127
+    x[20:, 0] = 127
+    x[20:].clamp_(-127, 127)
+    rows = rows_of(x, (width + 15) // 16 * 16, dtype)
+    w = torch.randn(width, generator=g, device="cuda")
+    for weights in (None, w):
+        q, s = norm(rows.clone(), None, weights, width, (width + 15) // 16 * 16)
+        t = rows[:, :width].float()
+        if weights is not None:
+            t = t * weights
+        m = t.abs().amax(1, keepdim=True)
+        assert torch.equal(q.float(), torch.round(t * (127 / m.double()).float()))
+        if weights is None:
+            assert torch.equal(s.float(), (m.double() / 127).float()[:, 0])
