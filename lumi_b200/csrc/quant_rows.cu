@@ -54,75 +54,49 @@ __device__ __forceinline__ void unpack(const Words<__nv_bfloat16, E>& w, float (
     }
 }
 // Of the norm's weights, which no store of the kernel changes: loads that may pass the stores of x, but not the dependency wait.
-template <bool RAGGED>
-__device__ __forceinline__ void load_weights(const float* p, int n, float& a, float& b, float& c, float& d) {
-    a = b = c = d = 0.f;
-    if (RAGGED ? n >= 4 : n > 0) {
-        asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(a), "=f"(b), "=f"(c), "=f"(d) : "l"(p));
-    } else if (RAGGED) {
-        if (n > 0) a = p[0];
-        if (n > 1) b = p[1];
-        if (n > 2) c = p[2];
-    }
+__device__ __forceinline__ void load_weights(const float* p, float& a, float& b, float& c, float& d) {
+    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(a), "=f"(b), "=f"(c), "=f"(d) : "l"(p));
 }
-// The row ends n numbers from here (n <= 0: before); what is behind it is neither read nor counted.  RAGGED: it may end within these E.
-template <bool RAGGED, typename T, int E>
-__device__ __forceinline__ void load_some(const T* p, int n, Words<T, E>& w) {
+// The row ends n numbers from here.  Numbers are taken E at a time where a row has that many; those behind the last whole E (`tail`s, up to seven) go to the first
+// threads of the row, one each.  What is behind a row is neither read nor written.
+template <typename T, int E>
+__device__ __forceinline__ void load_whole(const T* p, int n, Words<T, E>& w) {
     constexpr int N = E * (int)sizeof(T) / 4;
 #pragma unroll
     for (int i = 0; i < N; ++i) w.u[i] = 0;
-    if (RAGGED ? n >= E : n > 0) {
-        if constexpr (N == 2) {
-            const uint2 t = *reinterpret_cast<const uint2*>(p);
-            w.u[0] = t.x; w.u[1] = t.y;
-        } else {
+    if (n < E) return;
+    if constexpr (N == 2) {
+        const uint2 t = *reinterpret_cast<const uint2*>(p);
+        w.u[0] = t.x; w.u[1] = t.y;
+    } else {
 #pragma unroll
-            for (int i = 0; i < N / 4; ++i) {
-                const uint4 t = reinterpret_cast<const uint4*>(p)[i];
-                w.u[4 * i] = t.x; w.u[4 * i + 1] = t.y; w.u[4 * i + 2] = t.z; w.u[4 * i + 3] = t.w;
-            }
-        }
-    } else if (RAGGED && n > 0) {
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int i = 0; i < E; ++i) if (i < n) w.u[i] = reinterpret_cast<const uint32_t*>(p)[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < E; ++i) if (i < n) w.u[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
+        for (int i = 0; i < N / 4; ++i) {
+            const uint4 t = reinterpret_cast<const uint4*>(p)[i];
+            w.u[4 * i] = t.x; w.u[4 * i + 1] = t.y; w.u[4 * i + 2] = t.z; w.u[4 * i + 3] = t.w;
         }
     }
 }
+__device__ __forceinline__ float number(const float* p) { return *p; }
+__device__ __forceinline__ float number(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void put_one(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put_one(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ float stored(float v, const float*) { return v; }
 __device__ __forceinline__ float stored(float v, const __nv_bfloat16*) { return __bfloat162float(__float2bfloat16_rn(v)); }
-template <bool RAGGED, int E>
-__device__ __forceinline__ void store_some(float* p, int n, const float (&v)[E]) {
-    if (RAGGED ? n >= E : n > 0) {
+template <int E>
+__device__ __forceinline__ void store_whole(float* p, const float (&v)[E]) {
 #pragma unroll
-        for (int i = 0; i < E / 4; ++i) *reinterpret_cast<float4*>(p + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        return;
-    }
-    if (RAGGED)
-#pragma unroll
-        for (int i = 0; i < E; ++i) if (i < n) p[i] = v[i];
+    for (int i = 0; i < E / 4; ++i) *reinterpret_cast<float4*>(p + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
 }
-template <bool RAGGED, int E>
-__device__ __forceinline__ void store_some(__nv_bfloat16* p, int n, const float (&v)[E]) {
+template <int E>
+__device__ __forceinline__ void store_whole(__nv_bfloat16* p, const float (&v)[E]) {
     static_assert(E == 8, "");
-    if (RAGGED ? n >= E : n > 0) {
-        uint32_t u[4];
+    uint32_t u[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-            u[i] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-        *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
-        return;
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        u[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
-    if (RAGGED)
-#pragma unroll
-        for (int i = 0; i < E; ++i) if (i < n) p[i] = __float2bfloat16_rn(v[i]);
+    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
 }
 
 // ---- sources of rows: load(): what memory holds of E numbers; values(): the numbers to be held in 8 bits, with the sum of squares
@@ -135,9 +109,10 @@ __device__ __forceinline__ void store_some(__nv_bfloat16* p, int n, const float 
 // kStay: as many blocks as run at once stay for row after row, the next one's loads ahead of this one's reduction.  It wins where a row is few bytes and has a residual's
 //   sum to write (bf16, 16384 x 2048: 41 against 59), and loses elsewhere: the registers cost more blocks (gate of 32768 x 2816 bf16 rows: 94 against 75).
 // Norm, or rows as they are.  ADD: x += o first, rounded to x's type, so that the norm sees what later readers of x see.
-template <typename XT, typename OT, bool ADD, bool NORM, bool RAGGED>
+// TAIL: widths are no multiples of E.
+template <typename XT, typename OT, bool ADD, bool NORM, bool TAIL>
 struct NormSource {
-    static constexpr bool kRagged = RAGGED;
+    static constexpr bool kTail = TAIL;
     static constexpr int E = sizeof(XT) == 4 ? 4 : 8;
     static constexpr bool kNorm = NORM, kStay = E == 8 && ADD;
     static constexpr int kEights = ADD ? 1 : (E == 8 ? 4 : 2), kWarp = E == 8 || !ADD ? 1024 : 512;
@@ -149,8 +124,8 @@ struct NormSource {
     struct Raw { Words<XT, E> x; std::conditional_t<ADD, Words<OT, E>, None> o; };
     template <bool AGAIN>
     __device__ __forceinline__ void load(long row, int c, Raw& r) const {
-        load_some<RAGGED>(x + row * ldx + c, width - c, r.x);
-        if constexpr (ADD && !AGAIN) load_some<RAGGED>(o + row * ldo + c, width - c, r.o);
+        load_whole(x + row * ldx + c, width - c, r.x);
+        if constexpr (ADD && !AGAIN) load_whole(o + row * ldo + c, width - c, r.o);
     }
     // AGAIN: x has been added to already
     template <bool AGAIN>
@@ -161,12 +136,17 @@ struct NormSource {
             unpack(r.o, add);
 #pragma unroll
             for (int i = 0; i < E; ++i) t[i] = stored(t[i] + add[i], x);
-            store_some<RAGGED, E>(x + row * ldx + c, width - c, t);
+            if (width - c >= E) store_whole<E>(x + row * ldx + c, t);
         }
         if constexpr (NORM) {
             float f[E];
+            if (width - c >= E) {
 #pragma unroll
-            for (int i = 0; i < E; i += 4) load_weights<RAGGED>(w + c + i, width - c - i, f[i], f[i + 1], f[i + 2], f[i + 3]);
+                for (int i = 0; i < E; i += 4) load_weights(w + c + i, f[i], f[i + 1], f[i + 2], f[i + 3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; ++i) f[i] = 0.f;
+            }
 #pragma unroll
             for (int i = 0; i < E; ++i) {
                 sum = fmaf(t[i], t[i], sum);
@@ -174,7 +154,25 @@ struct NormSource {
             }
         }
     }
-    // sum of squares of E numbers times k, from memory
+    // the same of one number
+    struct Tail { float x, o; };
+    template <bool AGAIN>
+    __device__ __forceinline__ void load_tail(long row, int c, Tail& r) const {
+        r.x = number(x + row * ldx + c);
+        if constexpr (ADD && !AGAIN) r.o = number(o + row * ldo + c);
+    }
+    template <bool AGAIN>
+    __device__ __forceinline__ float tail(long row, int c, const Tail& r, float& sum) const {
+        float v = r.x;
+        if constexpr (ADD && !AGAIN) {
+            v = stored(v + r.o, x);
+            put_one(x + row * ldx + c, v);
+        }
+        if constexpr (!NORM) return v;
+        sum = fmaf(v, v, sum);
+        return v * number(w + c);
+    }
+    // sums of squares of numbers times k, from memory
     __device__ __forceinline__ float squares(long row, int c, float k) const {
         Raw r;
         float v[E], part = 0.f;
@@ -184,12 +182,16 @@ struct NormSource {
         for (int i = 0; i < E; ++i) part = fmaf(v[i] * k, v[i] * k, part);
         return part;
     }
+    __device__ __forceinline__ float squares_tail(long row, int c, float k) const {
+        const float v = number(x + row * ldx + c) * k;
+        return v * v;
+    }
 };
 
 // Gate: rows hold gates, and from column `up` on as many ups.
-template <typename XT, bool SILU, bool RAGGED>
+template <typename XT, bool SILU, bool TAIL>
 struct GateSource {
-    static constexpr bool kRagged = RAGGED;
+    static constexpr bool kTail = TAIL;
     static constexpr int E = sizeof(XT) == 4 ? 4 : 8;
     static constexpr bool kNorm = false, kStay = false;
     static constexpr int kEights = E == 8 ? 4 : 1, kWarp = E == 8 ? 1024 : 512;
@@ -199,8 +201,8 @@ struct GateSource {
     struct Raw { Words<XT, E> g, u; };
     template <bool AGAIN>
     __device__ __forceinline__ void load(long row, int c, Raw& r) const {
-        load_some<RAGGED>(gu + row * ld + c, width - c, r.g);
-        load_some<RAGGED>(gu + row * ld + up + c, width - c, r.u);
+        load_whole(gu + row * ld + c, width - c, r.g);
+        load_whole(gu + row * ld + up + c, width - c, r.u);
     }
     template <bool AGAIN>
     __device__ __forceinline__ void values(long, int, const Raw& r, float (&t)[E], float&) const {
@@ -208,10 +210,19 @@ struct GateSource {
         unpack(r.g, t);
         unpack(r.u, u);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float z = fast_sigmoid(t[i]);
-            t[i] = (SILU ? t[i] * z : z) * u[i];
-        }
+        for (int i = 0; i < E; ++i) t[i] = gated(t[i], u[i]);
+    }
+    struct Tail { float g, u; };
+    template <bool AGAIN>
+    __device__ __forceinline__ void load_tail(long row, int c, Tail& r) const {
+        r.g = number(gu + row * ld + c);
+        r.u = number(gu + row * ld + up + c);
+    }
+    template <bool AGAIN>
+    __device__ __forceinline__ float tail(long, int, const Tail& r, float&) const { return gated(r.g, r.u); }
+    static __device__ __forceinline__ float gated(float gate, float v) {
+        const float z = fast_sigmoid(gate);
+        return (SILU ? gate * z : z) * v;
     }
 };
 
@@ -221,31 +232,28 @@ __device__ __forceinline__ void largest(const float (&t)[E], float& m) {
 #pragma unroll
     for (int i = 0; i < E; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(t[i])));
 }
+__device__ __forceinline__ void largest(float t, float& m) { asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(t))); }
 
 // t * inv, rounded to fp32, to the nearest integer, ties to even: added to 1.5 * 2^23, the integer is the sum's low byte.  (Without the first rounding a quotient that lies on a half
 // falls to the side that the reciprocal's error points to.)  Zeros where the row is not all numbers.
-template <bool RAGGED, int E>
+__device__ __forceinline__ uint32_t rounded(float t, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(t, inv), 12582912.f)); }
+template <int E>
 __device__ __forceinline__ void put(int8_t* q, int n, const float (&t)[E], float inv, bool numbers) {
     uint32_t b[E];
     if (numbers) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(t[i], inv), 12582912.f));
+        for (int i = 0; i < E; ++i) b[i] = rounded(t[i], inv);
     } else {
 #pragma unroll
         for (int i = 0; i < E; ++i) b[i] = 0;
     }
-    if (RAGGED ? n >= E : n > 0) {
-        uint32_t u[E / 4];
+    if (n < E) return;
+    uint32_t u[E / 4];
 #pragma unroll
-        for (int i = 0; i < E / 4; ++i)
-            u[i] = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410);
-        if constexpr (E == 8) *reinterpret_cast<uint2*>(q) = make_uint2(u[0], u[1]);
-        else *reinterpret_cast<uint32_t*>(q) = u[0];
-        return;
-    }
-    if (RAGGED)
-#pragma unroll
-        for (int i = 0; i < E; ++i) if (i < n) q[i] = (int8_t)b[i];
+    for (int i = 0; i < E / 4; ++i)
+        u[i] = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410);
+    if constexpr (E == 8) *reinterpret_cast<uint2*>(q) = make_uint2(u[0], u[1]);
+    else *reinterpret_cast<uint32_t*>(q) = u[0];
 }
 
 // Sum (SUM) and maximum over the threads of a row: a warp's, or the block's.  turn counts a block's reductions.
@@ -299,35 +307,46 @@ __global__ void __launch_bounds__(NT) quant_wide_kernel(SRC src, QuantOut out) {
     const long row = blockIdx.x;
     pdl_release();
     pdl_sync();
-    float sum = 0.f;
-    float m = 0.f;
+    const int whole = src.width / E * E, tail_at = whole + threadIdx.x;
+    const bool has_tail = SRC::kTail && tail_at < src.width;
+    float sum = 0.f, m = 0.f;
     uint32_t turn = 0;
-    for (int c = threadIdx.x * E; c < src.width; c += NT * E) {
+    for (int c = threadIdx.x * E; c < whole; c += NT * E) {
         typename SRC::Raw r;
         float t[E];
         src.template load<false>(row, c, r);
         src.template values<false>(row, c, r, t, sum);
         largest<E>(t, m);
     }
+    typename SRC::Tail r1{};
+    if (has_tail) {
+        src.template load_tail<false>(row, tail_at, r1);
+        largest(src.template tail<false>(row, tail_at, r1, sum), m);
+    }
     reduce_row<false, SRC::kNorm>(sum, m, turn);
     const bool numbers = m < __uint_as_float(kInfBits);
     Factor f{0.f, 1.f};
     if constexpr (SRC::kNorm)
         f = norm_sum(sum, src.eps, [&](float k) {
-            float part = 0.f;
-            float unused = 0.f;
-            for (int c = threadIdx.x * E; c < src.width; c += NT * E) part += src.squares(row, c, k);
+            float part = has_tail ? src.squares_tail(row, tail_at, k) : 0.f, unused = 0.f;
+            for (int c = threadIdx.x * E; c < whole; c += NT * E) part += src.squares(row, c, k);
             reduce_row<false, true>(part, unused, turn);
             return part;
         });
     const float top = fmaxf(m, kLeast), inv = __fdiv_rn(127.f, top);
     if (threadIdx.x == 0) out.scale[row] = row_scale(src, f, numbers, top);
-    for (int c = threadIdx.x * E; c < src.width; c += NT * E) {
+    int8_t* const q = out.q + row * out.ldq;
+    float unused = 0.f;
+    for (int c = threadIdx.x * E; c < whole; c += NT * E) {
         typename SRC::Raw r;
-        float t[E], unused = 0.f;
+        float t[E];
         src.template load<true>(row, c, r);
         src.template values<true>(row, c, r, t, unused);
-        put<SRC::kRagged, E>(out.q + row * out.ldq + c, src.width - c, t, inv, numbers);
+        put<E>(q + c, E, t, inv, numbers);
+    }
+    if (has_tail) {
+        src.template load_tail<true>(row, tail_at, r1);
+        q[tail_at] = numbers ? (int8_t)rounded(src.template tail<true>(row, tail_at, r1, unused), inv) : 0;
     }
 }
 
@@ -343,36 +362,47 @@ __global__ void __launch_bounds__(WARP ? 128 : 512, SRC::E == 8 && !WARP ? 2 : 1
     pdl_release();
     pdl_sync();
     if (row >= rows) return;                              // whole warps, and only where a row is a warp's
+    const int tail_at = src.width / E * E + tid;
+    const bool has_tail = SRC::kTail && tail_at < src.width;
     typename SRC::Raw r[NC];
+    typename SRC::Tail r1{};
 #pragma unroll
     for (int i = 0; i < NC; ++i) src.template load<false>(row, (i * NT + tid) * E, r[i]);
+    if (has_tail) src.template load_tail<false>(row, tail_at, r1);
     for (; row < rows; row += step) {
-        float sum = 0.f, t[NC][E], m = 0.f;
+        float sum = 0.f, t[NC][E], m = 0.f, t1 = 0.f;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             src.template values<false>(row, (i * NT + tid) * E, r[i], t[i], sum);
             largest<E>(t[i], m);
         }
-        if (SRC::kStay && row + step < rows)
+        if (has_tail) {
+            t1 = src.template tail<false>(row, tail_at, r1, sum);
+            largest(t1, m);
+        }
+        if (SRC::kStay && row + step < rows) {
 #pragma unroll
             for (int i = 0; i < NC; ++i) src.template load<false>(row + step, (i * NT + tid) * E, r[i]);
+            if (has_tail) src.template load_tail<false>(row + step, tail_at, r1);
+        }
         reduce_row<WARP, SRC::kNorm>(sum, m, turn);
         const bool numbers = m < __uint_as_float(kInfBits);
         Factor f{0.f, 1.f};
         if constexpr (SRC::kNorm)
             f = norm_sum(sum, src.eps, [&](float k) {
-                float part = 0.f;
-                float unused = 0.f;
+                float part = has_tail ? src.squares_tail(row, tail_at, k) : 0.f, unused = 0.f;
                 for (int i = 0; i < NC; ++i) part += src.squares(row, (i * NT + tid) * E, k);
                 reduce_row<WARP, true>(part, unused, turn);
                 return part;
             });
         const float top = fmaxf(m, kLeast), inv = __fdiv_rn(127.f, top);
+        int8_t* const q = out.q + row * out.ldq;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             const int c = (i * NT + tid) * E;
-            put<SRC::kRagged, E>(out.q + row * out.ldq + c, src.width - c, t[i], inv, numbers);
+            put<E>(q + c, src.width - c, t[i], inv, numbers);
         }
+        if (has_tail) q[tail_at] = numbers ? (int8_t)rounded(t1, inv) : 0;
         if (tid == 0) out.scale[row] = row_scale(src, f, numbers, top);      // by one thread: its divisions and root take longer than a row's numbers
         if constexpr (!SRC::kStay) break;
     }
@@ -401,7 +431,7 @@ int32_t launch_rows_of(const SRC& src, const QuantOut& out, int rows, cudaStream
         regs = at.numRegs;
         registers.store(regs, std::memory_order_relaxed);
     }
-    const int chunks = (src.width + SRC::E - 1) / SRC::E, threads = WARP ? 128 : ((chunks + NC - 1) / NC + 31) / 32 * 32;
+    const int chunks = std::max(1, src.width / SRC::E), threads = WARP ? 128 : ((chunks + NC - 1) / NC + 31) / 32 * 32;
     // as many blocks as run at once; registers are given out by eights per thread
     const int per_sm = std::max(1, std::min({32, 2048 / threads, 65536 / ((regs + 7) / 8 * 8 * threads)}));
     const long blocks = WARP ? ((long)rows + 3) / 4 : rows;
@@ -412,9 +442,9 @@ int32_t launch_rows_of(const SRC& src, const QuantOut& out, int rows, cudaStream
 }
 
 // Two eights of numbers per thread instead of four, where whole warps then leave fewer threads without numbers: 1536 columns are 192 eights, 64 threads of four or 96 of
-// two.  Gate of 32768 x 1536 bf16 rows 42 -> 37 us, 16384 x 2400 35 -> 31; rows that end within an eight are slower so (32768 x 1111 50 -> 54).
+// two.  Gate of 32768 x 1536 bf16 rows 42 -> 37 us, 16384 x 2400 35 -> 31.
 inline bool two_eights(int width) {
-    const int n = (width + 7) / 8;
+    const int n = width / 8;
     auto slots = [&](int per) { return ((n + per - 1) / per + 31) / 32 * 32 * per; };
     return 10 * slots(2) < 9 * slots(4);
 }
@@ -433,9 +463,7 @@ int32_t launch(const SRC& src, const QuantOut& out, int rows, cudaStream_t st) {
     if constexpr (SRC::kEights == 1) {
         if (width <= 256 * 8) return launch_rows_of<SRC, false, L>(src, out, rows, st);
     }
-    if constexpr (SRC::kEights <= 2 || !SRC::kRagged) {
-        if (width <= 512 * 16 && (SRC::kEights <= 2 || two_eights(width))) return launch_rows_of<SRC, false, 2 * L>(src, out, rows, st);
-    }
+    if (width <= 512 * 16 && (SRC::kEights <= 2 || two_eights(width))) return launch_rows_of<SRC, false, 2 * L>(src, out, rows, st);
     if (width <= 512 * 32) return launch_rows_of<SRC, false, 4 * L>(src, out, rows, st);
     cudaLaunchAttribute attr[1];
     const cudaLaunchConfig_t cfg = dependent_launch(dim3((unsigned)rows), 1024, attr, st);
@@ -450,12 +478,12 @@ int32_t launch_norm(uint64_t x, int ldx, uint64_t o, int ldo, uint64_t w, const 
         src.ldx = ldx; src.ldo = ldo; src.width = width; src.eps = eps;
         return launch(src, out, rows, st);
     };
-    auto ragged = [&](auto r) {
-        constexpr bool R = decltype(r)::value;
-        if (o) return w ? go(NormSource<XT, OT, true, true, R>{}) : go(NormSource<XT, OT, true, false, R>{});
-        return w ? go(NormSource<XT, XT, false, true, R>{}) : go(NormSource<XT, XT, false, false, R>{});
+    auto with_tail = [&](auto tail) {
+        constexpr bool T = decltype(tail)::value;
+        if (o) return w ? go(NormSource<XT, OT, true, true, T>{}) : go(NormSource<XT, OT, true, false, T>{});
+        return w ? go(NormSource<XT, XT, false, true, T>{}) : go(NormSource<XT, XT, false, false, T>{});
     };
-    return width % NormSource<XT, OT, true, true, true>::E != 0 ? ragged(std::true_type{}) : ragged(std::false_type{});
+    return width % NormSource<XT, OT, true, true, true>::E != 0 ? with_tail(std::true_type{}) : with_tail(std::false_type{});
 }
 
 // ---- rows back as numbers: y = q s.  A warp takes up to 1024 numbers of a row, 16 bytes of y per lane at a time.  ANY: rows of y begin anywhere, or end within
@@ -512,7 +540,7 @@ __global__ void __launch_bounds__(256) dequant_kernel(const int8_t* q, long ldq,
             float v[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = byte_value(u[i][e / 4], e & 3, s);
-            if (j < pieces) store_some<false, E>(y + head + j * E, E, v);
+            if (j < pieces) store_whole<E>(y + head + j * E, v);
         }
     }
 }
@@ -560,12 +588,12 @@ extern "C" int32_t lumi_k_gate_quant(uint64_t gu, int32_t dtype, int32_t ld, int
         src.ld = ld; src.up = up; src.width = width;
         return launch<SRC>(src, out, rows, st);
     };
-    auto ragged = [&](auto r) {
-        constexpr bool R = decltype(r)::value;
-        if (dtype == LUMI_DTYPE_F32) return act ? go(GateSource<float, true, R>{}) : go(GateSource<float, false, R>{});
-        return act ? go(GateSource<__nv_bfloat16, true, R>{}) : go(GateSource<__nv_bfloat16, false, R>{});
+    auto with_tail = [&](auto tail) {
+        constexpr bool T = decltype(tail)::value;
+        if (dtype == LUMI_DTYPE_F32) return act ? go(GateSource<float, true, T>{}) : go(GateSource<float, false, T>{});
+        return act ? go(GateSource<__nv_bfloat16, true, T>{}) : go(GateSource<__nv_bfloat16, false, T>{});
     };
-    return width % (dtype == LUMI_DTYPE_F32 ? 4 : 8) != 0 ? ragged(std::true_type{}) : ragged(std::false_type{});
+    return width % (dtype == LUMI_DTYPE_F32 ? 4 : 8) != 0 ? with_tail(std::true_type{}) : with_tail(std::false_type{});
 }
 
 extern "C" int32_t lumi_k_dequant_rows(uint64_t q, int32_t ldq, uint64_t scale, uint64_t y, int32_t y_dtype, int32_t ldy, int32_t rows, int32_t width,
