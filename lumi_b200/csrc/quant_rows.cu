@@ -7,7 +7,7 @@
 //
 // What bounds them is memory: each number is read once and written once.  Arithmetic comes close where rows are bf16: the norm of 8192 x 4096 rows without a residual
 // (3 bytes per number, about 10 instructions) takes 21 us where DRAM takes 15.  Against rates that a plain copy reaches (6.55 TB/s): norm of 32768 x 1024 fp32 rows with a
-// residual 66 us, 101 %; gate of 32768 x 2816 bf16 rows 71 us, 99 %; these back as bf16 46 us, 93 %.  One row takes 1.7 us, which is its launch.
+// residual 66 us, 101 %; gate of 32768 x 2816 bf16 rows 72 us, 97 %; these back as bf16 45 us, 93 %.  One row takes 1.8 us, which is its launch.
 #include "device_args.h"
 #include "rows.cuh"
 
