@@ -528,16 +528,17 @@ __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUten
 // ---- many rows: pairs of CTAs ------------------------------------------------------------------------
 // Two CTAs of a cluster (two SMs) take tiles of 256 rows of W and `cols` rows of A (cta_group::2): each stages its 128 rows of W and half of the rows of A, the
 // first one issues the MMAs for both, each finishes its own rows of W.  Persistent, with two accumulators: a tile is finished while the next is multiplied.
-// Tiles go in blocks of 16 tiles of rows of A, rows of W by rows of W within a block, so that both operands come out of L2.
+// Tiles go in blocks of four tiles of rows of A, rows of W by rows of W within a block, so that both operands come out of L2 (back to back for a second, in blocks of 16 / 8 / 4 / 2:
+// 8192 x 2048 x 8448 into an fp32 stream 117 / 114 / 112 / 113 us, 8192 x 8192 x 4096 189 / 192 / 190 / 189, of 64: 135 for the first).
 // Warp 0: copies.  Warp 1: TMEM and MMA.  Warps 2 to 9: accumulators, two warps per quarter of the lanes, strips of 32 columns in turn.
 //
 // Results go through shared memory to tensor-map stores where D's rows allow it, old values of D come the same way, asked for a strip ahead (4096 x 7360 x 1024 into fp32: 51 us; by
 // single loads 71).  The arrival that gives an accumulator back is relaxed: as a release it waited for the results to reach memory (4096 x 7360 x 1024 35 -> 29 us).  Copies and MMAs are issued
 // by whole warps with one lane elected (29 -> 28 us; 8192 x 8192 x 8192 325 -> 316).
 //
-// What bounds it, 10^12 operations a second (twice the measured bf16 rate: 3342): 8192 x 8192 x 8192 3520, the tensor cores; 8192 x 2048 x 8448 into an fp32 stream 2890; at short K the
+// What bounds it, 10^12 operations a second (twice the measured bf16 rate: 3342): 8192 x 8192 x 8192 3520, the tensor cores; 8192 x 2048 x 8448 into an fp32 stream 3020; at short K the
 // shared memory, which operands, their copies and the results share: 4096 x 7360 x 1024 2360 (26 us; 28 with the results of a bf16 strip put one by one), and 2950 with the results left
-// out.  Called back to back for a second, the power limit takes the clock from 1.97 to 1.55 GHz there (32 us) and to 1.3 GHz at long K (8192 x 2048 x 8448: 98 -> 117 us).
+// out.  Called back to back for a second, the power limit takes the clock from 1.97 to 1.55 GHz there (32 us) and to 1.3 GHz at long K (8192 x 2048 x 8448: 94 -> 111 us).
 constexpr int kPairThreads = 320;
 struct PairTail {
     uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], drain;
@@ -546,7 +547,7 @@ struct PairTail {
     alignas(16) float scales[8][32];
 };
 static_assert(sizeof(PairTail) <= kTailBytes, "tail of the shared memory");
-constexpr int kBlockTiles = 16;
+constexpr int kBlockTiles = 4;
 
 // staged: results (and old values) travel by tensor-map copies, which want D's rows to begin and end on 16-byte boundaries
 struct PairShape { int cols, stages, tiles_a, tiles, staged; };
