@@ -381,7 +381,7 @@ int32_t lumi_k_dequant_rows(uint64_t q, int32_t ldq, uint64_t scale, uint64_t y,
  * integers (-128 is allowed), sums in 32-bit integers and so exact, the rest in fp32, rounded once to D's type (d_dtype LUMI_DTYPE_*, rows of ldd
  * elements; no alignment beyond the element's).  bias may be 0.  K <= 131071, M and N <= 2^30 (LUMI_E_UNSUPPORTED beyond; longer sums could overflow); lda and ldw are
  * multiples of 16, a and w 16-byte aligned; D overlaps none of the operands.  status: a device int32 or 0; a bounded wait on the device that gave up
- * sets the bit 4 of it and leaves NaN in the results that it cost. */
+ * sets its bit of value 4 and leaves NaN in the results that it cost. */
 int32_t lumi_k_gemm_i8(uint64_t a, int32_t lda, uint64_t a_scale, uint64_t w, int32_t ldw, uint64_t w_scale, uint64_t bias, uint64_t d, int32_t d_dtype,
                        int32_t ldd, int32_t M, int32_t N, int32_t K, int32_t accumulate, uint64_t status, uint64_t stream);
 

@@ -349,6 +349,46 @@ __device__ __forceinline__ void finish_strip(const I8Args& g, uint32_t acc, cons
     else finish_columns<false, DT>(g, sum, a_scale, d, live, in, sw, bias);
 }
 
+// The same for a kernel that knows whether it adds, with old values that were asked for ahead: `old` has this strip's and then takes the next one's, from m_next on (-1: there is none).
+template <typename DT>
+__device__ __forceinline__ void load_old(const I8Args& g, int m0, int n, float (&old)[32]) {
+    const int live = n < g.N ? g.M - m0 : 0;
+    const DT* p = (const DT*)g.d + (long)m0 * g.ldd + n;
+#pragma unroll
+    for (int j = 0; j < 32; ++j, p += g.ldd) old[j] = j < live ? old_value(p) : 0.f;
+}
+template <bool ADD, typename DT>
+__device__ __forceinline__ void tile_strip(const I8Args& g, uint32_t acc, const float* a_scale, int m0, int n, float sw, float bias, float (&old)[32], int m_next) {
+    const int live = n < g.N ? g.M - m0 : 0;
+    DT* d = (DT*)g.d + (long)m0 * g.ldd + n;
+    uint32_t sum[32];
+    tmem_ld32(acc, sum);
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) shared_load4(smem_u32(a_scale), v, j);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = scaled((int)sum[j], v[j], sw, bias);
+    if constexpr (ADD) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __fadd_rn(v[j], old[j]);
+        if (m_next >= 0) load_old<DT>(g, m_next, n, old);
+    }
+    if (live >= 32) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j, d += g.ldd) put_value(d, v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j, d += g.ldd) if (j < live) put_value(d, v[j]);
+    }
+}
+// Results that a lost wait cost.
+template <typename DT>
+__device__ __forceinline__ void lose_strip(const I8Args& g, int m0, int n) {
+    if (n < g.N)
+#pragma unroll 1
+        for (int m = m0; m < min(m0 + 32, g.M); ++m) put_value((DT*)g.d + (long)m * g.ldd + n, __uint_as_float(0x7fffffffu));
+}
+
 struct TileTail {
     uint64_t full[kMaxStages], empty[kMaxStages], done, drain;
     uint32_t tmem_slot;
@@ -364,8 +404,8 @@ struct TileShape { int cols, stages, splits; };
 // Warp 0: copies.  Warp 1: TMEM and MMA.  All eight: accumulators (warp w reads the lanes of quarter w % 4, strips of 32 columns in turn).
 // What bounds it is a chain: launch and barriers, the first copies, 0.19 us per k-block (a wait, four MMAs, a commit; issued by one lane in a branch of its own it took 0.25, with
 // descriptors composed anew 0.29; copies by two threads or sums in turn in four accumulators changed nothing), the results.  203 x 2053 x 1111: 4.3 us, DRAM's floor 0.5.
-template <typename DT>
-__global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, I8Args g, TileShape sh) {
+template <typename DT, bool ADD>
+__global__ void __launch_bounds__(256, 2) tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, I8Args g, TileShape sh) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int S = sh.stages, cols = sh.cols, splits = sh.splits, stage = kWBytes + cols * kBlockK;
@@ -454,12 +494,15 @@ __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUten
     DT* const d = (DT*)g.d + (long)mine * g.ldd + n;
     auto old_of = [&](int r, float (&o)[4]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = g.accumulate && n < g.N && r + e < RB && mine + r + e < g.M ? old_value(d + (r + e) * g.ldd) : 0.f;
+        for (int e = 0; e < 4; ++e) o[e] = ADD && n < g.N && r + e < RB && mine + r + e < g.M ? old_value(d + (r + e) * g.ldd) : 0.f;
     };
     float ahead[4] = {0.f, 0.f, 0.f, 0.f};
+    float old[32];                                                      // K not shared: of this warp's next strip
     if (splits > 1) {
         old_of(4 * half, ahead);
         cluster_wait();                                                 // every CTA of the cluster runs
+    } else if (ADD) {
+        load_old<DT>(g, m0 + half * 32, n, old);
     }
     __syncthreads();                                                    // the rows' scales are there
     if (!wait_for(&tl.done, 0, g.wait_ns)) timed_out = true;
@@ -471,7 +514,8 @@ __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUten
 #pragma unroll 1
         for (int cb = half; cb < cols / 32; cb += 2) {
             if (m0 + cb * 32 >= g.M) break;
-            finish_strip<DT>(g, lanes + (uint32_t)(cb * 32), tl.a_scale + cb * 32, m0 + cb * 32, n, sw, bias, lost);
+            if (lost) lose_strip<DT>(g, m0 + cb * 32, n);
+            else tile_strip<ADD, DT>(g, lanes + (uint32_t)(cb * 32), tl.a_scale + cb * 32, m0 + cb * 32, n, sw, bias, old, cb + 2 < cols / 32 ? m0 + (cb + 2) * 32 : -1);
         }
     } else {
         if (lost) {
@@ -519,7 +563,7 @@ __global__ void __launch_bounds__(256) tile_kernel(const __grid_constant__ CUten
         const float v[4] = {scaled(sum.x, sa.x, sw, bias), scaled(sum.y, sa.y, sw, bias), scaled(sum.z, sa.z, sw, bias), scaled(sum.w, sa.w, sw, bias)};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            if (mine + r + e < g.M) put_value(d + (r + e) * g.ldd, any_lost ? __uint_as_float(0x7fffffffu) : (g.accumulate ? __fadd_rn(v[e], ahead[e]) : v[e]));
+            if (mine + r + e < g.M) put_value(d + (r + e) * g.ldd, any_lost ? __uint_as_float(0x7fffffffu) : (ADD ? __fadd_rn(v[e], ahead[e]) : v[e]));
             ahead[e] = next[e];
         }
     }
@@ -950,17 +994,17 @@ TileShape tile_shape(const I8Args& g) {
     return best;
 }
 
-template <typename DT>
+template <typename DT, bool ADD>
 int32_t launch_tile(const I8Args& g, const TileShape& sh, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
     CUtensorMap ma, mw;
     LUMI_TRY(make_i8_map(&ma, g.a, g.lda, g.M, g.K, sh.cols));
     LUMI_TRY(make_i8_map(&mw, g.w, g.ldw, g.N, g.K, kWRows));
-    LUMI_TRY(allow_smem((const void*)tile_kernel<DT>, ready));
+    LUMI_TRY(allow_smem((const void*)tile_kernel<DT, ADD>, ready));
     const int part = sh.splits > 1 ? sh.cols * kWRows * 4 : 0;
     Launch l(dim3((unsigned)((g.N + kWRows - 1) / kWRows * sh.splits), (unsigned)((g.M + sh.cols - 1) / sh.cols)), 256,
              sh.stages * (kWBytes + sh.cols * kBlockK) + part + kTailBytes + 1024, sh.splits, st);
-    LUMI_CUDA(cudaLaunchKernelEx(&l.cfg, tile_kernel<DT>, ma, mw, g, sh));
+    LUMI_CUDA(cudaLaunchKernelEx(&l.cfg, tile_kernel<DT, ADD>, ma, mw, g, sh));
     return LUMI_OK;
 }
 
@@ -1001,7 +1045,8 @@ template <typename DT>
 int32_t launch_product(const I8Args& g, cudaStream_t st) {
     if (g.M <= 2 || (g.M <= kFewRows && g.K <= kFewK && (long)g.N * g.K <= kFewBytes)) return launch_few<DT>(g, st);
     const TileShape sh = tile_shape(g);
-    return sh.cols != 0 ? launch_tile<DT>(g, sh, st) : launch_pair<DT>(g, pair_cols(g), st);
+    if (sh.cols == 0) return launch_pair<DT>(g, pair_cols(g), st);
+    return g.accumulate ? launch_tile<DT, true>(g, sh, st) : launch_tile<DT, false>(g, sh, st);
 }
 
 }  // namespace
