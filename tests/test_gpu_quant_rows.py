@@ -273,3 +273,33 @@ def test_the_definitions_own_bits(width, dtype):
         assert torch.equal(q.float(), torch.round(t * (127 / m.double()).float()))
         if weights is None:
             assert torch.equal(s.float(), (m.double() / 127).float()[:, 0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [16, 704, 4096, 20000])
+def test_gates_far_from_zero(dtype, width):
+    """Gates at +-100, +-88, +-30 and, for the sigmoid, infinite ones: open or closed, and closed to zero.  (Below -16 the gate's relative error grows to |gate| 2^-23, of numbers
+    under e^-16 of the row's largest: nothing beside half a step.)  An open silu of an infinity is an infinity: that row is NaN, and its neighbours are not."""
+    g = torch.Generator(device="cuda").manual_seed(width)
+    some = torch.tensor([-100.0, -88, -30, -17, 0, 17, 30, 88, 100, -1000], device="cuda")
+    gate = some[torch.randint(0, 10, (4, width), generator=g, device="cuda")]
+    ups = torch.randn(4, width, generator=g, device="cuda")
+    gate[:, 0], ups[:, 0] = 100, 1
+    for act in (0, 1):
+        z = gate.clone()
+        if act == 0:
+            z[1, 1], z[2, 2] = float("-inf"), float("inf")
+        else:
+            z[2, 2] = float("inf")
+            ups[2, 2] = 1
+        gu = torch.cat([z, ups], 1).to(dtype).contiguous()
+        q = torch.zeros(4, (width + 15) // 16 * 16, device="cuda", dtype=torch.int8)
+        s = torch.zeros(4, device="cuda")
+        call("lumi_k_gate_quant", gu.data_ptr(), code(gu), 2 * width, width, act, q.data_ptr(), q.stride(0), s.data_ptr(), 4, width, 0)
+        torch.cuda.synchronize()
+        zd, ud = gu[:, :width].double(), gu[:, width:].double()
+        t = torch.sigmoid(zd) * ud * (zd if act else 1)
+        keep = [0, 1, 2, 3] if act == 0 else [0, 1, 3]
+        check(q[keep][:, :width].double(), s[keep].double(), t[keep], torch.ones(len(keep), 1, device="cuda", dtype=torch.float64), 2.0 ** -18)
+        if act == 1:
+            assert bool(torch.isnan(s[2])) and bool((q[2] == 0).all())
