@@ -282,9 +282,6 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_ahi, const __grid
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int num_kb = K / BK;
 
-    // A successor launched with programmatic dependent launch may become resident now and run the part of its
-    // prologue that does not depend on this kernel (the state step requests its state tiles there).
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (status != nullptr && (*reinterpret_cast<volatile int32_t*>(status) & STATUS_TIMEOUT)) {
         if constexpr (PAIR) ntiles = 0;           // no work, but the cluster's barriers are taken
         else return;
@@ -312,6 +309,10 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_ahi, const __grid
     if constexpr (PAIR) { __syncwarp(); cluster_arrive(); cluster_wait(); }      // the other CTA's barriers exist, its TMEM is allocated
     else __syncthreads();
     tc_fence_after();
+    // A successor launched with programmatic dependent launch may become resident now and run the part of its
+    // prologue that does not depend on this kernel (the state step requests its state tiles there).  Behind the allocation: a successor
+    // may want TMEM too, and would keep it while it waits for this kernel.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
     // Launched with programmatic dependent launch (small batches), this CTA may have become resident and done all of the
     // above — barrier set-up, TMEM allocation — while its predecessor (the state step) still ran; everything below reads
