@@ -438,11 +438,12 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const __grid_constant__ CU
     if (splits > 1) cluster_arrive();                                   // "this CTA runs": sums may be sent to it
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tl.tmem_slot);
     bool timed_out = false;
+    int issued = 0;                                                     // (warp 0) k-blocks whose copies are on their way or have landed
     pdl_sync();
 
     if (warp == 0) {
         if ((int)(blockIdx.y * gridDim.x + blockIdx.x) != g.skip_unit) {
-            int s = 0, issued = 0;
+            int s = 0;
             uint32_t ph = 0;
             for (int i = 0; i < nkb; ++i) {
                 if (!__all_sync(0xffffffffu, wait_for(&tl.empty[s], ph ^ 1u, g.wait_ns))) { timed_out = true; break; }
@@ -455,8 +456,6 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const __grid_constant__ CU
                 issued = i + 1;
                 if (++s == S) { s = 0; ph ^= 1u; }
             }
-            if (timed_out)                                              // let the copies land (bounded) that nobody may consume
-                for (int i = max(0, issued - S); i < issued; ++i) wait_for(&tl.full[i % S], (uint32_t)(i / S) & 1u, g.wait_ns);
         }
     } else if (warp == 1) {
         const uint32_t idesc = i8_idesc(kWRows, cols), units = (uint32_t)stage >> 4;
@@ -478,7 +477,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const __grid_constant__ CU
         }
         if (timed_out && elect_one()) {                                 // let every MMA issued so far finish (bounded), then pass the word on
             umma_commit(&tl.drain);
-            wait_for(&tl.drain, 0, g.wait_ns);
+            wait_for(&tl.drain, 0, kWaitLimitNs);
             *reinterpret_cast<volatile int*>(&tl.lost) = 1;
             mbar_arrive(&tl.done);
         }
@@ -505,7 +504,8 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const __grid_constant__ CU
         load_old<DT>(g, m0 + half * 32, n, old);
     }
     __syncthreads();                                                    // the rows' scales are there
-    if (!wait_for(&tl.done, 0, g.wait_ns)) timed_out = true;
+    // (the warp that issued the MMAs frees their TMEM below: it does not go by a caller's shorter limit)
+    if (!wait_for(&tl.done, 0, warp == 1 ? max(g.wait_ns, kWaitLimitNs) : g.wait_ns)) timed_out = true;
     timed_out = __any_sync(0xffffffffu, timed_out);                     // tcgen05.ld below is warp-collective
     const bool lost = timed_out || *reinterpret_cast<volatile int*>(&tl.lost) != 0;
     tc_fence_after();
@@ -544,10 +544,13 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const __grid_constant__ CU
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
     }
     if (timed_out && g.status != nullptr) atomicOr(g.status, STATUS_TIMEOUT);
+    const bool any_lost = *reinterpret_cast<volatile int*>(&tl.lost) != 0;
+    // copies that no MMA waited for land (bounded) before this CTA's memory goes away, whichever of its waits ran out
+    if (any_lost && warp == 0)
+        for (int i = max(0, issued - S); i < issued; ++i) wait_for(&tl.full[i % S], (uint32_t)(i / S) & 1u, kWaitLimitNs);
     if (splits == 1) return;
 
     // ---- the rows of A that this CTA finishes
-    const bool any_lost = *reinterpret_cast<volatile int*>(&tl.lost) != 0;
     if (n >= g.N) return;
     for (int r = 4 * half; r < RB; r += 8) {
         if (mine + r >= g.M) break;
