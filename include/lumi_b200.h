@@ -386,7 +386,8 @@ int32_t lumi_k_gemm_i8(uint64_t a, int32_t lda, uint64_t a_scale, uint64_t w, in
                        int32_t ldd, int32_t M, int32_t N, int32_t K, int32_t accumulate, uint64_t status, uint64_t stream);
 
 /* Failure-path test hook of that product: waits limited to wait_limit_ns, the operands of tile skip_unit (-1: none; in launch order, a pair's second CTA's) never
- * arrive.  status: a zeroed device int32.  Returns LUMI_E_TIMEOUT when a wait gave up; the kernel has then returned cleanly and further calls work.  (Up to eight
+ * arrive; skip_unit = -2 - t: everything arrives, but of tile t one wait runs out at once (the one in front of its MMAs; a pair's: of one of the second CTA's warps that finish
+ * it).  status: a zeroed device int32.  Returns LUMI_E_TIMEOUT when a wait gave up; the kernel has then returned cleanly and further calls work.  (Up to eight
  * rows may have kernels without waits.)  Synchronises the default stream. */
 int32_t lumi_debug_gemm_i8_wait_timeout(uint64_t a, int32_t lda, uint64_t a_scale, uint64_t w, int32_t ldw, uint64_t w_scale, uint64_t d, int32_t d_dtype,
                                         int32_t ldd, int32_t M, int32_t N, int32_t K, int32_t accumulate, uint64_t wait_limit_ns, int32_t skip_unit, uint64_t status);

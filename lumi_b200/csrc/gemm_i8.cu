@@ -32,6 +32,7 @@ struct I8Args {
     int32_t* status;
     uint64_t wait_ns;
     int skip_unit;                           // failure tests: operands of this tile never arrive
+    int give_up;                             // failure tests: a wait of this tile runs out at once (tile_kernel: the MMA warp's first; pair_kernel: one finishing warp's for the sums)
 };
 
 __device__ __forceinline__ float old_value(const float* p) { return *p; }
@@ -462,7 +463,9 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const __grid_constant__ CU
         const uint64_t w0 = make_smem_desc(smem_u32(base)), a0 = make_smem_desc(smem_u32(base) + kWBytes);
         int s = 0;
         uint32_t ph = 0;
-        for (int i = 0; i < nkb; ++i) {
+        timed_out = (int)(blockIdx.y * gridDim.x + blockIdx.x) == g.give_up;
+        const int steps = timed_out ? 0 : nkb;
+        for (int i = 0; i < steps; ++i) {
             if (!__all_sync(0xffffffffu, wait_for(&tl.full[s], ph, g.wait_ns))) { timed_out = true; break; }
             tc_fence_after();
             if (elect_one()) {
@@ -752,16 +755,18 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
 #pragma unroll
             for (int i = 0; i < kMaxCols / 64; ++i) sa[i] = next_a[i];
             // after a wait that ran out, this tile and all that follow are left as NaN
-            if (!timed_out && !wait_for(&tl.acc_full[as], aph, g.wait_ns)) timed_out = true;
+            if (!timed_out && ((t == g.give_up && warp == 2 && rank == 1) || !wait_for(&tl.acc_full[as], aph, g.wait_ns))) timed_out = true;
             timed_out = __any_sync(0xffffffffu, timed_out);             // tcgen05.ld is warp-collective
             tc_fence_after();
             const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + as * kMaxCols;
             ask(t + at_once);
             auto column = [&](int i) { return (uint32_t)(half + 2 * i) * 32u; };
-            auto release = [&]() {                                      // this warp has read its share of the accumulator
+            // This warp has read its share of the accumulator.  After a lost wait it stays silent: it runs ahead of the others, and its arrivals would stand in for theirs, so that an
+            // accumulator were written that they still read.  The MMAs' wait for it then runs out too.
+            auto release = [&]() {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_relaxed(map_to_rank(smem_u32(&tl.acc_empty[as]), 0));
+                if (lane == 0 && !timed_out) mbar_arrive_relaxed(map_to_rank(smem_u32(&tl.acc_empty[as]), 0));
             };
             auto set_scales = [&](int i) {
                 __syncwarp();                                           // the last strip's have been read
@@ -1070,7 +1075,7 @@ static int32_t check_and_run(const char* name, uint64_t a, int32_t lda, uint64_t
     if (M == 0 || N == 0) return LUMI_OK;
     LUMI_TRY(check_device_memory(name, {a, a_scale, w, w_scale, bias, d, status}));
     const I8Args g{(const int8_t*)a, (const int8_t*)w, (const float*)a_scale, (const float*)w_scale, (const float*)bias, (void*)d, lda, ldw, ldd, M, N, K, accumulate,
-                   (int32_t*)status, wait_ns, skip_unit};
+                   (int32_t*)status, wait_ns, skip_unit, skip_unit < -1 ? -2 - skip_unit : -1};
     return d_dtype == LUMI_DTYPE_F32 ? launch_product<float>(g, st) : launch_product<__nv_bfloat16>(g, st);
 }
 
@@ -1079,7 +1084,7 @@ extern "C" int32_t lumi_k_gemm_i8(uint64_t a, int32_t lda, uint64_t a_scale, uin
     return check_and_run("lumi_k_gemm_i8", a, lda, a_scale, w, ldw, w_scale, bias, d, d_dtype, ldd, M, N, K, accumulate, status, kWaitLimitNs, -1, (cudaStream_t)stream);
 }
 
-// Failure-path test hook: waits limited by the caller and a tile whose operands (a pair: the second CTA's) never arrive.
+// Failure-path test hook: waits limited by the caller and a tile whose operands (a pair: the second CTA's) never arrive, or (skip_unit < -1) one wait that runs out at once.
 extern "C" int32_t lumi_debug_gemm_i8_wait_timeout(uint64_t a, int32_t lda, uint64_t a_scale, uint64_t w, int32_t ldw, uint64_t w_scale, uint64_t d, int32_t d_dtype,
                                                    int32_t ldd, int32_t M, int32_t N, int32_t K, int32_t accumulate, uint64_t wait_limit_ns, int32_t skip_unit,
                                                    uint64_t status) {
