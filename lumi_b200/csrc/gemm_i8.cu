@@ -700,11 +700,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
                     if (++s == S) { s = 0; ph ^= 1u; }
                 }
             }
-            if (timed_out && elect_one()) {                             // let every MMA issued so far finish (bounded) before TMEM is freed
-                umma_commit_pair(&tl.drain);
-                wait_for(&tl.drain, 0, g.wait_ns);
-            }
-            __syncwarp();
         }
     } else {
         const int q = warp & 3, half = (warp - 2) >> 2, strips_here = (cols / 32 - half + 1) >> 1;
@@ -854,7 +849,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
         }
         if (lane == 0) {
             asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-            for (int i = 0; i < 2; ++i) if (waited >> i & 1) wait_for(&old[i], (arrivals >> i) & 1u, g.wait_ns);      // (after a lost wait) copies under way
+            for (int i = 0; i < 2; ++i) if (waited >> i & 1) wait_for(&old[i], (arrivals >> i) & 1u, kWaitLimitNs);      // (after a lost wait) copies under way
         }
         __syncwarp();
     }
@@ -866,7 +861,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
     __syncwarp();
     cluster_arrive();
     cluster_wait();
-    if (*reinterpret_cast<volatile uint32_t*>(&tl.gave_up) != 0) {      // ... nor under a copy: the first CTA waits (bounded) for both CTAs' copies
+    if (*reinterpret_cast<volatile uint32_t*>(&tl.gave_up) != 0) {      // ... whoever's wait ran out: the first CTA waits (bounded) for both CTAs' MMAs and copies
+        if (rank == 0 && warp == 1) {
+            if (elect_one()) {                                          // (the lane that issued the MMAs)
+                umma_commit_pair(&tl.drain);
+                wait_for(&tl.drain, 0, kWaitLimitNs);
+            }
+            __syncwarp();
+        }
         if (rank == 0 && threadIdx.x == 0) {
             volatile uint32_t* issued = tl.issued;
             const uint32_t i0 = issued[0], i1 = issued[1], lo = min(i0, i1), hi = max(i0, i1);      // at most S apart: neither gets past an unconsumed stage
@@ -874,7 +876,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_cons
                 if (i0 > i1) mbar_complete_tx(&tl.full[k % S], (uint32_t)stage);
                 else mbar_expect_tx(&tl.full[k % S], (uint32_t)stage);
             }
-            for (uint32_t k = hi > (uint32_t)S ? hi - S : 0; k < hi; ++k) wait_for(&tl.full[k % S], (k / S) & 1u, g.wait_ns);
+            for (uint32_t k = hi > (uint32_t)S ? hi - S : 0; k < hi; ++k) wait_for(&tl.full[k % S], (k / S) & 1u, kWaitLimitNs);
         }
         __syncwarp();
         cluster_arrive();

@@ -39,3 +39,21 @@ def test_tiles(M, N, K, add, d):
 @pytest.mark.parametrize("d", [torch.float32, torch.bfloat16])
 def test_pairs(M, N, K, add, d):
     give_up(M, N, K, add, d, [0, 1, 75, 150])
+
+
+@pytest.mark.parametrize("M,N,K,add", [(300, 520, 4096, True), (16, 1024, 2816, False), (4096, 7360, 256, True), (4100, 7361, 640, False)])
+@pytest.mark.parametrize("limit", [1, 1000, 20_000])
+def test_limits_that_are_too_short(M, N, K, add, limit):
+    """What a call with a short limit clears up is waited for by the library's own limit: the call says whether a wait ran out, and the next one is right."""
+    c = Case(M, N, K, add=add, seed=N)
+    want = c.run().d[:M, :N].clone()
+    status = torch.zeros(1, device="cuda", dtype=torch.int32)
+    for _ in range(5):
+        c.d.copy_(c.old)
+        status.zero_()
+        rc = lumi_b200.lib().lumi_debug_gemm_i8_wait_timeout(c.a.data_ptr(), c.a.stride(0), c.sa.data_ptr(), c.w.data_ptr(), c.w.stride(0), c.sw.data_ptr(), c.d.data_ptr(), 0, c.ldd,
+                                                             M, N, K, int(add), limit, -1, status.data_ptr())
+        lost = torch.isnan(c.d[:M, :N])
+        assert rc == (-7 if bool(lost.any()) else 0) and torch.equal(c.d[:M, :N][~lost], want[~lost])
+        c.d.copy_(c.old)
+        assert torch.equal(c.run().d[:M, :N], want)
