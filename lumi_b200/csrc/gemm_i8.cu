@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const __grid_constant__ CU
     if (splits > 1) {
         old_of(4 * half, ahead);
         cluster_wait();                                                 // every CTA of the cluster runs
-    } else if (ADD) {
+    } else if (ADD && half < cols / 32) {                               // (a tile of 32 rows of A has no strip for the second half: those rows are another CTA's)
         load_old<DT>(g, m0 + half * 32, n, old);
     }
     __syncthreads();                                                    // the rows' scales are there
