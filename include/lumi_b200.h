@@ -369,7 +369,8 @@ int32_t lumi_k_norm_quant(uint64_t x, int32_t x_dtype, int32_t ldx, uint64_t o, 
                           uint64_t scale, int32_t rows, int32_t width, float eps, uint64_t stream);
 
 /* The gate of a feed-forward: rows of gu hold `width` gates and, from column `up` on, `width` ups; act(gate) * up as q and scale.  act: 0 sigmoid (the
- * hybrid's, inference/src/model.rs:550-552), 1 silu.  up and ld are multiples of 4 (fp32) or 8 (bf16) elements, up >= width. */
+ * hybrid's, inference/src/model.rs:550-552), 1 silu.  The sigmoid of fp32 gates is good to 2^-21 of itself, zero below -88.7 (as in lumi_k_gate_mul); of bf16 gates, by the hardware's
+ * exponential, to (2 + |gate| / 4) 2^-21, zero below -87.3: next to nothing beside half a step of an 8-bit integer, but seen in the scale's last bits.  up and ld are multiples of 4 (fp32) or 8 (bf16) elements, up >= width. */
 int32_t lumi_k_gate_quant(uint64_t gu, int32_t dtype, int32_t ld, int32_t up, int32_t act, uint64_t q, int32_t ldq, uint64_t scale, int32_t rows,
                           int32_t width, uint64_t stream);
 

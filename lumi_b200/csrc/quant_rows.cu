@@ -28,9 +28,17 @@ struct QuantOut {
     int ldq;
 };
 
-// e^-v and the quotient by the hardware's approximations: a relative error of 2^-21 and, where v is far below zero, of |v| 2^-23.  With the accurate forms
-// the arithmetic of a bf16 gate takes longer than its bytes.
-__device__ __forceinline__ float fast_sigmoid(float v) {
+// 1 / (1 + e^-v).  Of fp32 gates: expf (one ulp), then the hardware's reciprocal (one ulp) of an eighth of the sum, which stays in its range where the sigmoid no longer is a normal
+// number: under 2^-21 of it for all v above -88.7, below which expf leaves fp32's range and the gate is closed.  Their bytes take longer than that: 32768 x 2816 116 us, with both
+// approximations of the bf16 form too, with a rounded division 136.
+// Of bf16 gates: hardware exponential and reciprocal, a relative error of 2^-21 and, below zero, of |v| 2^-23 (the rounding of the exponent), closed below -87.3.  These are few
+// instructions, which such rows are close to being bound by: 32768 x 2816 72 us, with expf 86, with a rounded division too 115.  Half a step of an 8-bit integer is 2^-8.
+__device__ __forceinline__ float gate_sigmoid(float v, const float*) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(expf(-v), 0.125f, 0.125f)));
+    return r * 0.125f;
+}
+__device__ __forceinline__ float gate_sigmoid(float v, const __nv_bfloat16*) {
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
@@ -155,6 +163,7 @@ struct NormSource {
         }
     }
     // the same of one number
+    static constexpr bool kTailFree = false;
     struct Tail { float x, o; };
     template <bool AGAIN>
     __device__ __forceinline__ void load_tail(long row, int c, Tail& r) const {
@@ -212,6 +221,8 @@ struct GateSource {
 #pragma unroll
         for (int i = 0; i < E; ++i) t[i] = gated(t[i], u[i]);
     }
+    // A tail of zeros is zero: taken by all threads without a branch, it runs beside the other numbers (fp32, 45248 x 1111 80 -> 73 us; bf16 no gain).
+    static constexpr bool kTailFree = E == 4;
     struct Tail { float g, u; };
     template <bool AGAIN>
     __device__ __forceinline__ void load_tail(long row, int c, Tail& r) const {
@@ -221,7 +232,7 @@ struct GateSource {
     template <bool AGAIN>
     __device__ __forceinline__ float tail(long, int, const Tail& r, float&) const { return gated(r.g, r.u); }
     static __device__ __forceinline__ float gated(float gate, float v) {
-        const float z = fast_sigmoid(gate);
+        const float z = gate_sigmoid(gate, (const XT*)nullptr);
         return (SILU ? gate * z : z) * v;
     }
 };
@@ -362,8 +373,11 @@ __global__ void __launch_bounds__(NT) quant_wide_kernel(SRC src, QuantOut out) {
 
 // The numbers of a row in the registers of a warp (WARP) or a block, NC times E for each thread: memory is read once, all of it asked for before the first is
 // used, and the next row's while this one is reduced and written.
+// Blocks of 512 that have room on an SM, whatever the compiler would like: with fewer, an fp32 silu gate of 8192 x 8192 took 117 us (now 86), of 32768 x 1536 69 (65).
 template <typename SRC, bool WARP, int NC>
-__global__ void __launch_bounds__(WARP ? 128 : 512, SRC::E == 8 && !WARP ? 2 : 1) quant_rows_kernel(SRC src, QuantOut out, int rows) {
+constexpr int kRoom = WARP ? 1 : (SRC::E == 8 ? 2 : (SRC::kNorm ? 1 : (NC == 2 ? 3 : 2)));
+template <typename SRC, bool WARP, int NC>
+__global__ void __launch_bounds__(WARP ? 128 : 512, kRoom<SRC, WARP, NC>) quant_rows_kernel(SRC src, QuantOut out, int rows) {
     constexpr int E = SRC::E;
     const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, NT = WARP ? 32 : blockDim.x;
     const long step = WARP ? 4l * gridDim.x : (long)gridDim.x;
@@ -386,7 +400,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 512, SRC::E == 8 && !WARP ? 2 : 1
             src.template values<false>(row, (i * NT + tid) * E, r[i], t[i], sum);
             largest<E>(t[i], m);
         }
-        if (has_tail) {
+        if (SRC::kTail && (has_tail || SRC::kTailFree)) {
             t1 = src.template tail<false>(row, tail_at, r1, sum);
             largest(t1, m);
         }
