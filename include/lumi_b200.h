@@ -358,13 +358,14 @@ int32_t lumi_k_gate_mul(uint64_t gu, int32_t ld, uint64_t out32, uint64_t hi, ui
  * m = max(max |t|, 2^-100): t is about q * s.  A row that holds an infinity or a NaN gets q = 0 and s = NaN, so that all that is made from it is NaN.
  * These calls have no counterpart in the reference.  All pointers are memory of the current device; what lies between a row's end and the next
  * row (ld) is neither read nor written, rows begin on 16-byte boundaries.  Nothing is allocated and no workspace is shared: calls may overlap on any
- * streams and be captured into graphs.  With no rows a call does nothing; rows of more than 2^30 numbers are LUMI_E_UNSUPPORTED. */
+ * streams and be captured into graphs.  With no rows a call does nothing, but checks its arguments all the same (pointers that have to be given may not be 0). */
 
 /* The norm in front of a projection: x[r] += o[r] (o = 0: x is left alone; the sum is rounded to x's type, and the norm sees the rounded row), then
  * the rows x[r] / sqrt(mean(x[r]^2) + eps) * w over `width` elements as q[rows][ldq] and scale[rows].  w = 0: no norm, the rows of x as they are (a
  * projection's weights [N][K] give q and w_scale of lumi_k_gemm_i8; eps is not looked at).  x_dtype, o_dtype: LUMI_DTYPE_*; w fp32, eps > 0.
  * ldx and ldo are multiples of 4 (fp32) or 8 (bf16) elements, ldq of 16; x, o, w and q are 16-byte aligned.  o may be x itself; nothing else overlaps.
- * A row for which x * w leaves fp32's range is one that holds an infinity.  Rows are independent: their results are the same bits alone and among others. */
+ * A row for which x * w leaves fp32's range is one that holds an infinity.  Rows are independent: their results are the same bits alone and among others.  Rows of more than
+ * 2^30 numbers are LUMI_E_UNSUPPORTED (those of lumi_k_gate_quant cannot be longer, by their ld; lumi_k_dequant_rows takes them). */
 int32_t lumi_k_norm_quant(uint64_t x, int32_t x_dtype, int32_t ldx, uint64_t o, int32_t o_dtype, int32_t ldo, uint64_t w, uint64_t q, int32_t ldq,
                           uint64_t scale, int32_t rows, int32_t width, float eps, uint64_t stream);
 
