@@ -586,9 +586,10 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const __grid_constant__ CU
 // single loads 71).  The arrival that gives an accumulator back is relaxed: as a release it waited for the results to reach memory (4096 x 7360 x 1024 35 -> 29 us).  Copies and MMAs are issued
 // by whole warps with one lane elected (29 -> 28 us; 8192 x 8192 x 8192 325 -> 316).
 //
-// What bounds it, 10^12 operations a second (twice the measured bf16 rate: 3342): 8192 x 8192 x 8192 3520, the tensor cores; 8192 x 2048 x 8448 into an fp32 stream 3020; at short K the
-// shared memory, which operands, their copies and the results share: 4096 x 7360 x 1024 2360 (26 us; 28 with the results of a bf16 strip put one by one), and 2950 with the results left
-// out.  Called back to back for a second, the power limit takes the clock from 1.97 to 1.55 GHz there (32 us) and to 1.3 GHz at long K (8192 x 2048 x 8448: 94 -> 111 us).
+// What bounds it, 10^12 operations a second (twice the measured bf16 rate: 3342): 8192 x 8192 x 8192 3520, the tensor cores; 8192 x 2048 x 8448 into an fp32 stream 3020; at short K rounds
+// of whole tiles and the results.  A round of 74 tiles of 256 x 256 takes 2.6 us in bf16 at K = 128, whose MMAs take 0.4 at that rate; 3.9 at K = 1024 (3.0); 6.2 at K = 2048 (5.9); in fp32
+// 3.5, 4.9 and 7.6.  4096 x 7360 x 1024 is 6.27 such rounds and takes the time of seven: 26 to 27 us (28 with the results of a bf16 strip put one by one), 21 with the results left out,
+// of which more than two are the last round, where 20 of 74 pairs have work.  Called back to back for a second, the power limit takes the clock from 1.97 to 1.55 GHz there (32 us) and to 1.3 GHz at long K (8192 x 2048 x 8448: 94 -> 111 us).
 constexpr int kPairThreads = 320;
 struct PairTail {
     uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], drain;
@@ -978,9 +979,9 @@ int32_t launch_few(const I8Args& g, cudaStream_t st) {
 
 // Tile and shares of K for a product whose tiles fit on the GPU at once (cols 0: they do not).  The estimate, in microseconds behind what every launch
 // takes: 0.19 per k-block, and for the results, or for sums that cross the cluster's shared memory, by the tile's width and the number of CTAs.  Measured, columns /
-// shares (CTAs): 16 x 7360 x 1024 32/1 (58) 4.4, 32/2 (116) 5.8; 64 x 1024 x 2816 32/2 (32) 5.4, 32/4 (64) 4.3, 32/8 (128) 4.6, 64/4 (32) 5.4; 512 x 1024 x 2816 32/1 (128) 6.8, 64/2 (128)
-// 9.4; 512 x 259 x 8192 32/2 (96) 12.0, 64/4 (96) 10.1; 512 x 5632 x 2048 192/1 (132) 8.8, 256/1 (88) 10.4.  A second round of CTAs costs as much as the first: 256 x 7360 x 1024 128/1
-// (116) 6.5, 32/1 (464) 11.1, 128/2 (232) 20.5 (with a slower issue).
+// shares (CTAs): 16 x 7360 x 1024 32/1 (58) 4.6, 32/2 (116) 5.6; 64 x 1024 x 2816 32/2 (32) 5.4, 32/4 (64) 4.4, 32/8 (128) 4.8, 64/4 (32) 5.3; 512 x 1024 x 2816 32/1 (128) 7.1, 64/2 (128)
+// 9.0; 512 x 259 x 8192 32/2 (96) 11.9, 64/4 (96) 9.9; 512 x 5632 x 2048 192/1 (132) 9.2, 256/1 (88) 10.9.  A second round of CTAs costs more than the first: 256 x 7360 x 1024 128/1
+// (116) 6.3, 32/1 (464) 16.5, 128/2 (232) 18.3.
 TileShape tile_shape(const I8Args& g) {
     const int num_kb = (g.K + kBlockK - 1) / kBlockK;
     const long tiles = ((long)g.N + kWRows - 1) / kWRows;
