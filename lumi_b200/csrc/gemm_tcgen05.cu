@@ -278,16 +278,14 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_ahi, const __grid
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
     volatile uint32_t* gave_up = tmem_slot + 1;   // PAIR: a wait of either CTA ran out; then (first CTA) the k-blocks that either issued
     volatile uint32_t* issued = tmem_slot + 2;
+    volatile uint32_t* skip = tmem_slot + 4;      // a wait that expired in an earlier launch, or in an earlier CTA of this one: no work
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int num_kb = K / BK;
 
-    if (status != nullptr && (*reinterpret_cast<volatile int32_t*>(status) & STATUS_TIMEOUT)) {
-        if constexpr (PAIR) ntiles = 0;           // no work, but the cluster's barriers are taken
-        else return;
-    }
-
     if (threadIdx.x == 0) {
+        // (one verdict for all threads of the CTA: the word may change while they look)
+        *skip = status != nullptr && (*reinterpret_cast<volatile int32_t*>(status) & STATUS_TIMEOUT) ? 1u : 0u;
         for (int s = 0; s < S; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&tmem_full[i], 1); mbar_init(&tmem_empty[i], PAIR ? 8 : 4); }
         mbar_init(drain_bar, 1);
@@ -314,6 +312,7 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_ahi, const __grid
     // may want TMEM too, and would keep it while it waits for this kernel.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+    if (*skip != 0) ntiles = 0;                   // (the barriers are taken all the same)
     // Launched with programmatic dependent launch (small batches), this CTA may have become resident and done all of the
     // above — barrier set-up, TMEM allocation — while its predecessor (the state step) still ran; everything below reads
     // what predecessors produced.  Without the launch attribute this is a no-op.
@@ -370,7 +369,7 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_ahi, const __grid
         }
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (by_rows) ntiles = __ldcg(ex.n_tiles) * tiles_pg;
+    if (by_rows && *skip == 0) ntiles = __ldcg(ex.n_tiles) * tiles_pg;
 
     bool timed_out = false;
     if (warp == 0) {

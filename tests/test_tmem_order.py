@@ -37,3 +37,12 @@ def test_dependents_are_released_behind_the_allocation(f, body):
     barrier = body.find("tc_fence_after()", alloc[-1])        # every thread of the CTA is behind the allocation here
     assert barrier > 0
     assert all(r > barrier for r in release), f
+
+
+@pytest.mark.parametrize("f,body", WITH_TMEM, ids=["%s-%d" % (f, i) for i, (f, _) in enumerate(WITH_TMEM)])
+def test_one_verdict_on_an_earlier_timeout(f, body):
+    """A kernel that does no work after a wait ran out elsewhere decides it once for all threads of a CTA: the word may change while they look, and warps that part over it would allocate
+    tensor memory, or read it, with half their lanes."""
+    for line in body.split("\n"):
+        if "& STATUS_TIMEOUT" in line:
+            assert "__syncthreads_or(" in line or re.match(r"\s*(tl\.|\*)skip = ", line), (f, line)      # (skip: one thread's word in shared memory)
