@@ -243,7 +243,7 @@ int32_t lumi_k_gemm_bf16_tcgen05(uint64_t a_hi, uint64_t a_lo, uint64_t w, uint6
                                  int32_t K, int32_t ldd, int32_t accumulate, uint64_t stream);
 
 /* Failure-path test hook for the bounded device-side waits (no counterpart in the reference, whose kernels never wait
- * on one another): runs the same GEMM with activations a_hi only, every device-side wait limited to wait_limit_ns, and
+ * on one another): runs the same GEMM with activations a_hi only, every device-side wait limited to wait_limit_ns (at least 10^6; 0: the library's own), and
  * the producer stopping before work unit `skip_unit` (units are 128-row x tile-width output tiles in launch order, CTAs
  * up to 64 rows; -1 = none), so that the waits of the consumers run out.  status_word: a zeroed device int32.  Returns LUMI_E_TIMEOUT
  * when a wait gave up — the kernel has then returned cleanly (copies drained, tensor memory freed) and further calls
@@ -259,7 +259,7 @@ int32_t lumi_debug_gemm_wait_timeout(uint64_t a_hi, uint64_t w, uint64_t d, int3
  * act: 0 none, 2 relu squared.  groups > 0: products of column blocks: group g multiplies columns [g K, (g + 1) K) of A (rows of lda) with rows
  * [g group_rows, ...) of W; its results go to columns g out_step + n, n < out_n, of D (ldd) and out_hi / out_lo (ldo), with gate (3 relu, 4 silu:
  * rows of W sixteen gates and sixteen ups in turn) and mul (times sigmoid(mul[row * ldmul + column])).
- * status_word given: waits are limited to wait_limit_ns, work unit skip_unit (-1: none) is not fed, the call synchronises and answers LUMI_E_TIMEOUT. */
+ * status_word given: waits are limited to wait_limit_ns (at least 10^6; 0: the library's own), work unit skip_unit (-1: none) is not fed, the call synchronises and answers LUMI_E_TIMEOUT. */
 typedef struct lumi_gemm_probe {
     uint64_t a_hi, a_lo, w, d;
     uint64_t bias, ssq_in, gamma_next, out_hi, out_lo, ssq_out, mul;

@@ -3087,9 +3087,16 @@ extern "C" int32_t lumi_debug_gemm_plan(int32_t M, int32_t N, int32_t K, int32_t
     return LUMI_OK;
 }
 
+// Limits of the test hooks of the bf16 products: what such a kernel waits for when it clears up (its own copies, its MMAs) goes by the same limit, and has to fit into it.
+static int32_t check_wait_limit(uint64_t ns) {
+    if (ns != 0 && ns < 1000000) return fail(LUMI_E_INVALID, "a wait limit of %llu ns (at least 1000000, or 0)", (unsigned long long)ns);
+    return LUMI_OK;
+}
+
 extern "C" int32_t lumi_debug_gemm_wait_timeout(uint64_t a_hi, uint64_t w, uint64_t d, int32_t M, int32_t N, int32_t K, uint64_t wait_limit_ns,
                                                 int32_t skip_unit, uint64_t status_word) {
     if (!a_hi || !w || !d || !status_word) return fail(LUMI_E_INVALID, "null device pointer");
+    LUMI_TRY(check_wait_limit(wait_limit_ns));
     GemmArgs g{(const __nv_bfloat16*)a_hi, nullptr, (const __nv_bfloat16*)w, (float*)d, N, M, N, K, 0, (int32_t*)status_word};
     g.few_rows = M <= 64;                                 // as a step's products; above, the persistent kernel
     g.wait_limit_ns = wait_limit_ns;
@@ -3104,6 +3111,7 @@ extern "C" int32_t lumi_debug_gemm_wait_timeout(uint64_t a_hi, uint64_t w, uint6
 
 extern "C" int32_t lumi_debug_gemm(const lumi_gemm_probe* q) {
     if (!q || !q->a_hi || !q->w || (!q->d && !q->out_hi)) return fail(LUMI_E_INVALID, "a product needs its operands and an output");
+    if (q->status_word) LUMI_TRY(check_wait_limit(q->wait_limit_ns));
     KernelScratch ks;
     if (q->split_k) LUMI_TRY(kernel_scratch(&ks));
     GemmArgs g{(const __nv_bfloat16*)q->a_hi, (const __nv_bfloat16*)q->a_lo, (const __nv_bfloat16*)q->w, (float*)q->d, q->ldd, q->M, q->N, q->K, q->accumulate,
