@@ -394,6 +394,63 @@ int32_t lumi_k_gemm_i8(uint64_t a, int32_t lda, uint64_t a_scale, uint64_t w, in
 int32_t lumi_debug_gemm_i8_wait_timeout(uint64_t a, int32_t lda, uint64_t a_scale, uint64_t w, int32_t ldw, uint64_t w_scale, uint64_t d, int32_t d_dtype,
                                         int32_t ldd, int32_t M, int32_t N, int32_t K, int32_t accumulate, uint64_t wait_limit_ns, int32_t skip_unit, uint64_t status);
 
+/* ---- keys and values in 4 bits: pages, rows in and out, attention ----------------------------
+ * A cache for requests of different lengths, in pages of 64 tokens that any request may be given.  These calls have no counterpart in the reference (its cache: inference/src/model.rs:
+ * 492-556).  All pointers are memory of the current device.  Nothing is allocated; calls may be captured into graphs.  With no rows (or sequences) a call does nothing, but checks
+ * its arguments all the same.
+ *
+ * A token's keys (dk numbers per head) and values (dv) lie in groups of 32, the last one possibly shorter.  A group t has the scale s = m / 7 rounded up to bf16, m = max(max |t|,
+ * 2^-100), and codes n = 8 + rint(t / s) (fp32 quotient, ties to even; 1 .. 15) in 4 bits: t is about (n - 8) s, off by s / 2 at most.  A group that holds an infinity or a NaN gets
+ * codes 8 and s = NaN.  A page has a block per head, 16-byte aligned:
+ *   keys' codes [group][token][16 bytes], keys' scales [group][token] bf16, values' codes, values' scales (groups of dk, then of dv).
+ * Of a group's 16 bytes, number i of the values is nibble i (low nibbles first); of the keys, four 32-bit words hold eight numbers each, number e of a word as nibble e / 2 + 4 (e % 2).
+ * Nibbles behind a head's last number are written as 8 and not looked at.
+ * The token at place t of page p has slot 64 p + t.  dk, dv <= 256; n_pages < 2^25 (LUMI_E_UNSUPPORTED beyond). */
+
+/* Bytes of one page: kv_heads blocks of (ceil(dk / 32) + ceil(dv / 32)) * 1152. */
+int32_t lumi_k_kv4_page_bytes(int32_t kv_heads, int32_t dk, int32_t dv, int64_t* bytes);
+
+/* What a step needs to know, from the lengths of its requests: tokens[nseq] that each sequence holds, len[nseq] new ones (0: none; negative: the request has ended, its pages come back
+ * and it holds no tokens then).  All arrays are 32-bit integers.
+ *   page_table [nseq][pages_per_seq]: page of positions 64 i .. 64 i + 63 of a sequence.  Entries of held tokens are read, those of new pages written, others left as they were.
+ *   free_pages [n_pages]: a stack of pool[0] page ids.  Pages that come back are laid on top of it in the order of sequences; new pages are taken from the top, for the first sequence first.
+ *   pool_after [2]: the new count; pool[1] with the bits below.  tokens_after [nseq].  (pool_after may be pool, tokens_after may be tokens; nothing else overlaps.)
+ *   row_start [nseq + 1]: the first row of each sequence and, last, the number of rows; pos, slot [rows]: position and slot of each row, -1 for rows behind the last sequence.
+ * A call whose inputs do not lie where its results go can be made again with the same results.  Bits of pool_after[1]: 1 there are not enough free pages (or the count is none), 2 a sequence
+ * would have more tokens than its row of the table (or holds a negative number), 4 more new tokens than `rows`.  Then nothing else changes: row_start is 0, pos and slot are -1.
+ * nseq <= 8192 (LUMI_E_UNSUPPORTED beyond). */
+int32_t lumi_k_page_plan(uint64_t tokens, uint64_t len, int32_t nseq, uint64_t page_table, int32_t pages_per_seq, uint64_t free_pages, int32_t n_pages, uint64_t pool,
+                         uint64_t pool_after, uint64_t tokens_after, uint64_t row_start, uint64_t pos, uint64_t slot, int32_t rows, uint64_t stream);
+
+/* Rows of keys [rows][ldk] (head h at columns h dk ...) and values [rows][ldv] into the slots of slot[rows]; rows whose slot is not one of the cache's (-1) are left out.  dtype:
+ * LUMI_DTYPE_* of both.  No alignment beyond the element's, but rows on 16-byte boundaries and heads of whole eights go faster.  The slots of a call differ. */
+int32_t lumi_k_kv4_append(uint64_t k, int32_t ldk, uint64_t v, int32_t ldv, int32_t dtype, uint64_t slot, uint64_t kv, int32_t n_pages, int32_t kv_heads, int32_t dk, int32_t dv,
+                          int32_t rows, uint64_t stream);
+
+/* The same rows back as numbers, (n - 8) s rounded once to the type; rows whose slot is not one of the cache's, and what lies behind a row's end, are left as they were. */
+int32_t lumi_k_kv4_read(uint64_t kv, int32_t n_pages, uint64_t slot, uint64_t k, int32_t ldk, uint64_t v, int32_t ldv, int32_t dtype, int32_t kv_heads, int32_t dk, int32_t dv,
+                        int32_t rows, uint64_t stream);
+
+/* Attention: y[r] = softmax(scale q[r] K^T) V over the cache of the row's sequence, the call's own rows (appended before) among it.  Sequence s has the rows row_start[s] ..
+ * row_start[s + 1] - 1 and holds tokens[s] tokens with them: row i of its n rows stands at position tokens[s] - n + i and sees the `window` positions that end with its own (0: all).
+ * sink: the softmax has one more score, 0, without a value.  heads a multiple of kv_heads; head h reads the cache's head h / (heads / kv_heads).
+ * q [rows][ldq], y [rows][ldy]: dtype LUMI_DTYPE_*, any alignment of theirs; fp32 rows are good to about 2^-20, bf16 rows to their own rounding.  rows behind row_start[nseq] are left as
+ * they were; rows <= 2^24.  max_new: at least the largest number of rows of a sequence; sequences of more are left out.
+ * work: at least lumi_k_kv4_attention_work_bytes, zero before its first call; calls that may run at the same time (other streams, other graphs) need areas of their own.
+ * status: a device int32 or 0.  Bit 1: a sequence's lengths do not fit its rows or its row of the table (its rows are left as they were), or a page that rows see is not one of the cache's (its tokens are
+ * passed over; a row that sees nothing is 0).  Bit 4: a bounded wait on the device gave up; rows that it cost are NaN. */
+int32_t lumi_k_kv4_attention_work_bytes(int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv, int64_t* bytes);
+int32_t lumi_k_kv4_attention(uint64_t q, int32_t ldq, int32_t dtype, uint64_t kv, int32_t n_pages, uint64_t page_table, int32_t pages_per_seq, uint64_t row_start, uint64_t tokens,
+                             uint64_t y, int32_t ldy, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv, int32_t window, float scale, int32_t sink, int32_t nseq, int32_t rows,
+                             int32_t max_new, uint64_t work, uint64_t work_bytes, uint64_t status, uint64_t stream);
+
+/* The norms around a block, with its gate and residual scale: x[r] += scale * gate[r] * (o[r] / sqrt(mean(o[r]^2) + eps) * w_post) (rounded to x's type), then
+ * y[r] = x[r] / sqrt(mean(x[r]^2) + eps) * w_pre of the rounded row.  w_post = 0: o as it is; gate = 0: none, else of o's type, ldg = 0: one row of gates for all rows; y = 0: x alone.
+ * *_dtype: LUMI_DTYPE_*; w_post, w_pre fp32.  Rows begin on 16-byte boundaries (ld* multiples of 4 fp32 or 8 bf16 numbers); what lies behind a row's end is neither read nor written.
+ * x, o, gate and y do not overlap.  width <= 32768 (LUMI_E_UNSUPPORTED beyond).  A row's results do not depend on the other rows. */
+int32_t lumi_k_block_norm(uint64_t x, int32_t x_dtype, int32_t ldx, uint64_t o, int32_t o_dtype, int32_t ldo, uint64_t w_post, uint64_t gate, int32_t ldg, float scale, uint64_t w_pre,
+                          uint64_t y, int32_t y_dtype, int32_t ldy, int32_t rows, int32_t width, float eps, uint64_t stream);
+
 /* One Mamba block (RMSNorm -> in_proj -> state step -> out_proj + residual, inference/src/model.rs:296-375
  * in arithmetic) WITHOUT any allocation.  This entry point has no counterpart in the reference.
  *
