@@ -40,6 +40,7 @@ struct AttendArgs {
     long ldq, ldy;
     int heads, kv_heads, group, dk, dv, window, sink, nseq, rows, max_new, n_pages, width;
     int few;                                               // columns per head of the cache up to which a sequence is the step kernel's
+    int wide_q, wide_y;                                    // rows and heads lie on boundaries of 16 bytes, of four numbers
     int slots, slot_bytes;                                 // of a warp's ring
     int skip;                                              // failure tests: the copy of this page of the line is not issued
     float scale;
@@ -47,12 +48,49 @@ struct AttendArgs {
 
 __device__ __forceinline__ float number(const float* p) { return *p; }
 __device__ __forceinline__ float number(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+// Eight numbers on a 16-byte boundary, or none.
+__device__ __forceinline__ void eight_numbers(const float* p, int n, float (&t)[8]) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+    if (n > 0) { x = reinterpret_cast<const float4*>(p)[0]; y = reinterpret_cast<const float4*>(p)[1]; }
+    t[0] = x.x; t[1] = x.y; t[2] = x.z; t[3] = x.w; t[4] = y.x; t[5] = y.y; t[6] = y.z; t[7] = y.w;
+}
+__device__ __forceinline__ void eight_numbers(const __nv_bfloat16* p, int n, float (&t)[8]) {
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (n > 0) x = *reinterpret_cast<const uint4*>(p);
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { t[2 * i] = __uint_as_float(u[i] << 16); t[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+}
+// Four results of a row, of which it has n.
+__device__ __forceinline__ void put_four(float* p, int n, bool wide, const float (&t)[4]) {
+    if (wide && n >= 4) *reinterpret_cast<float4*>(p) = make_float4(t[0], t[1], t[2], t[3]);
+    else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (i < n) p[i] = t[i];
+    }
+}
+__device__ __forceinline__ void put_four(__nv_bfloat16* p, int n, bool wide, const float (&t)[4]) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(t[0], t[1]), b = __floats2bfloat162_rn(t[2], t[3]);
+    if (wide && n >= 4) *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    else {
+        if (n > 0) p[0] = a.x;
+        if (n > 1) p[1] = a.y;
+        if (n > 2) p[2] = b.x;
+        if (n > 3) p[3] = b.y;
+    }
+}
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// Matrix loads may be moved as the arithmetic around them allows; what orders them is their address, which comes from pinned() behind what they have to wait for.
+__device__ __forceinline__ uint32_t pinned(uint32_t a) {
+    uint32_t b;
+    asm volatile("mov.u32 %0, %1;" : "=r"(b) : "r"(a) : "memory");
+    return b;
+}
 __device__ __forceinline__ void ldmatrix4(uint32_t a, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+    asm("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
 }
 __device__ __forceinline__ void ldmatrix4_trans(uint32_t a, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+    asm("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
 }
 __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
@@ -61,11 +99,29 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
 __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     mma16(d, a0, a1, a2, a3, b0, b1, d[0], d[1], d[2], d[3]);
 }
+// An 8 x 8 matrix of 16-bit numbers, one row per four lanes, two numbers each, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t u) {
+    uint32_t v;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(v) : "r"(u));
+    return v;
+}
 __device__ __forceinline__ uint32_t halves(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float2 unhalves(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+// two fp32 operations in one
+__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0, float c1) {
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mul2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void add2(float& d0, float& d1, float a0, float a1) {
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%0, %1};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(d0), "+f"(d1) : "f"(a0), "f"(a1));
+}
 __device__ __forceinline__ float low_bf16(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float high_bf16(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
@@ -100,7 +156,6 @@ struct StepShape {
     static constexpr int kCols = MODE == 1 ? 16 : 8;
     // registers: accumulators of values 4 NG per eight columns and number block, of their offsets, scores, q
     static constexpr int kWarps = NG == 8 ? 6 : MODE == 1 ? (NG == 4 ? 8 : 12) : (NG == 4 ? 12 : 16);
-    static constexpr int kStage = 1024;                    // of a warp: one group of its columns on their way into registers
 };
 
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -110,22 +165,26 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
 // One part of a unit: columns' largest score m (in units of log2), sum l and numbers o [column][dv], all relative to 2^m.  Where parts lie: m [cols], l [cols], o [cols][pad].
 __host__ __device__ inline int part_floats(int cols, int dv) { return cols * (2 + kv4_groups(dv) * kGroup); }
 
+__device__ __forceinline__ long long quotient(long long n, long long d) {       // of numbers that are nearly always small
+    return ((n | d) >> 32) == 0 ? (long long)((uint32_t)n / (uint32_t)d) : n / d;
+}
+
 struct Open { long long lo, hi; int s, unit; };
 
 template <typename T, int NG, int MODE>
 __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_kernel(const AttendArgs a) {
     using Shape = StepShape<NG, MODE>;
-    constexpr int W = Shape::kWarps, COLS = Shape::kCols, NT = W * 32, SETS = MODE == 1 ? 2 : 1;
+    constexpr int W = Shape::kWarps, COLS = Shape::kCols, THREADS = W * 32, NT = MODE == 1 ? 2 : 1;
     constexpr bool TWO = MODE == 2;                        // two terms of q and of the weights
     extern __shared__ __align__(128) uint8_t sm[];
-    __shared__ long long before[NT + 1];                   // pages of the sequences ahead of each thread's
+    __shared__ long long before[THREADS + 1];                   // pages of the sequences ahead of each thread's
     __shared__ uint64_t full[W][4];
     __shared__ long long warp_pages[W];
     __shared__ Open heads_s[W], tails_s[W];                // units that began ahead of a warp's run and end in it; that its run ends with and that it does not hold whole
-    __shared__ int last_s, lost_s;
+    __shared__ int last_s, lost_s, n_open_s, opens_s[32];
+    __shared__ long long line_s[3 + W];                    // pages of the line, the CTA's first and its end, runs' first ones: not kept in registers over the pages
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i8 = lane >> 2, j4 = lane & 3;
     uint8_t* const ring = sm + (size_t)warp * a.slots * a.slot_bytes;
-    uint8_t* const stage = sm + (size_t)W * a.slots * a.slot_bytes + warp * Shape::kStage;
     const int gk = kv4_groups(a.dk), gv = kv4_groups(a.dv), part = kv4_part(a.dk), block = kv4_block(a.dk, a.dv);
     const int rec = part_floats(COLS, a.dv), pad = gv * kGroup;
 
@@ -137,7 +196,7 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
     pdl_sync();
 
     // ---- the line of pages: each thread sums up a run of sequences
-    const int each = (a.nseq + NT - 1) / NT, s_lo = min(a.nseq, tid * each), s_hi = min(a.nseq, s_lo + each);
+    const int each = (a.nseq + THREADS - 1) / THREADS, s_lo = min(a.nseq, tid * each), s_hi = min(a.nseq, s_lo + each);
     long long mine = 0;
     bool any_bad = false;
     for (int s = s_lo; s < s_hi; ++s) {
@@ -156,19 +215,23 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
 #pragma unroll
     for (int w = 0; w < W; ++w) { const long long p = warp_pages[w]; if (w < warp) ahead += p; total += p; }
     before[tid] = ahead + run - mine;
-    if (tid == NT - 1) before[NT] = total;
+    if (tid == THREADS - 1) before[THREADS] = total;
     __syncthreads();
     // CTAs that get work: a page per warp at least.  CTA c takes the pages from c total / ctas on.
-    const int ctas = (int)min((long long)gridDim.x, (total + W - 1) / W), cta = blockIdx.x;
+    const int ctas = (int)min((long long)gridDim.x, quotient(total + W - 1, W)), cta = blockIdx.x;
     if (cta >= ctas) return;
-    const long long c_lo = total * cta / ctas, c_hi = total * (cta + 1) / ctas;
-    auto warp_from = [&](int w) { return c_lo + (c_hi - c_lo) * w / W; };
-    const long long x_lo = warp_from(warp), x_hi = warp_from(warp + 1);
+    const long long c_lo = quotient(total * cta, ctas), c_hi = quotient(total * (cta + 1), ctas);
+    auto warp_from = [&](int w) { return c_lo + quotient((c_hi - c_lo) * w, W); };
+    const int run_n = (int)(warp_from(warp + 1) - warp_from(warp));
+    if (lane == 0) line_s[3 + warp] = warp_from(warp);
+    if (tid == 0) { line_s[0] = total; line_s[1] = c_lo; line_s[2] = c_hi; }
+    __syncwarp();
+    volatile const long long* const x_lo_s = line_s + 3 + warp;
 
     // where page x of the line lies: sequence, unit, page of the unit's
     struct Spot { int s, unit, p, page; };
     auto find = [&](long long x) {
-        int lo = 0, hi = NT;
+        int lo = 0, hi = THREADS;
         while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (before[mid] <= x) lo = mid; else hi = mid; }
         long long at = before[lo];
         Spot r{0, 0, 0, -1};
@@ -179,7 +242,7 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
             if (x < at + n) {
                 const long long rel = x - at;
                 r.s = s;
-                r.unit = (int)(rel / q.pages);
+                r.unit = (int)quotient(rel, q.pages);
                 r.p = (int)(rel - (long long)r.unit * q.pages);
                 r.page = a.table[(size_t)s * a.width + q.page0 + r.p];
                 if (r.page < 0 || r.page >= a.n_pages) {
@@ -193,106 +256,107 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
         return r;
     };
 
-    // ---- state of the unit at hand
-    float O[SETS][2 * NG][4], OFF[SETS][NG][4], m[SETS], l[SETS];
-    uint32_t Q[2 * NG][4];
-    float qc[NG][2];                                       // what the scores' accumulators start at
-    float cx[SETS];                                        // factor from accumulators to scores in units of log2
-    int lo_pos[SETS], hi_pos[SETS];                        // positions that the column sees: lo .. hi
+    // ---- state of the unit at hand.  Lane 4 i + j: columns 2 j and 2 j + 1 of each eight, tokens i of each eight, numbers 4 i .. 4 i + 3 of each group.
+    float O[NT][2 * NG][4], m[NT][2], l[NT][2];
+    float OFF[NT][TWO ? NG : 2][2];                        // 8 sum p s: bf16 rows: row g of the accumulator is group g; fp32 rows: the lane's tokens' part
+    uint32_t Q[NT][2 * NG][TWO ? 4 : 2];                   // q as B, first and second term
+    float QC[NT][NG][2];                                   // -8 sum q of each group: what the scores' accumulators start at
+    float cx[NT][2];                                       // factor from accumulators to scores in units of log2
+    int lo_pos[NT][2], hi_pos[NT][2];                      // positions that the column sees: lo .. hi
     int e_v = 0;                                           // scales of values are below 2^e_v so far
-    int first_full = 0, last_full = 0;                     // pages whose every token is seen by every column, as positions: [first_full, last_full]
+    int first_full = 0, last_full = 0;                     // positions that every column sees
     bool dead = false;                                     // a wait gave up
     const float sign = a.scale < 0.f ? -1.f : 1.f;
 
     auto begin_unit = [&](const Sequence& q, int unit) {
-        const int cols = q.n * a.group, head = unit % a.kv_heads, col0 = unit / a.kv_heads * COLS;
-        float raw[COLS][NG];
-#pragma unroll
-        for (int c = 0; c < COLS; ++c) {
-            const int col = col0 + c;
-            const T* const p = (const T*)a.q + (long)(q.first + col / a.group) * a.ldq + (long)(head * a.group + col % a.group) * a.dk;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) raw[c][g] = col < cols && g * kGroup + lane < a.dk ? number(p + g * kGroup + lane) : 0.f;
-        }
-        // times a power of two that brings the column's largest to 2^13 .. 2^14
-        float by[COLS];
-#pragma unroll
-        for (int c = 0; c < COLS; ++c) {
-            uint32_t top = 0;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) top = max(top, __float_as_uint(raw[c][g]) & 0x7fffffffu);
-            top = __reduce_max_sync(0xffffffffu, top);
-            const int k = top >= 0x7f800000u || top == 0 ? 0 : min(126, 13 + 127 - (int)(top >> 23));
-            by[c] = power_of_two(k) * sign;
-        }
-        // number d of a group: word j, pair half, step; the second pair of a step meets codes that are 16 times as large
-        const int step = lane % 8 / 4, half = lane % 4 / 2, k8 = lane / 8 * 2 + lane % 2;
-        uint16_t* const to = reinterpret_cast<uint16_t*>(stage) + (step * 2 + half) * 128 + k8;
-        const float sixteenth = half ? 0.0625f : 1.f;
-        const uint32_t from = smem_u32(stage) + (lane / 16) * 256 + (lane % 16) * 16;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            if (g >= gk) break;
-#pragma unroll
-            for (int c = 0; c < COLS; ++c) {
-                const float v = raw[c][g] * by[c] * sixteenth;
-                const __half h = __float2half_rn(v);
-                to[c * 8] = __half_as_ushort(h);
-                if (TWO) to[(c + 8) * 8] = __half_as_ushort(__float2half_rn(v - __half2float(h)));
-                else if (COLS == 8) to[(c + 8) * 8] = 0;
-            }
-            __syncwarp();
-            ldmatrix4(from, Q[2 * g]);
-            ldmatrix4(from + 512, Q[2 * g + 1]);
-            __syncwarp();
-            float t[4];
-            mma16(t, Q[2 * g][0], Q[2 * g][1], Q[2 * g][2], Q[2 * g][3], 0x80088008u, 0x80808080u, 0.f, 0.f, 0.f, 0.f);          // -8 2^-24 and -128 2^-24
-            mma16(t, Q[2 * g + 1][0], Q[2 * g + 1][1], Q[2 * g + 1][2], Q[2 * g + 1][3], 0x80088008u, 0x80808080u);
-            qc[g][0] = t[0]; qc[g][1] = t[2];
-        }
+        const int cols = q.n * a.group, tile = unit / a.kv_heads, head = unit - tile * a.kv_heads, col0 = tile * COLS;
         first_full = 0; last_full = 0x7fffffff;
 #pragma unroll
-        for (int set = 0; set < SETS; ++set) {
-            float b = 1.f;
+        for (int nt = 0; nt < NT; ++nt) {
+            const int col = col0 + nt * 8 + i8, row = min(col, cols - 1) / a.group, h = min(col, cols - 1) - row * a.group;
+            const T* const p = (const T*)a.q + (long)(q.first + row) * a.ldq + (long)(head * a.group + h) * a.dk + j4 * 8;
+            float raw[NG][8];                              // numbers 8 j .. 8 j + 7 of each group of column i
 #pragma unroll
-            for (int c = 0; c < 8; ++c) if (c == i8) b = by[set * 8 + c] * sign;
-            cx[set] = fminf(fmaxf(__fdiv_rn(fabsf(a.scale) * kLog2e, b) * 16777216.f, 1e-37f), 3.4e38f);      // (not 0: hidden scores are -inf)
-            const int row = min(col0 + set * 8 + i8, cols - 1) / a.group, pos = q.total - q.n + row;
-            hi_pos[set] = pos;
-            lo_pos[set] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-            m[set] = -INFINITY;
-            l[set] = 0.f;
-        }
-        {
-            const int row0 = col0 / a.group, row1 = min(col0 + COLS, cols) - 1;
-            last_full = q.total - q.n + row0;
-            const int far = q.total - q.n + row1 / a.group;
-            first_full = a.window > 0 ? max(0, far - a.window + 1) : 0;
+            for (int g = 0; g < NG; ++g) {
+                const int n = col < cols ? a.dk - g * kGroup - j4 * 8 : 0;
+                if (a.wide_q) eight_numbers(p + g * kGroup, n, raw[g]);
+                else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) raw[g][e] = e < n ? number(p + g * kGroup + e) : 0.f;
+                }
+            }
+            // times a power of two that brings the column's largest to 2^13 .. 2^14
+            uint32_t top = 0;
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(raw[g][e]) & 0x7fffffffu);
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float by = power_of_two(top >= 0x7f800000u || top == 0 ? 0 : min(126, 13 + 127 - (int)(top >> 23)));
+            const float c = fminf(fmaxf(__fdiv_rn(fabsf(a.scale) * kLog2e, by) * 16777216.f, 1e-37f), 3.4e38f);      // (not 0: hidden scores are -inf)
+            const int pos = q.total - q.n + row, lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                cx[nt][e] = __shfl_sync(0xffffffffu, c, 8 * j4 + 4 * e);
+                hi_pos[nt][e] = __shfl_sync(0xffffffffu, pos, 8 * j4 + 4 * e);
+                lo_pos[nt][e] = __shfl_sync(0xffffffffu, lo, 8 * j4 + 4 * e);
+                m[nt][e] = -INFINITY;
+                l[nt][e] = 0.f;
+            }
+            last_full = min(last_full, __reduce_min_sync(0xffffffffu, pos));
+            first_full = max(first_full, __reduce_max_sync(0xffffffffu, lo));
+            const float f = by * sign, f16 = f * 0.0625f;  // the second pair of a step meets codes that are 16 times as large
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int step = 0; step < 2; ++step) {
+                    const float(&v)[8] = raw[g];
+                    const float v0 = v[step * 4] * f, v1 = v[step * 4 + 1] * f, v2 = v[step * 4 + 2] * f16, v3 = v[step * 4 + 3] * f16;
+                    auto& to = Q[nt][2 * g + step];
+                    to[0] = halves(v0, v1);
+                    to[1] = halves(v2, v3);
+                    if constexpr (TWO) {
+                        const float2 h0 = unhalves(to[0]), h1 = unhalves(to[1]);
+                        to[2] = halves(v0 - h0.x, v1 - h0.y);
+                        to[3] = halves(v2 - h1.x, v3 - h1.y);
+                    }
+                }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int step = 0; step < 2; ++step) {
+                    const auto& b = Q[nt][2 * g + step];
+                    mma16(t, 0x80088008u, 0x80088008u, 0x80808080u, 0x80808080u, b[0], b[1]);                // -8 2^-24 and -128 2^-24
+                    if constexpr (TWO) mma16(t, 0x80088008u, 0x80088008u, 0x80808080u, 0x80808080u, b[2], b[3]);
+                }
+                QC[nt][g][0] = t[0]; QC[nt][g][1] = t[1];
+            }
+#pragma unroll
+            for (int t = 0; t < 2 * NG; ++t) O[nt][t][0] = O[nt][t][1] = O[nt][t][2] = O[nt][t][3] = 0.f;
+#pragma unroll
+            for (int g = 0; g < (TWO ? NG : 2); ++g) OFF[nt][g][0] = OFF[nt][g][1] = 0.f;
         }
         e_v = -90;
-#pragma unroll
-        for (int set = 0; set < SETS; ++set) {
-#pragma unroll
-            for (int t = 0; t < 2 * NG; ++t) O[set][t][0] = O[set][t][1] = O[set][t][2] = O[set][t][3] = 0.f;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) OFF[set][g][0] = OFF[set][g][1] = OFF[set][g][2] = OFF[set][g][3] = 0.f;
-        }
     };
-    auto scale_values = [&](int set, float f0, float f1) {     // of columns 2 j and 2 j + 1
+    auto scale_values = [&](int nt, float f0, float f1) {
 #pragma unroll
-        for (int t = 0; t < 2 * NG; ++t) { O[set][t][0] *= f0; O[set][t][1] *= f1; O[set][t][2] *= f0; O[set][t][3] *= f1; }
+        for (int t = 0; t < 2 * NG; ++t) { O[nt][t][0] *= f0; O[nt][t][1] *= f1; O[nt][t][2] *= f0; O[nt][t][3] *= f1; }
 #pragma unroll
-        for (int g = 0; g < NG; ++g) { OFF[set][g][0] *= f0; OFF[set][g][1] *= f1; OFF[set][g][2] *= f0; OFF[set][g][3] *= f1; }
+        for (int g = 0; g < (TWO ? NG : 2); ++g) { OFF[nt][g][0] *= f0; OFF[nt][g][1] *= f1; }
     };
 
     // ---- one page of the unit
     auto work_page = [&](uint8_t* slot, int pos0) {
-        const uint32_t base = smem_u32(slot);
         const bool edge = pos0 < first_full || pos0 + kPage - 1 > last_full;
         if (edge) {
             // scales of tokens that no column sees may be any bits: they become 0
-            const int lo = __reduce_min_sync(0xffffffffu, SETS == 2 ? min(lo_pos[0], lo_pos[SETS - 1]) : lo_pos[0]);
-            const int hi = __reduce_max_sync(0xffffffffu, SETS == 2 ? max(hi_pos[0], hi_pos[SETS - 1]) : hi_pos[0]);
+            int lo = lo_pos[0][0], hi = hi_pos[0][0];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) { lo = min(lo, min(lo_pos[nt][0], lo_pos[nt][1])); hi = max(hi, max(hi_pos[nt][0], hi_pos[nt][1])); }
+            lo = __reduce_min_sync(0xffffffffu, lo);
+            hi = __reduce_max_sync(0xffffffffu, hi);
             uint16_t* const sv = reinterpret_cast<uint16_t*>(slot + part + gv * kPlane);
             for (int k = lane; k < gv * kPage; k += 32) {
                 const int pos = pos0 + k % kPage;
@@ -301,47 +365,66 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         }
-        float S[SETS][8][2];
+        const uint32_t base = pinned(smem_u32(slot));
+        // scales of a pair of groups, of tokens i of four eights: the transposing load finds the pair's planes in its odd and even rows
+        auto pair_scales = [&](uint32_t scales, int g, int groups, int h, uint32_t (&sc)[4]) {
+            ldmatrix4_trans(scales + min(g + lane % 2, groups - 1) * kScales + h * 64 + (lane / 8) * 16, sc);
+        };
+        float S[NT][8][2];                                 // token i of each eight
 #pragma unroll
-        for (int set = 0; set < SETS; ++set)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int t = 0; t < 8; ++t) S[set][t][0] = S[set][t][1] = 0.f;
-        // scores
+            for (int t = 0; t < 8; ++t) S[nt][t][0] = S[nt][t][1] = 0.f;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            if (g >= gk) break;
-            const uint32_t codes = base + g * kPlane + lane * 16, scales = base + gk * kPlane + g * kScales + (lane / 8) * 16;
+        for (int h = 0; h < 2; ++h) {
+            uint32_t sc[4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t w[4], sc[4];
-                ldmatrix4(codes + h * 512, w);
-                ldmatrix4(scales + h * 64, sc);
+            for (int g = 0; g < NG; ++g) {
+                if (g >= gk) break;
+                if (g % 2 == 0) pair_scales(base + gk * kPlane, g, gk, h, sc);
+                uint32_t w[4];
+                ldmatrix4(base + g * kPlane + lane * 16 + h * 512, w);
+                float d[NT][2][4];                         // (products that do not wait for one another side by side)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    float d[4];
-                    mma16(d, Q[2 * g][0], Q[2 * g][1], Q[2 * g][2], Q[2 * g][3], w[t] & 0x000f000fu, w[t] & 0x00f000f0u, qc[g][0], qc[g][0], qc[g][1], qc[g][1]);
-                    const uint32_t u = w[t] >> 8;
-                    mma16(d, Q[2 * g + 1][0], Q[2 * g + 1][1], Q[2 * g + 1][2], Q[2 * g + 1][3], u & 0x000f000fu, u & 0x00f000f0u);
-                    const float s0 = low_bf16(sc[t]), s1 = high_bf16(sc[t]);
-                    if (TWO) { d[0] += d[2]; d[1] += d[3]; }
-                    S[0][h * 4 + t][0] = fmaf(d[0], s0, S[0][h * 4 + t][0]);
-                    S[0][h * 4 + t][1] = fmaf(d[1], s1, S[0][h * 4 + t][1]);
-                    if (SETS == 2) {
-                        S[SETS - 1][h * 4 + t][0] = fmaf(d[2], s0, S[SETS - 1][h * 4 + t][0]);
-                        S[SETS - 1][h * 4 + t][1] = fmaf(d[3], s1, S[SETS - 1][h * 4 + t][1]);
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint32_t a0 = w[2 * k] & 0x000f000fu, a1 = w[2 * k + 1] & 0x000f000fu, a2 = w[2 * k] & 0x00f000f0u, a3 = w[2 * k + 1] & 0x00f000f0u;
+                        const auto& q = Q[nt][2 * g];
+                        mma16(d[nt][k], a0, a1, a2, a3, q[0], q[1], QC[nt][g][0], QC[nt][g][1], QC[nt][g][0], QC[nt][g][1]);
+                        if constexpr (TWO) mma16(d[nt][k], a0, a1, a2, a3, q[2], q[3]);
+                    }
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint32_t u0 = w[2 * k] >> 8, u1 = w[2 * k + 1] >> 8;
+                        const uint32_t a0 = u0 & 0x000f000fu, a1 = u1 & 0x000f000fu, a2 = u0 & 0x00f000f0u, a3 = u1 & 0x00f000f0u;
+                        const auto& q = Q[nt][2 * g + 1];
+                        mma16(d[nt][k], a0, a1, a2, a3, q[0], q[1]);
+                        if constexpr (TWO) mma16(d[nt][k], a0, a1, a2, a3, q[2], q[3]);
+                    }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float s0 = g % 2 ? high_bf16(sc[2 * k]) : low_bf16(sc[2 * k]), s1 = g % 2 ? high_bf16(sc[2 * k + 1]) : low_bf16(sc[2 * k + 1]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float(&x)[2] = S[nt][4 * h + 2 * k], (&y)[2] = S[nt][4 * h + 2 * k + 1];
+                        x[0] = fmaf(d[nt][k][0], s0, x[0]); x[1] = fmaf(d[nt][k][1], s0, x[1]);
+                        y[0] = fmaf(d[nt][k][2], s1, y[0]); y[1] = fmaf(d[nt][k][3], s1, y[1]);
                     }
                 }
             }
         }
         if (edge) {
 #pragma unroll
-            for (int set = 0; set < SETS; ++set)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int t = 0; t < 8; ++t)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const int pos = pos0 + t * 8 + 2 * j4 + e;
-                        if (pos < lo_pos[set] || pos > hi_pos[set]) S[set][t][e] = -INFINITY;
+                        const int pos = pos0 + t * 8 + i8;
+                        if (pos < lo_pos[nt][e] || pos > hi_pos[nt][e]) S[nt][t][e] = -INFINITY;
                     }
         }
         // the largest scale of values: a lane looks at eight of them
@@ -365,165 +448,196 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                 const int to = __reduce_max_sync(0xffffffffu, e), by = max(e_v - to, -252);
                 const float f = power_of_two(by / 2), f2 = power_of_two(by - by / 2);
 #pragma unroll
-                for (int set = 0; set < SETS; ++set) {
-                    scale_values(set, f, f);
-                    scale_values(set, f2, f2);
-                    l[set] = l[set] * f * f2;
+                for (int nt = 0; nt < NT; ++nt) {
+                    scale_values(nt, f, f);
+                    scale_values(nt, f2, f2);
+                    l[nt][0] = l[nt][0] * f * f2; l[nt][1] = l[nt][1] * f * f2;
                 }
                 e_v = to;
             }
         }
         // weights relative to the running maximum, which moves where it would have to by more than 2^8
-        const int up = 7 - e_v;
         bool moves = false;
-        float top[SETS];
+        float top[NT][2];
 #pragma unroll
-        for (int set = 0; set < SETS; ++set) {
-            float t = S[set][0][0];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) t = fmaxf(t, fmaxf(S[set][k][0], S[set][k][1]));
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-            top[set] = t * cx[set];
-            moves |= top[set] > m[set] + 8.f || (m[set] == -INFINITY && top[set] > -INFINITY);
-        }
+            for (int e = 0; e < 2; ++e) {
+                float t = S[nt][0][e];
+#pragma unroll
+                for (int k = 1; k < 8; ++k) t = fmaxf(t, S[nt][k][e]);
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+                top[nt][e] = t * cx[nt][e];
+                moves |= top[nt][e] > m[nt][e] + 8.f || (m[nt][e] == -INFINITY && top[nt][e] > -INFINITY);
+            }
         if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
-            for (int set = 0; set < SETS; ++set) {
-                const float to = fmaxf(m[set], top[set]);
-                const float f = m[set] == -INFINITY ? 0.f : exp2_fast(m[set] - to);      // nothing so far: the numbers are 0
-                m[set] = to;
-                l[set] *= f;
-                scale_values(set, __shfl_sync(0xffffffffu, f, 8 * j4), __shfl_sync(0xffffffffu, f, 8 * j4 + 4));
+            for (int nt = 0; nt < NT; ++nt) {
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float to = fmaxf(m[nt][e], top[nt][e]);
+                    f[e] = m[nt][e] == -INFINITY ? 0.f : exp2_fast(m[nt][e] - to);      // nothing so far: the numbers are 0
+                    m[nt][e] = to;
+                    l[nt][e] *= f[e];
+                }
+                scale_values(nt, f[0], f[1]);
             }
         }
 #pragma unroll
-        for (int set = 0; set < SETS; ++set) {
-            const float off = m[set] == -INFINITY ? 0.f : (float)up - m[set];
+        for (int nt = 0; nt < NT; ++nt) {
+            const float up = (float)(7 - e_v), off0 = m[nt][0] == -INFINITY ? 0.f : up - m[nt][0], off1 = m[nt][1] == -INFINITY ? 0.f : up - m[nt][1];
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
-                S[set][t][0] = exp2_fast(fmaf(S[set][t][0], cx[set], off));
-                S[set][t][1] = exp2_fast(fmaf(S[set][t][1], cx[set], off));
-                l[set] += S[set][t][0] + S[set][t][1];
+                float(&x)[2] = S[nt][t];
+                fma2(x[0], x[1], x[0], x[1], cx[nt][0], cx[nt][1], off0, off1);
+                x[0] = exp2_fast(x[0]);
+                x[1] = exp2_fast(x[1]);
+                add2(l[nt][0], l[nt][1], x[0], x[1]);
             }
         }
-        // values
+        // values: 32 tokens, then group after group, so that products into the same accumulators lie apart
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            if (g >= gv) break;
-            const uint32_t codes = base + part + g * kPlane + lane * 16, scales = base + part + gv * kPlane + g * kScales + (lane / 8) * 16;
+        for (int h = 0; h < 2; ++h) {
+            uint32_t sc[4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t w[4], sc[4];
-                ldmatrix4_trans(codes + h * 512, w);
-                ldmatrix4(scales + h * 64, sc);
+            for (int g = 0; g < NG; ++g) {
+                if (g >= gv) break;
+                if (g % 2 == 0) pair_scales(base + part + gv * kPlane, g, gv, h, sc);
+                const uint32_t eights = i8 == g ? 0x00080008u : 0u;
+                uint32_t w[4];
+                ldmatrix4_trans(base + part + g * kPlane + lane * 16 + h * 512, w);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const uint32_t r0 = w[2 * k], r1 = w[2 * k + 1], u0 = r0 >> 8, u1 = r1 >> 8;
-                    const float s0 = low_bf16(sc[2 * k]), s1 = high_bf16(sc[2 * k]), s2 = low_bf16(sc[2 * k + 1]), s3 = high_bf16(sc[2 * k + 1]);
+                    const float s0 = g % 2 ? high_bf16(sc[2 * k]) : low_bf16(sc[2 * k]), s1 = g % 2 ? high_bf16(sc[2 * k + 1]) : low_bf16(sc[2 * k + 1]);
 #pragma unroll
-                    for (int set = 0; set < SETS; ++set) {
-                        const float(&p)[2] = S[set][h * 4 + 2 * k];
-                        const float(&q)[2] = S[set][h * 4 + 2 * k + 1];
-                        const float v0 = p[0] * s0, v1 = p[1] * s1, v2 = q[0] * s2, v3 = q[1] * s3;
-                        uint32_t b0 = halves(v0, v1), b1 = halves(v2, v3);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const float(&x)[2] = S[nt][4 * h + 2 * k], (&y)[2] = S[nt][4 * h + 2 * k + 1];
+                        const float v0 = x[0] * s0, v1 = x[1] * s0, v2 = y[0] * s1, v3 = y[1] * s1;
+                        const uint32_t p0 = halves(v0, v1), p1 = halves(v2, v3);
 #pragma unroll
                         for (int term = 0; term < (TWO ? 2 : 1); ++term) {
-                            mma16(O[set][2 * g], r0 & 0x000f000fu, r0 & 0x00f000f0u, r1 & 0x000f000fu, r1 & 0x00f000f0u, b0, b1);
-                            mma16(O[set][2 * g + 1], u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, b0, b1);
-                            mma16(OFF[set][g], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, b0, b1);
-                            if (TWO && term == 0) {
-                                const float2 h0 = unhalves(b0), h1 = unhalves(b1);
+                            uint32_t b0 = p0, b1 = p1;
+                            if (term == 1) {
+                                const float2 h0 = unhalves(p0), h1 = unhalves(p1);
                                 b0 = halves(v0 - h0.x, v1 - h0.y);
                                 b1 = halves(v2 - h1.x, v3 - h1.y);
                             }
+                            b0 = transposed(b0);
+                            b1 = transposed(b1);
+                            mma16(O[nt][2 * g], r0 & 0x000f000fu, r0 & 0x00f000f0u, r1 & 0x000f000fu, r1 & 0x00f000f0u, b0, b1);
+                            mma16(O[nt][2 * g + 1], u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, b0, b1);
+                            if constexpr (!TWO) {
+                                float t[4] = {OFF[nt][0][0], OFF[nt][0][1], OFF[nt][1][0], OFF[nt][1][1]};
+                                mma16(t, eights, 0u, eights, 0u, b0, b1);
+                                OFF[nt][0][0] = t[0]; OFF[nt][0][1] = t[1]; OFF[nt][1][0] = t[2]; OFF[nt][1][1] = t[3];
+                            }
+                        }
+                        if constexpr (TWO) {
+                            add2(OFF[nt][g][0], OFF[nt][g][1], v0, v1);
+                            add2(OFF[nt][g][0], OFF[nt][g][1], v2, v3);
                         }
                     }
                 }
             }
         }
+        // the slot's numbers have been read when these are known
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int t = 0; t < 2 * NG; ++t) asm volatile("" : "+f"(O[nt][t][0]), "+f"(O[nt][t][1]), "+f"(O[nt][t][2]), "+f"(O[nt][t][3]) : : "memory");
+#pragma unroll
+            for (int g = 0; g < (TWO ? NG : 2); ++g) asm volatile("" : "+f"(OFF[nt][g][0]), "+f"(OFF[nt][g][1]) : : "memory");
+        }
     };
 
     // ---- what a unit leaves: numbers 4 i .. 4 i + 3 of each group, of columns 2 j and 2 j + 1, before the division by the sum
-    auto number_at = [&](int set, int g, int t, int col) { return (O[set][2 * g + (t >> 1)][(t & 1) * 2 + col] * ((t & 1) ? 0.0625f : 1.f) - OFF[set][g][col]); };
+    auto over_tokens = [&](float v) {
+        v += __shfl_xor_sync(0xffffffffu, v, 4);
+        v += __shfl_xor_sync(0xffffffffu, v, 8);
+        return v + __shfl_xor_sync(0xffffffffu, v, 16);
+    };
+    auto offset_of = [&](int nt, int g, int e) {
+        if constexpr (TWO) return over_tokens(OFF[nt][g][e]) * 4.76837158203125e-07f;      // 8 2^-24
+        else return __shfl_sync(0xffffffffu, OFF[nt][0][e], g * 4 + j4);
+    };
+    auto number_at = [&](int nt, int g, int t, int e, float off) { return O[nt][2 * g + (t >> 1)][(t & 1) * 2 + e] * ((t & 1) ? 0.0625f : 1.f) - off; };
     auto finish_unit = [&](int s, int unit) {              // the whole unit was this warp's
         Sequence q;
         lengths_of(a, s, q);
-        const int cols = q.n * a.group, head = unit % a.kv_heads, col0 = unit / a.kv_heads * COLS;
+        const int cols = q.n * a.group, tile = unit / a.kv_heads, head = unit - tile * a.kv_heads;
 #pragma unroll
-        for (int set = 0; set < SETS; ++set) {
-            float sum = l[set];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            if (a.sink && m[set] != -INFINITY) sum += exp2_fast((float)(7 - e_v) - m[set]);
-            const float inv = dead ? __uint_as_float(0x7fc00000u) : m[set] == -INFINITY && sum == 0.f ? 0.f : __fdiv_rn(16777216.f, sum);
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float f = __shfl_sync(0xffffffffu, inv, 8 * j4 + 4 * e);
-                const int col = col0 + set * 8 + 2 * j4 + e;
+                float sum = over_tokens(l[nt][e]);
+                if (a.sink && m[nt][e] != -INFINITY) sum += exp2_fast((float)(7 - e_v) - m[nt][e]);
+                const float f = dead ? __uint_as_float(0x7fc00000u) : m[nt][e] == -INFINITY && sum == 0.f ? 0.f : __fdiv_rn(16777216.f, sum);
+                float off[NG];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) off[g] = offset_of(nt, g, e);
+                const int col = tile * COLS + nt * 8 + 2 * j4 + e, row = col / a.group, h = col - row * a.group;
                 if (col >= cols) continue;
-                T* const y = (T*)a.y + (long)(q.first + col / a.group) * a.ldy + (long)(head * a.group + col % a.group) * a.dv;
+                T* const y = (T*)a.y + (long)(q.first + row) * a.ldy + (long)(head * a.group + h) * a.dv;
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     if (g >= gv) break;
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const int d = g * kGroup + 4 * i8 + t;
-                        if (d < a.dv) y[d] = (T)(number_at(set, g, t, e) * f);
-                    }
+                    const int d = g * kGroup + 4 * i8;
+                    const float v[4] = {number_at(nt, g, 0, e, off[g]) * f, number_at(nt, g, 1, e, off[g]) * f, number_at(nt, g, 2, e, off[g]) * f, number_at(nt, g, 3, e, off[g]) * f};
+                    put_four(y + d, a.dv - d, a.wide_y, v);
                 }
             }
-        }
     };
     auto leave_part = [&](float* to) {
         const float by = power_of_two(e_v / 2), by2 = power_of_two(e_v - e_v / 2);          // back from 2^(7 - e_v)
 #pragma unroll
-        for (int set = 0; set < SETS; ++set) {
-            float sum = l[set];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            if (j4 == 0) {
-                to[set * 8 + i8] = m[set];
-                to[COLS + set * 8 + i8] = dead ? __uint_as_float(0x7fc00000u) : sum * 0.0078125f * by * by2;
-            }
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e) {
+                const int col = nt * 8 + 2 * j4 + e;
+                const float sum = over_tokens(l[nt][e]);
+                if (i8 == 0) {
+                    to[col] = m[nt][e];
+                    to[COLS + col] = dead ? __uint_as_float(0x7fc00000u) : sum * 0.0078125f * by * by2;
+                }
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     if (g >= gv) break;
+                    const float off = offset_of(nt, g, e);
                     float v[4];
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) v[t] = number_at(set, g, t, e) * 131072.f * by * by2;
-                    *reinterpret_cast<float4*>(to + 2 * COLS + (set * 8 + 2 * j4 + e) * pad + g * kGroup + 4 * i8) = make_float4(v[0], v[1], v[2], v[3]);
+                    for (int t = 0; t < 4; ++t) v[t] = number_at(nt, g, t, e, off) * 131072.f * by * by2;
+                    *reinterpret_cast<float4*>(to + 2 * COLS + col * pad + g * kGroup + 4 * i8) = make_float4(v[0], v[1], v[2], v[3]);
                 }
-        }
+            }
     };
 
     // ---- the warp's run
     float* const head_part = a.parts + (size_t)kMaxCtas * 2 * rec + ((size_t)cta * W + warp) * rec;
     uint32_t pending = 0, phases = 0;                      // bits of slots: a copy is on its way; parity of the next one's end
     Spot now{0, 0, 0, -1}, then{0, 0, 0, -1};              // of the 32 pages at hand, one per lane, and of the next 32
-    auto issue = [&](long long x, int slot, int page, int unit) {      // (uniform)
+    auto issue = [&](int x, int slot, int page, int unit) {      // (uniform)
         if (page < 0) return;
         pending |= 1u << slot;
         if (lane == 0) {
             mbar_expect_tx(&full[warp][slot], block);
-            if (x != a.skip) bulk_copy(smem_u32(ring) + slot * a.slot_bytes, a.kv + ((size_t)page * a.kv_heads + unit % a.kv_heads) * block, block, &full[warp][slot]);
+            if (a.skip < 0 || *x_lo_s + x != a.skip) bulk_copy(smem_u32(ring) + slot * a.slot_bytes, a.kv + ((size_t)page * a.kv_heads + unit % a.kv_heads) * block, block, &full[warp][slot]);
         }
     };
     int s = 0, unit = 0, pages = 0, page0 = 0;             // the unit at hand
-    long long unit_lo = -1, unit_hi = -1;                  // its pages of the line
-    if (x_lo < x_hi) {
-        long long batch = x_lo, asked = x_lo;
-        if (batch + lane < x_hi) now = find(batch + lane);
-        for (; asked < min(x_hi, x_lo + a.slots); ++asked) {
-            const int k = (int)(asked - batch);
-            issue(asked, k, __shfl_sync(0xffffffffu, now.page, k), __shfl_sync(0xffffffffu, now.unit, k));
-        }
+    int unit_lo = 0, unit_hi = 0;                          // its pages, counted from the run's first
+    if (run_n > 0) {
+        int batch = 0, asked = 0;
+        if (lane < run_n) now = find(*x_lo_s + lane);
+        __syncwarp();
+        for (; asked < min(run_n, a.slots); ++asked) issue(asked, asked, __shfl_sync(0xffffffffu, now.page, asked), __shfl_sync(0xffffffffu, now.unit, asked));
         int slot = 0;
-        for (long long x = x_lo; x < x_hi; ++x) {
-            const int k = (int)(x - batch), p = __shfl_sync(0xffffffffu, now.p, k);
-            if (x == x_lo || p == 0) {
+        for (int x = 0; x < run_n; ++x) {
+            const int k = x - batch, p = __shfl_sync(0xffffffffu, now.p, k);
+            if (x == 0 || p == 0) {
                 s = __shfl_sync(0xffffffffu, now.s, k);
                 unit = __shfl_sync(0xffffffffu, now.unit, k);
                 bool bad;
@@ -532,7 +646,7 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                 unit_lo = x - p; unit_hi = unit_lo + pages;
                 begin_unit(q, unit);
             }
-            if (k == 8 && batch + 32 < x_hi && batch + 32 + lane < x_hi) then = find(batch + 32 + lane);
+            if (k == 8 && batch + 32 + lane < run_n) then = find(*x_lo_s + batch + 32 + lane);
             __syncwarp();
             if (pending >> slot & 1) {
                 if (!dead) dead = __any_sync(0xffffffffu, !mbar_wait(&full[warp][slot], phases >> slot & 1, a.wait_ns));
@@ -544,15 +658,15 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                 }
             }
             if (p == pages - 1) {
-                if (unit_lo >= x_lo) finish_unit(s, unit);
-                else if (x + 1 < x_hi) {
+                if (unit_lo >= 0) finish_unit(s, unit);
+                else if (x + 1 < run_n) {
                     leave_part(head_part);
-                    if (lane == 0) heads_s[warp] = Open{unit_lo, unit_hi, s, unit};
+                    if (lane == 0) heads_s[warp] = Open{*x_lo_s + unit_lo, *x_lo_s + unit_hi, s, unit};
                 }
             }
             // the slot is free for the page `slots` further on
-            if (asked < x_hi && !dead) {
-                const int kk = (int)(asked - batch);
+            if (asked < run_n && !dead) {
+                const int kk = asked - batch;
                 const int page = __shfl_sync(0xffffffffu, kk < 32 ? now.page : then.page, kk & 31), u = __shfl_sync(0xffffffffu, kk < 32 ? now.unit : then.unit, kk & 31);
                 issue(asked, slot, page, u);
                 ++asked;
@@ -566,70 +680,88 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
             lost_s = 1;
             if (a.status != nullptr) atomicOr(a.status, STATUS_TIMEOUT);
         }
-        const bool open = unit_hi > x_hi || unit_lo < x_lo;    // the last unit goes on, or began ahead and ends with the run
+        const bool open = unit_hi > run_n || unit_lo < 0;    // the last unit goes on, or began ahead and ends with the run
         if (open) {
             leave_part(reinterpret_cast<float*>(ring));
-            if (lane == 0) tails_s[warp] = Open{unit_lo, unit_hi, s, unit};
+            if (lane == 0) tails_s[warp] = Open{*x_lo_s + unit_lo, *x_lo_s + unit_hi, s, unit};
         }
     }
     __syncthreads();
 
-    // ---- parts of units, joined: numbers 4 at a time, a column's weights by each thread for itself
-    auto put_numbers = [&](int s, int unit, int col, int d, float4 v, float m, float sum) {      // sums over all of the unit
+    // ---- parts of units, joined, four numbers of a column at a time
+    // Open units of the CTA in their order: each begins with a head of a run (only the first run's, of a unit of CTAs ahead) or with a tail.
+    if (warp == 0) {
+        bool first = false;
+        const int w = lane / 2, tail = lane % 2;
+        if (w < W) {
+            const long long lo = tail ? tails_s[w].lo : heads_s[w].lo;
+            first = lo >= 0;
+            for (int v = 0; v < w; ++v) first &= tails_s[v].lo != lo;
+        }
+        const uint32_t all = __ballot_sync(0xffffffffu, first);
+        if (first) opens_s[__popc(all & ((1u << lane) - 1))] = lane;
+        if (lane == 0) n_open_s = __popc(all);
+    }
+    __syncthreads();
+    const int n_open = n_open_s, items = COLS * pad / 4;
+    const long long all_pages = line_s[0], cta_lo = line_s[1], cta_hi = line_s[2];
+    const int sharers = (int)min((long long)gridDim.x, quotient(all_pages + W - 1, W));
+    auto put_numbers = [&](const Open& u, int col, int d, float4 v, float m, float sum) {      // sums over all of the unit
         Sequence q;
-        lengths_of(a, s, q);
-        const int cols = q.n * a.group, head = unit % a.kv_heads;
-        col += unit / a.kv_heads * COLS;
+        lengths_of(a, u.s, q);
+        const int cols = q.n * a.group, tile = u.unit / a.kv_heads, head = u.unit - tile * a.kv_heads;
+        col += tile * COLS;
         if (col >= cols) return;
         if (a.sink && m != -INFINITY) sum += exp2_fast(-m);
         const float f = lost_s ? __uint_as_float(0x7fc00000u) : m == -INFINITY && sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-        T* const y = (T*)a.y + (long)(q.first + col / a.group) * a.ldy + (long)(head * a.group + col % a.group) * a.dv + d;
+        const int row = col / a.group, h = col - row * a.group;
         const float t[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) if (d + i < a.dv) y[i] = (T)t[i];
+        put_four((T*)a.y + (long)(q.first + row) * a.ldy + (long)(head * a.group + h) * a.dv + d, a.dv - d, a.wide_y, t);
     };
-    // adds a part, given its largest score, to sums relative to m
-    auto join = [](float& m, float& sum, float4& o, float pm, float ps, float4 po) {
-        const float to = fmaxf(m, pm), f = m == -INFINITY ? 0.f : exp2_fast(m - to), g = pm == -INFINITY ? 0.f : exp2_fast(pm - to);
-        m = to;
-        sum = sum * f + (ps == ps ? ps * g : ps);
-        o.x = o.x * f + po.x * g; o.y = o.y * f + po.y * g; o.z = o.z * f + po.z * g; o.w = o.w * f + po.w * g;
+    // (a part that has seen nothing counts for nothing, unless its sum is no number)
+    auto weight = [](float pm, float m) { return pm == -INFINITY ? 0.f : exp2_fast(pm - m); };
+    auto add_part = [](float& sum, float4& o, float w, float ps, float4 po) {
+        sum += ps == ps ? ps * w : ps;
+        o.x = fmaf(po.x, w, o.x); o.y = fmaf(po.y, w, o.y); o.z = fmaf(po.z, w, o.z); o.w = fmaf(po.w, w, o.w);
     };
-    Open shared_units[2];
-    shared_units[0].lo = shared_units[1].lo = -1;
-    for (int w = 0; w < W; ++w)
-        for (int kind = 0; kind < 2; ++kind) {             // a run's head lies ahead of its tail
-            const Open u = kind == 0 ? heads_s[w] : tails_s[w];
-            if (u.lo < 0) continue;
-            bool first = true;
-            for (int v = 0; v < w; ++v) first &= tails_s[v].lo != u.lo;
-            if (!first) continue;
-            const bool whole = u.lo >= c_lo && u.hi <= c_hi;
-            const int place = u.lo < c_lo ? 0 : 1;
-            float* const to = a.parts + ((size_t)cta * 2 + place) * rec;
-            for (int i = tid; i < COLS * pad / 4; i += NT) {
-                const int col = i * 4 / pad, d = i * 4 % pad;
-                float m = -INFINITY, sum = 0.f;
-                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int v = w; v < W; ++v)
-                    for (int k2 = v == w ? kind : 0; k2 < 2; ++k2) {
-                        if ((k2 == 0 ? heads_s[v].lo : tails_s[v].lo) != u.lo) continue;
-                        const float* const p = k2 == 0 ? a.parts + (size_t)kMaxCtas * 2 * rec + ((size_t)cta * W + v) * rec : reinterpret_cast<const float*>(sm + (size_t)v * a.slots * a.slot_bytes);
-                        join(m, sum, o, p[col], p[COLS + col], *reinterpret_cast<const float4*>(p + 2 * COLS + i * 4));
-                    }
-                if (whole) put_numbers(u.s, u.unit, col, d, o, m, sum);
-                else {
-                    *reinterpret_cast<float4*>(to + 2 * COLS + i * 4) = o;
-                    if (d == 0) { to[col] = m; to[COLS + col] = lost_s ? __uint_as_float(0x7fc00000u) : sum; }
-                }
+    for (int x = tid; x < n_open * items; x += THREADS) {
+        const int k = x / items, i = x - k * items, col = i * 4 / pad, d = i * 4 - col * pad, w0 = opens_s[k] / 2;
+        const bool head = opens_s[k] % 2 == 0;
+        const Open u = head ? heads_s[w0] : tails_s[w0];
+        // its parts: the first run's head; tails of runs from w0 on; the head of the run in which it ends
+        const float* const first_head = a.parts + (size_t)kMaxCtas * 2 * rec + ((size_t)cta * W + w0) * rec;
+        int w1 = w0;                                       // tails w0 .. w1 - 1 (empty runs between them have none)
+        const float* last_head = nullptr;
+        if (!head) {
+            for (int v = w0; v < W; ++v) {
+                if (tails_s[v].lo == u.lo) w1 = v + 1;
+                if (v > w0 && heads_s[v].lo == u.lo) last_head = a.parts + (size_t)kMaxCtas * 2 * rec + ((size_t)cta * W + v) * rec;
             }
-            if (!whole) shared_units[place] = u;
         }
-    // ---- units that CTAs share: who arrives last joins them, in their order
+        auto tail = [&](int v) { return reinterpret_cast<const float*>(sm + (size_t)v * a.slots * a.slot_bytes); };
+        float m = -INFINITY, sum = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (head) m = first_head[col];
+        if (last_head != nullptr) m = last_head[col];
+        for (int v = w0; v < w1; ++v) if (tails_s[v].lo == u.lo) m = fmaxf(m, tail(v)[col]);
+        if (head) add_part(sum, o, weight(m, m), first_head[COLS + col], *reinterpret_cast<const float4*>(first_head + 2 * COLS + i * 4));
+        for (int v = w0; v < w1; ++v)
+            if (tails_s[v].lo == u.lo) add_part(sum, o, weight(tail(v)[col], m), tail(v)[COLS + col], *reinterpret_cast<const float4*>(tail(v) + 2 * COLS + i * 4));
+        if (last_head != nullptr) add_part(sum, o, weight(last_head[col], m), last_head[COLS + col], *reinterpret_cast<const float4*>(last_head + 2 * COLS + i * 4));
+        if (u.lo >= cta_lo && u.hi <= cta_hi) put_numbers(u, col, d, o, m, sum);
+        else {
+            float* const to = a.parts + ((size_t)cta * 2 + (u.lo < cta_lo ? 0 : 1)) * rec;
+            *reinterpret_cast<float4*>(to + 2 * COLS + i * 4) = o;
+            if (d == 0) { to[col] = m; to[COLS + col] = lost_s ? __uint_as_float(0x7fc00000u) : sum; }
+        }
+    }
+    // ---- units that CTAs share: who arrives last joins them, in their order.  They are the CTA's first and last open ones.
     for (int place = 0; place < 2; ++place) {
-        const Open u = shared_units[place];
-        if (u.lo < 0) continue;                            // (the same for all threads)
-        const int c0 = (int)(((u.lo + 1) * ctas - 1) / total), c1 = (int)((u.hi * ctas - 1) / total);
+        if (n_open == 0) break;
+        const int k = opens_s[place == 0 ? 0 : n_open - 1];
+        const Open u = k % 2 == 0 ? heads_s[k / 2] : tails_s[k / 2];
+        if (place == 0 ? u.lo >= cta_lo : u.lo < cta_lo || u.hi <= cta_hi) continue;      // (the same for all threads)
+        const int c0 = (int)quotient((u.lo + 1) * sharers - 1, all_pages), c1 = (int)quotient(u.hi * sharers - 1, all_pages);
         __threadfence();
         __syncthreads();
         if (tid == 0) {
@@ -640,16 +772,19 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
         __syncthreads();
         if (!last_s) continue;
         __threadfence();
-        for (int i = tid; i < COLS * pad / 4; i += NT) {
-            const int col = i * 4 / pad, d = i * 4 % pad;
+        for (int i = tid; i < items; i += THREADS) {
+            const int col = i * 4 / pad, d = i * 4 - col * pad;
             float m = -INFINITY, sum = 0.f;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+            auto place_of = [&](int c) { return a.parts + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * rec; };
+#pragma unroll 8
+            for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(place_of(c) + col));
+#pragma unroll 8
             for (int c = c0; c <= c1; ++c) {
-                const float* const p = a.parts + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * rec;
-                join(m, sum, o, __ldcg(p + col), __ldcg(p + COLS + col), __ldcg(reinterpret_cast<const float4*>(p + 2 * COLS + i * 4)));
+                const float* const p = place_of(c);
+                add_part(sum, o, weight(__ldcg(p + col), m), __ldcg(p + COLS + col), __ldcg(reinterpret_cast<const float4*>(p + 2 * COLS + i * 4)));
             }
-            put_numbers(u.s, u.unit, col, d, o, m, sum);
+            put_numbers(u, col, d, o, m, sum);
         }
         __syncthreads();
     }
@@ -662,10 +797,10 @@ int32_t launch_step(AttendArgs a, uint64_t work, cudaStream_t st) {
     const int rec = part_floats(Shape::kCols, a.dv) * 4;
     a.slot_bytes = (std::max(kv4_block(a.dk, a.dv), rec) + 127) / 128 * 128;
     // 232448 bytes of shared memory per CTA, less what is declared in the kernel
-    a.slots = std::min(4, (int)((232448 - 1024 - W * (Shape::kStage + 360)) / (W * a.slot_bytes)));
+    a.slots = std::min(4, (int)((232448 - 1024 - W * 512) / (W * a.slot_bytes)));
     a.tickets = (int32_t*)work;
     a.parts = (float*)(work + 4096);
-    const size_t smem = (size_t)W * (a.slots * a.slot_bytes + Shape::kStage);
+    const size_t smem = (size_t)W * a.slots * a.slot_bytes;
     LUMI_CUDA(cudaFuncSetAttribute(kv4_step_kernel<T, NG, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const int ctas = std::min(kMaxCtas, sm_count());
     cudaLaunchConfig_t cfg = {};
@@ -731,6 +866,8 @@ extern "C" int32_t lumi_k_kv4_attention(uint64_t q, int32_t ldq, int32_t dtype, 
     a.table = (const int32_t*)page_table; a.row_start = (const int32_t*)row_start; a.tokens = (const int32_t*)tokens; a.status = (int32_t*)status;
     a.ldq = ldq; a.ldy = ldy; a.heads = heads; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.dk = dk; a.dv = dv;
     a.window = window; a.sink = sink != 0; a.nseq = nseq; a.rows = rows; a.max_new = max_new; a.n_pages = n_pages; a.width = pages_per_seq; a.scale = scale;
+    a.wide_q = (q & 15) == 0 && dk % 8 == 0 && (long)ldq * (f32 ? 4 : 2) % 16 == 0;
+    a.wide_y = (y & (f32 ? 15 : 7)) == 0 && dv % 4 == 0 && ldy % 4 == 0;
     a.few = 1 << 30; a.wait_ns = kWaitLimitNs; a.skip = -1;
     return f32 ? step<float>(a, work, (cudaStream_t)stream) : step<__nv_bfloat16>(a, work, (cudaStream_t)stream);
 }
