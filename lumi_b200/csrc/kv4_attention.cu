@@ -115,10 +115,6 @@ __device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, f
     asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
         : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
 }
-__device__ __forceinline__ void mul2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
-}
 __device__ __forceinline__ void add2(float& d0, float& d1, float a0, float a1) {
     asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%0, %1};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(d0), "+f"(d1) : "f"(a0), "f"(a1));
 }
@@ -181,7 +177,8 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
     __shared__ uint64_t full[W][4];
     __shared__ long long warp_pages[W];
     __shared__ Open heads_s[W], tails_s[W];                // units that began ahead of a warp's run and end in it; that its run ends with and that it does not hold whole
-    __shared__ int last_s, lost_s, n_open_s, opens_s[32];
+    __shared__ int lost_s, n_open_s;
+    __shared__ int4 opens_s[2 * W], shared_s[2];
     __shared__ long long line_s[3 + W];                    // pages of the line, the CTA's first and its end, runs' first ones: not kept in registers over the pages
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i8 = lane >> 2, j4 = lane & 3;
     uint8_t* const ring = sm + (size_t)warp * a.slots * a.slot_bytes;
@@ -221,7 +218,8 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
     const int ctas = (int)min((long long)gridDim.x, quotient(total + W - 1, W)), cta = blockIdx.x;
     if (cta >= ctas) return;
     const long long c_lo = quotient(total * cta, ctas), c_hi = quotient(total * (cta + 1), ctas);
-    auto warp_from = [&](int w) { return c_lo + quotient((c_hi - c_lo) * w, W); };
+    const int runs = (int)min((long long)W, c_hi - c_lo);    // runs that are not empty come first
+    auto warp_from = [&](int w) { return c_lo + quotient((c_hi - c_lo) * min(w, runs), runs); };
     const int run_n = (int)(warp_from(warp + 1) - warp_from(warp));
     if (lane == 0) line_s[3 + warp] = warp_from(warp);
     if (tid == 0) { line_s[0] = total; line_s[1] = c_lo; line_s[2] = c_hi; }
@@ -340,13 +338,6 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
         }
         e_v = -90;
     };
-    auto scale_values = [&](int nt, float f0, float f1) {
-#pragma unroll
-        for (int t = 0; t < 2 * NG; ++t) { O[nt][t][0] *= f0; O[nt][t][1] *= f1; O[nt][t][2] *= f0; O[nt][t][3] *= f1; }
-#pragma unroll
-        for (int g = 0; g < (TWO ? NG : 2); ++g) { OFF[nt][g][0] *= f0; OFF[nt][g][1] *= f1; }
-    };
-
     // ---- one page of the unit
     auto work_page = [&](uint8_t* slot, int pos0) {
         const bool edge = pos0 < first_full || pos0 + kPage - 1 > last_full;
@@ -428,6 +419,7 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                     }
         }
         // the largest scale of values: a lane looks at eight of them
+        int e_top;
         {
             uint32_t top = 0;
             const uint4* const sv = reinterpret_cast<const uint4*>(slot + part + gv * kPlane);
@@ -443,21 +435,10 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                     top = max(top, max(b0 < 0x7f80u ? b0 : 0u, b1 < 0x7f80u ? b1 : 0u));      // what is no number has no size
                 }
             }
-            const int e = min(127, (int)(top >> 7) - 126);     // the largest is below 2^e
-            if (__any_sync(0xffffffffu, e > e_v)) {
-                const int to = __reduce_max_sync(0xffffffffu, e), by = max(e_v - to, -252);
-                const float f = power_of_two(by / 2), f2 = power_of_two(by - by / 2);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    scale_values(nt, f, f);
-                    scale_values(nt, f2, f2);
-                    l[nt][0] = l[nt][0] * f * f2; l[nt][1] = l[nt][1] * f * f2;
-                }
-                e_v = to;
-            }
+            e_top = min(127, (int)(top >> 7) - 126);       // the largest is below 2^e
         }
-        // weights relative to the running maximum, which moves where it would have to by more than 2^8
-        bool moves = false;
+        // weights are relative to the running maximum, which moves where it would have to by more than 2^8, and to 2^(e_v - 7)
+        bool moves = e_top > e_v;
         float top[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -473,18 +454,27 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                 moves |= top[nt][e] > m[nt][e] + 8.f || (m[nt][e] == -INFINITY && top[nt][e] > -INFINITY);
             }
         if (__any_sync(0xffffffffu, moves)) {
+            const int to_e = max(e_v, __reduce_max_sync(0xffffffffu, e_top));
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float f[2];
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const float to = fmaxf(m[nt][e], top[nt][e]);
-                    f[e] = m[nt][e] == -INFINITY ? 0.f : exp2_fast(m[nt][e] - to);      // nothing so far: the numbers are 0
+                    top[nt][e] = m[nt][e] == -INFINITY ? 0.f : exp2_fast(0.5f * (m[nt][e] - to + (float)(e_v - to_e)));      // (nothing so far: the numbers are 0)
                     m[nt][e] = to;
-                    l[nt][e] *= f[e];
                 }
-                scale_values(nt, f[0], f[1]);
-            }
+            e_v = to_e;
+#pragma unroll 1
+            for (int twice = 0; twice < 2; ++twice)        // the factor's root: scales of values may differ by more than fp32's range
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float f0 = top[nt][0], f1 = top[nt][1];
+#pragma unroll
+                    for (int t = 0; t < 2 * NG; ++t) { O[nt][t][0] *= f0; O[nt][t][1] *= f1; O[nt][t][2] *= f0; O[nt][t][3] *= f1; }
+#pragma unroll
+                    for (int g = 0; g < (TWO ? NG : 2); ++g) { OFF[nt][g][0] *= f0; OFF[nt][g][1] *= f1; }
+                    l[nt][0] *= f0; l[nt][1] *= f1;
+                }
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -565,52 +555,33 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
         else return __shfl_sync(0xffffffffu, OFF[nt][0][e], g * 4 + j4);
     };
     auto number_at = [&](int nt, int g, int t, int e, float off) { return O[nt][2 * g + (t >> 1)][(t & 1) * 2 + e] * ((t & 1) ? 0.0625f : 1.f) - off; };
-    auto finish_unit = [&](int s, int unit) {              // the whole unit was this warp's
+    // to == nullptr: the whole unit was this warp's, rows of y; else a part of it
+    auto leave_unit = [&](int s, int unit, float* to) {
         Sequence q;
         lengths_of(a, s, q);
         const int cols = q.n * a.group, tile = unit / a.kv_heads, head = unit - tile * a.kv_heads;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float sum = over_tokens(l[nt][e]);
-                if (a.sink && m[nt][e] != -INFINITY) sum += exp2_fast((float)(7 - e_v) - m[nt][e]);
-                const float f = dead ? __uint_as_float(0x7fc00000u) : m[nt][e] == -INFINITY && sum == 0.f ? 0.f : __fdiv_rn(16777216.f, sum);
-                float off[NG];
-#pragma unroll
-                for (int g = 0; g < NG; ++g) off[g] = offset_of(nt, g, e);
-                const int col = tile * COLS + nt * 8 + 2 * j4 + e, row = col / a.group, h = col - row * a.group;
-                if (col >= cols) continue;
-                T* const y = (T*)a.y + (long)(q.first + row) * a.ldy + (long)(head * a.group + h) * a.dv;
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    if (g >= gv) break;
-                    const int d = g * kGroup + 4 * i8;
-                    const float v[4] = {number_at(nt, g, 0, e, off[g]) * f, number_at(nt, g, 1, e, off[g]) * f, number_at(nt, g, 2, e, off[g]) * f, number_at(nt, g, 3, e, off[g]) * f};
-                    put_four(y + d, a.dv - d, a.wide_y, v);
-                }
-            }
-    };
-    auto leave_part = [&](float* to) {
         const float by = power_of_two(e_v / 2), by2 = power_of_two(e_v - e_v / 2);          // back from 2^(7 - e_v)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int col = nt * 8 + 2 * j4 + e;
-                const float sum = over_tokens(l[nt][e]);
-                if (i8 == 0) {
-                    to[col] = m[nt][e];
-                    to[COLS + col] = dead ? __uint_as_float(0x7fc00000u) : sum * 0.0078125f * by * by2;
-                }
+                float sum = over_tokens(l[nt][e]) * 0.0078125f * by * by2;
+                if (to == nullptr && a.sink && m[nt][e] != -INFINITY) sum += exp2_fast(-m[nt][e]);
+                if (dead) sum = __uint_as_float(0x7fc00000u);
+                const float f = to != nullptr ? 1.f : m[nt][e] == -INFINITY && sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+                const int c8 = nt * 8 + 2 * j4 + e, col = tile * COLS + c8, row = col / a.group, h = col - row * a.group;
+                if (to != nullptr && i8 == 0) { to[c8] = m[nt][e]; to[COLS + c8] = sum; }
+                T* const y = (T*)a.y + (long)(q.first + row) * a.ldy + (long)(head * a.group + h) * a.dv;
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     if (g >= gv) break;
                     const float off = offset_of(nt, g, e);
                     float v[4];
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) v[t] = number_at(nt, g, t, e, off) * 131072.f * by * by2;
-                    *reinterpret_cast<float4*>(to + 2 * COLS + col * pad + g * kGroup + 4 * i8) = make_float4(v[0], v[1], v[2], v[3]);
+                    for (int t = 0; t < 4; ++t) v[t] = number_at(nt, g, t, e, off) * 131072.f * by * by2 * f;
+                    const int d = g * kGroup + 4 * i8;
+                    if (to != nullptr) *reinterpret_cast<float4*>(to + 2 * COLS + c8 * pad + d) = make_float4(v[0], v[1], v[2], v[3]);
+                    else if (col < cols) put_four(y + d, a.dv - d, a.wide_y, v);
                 }
             }
     };
@@ -630,13 +601,21 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
     int s = 0, unit = 0, pages = 0, page0 = 0;             // the unit at hand
     int unit_lo = 0, unit_hi = 0;                          // its pages, counted from the run's first
     if (run_n > 0) {
-        int batch = 0, asked = 0;
-        if (lane < run_n) now = find(*x_lo_s + lane);
-        __syncwarp();
-        for (; asked < min(run_n, a.slots); ++asked) issue(asked, asked, __shfl_sync(0xffffffffu, now.page, asked), __shfl_sync(0xffffffffu, now.unit, asked));
-        int slot = 0;
+        int batch = 0, asked = 0, slot = 0;
         for (int x = 0; x < run_n; ++x) {
-            const int k = x - batch, p = __shfl_sync(0xffffffffu, now.p, k);
+            const int k = x - batch;
+            if (x == 0 || k == 8) {                        // places of the first 32 pages; of the 32 behind these
+                const int at = x == 0 ? 0 : batch + 32;
+                Spot found{0, 0, 0, -1};
+                if (at + lane < run_n) found = find(*x_lo_s + at + lane);
+                __syncwarp();
+                if (x == 0) {
+                    now = found;
+#pragma unroll 1
+                    for (; asked < min(run_n, a.slots); ++asked) issue(asked, asked, __shfl_sync(0xffffffffu, now.page, asked), __shfl_sync(0xffffffffu, now.unit, asked));
+                } else then = found;
+            }
+            const int p = __shfl_sync(0xffffffffu, now.p, k);
             if (x == 0 || p == 0) {
                 s = __shfl_sync(0xffffffffu, now.s, k);
                 unit = __shfl_sync(0xffffffffu, now.unit, k);
@@ -646,8 +625,6 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                 unit_lo = x - p; unit_hi = unit_lo + pages;
                 begin_unit(q, unit);
             }
-            if (k == 8 && batch + 32 + lane < run_n) then = find(*x_lo_s + batch + 32 + lane);
-            __syncwarp();
             if (pending >> slot & 1) {
                 if (!dead) dead = __any_sync(0xffffffffu, !mbar_wait(&full[warp][slot], phases >> slot & 1, a.wait_ns));
                 if (!dead) {
@@ -657,12 +634,17 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                     __syncwarp();
                 }
             }
-            if (p == pages - 1) {
-                if (unit_lo >= 0) finish_unit(s, unit);
-                else if (x + 1 < run_n) {
-                    leave_part(head_part);
-                    if (lane == 0) heads_s[warp] = Open{*x_lo_s + unit_lo, *x_lo_s + unit_hi, s, unit};
+            // the unit ends here, or the run does
+            if (p == pages - 1 || x == run_n - 1) {
+                float* to = nullptr;
+                if (unit_lo < 0 || p < pages - 1) {
+                    to = x + 1 < run_n ? head_part : reinterpret_cast<float*>(ring);
+                    if (x == run_n - 1)                    // (only after a wait gave up: copies in flight land before their places are used again)
+#pragma unroll 1
+                        for (int i = 0; i < a.slots; ++i) if (pending >> i & 1) mbar_wait(&full[warp][i], phases >> i & 1, a.wait_ns);
+                    if (lane == 0) (x + 1 < run_n ? heads_s : tails_s)[warp] = Open{*x_lo_s + unit_lo, *x_lo_s + unit_hi, s, unit};
                 }
+                leave_unit(s, unit, to);
             }
             // the slot is free for the page `slots` further on
             if (asked < run_n && !dead) {
@@ -674,38 +656,41 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
             if (k == 31) { now = then; batch += 32; }
             slot = slot + 1 == a.slots ? 0 : slot + 1;
         }
-        for (int i = 0; i < a.slots; ++i)                  // (only after a wait gave up: copies in flight land before the CTA ends)
-            if (pending >> i & 1) mbar_wait(&full[warp][i], phases >> i & 1, a.wait_ns);
-        if (dead && lane == 0) {
-            lost_s = 1;
-            if (a.status != nullptr) atomicOr(a.status, STATUS_TIMEOUT);
-        }
-        const bool open = unit_hi > run_n || unit_lo < 0;    // the last unit goes on, or began ahead and ends with the run
-        if (open) {
-            leave_part(reinterpret_cast<float*>(ring));
-            if (lane == 0) tails_s[warp] = Open{*x_lo_s + unit_lo, *x_lo_s + unit_hi, s, unit};
+        if (dead) {
+#pragma unroll 1
+            for (int i = 0; i < a.slots; ++i) if (pending >> i & 1) mbar_wait(&full[warp][i], phases >> i & 1, a.wait_ns);
+            if (lane == 0) {
+                lost_s = 1;
+                if (a.status != nullptr) atomicOr(a.status, STATUS_TIMEOUT);
+            }
         }
     }
     __syncthreads();
 
     // ---- parts of units, joined, four numbers of a column at a time
-    // Open units of the CTA in their order: each begins with a head of a run (only the first run's, of a unit of CTAs ahead) or with a tail.
+    // Open units of the CTA in their order: each begins with a head of a run (only the first run's, of a unit of CTAs ahead) or with a tail, goes on with tails and may end with a head.
     if (warp == 0) {
         bool first = false;
+        int last_tail = -1, last_head = -1;
         const int w = lane / 2, tail = lane % 2;
         if (w < W) {
             const long long lo = tail ? tails_s[w].lo : heads_s[w].lo;
             first = lo >= 0;
             for (int v = 0; v < w; ++v) first &= tails_s[v].lo != lo;
+            for (int v = w; v < W; ++v) {
+                if (tails_s[v].lo == lo) last_tail = v;
+                if ((v > w || !tail) && heads_s[v].lo == lo) last_head = v;
+            }
         }
         const uint32_t all = __ballot_sync(0xffffffffu, first);
-        if (first) opens_s[__popc(all & ((1u << lane) - 1))] = lane;
+        if (first) opens_s[__popc(all & ((1u << lane) - 1))] = make_int4(w, tail ? last_tail : w - 1, last_head, 0);
         if (lane == 0) n_open_s = __popc(all);
     }
     __syncthreads();
     const int n_open = n_open_s, items = COLS * pad / 4;
     const long long all_pages = line_s[0], cta_lo = line_s[1], cta_hi = line_s[2];
     const int sharers = (int)min((long long)gridDim.x, quotient(all_pages + W - 1, W));
+    auto open_unit = [&](int k) { const int4 o = opens_s[k]; return o.y < o.x ? heads_s[o.z] : tails_s[o.x]; };
     auto put_numbers = [&](const Open& u, int col, int d, float4 v, float m, float sum) {      // sums over all of the unit
         Sequence q;
         lengths_of(a, u.s, q);
@@ -725,29 +710,18 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
         o.x = fmaf(po.x, w, o.x); o.y = fmaf(po.y, w, o.y); o.z = fmaf(po.z, w, o.z); o.w = fmaf(po.w, w, o.w);
     };
     for (int x = tid; x < n_open * items; x += THREADS) {
-        const int k = x / items, i = x - k * items, col = i * 4 / pad, d = i * 4 - col * pad, w0 = opens_s[k] / 2;
-        const bool head = opens_s[k] % 2 == 0;
-        const Open u = head ? heads_s[w0] : tails_s[w0];
-        // its parts: the first run's head; tails of runs from w0 on; the head of the run in which it ends
-        const float* const first_head = a.parts + (size_t)kMaxCtas * 2 * rec + ((size_t)cta * W + w0) * rec;
-        int w1 = w0;                                       // tails w0 .. w1 - 1 (empty runs between them have none)
-        const float* last_head = nullptr;
-        if (!head) {
-            for (int v = w0; v < W; ++v) {
-                if (tails_s[v].lo == u.lo) w1 = v + 1;
-                if (v > w0 && heads_s[v].lo == u.lo) last_head = a.parts + (size_t)kMaxCtas * 2 * rec + ((size_t)cta * W + v) * rec;
-            }
-        }
-        auto tail = [&](int v) { return reinterpret_cast<const float*>(sm + (size_t)v * a.slots * a.slot_bytes); };
-        float m = -INFINITY, sum = 0.f;
+        const int k = x / items, i = x - k * items, col = i * 4 / pad, d = i * 4 - col * pad;
+        const int4 parts = opens_s[k];                     // tails x .. y, head z
+        const Open u = open_unit(k);
+        const float* const head = a.parts + (size_t)kMaxCtas * 2 * rec + ((size_t)cta * W + max(parts.z, 0)) * rec;
+        auto tail = [&](int v) { return reinterpret_cast<const float*>(sm + v * a.slots * a.slot_bytes); };
+        float m = parts.z >= 0 ? head[col] : -INFINITY, sum = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (head) m = first_head[col];
-        if (last_head != nullptr) m = last_head[col];
-        for (int v = w0; v < w1; ++v) if (tails_s[v].lo == u.lo) m = fmaxf(m, tail(v)[col]);
-        if (head) add_part(sum, o, weight(m, m), first_head[COLS + col], *reinterpret_cast<const float4*>(first_head + 2 * COLS + i * 4));
-        for (int v = w0; v < w1; ++v)
-            if (tails_s[v].lo == u.lo) add_part(sum, o, weight(tail(v)[col], m), tail(v)[COLS + col], *reinterpret_cast<const float4*>(tail(v) + 2 * COLS + i * 4));
-        if (last_head != nullptr) add_part(sum, o, weight(last_head[col], m), last_head[COLS + col], *reinterpret_cast<const float4*>(last_head + 2 * COLS + i * 4));
+#pragma unroll 4
+        for (int v = parts.x; v <= parts.y; ++v) m = fmaxf(m, tail(v)[col]);
+#pragma unroll 4
+        for (int v = parts.x; v <= parts.y; ++v) add_part(sum, o, weight(tail(v)[col], m), tail(v)[COLS + col], *reinterpret_cast<const float4*>(tail(v) + 2 * COLS + i * 4));
+        if (parts.z >= 0) add_part(sum, o, weight(head[col], m), head[COLS + col], *reinterpret_cast<const float4*>(head + 2 * COLS + i * 4));
         if (u.lo >= cta_lo && u.hi <= cta_hi) put_numbers(u, col, d, o, m, sum);
         else {
             float* const to = a.parts + ((size_t)cta * 2 + (u.lo < cta_lo ? 0 : 1)) * rec;
@@ -756,22 +730,25 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
         }
     }
     // ---- units that CTAs share: who arrives last joins them, in their order.  They are the CTA's first and last open ones.
-    for (int place = 0; place < 2; ++place) {
-        if (n_open == 0) break;
-        const int k = opens_s[place == 0 ? 0 : n_open - 1];
-        const Open u = k % 2 == 0 ? heads_s[k / 2] : tails_s[k / 2];
-        if (place == 0 ? u.lo >= cta_lo : u.lo < cta_lo || u.hi <= cta_hi) continue;      // (the same for all threads)
+    if (n_open == 0) return;
+    const Open ends[2] = {open_unit(0), open_unit(n_open - 1)};
+    const bool shared[2] = {ends[0].lo < cta_lo, ends[1].lo >= cta_lo && ends[1].hi > cta_hi};
+    if (!shared[0] && !shared[1]) return;
+    __threadfence();
+    __syncthreads();
+    if (tid < 2 && shared[tid]) {
+        const Open u = ends[tid];
         const int c0 = (int)quotient((u.lo + 1) * sharers - 1, all_pages), c1 = (int)quotient(u.hi * sharers - 1, all_pages);
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-            const int n = atomicAdd(a.tickets + c0, 1);
-            last_s = n == c1 - c0;
-            if (last_s) a.tickets[c0] = 0;
-        }
-        __syncthreads();
-        if (!last_s) continue;
-        __threadfence();
+        const bool last = atomicAdd(a.tickets + c0, 1) == c1 - c0;
+        if (last) a.tickets[c0] = 0;
+        shared_s[tid] = make_int4(c0, c1, last, 0);
+    }
+    __syncthreads();
+    __threadfence();
+    for (int place = 0; place < 2; ++place) {
+        if (!shared[place] || !shared_s[place].z) continue;
+        const Open u = ends[place];
+        const int c0 = shared_s[place].x, c1 = shared_s[place].y;
         for (int i = tid; i < items; i += THREADS) {
             const int col = i * 4 / pad, d = i * 4 - col * pad;
             float m = -INFINITY, sum = 0.f;
@@ -786,7 +763,6 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
             }
             put_numbers(u, col, d, o, m, sum);
         }
-        __syncthreads();
     }
 }
 
