@@ -18,7 +18,7 @@ CLI = os.path.join(LIBDIR, "lumi-infer-b200")
 
 SOURCES = ["api.cu", "kernels.cu", "gemm_tcgen05.cu", "gemm_few_rows.cu", "gemm_rows_f32.cu", "attention.cu", "decode_b1.cu", "block_static.cu", "prefill_ssd.cu", "prefill_rows.cu", "safetensors.cpp",
            "architectures.cpp", "sublayer.cu", "delta_rule.cu", "window_attention.cu", "block_product.cu", "retention.cu", "rglru.cu", "latent_attention.cu",
-           "moe.cu", "quant_rows.cu", "gemm_i8.cu", "kv4_cache.cu", "kv4_attention.cu", "block_norm.cu"]
+           "moe.cu", "quant_rows.cu", "gemm_i8.cu", "kv4_cache.cu", "kv4_attention.cu", "kv4_prompt.cu", "block_norm.cu"]
 HEADERS = ["internal.h", "json_min.h", "rows.cuh", "tf32.cuh", "tcgen05.cuh", "embed_post.cuh", "device_args.h", "kv4.cuh", os.path.join("..", "..", "include", "lumi_b200.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-ccbin", "/usr/bin/g++"]

@@ -15,71 +15,18 @@
 #include "device_args.h"
 #include "kv4.cuh"
 #include "rows.cuh"
-#include "tcgen05.cuh"
-
-#include <cuda_fp16.h>
 
 #include <algorithm>
 
 namespace lumi {
 namespace {
 
-constexpr int kMaxRows = 1 << 24;                          // numbers of parts of work are 32-bit numbers
-constexpr int kBadPage = 1;                                // bit of the status word: a page or a length outside of what the cache holds
 constexpr int kMaxCtas = 296;                              // of the step kernel: places for parts
-constexpr float kLog2e = 1.4426950408889634f;
+// Fewer pages than these for each CTA are taken by fewer CTAs (us of one sequence of 4000 tokens and four heads of 64, and of 8 x 1000 and eight of 128): 4 pages 16.8, 19.7; 6 16.5, 19.6;
+// 8 15.1, 16.7; 12 18.0, 20.3.
+constexpr int kCtaPages = 8;
+constexpr int kFewColumns = 32;                            // of a sequence, that the step kernel still takes
 
-struct AttendArgs {
-    const void* q; void* y;
-    const uint8_t* kv;
-    const int32_t *table, *row_start, *tokens;
-    int32_t* status;
-    int32_t* tickets;                                      // [kMaxCtas], zero between calls
-    float* parts;                                          // [kMaxCtas][2] parts of units that CTAs share, then [kMaxCtas][warps] of units that end within a warp's run
-    uint64_t wait_ns;
-    long ldq, ldy;
-    int heads, kv_heads, group, dk, dv, window, sink, nseq, rows, max_new, n_pages, width;
-    int few;                                               // columns per head of the cache up to which a sequence is the step kernel's
-    int wide_q, wide_y;                                    // rows and heads lie on boundaries of 16 bytes, of four numbers
-    int slots, slot_bytes;                                 // of a warp's ring
-    int skip;                                              // failure tests: the copy of this page of the line is not issued
-    float scale;
-};
-
-__device__ __forceinline__ float number(const float* p) { return *p; }
-__device__ __forceinline__ float number(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-// Eight numbers on a 16-byte boundary, or none.
-__device__ __forceinline__ void eight_numbers(const float* p, int n, float (&t)[8]) {
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-    if (n > 0) { x = reinterpret_cast<const float4*>(p)[0]; y = reinterpret_cast<const float4*>(p)[1]; }
-    t[0] = x.x; t[1] = x.y; t[2] = x.z; t[3] = x.w; t[4] = y.x; t[5] = y.y; t[6] = y.z; t[7] = y.w;
-}
-__device__ __forceinline__ void eight_numbers(const __nv_bfloat16* p, int n, float (&t)[8]) {
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (n > 0) x = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { t[2 * i] = __uint_as_float(u[i] << 16); t[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
-}
-// Four results of a row, of which it has n.
-__device__ __forceinline__ void put_four(float* p, int n, bool wide, const float (&t)[4]) {
-    if (wide && n >= 4) *reinterpret_cast<float4*>(p) = make_float4(t[0], t[1], t[2], t[3]);
-    else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) if (i < n) p[i] = t[i];
-    }
-}
-__device__ __forceinline__ void put_four(__nv_bfloat16* p, int n, bool wide, const float (&t)[4]) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(t[0], t[1]), b = __floats2bfloat162_rn(t[2], t[3]);
-    if (wide && n >= 4) *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-    else {
-        if (n > 0) p[0] = a.x;
-        if (n > 1) p[1] = a.y;
-        if (n > 2) p[2] = b.x;
-        if (n > 3) p[3] = b.y;
-    }
-}
-__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 // Matrix loads may be moved as the arithmetic around them allows; what orders them is their address, which comes from pinned() behind what they have to wait for.
 __device__ __forceinline__ uint32_t pinned(uint32_t a) {
     uint32_t b;
@@ -105,11 +52,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t u) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(v) : "r"(u));
     return v;
 }
-__device__ __forceinline__ uint32_t halves(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unhalves(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 // two fp32 operations in one
 __device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0, float c1) {
     asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
@@ -117,19 +59,6 @@ __device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, f
 }
 __device__ __forceinline__ void add2(float& d0, float& d1, float a0, float a1) {
     asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%0, %1};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(d0), "+f"(d1) : "f"(a0), "f"(a1));
-}
-__device__ __forceinline__ float low_bf16(uint32_t u) { return __uint_as_float(u << 16); }
-__device__ __forceinline__ float high_bf16(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
-__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
-
-// What a sequence is to the call.
-struct Sequence { int first, n, total, page0, pages, units; };
-__device__ __forceinline__ bool lengths_of(const AttendArgs& a, int s, Sequence& q) {      // false: they make no sense
-    q.first = a.row_start[s];
-    const int end = a.row_start[s + 1];
-    q.total = a.tokens[s];
-    q.n = end - q.first;
-    return q.first >= 0 && end >= q.first && end <= a.rows && q.total >= q.n && q.total <= (long)a.width * kPage;
 }
 // Pages that any of its rows sees, and units of `cols` columns.  Nothing of a sequence that is left out, or that is another kernel's.
 __device__ __forceinline__ Sequence step_sequence(const AttendArgs& a, int s, int cols, bool& bad) {
@@ -154,16 +83,8 @@ struct StepShape {
     static constexpr int kWarps = NG == 8 ? 6 : MODE == 1 ? (NG == 4 ? 8 : 12) : (NG == 4 ? 12 : 16);
 };
 
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
-}
-
 // One part of a unit: columns' largest score m (in units of log2), sum l and numbers o [column][dv], all relative to 2^m.  Where parts lie: m [cols], l [cols], o [cols][pad].
 __host__ __device__ inline int part_floats(int cols, int dv) { return cols * (2 + kv4_groups(dv) * kGroup); }
-
-__device__ __forceinline__ long long quotient(long long n, long long d) {       // of numbers that are nearly always small
-    return ((n | d) >> 32) == 0 ? (long long)((uint32_t)n / (uint32_t)d) : n / d;
-}
 
 struct Open { long long lo, hi; int s, unit; };
 
@@ -214,8 +135,8 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
     before[tid] = ahead + run - mine;
     if (tid == THREADS - 1) before[THREADS] = total;
     __syncthreads();
-    // CTAs that get work: a page per warp at least.  CTA c takes the pages from c total / ctas on.
-    const int ctas = (int)min((long long)gridDim.x, quotient(total + W - 1, W)), cta = blockIdx.x;
+    // CTAs that get work: some pages each.  CTA c takes the pages from c total / ctas on.
+    const int ctas = (int)min((long long)gridDim.x, quotient(total + kCtaPages - 1, kCtaPages)), cta = blockIdx.x;
     if (cta >= ctas) return;
     const long long c_lo = quotient(total * cta, ctas), c_hi = quotient(total * (cta + 1), ctas);
     const int runs = (int)min((long long)W, c_hi - c_lo);    // runs that are not empty come first
@@ -689,7 +610,7 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
     __syncthreads();
     const int n_open = n_open_s, items = COLS * pad / 4;
     const long long all_pages = line_s[0], cta_lo = line_s[1], cta_hi = line_s[2];
-    const int sharers = (int)min((long long)gridDim.x, quotient(all_pages + W - 1, W));
+    const int sharers = (int)min((long long)gridDim.x, quotient(all_pages + kCtaPages - 1, kCtaPages));
     auto open_unit = [&](int k) { const int4 o = opens_s[k]; return o.y < o.x ? heads_s[o.z] : tails_s[o.x]; };
     auto put_numbers = [&](const Open& u, int col, int d, float4 v, float m, float sum) {      // sums over all of the unit
         Sequence q;
@@ -844,6 +765,7 @@ extern "C" int32_t lumi_k_kv4_attention(uint64_t q, int32_t ldq, int32_t dtype, 
     a.window = window; a.sink = sink != 0; a.nseq = nseq; a.rows = rows; a.max_new = max_new; a.n_pages = n_pages; a.width = pages_per_seq; a.scale = scale;
     a.wide_q = (q & 15) == 0 && dk % 8 == 0 && (long)ldq * (f32 ? 4 : 2) % 16 == 0;
     a.wide_y = (y & (f32 ? 15 : 7)) == 0 && dv % 4 == 0 && ldy % 4 == 0;
-    a.few = 1 << 30; a.wait_ns = kWaitLimitNs; a.skip = -1;
-    return f32 ? step<float>(a, work, (cudaStream_t)stream) : step<__nv_bfloat16>(a, work, (cudaStream_t)stream);
+    a.few = kFewColumns; a.wait_ns = kWaitLimitNs; a.skip = -1;
+    LUMI_TRY(f32 ? step<float>(a, work, (cudaStream_t)stream) : step<__nv_bfloat16>(a, work, (cudaStream_t)stream));
+    return (long)max_new * a.group > a.few ? launch_kv4_prompt(a, f32, work, (cudaStream_t)stream) : LUMI_OK;
 }

@@ -1,0 +1,667 @@
+// Attention over the paged cache in 4 bits for many rows per sequence, on the tensor cores (tcgen05): prompts, and slices behind what a sequence holds already.
+//
+// A tile is 128 columns (a column: a row and a query head that reads the unit's cache head), two tiles of a unit at once for heads of up to 128 numbers.  CTAs take equal runs of the
+// line of pages of all units, whatever the lengths; a unit that CTAs share is joined by the one that arrives last.  Per page of 64 tokens:
+//
+//   copy warp        the page's block into a ring, by one bulk copy
+//   4 dequant warps  codes and scales to (n - 8) s as fp16 tiles of keys and values, times a power of two per page (keys) or per unit so far (values): exact, since a number has 3 + 8
+//                    significant bits, down to 2^-8 of the largest scale, and to 2^-19 of it below
+//   MMA warp         S = Q K^T (128 x 64 per tile), O += P V, P from tensor memory
+//   softmax warps    4 per tile, a thread per column: S from tensor memory, running maximum and sum, P back as fp16; O is scaled in place where the maximum moves by more than 2^8
+//
+// fp32 rows: q and P as two fp16 terms each, their products into the same accumulators (2^-22).  Products and exponentials need about the same time (16 exponentials per SM and clock,
+// 4096 multiply-adds): 1024 clocks each per page and two tiles at heads of 128.
+#include "device_args.h"
+#include "kv4.cuh"
+#include "rows.cuh"
+
+#include <algorithm>
+
+namespace lumi {
+namespace {
+
+constexpr int kTile = 128;
+constexpr int kPromptCtas = 160;                           // places for parts
+constexpr int kTicketsAt = 320;                            // behind the step kernel's
+constexpr int kRunPages = 4;                               // a CTA's, at least
+constexpr int kMaxRing = 4;
+
+template <int NG, bool TWO>
+struct PromptShape {
+    static constexpr int kTiles = NG <= 4 ? 2 : 1;
+    static constexpr int kCols = kTile * kTiles;
+    static constexpr int kTerms = TWO ? 2 : 1;
+    static constexpr int kBlocks = NG / 2;                 // of 64 numbers: one 128-byte row each
+    static constexpr int kBufs = NG == 8 && TWO ? 1 : 2;   // tiles of keys and of values
+    static constexpr int kQ = kTiles * kTerms * kBlocks * kTile * 128, kKv = kBlocks * kPage * 128;
+    static constexpr int kFixed = kQ + 2 * kBufs * kKv;
+    static constexpr int kThreads = (kTiles * 4 + 4 + 2) * 32;
+    // tensor memory: O of each tile, S, P
+    static constexpr int kO = NG * kGroup, kS = kTiles * kO, kP = kS + kTiles * kPage, kPCols = TWO ? 64 : 32;
+};
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+        "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// A from tensor memory
+__device__ __forceinline__ void umma_tmem_a(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Values: 64 numbers of a token are a 128-byte row (the operand's N), tokens go along K: groups of eight 1024 bytes apart, blocks of 64 numbers kPage * 128.
+__device__ __forceinline__ uint64_t values_desc(uint32_t addr) {
+    uint64_t d = make_smem_desc(addr) & ~((uint64_t)0x3fff << 16);
+    return d | (uint64_t)((kPage * 128) >> 4) << 16;
+}
+__device__ __forceinline__ void group_barrier(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+
+struct PageInfo { int e_k, e_v, absent; uint32_t no_number[2]; };      // exponents of keys and values; tokens with values that are no numbers
+
+struct Cursor { int s, head, tile, skip; };                // a unit, and pages of it that are the CTA's ahead
+
+template <typename T, int NG>
+__global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) kv4_prompt_kernel(const AttendArgs a, const int ring_n) {
+    constexpr bool TWO = sizeof(T) == 4;
+    using Shape = PromptShape<NG, TWO>;
+    constexpr int TILES = Shape::kTiles, COLS = Shape::kCols, TERMS = Shape::kTerms, BLOCKS = Shape::kBlocks, BUFS = Shape::kBufs, THREADS = Shape::kThreads;
+    extern __shared__ __align__(1024) uint8_t sm_raw[];
+    uint8_t* const sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
+    uint8_t *const q_sm = sm, *const k_sm = q_sm + Shape::kQ, *const v_sm = k_sm + BUFS * Shape::kKv, *const ring = v_sm + BUFS * Shape::kKv;
+    __shared__ uint64_t raw_full[kMaxRing], raw_empty[kMaxRing], k_full[2], k_empty[2], v_full[2], v_empty[2], q_full[2], s_full[2], s_empty[2], p_full[2], o_done[2], info_full[4], all_done;
+    __shared__ PageInfo info[4];
+    __shared__ int absent_s[kMaxRing];
+    __shared__ int red_s[4][2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int dead_flag, last_s[2];
+    __shared__ long long before[THREADS + 1], warp_pages[THREADS / 32];
+    __shared__ Cursor start_s;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    volatile int* const dead_s = &dead_flag;
+    const int gk = kv4_groups(a.dk), gv = kv4_groups(a.dv), part = kv4_part(a.dk), block = kv4_block(a.dk, a.dv), pad = gv * kGroup;
+
+    if (tid == 0) {
+        for (int i = 0; i < kMaxRing; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], 4); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 4); mbar_init(&v_empty[i], 1);
+            mbar_init(&q_full[i], 4); mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 4); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) mbar_init(&info_full[i], 4);
+        mbar_init(&all_done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        dead_flag = 0;
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_release();
+    pdl_sync();
+    const uint32_t tmem = tmem_slot;
+
+    // ---- the line of pages
+    auto unit_pages = [&](const Sequence& q, int tile, int& lo, int& hi) {
+        const int cols = q.n * a.group, row0 = tile * COLS / a.group, row1 = (min((tile + 1) * COLS, cols) - 1) / a.group;
+        lo = a.window > 0 ? max(0, q.total - q.n + row0 - a.window + 1) / kPage : 0;
+        hi = (q.total - q.n + row1) / kPage + 1;
+    };
+    auto tiles_of = [&](const Sequence& q) { return (q.n * a.group + COLS - 1) / COLS; };
+    // pages of one head; 0: nothing of this kernel's
+    auto head_pages = [&](int s, Sequence& q, bool& bad) {
+        bad = !lengths_of(a, s, q);
+        if (bad || q.n <= 0 || q.n > a.max_new || (long)q.n * a.group <= a.few) return 0ll;
+        long long sum = 0;
+        for (int t = 0, n = tiles_of(q); t < n; ++t) {
+            int lo, hi;
+            unit_pages(q, t, lo, hi);
+            sum += hi - lo;
+        }
+        return sum;
+    };
+    const int each = (a.nseq + THREADS - 1) / THREADS, s_lo = min(a.nseq, tid * each), s_hi = min(a.nseq, s_lo + each);
+    long long mine = 0;
+    for (int s = s_lo; s < s_hi; ++s) {
+        Sequence q;
+        bool bad;
+        mine += head_pages(s, q, bad) * a.kv_heads;
+    }
+    long long run = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const long long t = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += t; }
+    if (lane == 31) warp_pages[warp] = run;
+    __syncthreads();
+    long long ahead = 0, total = 0;
+    for (int w = 0; w < THREADS / 32; ++w) { const long long p = warp_pages[w]; if (w < warp) ahead += p; total += p; }
+    before[tid] = ahead + run - mine;
+    if (tid == 0) before[THREADS] = total;
+    __syncthreads();
+    const int ctas = (int)min((long long)gridDim.x, quotient(total + kRunPages - 1, kRunPages)), cta = blockIdx.x;
+    const bool works = cta < ctas;
+    const long long c_lo = works ? quotient(total * cta, ctas) : 0, c_hi = works ? quotient(total * (cta + 1), ctas) : 0;
+    if (works && mine > 0 && before[tid] <= c_lo && c_lo < before[tid] + mine) {      // one thread's sequences hold the CTA's first page
+        long long at = before[tid];
+        for (int s = s_lo; s < s_hi; ++s) {
+            Sequence q;
+            bool bad;
+            const long long per = head_pages(s, q, bad), n = per * a.kv_heads;
+            if (c_lo < at + n) {
+                long long rel = c_lo - at;
+                Cursor c;
+                c.s = s;
+                c.head = (int)quotient(rel, per);
+                rel -= c.head * per;
+                for (c.tile = 0;; ++c.tile) {
+                    int lo, hi;
+                    unit_pages(q, c.tile, lo, hi);
+                    if (rel < hi - lo) break;
+                    rel -= hi - lo;
+                }
+                c.skip = (int)rel;
+                start_s = c;
+                break;
+            }
+            at += n;
+        }
+    }
+    __syncthreads();
+
+    // ---- what all roles walk over: the CTA's share of one unit after another
+    struct Segment { Sequence q; int s, head, tile, cols, lo, hi, p0, p1; };      // pages lo .. hi of the unit, p0 .. p1 of them here
+    auto walk = [&](auto&& body) {
+        if (!works) return;
+        Cursor c = start_s;
+        long long left = c_hi - c_lo, at = c_lo;
+        while (left > 0) {
+            Segment g;
+            lengths_of(a, c.s, g.q);
+            g.s = c.s; g.head = c.head; g.tile = c.tile;
+            g.cols = g.q.n * a.group;
+            unit_pages(g.q, c.tile, g.lo, g.hi);
+            g.p0 = g.lo + c.skip;
+            g.p1 = g.p0 + (int)min(left, (long long)(g.hi - g.p0));
+            body(g, at - c.skip);
+            left -= g.p1 - g.p0;
+            at += g.p1 - g.p0;
+            if (left <= 0) break;
+            c.skip = 0;
+            if (++c.tile * COLS >= g.cols) {
+                c.tile = 0;
+                if (++c.head == a.kv_heads) {
+                    c.head = 0;
+                    Sequence q;
+                    do {
+                        ++c.s;                             // (there is one more: pages are left)
+                        if (!lengths_of(a, c.s, q)) continue;
+                    } while (c.s + 1 < a.nseq && !(lengths_of(a, c.s, q) && q.n > 0 && q.n <= a.max_new && (long)q.n * a.group > a.few));
+                }
+            }
+        }
+    };
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!*dead_s && !mbar_wait(bar, parity & 1, a.wait_ns)) *dead_s = 1;
+        __syncwarp();
+    };
+    auto arrive = [&](uint64_t* bar) {                     // one of four warps, all of its lanes
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+    };
+    int copied = 0;                                        // (copy warp) copies issued
+
+    if (warp < TILES * 4) {
+        // ---- softmax: a thread per column
+        const int tile = warp / 4, r = tid % kTile;
+        const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+        const uint32_t t_o = tmem + tile * Shape::kO + lanes, t_s = tmem + Shape::kS + tile * kPage + lanes, t_p = tmem + Shape::kP + tile * Shape::kPCols + lanes;
+        uint32_t pages = 0, done = 0;                      // of the CTA, of this tile
+        walk([&](const Segment& g, long long unit_lo) {
+            const int col0 = g.tile * COLS + tile * kTile, n_pages = g.p1 - g.p0;
+            if (col0 >= g.cols) { pages += n_pages; return; }
+            const int col = min(col0 + r, g.cols - 1), row = col / a.group, h = col - row * a.group;
+            const bool valid = col0 + r < g.cols;
+            const int pos = g.q.total - g.q.n + row, lo_pos = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+            const long out_row = g.q.first + row;
+            const int out_head = g.head * a.group + h;
+            // q: times a power of two that brings the column's largest to 2^13 .. 2^14
+            float cx;
+            {
+                const T* const p = (const T*)a.q + out_row * a.ldq + (long)out_head * a.dk;
+                auto eight = [&](int d, float(&t)[8]) {
+                    const int n = valid ? a.dk - d : 0;
+                    if (a.wide_q) eight_numbers(p + d, n, t);
+                    else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) t[e] = e < n ? number(p + d + e) : 0.f;
+                    }
+                };
+                uint32_t top = 0;
+#pragma unroll 4
+                for (int d = 0; d < a.dk; d += 8) {
+                    float t[8];
+                    eight(d, t);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(t[e]) & 0x7fffffffu);
+                }
+                const float by = power_of_two(top >= 0x7f800000u || top == 0 ? 0 : min(126, 13 + 127 - (int)(top >> 23)));
+                cx = fminf(fmaxf(__fdiv_rn(fabsf(a.scale) * kLog2e, by), 1e-37f), 3.4e38f);
+                const float f = a.scale < 0.f ? -by : by;
+#pragma unroll 2
+                for (int d = 0; d < gk * kGroup; d += 8) {
+                    float t[8];
+                    eight(d, t);
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = t[2 * e] * f, y = t[2 * e + 1] * f;
+                        hi[e] = halves(x, y);
+                        if (TWO) { const float2 b = unhalves(hi[e]); lo[e] = halves(x - b.x, y - b.y); }
+                    }
+                    uint8_t* const to = q_sm + ((tile * TERMS) * BLOCKS + d / 64) * (kTile * 128) + r * 128 + ((d / 8 % 8) ^ (r & 7)) * 16;
+                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if (TWO) *reinterpret_cast<uint4*>(to + BLOCKS * (kTile * 128)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                arrive(&q_full[tile]);
+            }
+            float m = -INFINITY, l = 0.f;
+            int e_v = 0;
+            for (int i = 0; i < n_pages; ++i, ++pages, ++done) {
+                wait(&s_full[tile], done);
+                wait(&info_full[pages % 4], pages / 4);
+                const PageInfo& of = info[pages % 4];
+                tc_fence_after();
+                float s[64];
+                tmem_ld32(t_s, reinterpret_cast<uint32_t(&)[32]>(s[0]));
+                tmem_ld32(t_s + 32, reinterpret_cast<uint32_t(&)[32]>(s[32]));
+                tc_fence_before();
+                arrive(&s_empty[tile]);
+                const int up = of.e_k + 9;
+                const float c = fmaxf(cx * power_of_two(up / 2) * power_of_two(up - up / 2), 1e-37f);
+                const int pos0 = (g.p0 + i) * kPage, new_e = of.e_v;
+                if (__any_sync(0xffffffffu, pos0 < lo_pos || pos0 + kPage - 1 > pos || of.absent)) {
+#pragma unroll
+                    for (int k = 0; k < 64; ++k)
+                        if (pos0 + k < lo_pos || pos0 + k > pos || of.absent) s[k] = -INFINITY;
+                }
+                float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int k = 4; k < 64; ++k) top[k % 4] = fmaxf(top[k % 4], s[k]);
+                const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+                const bool moves = t > m + 8.f || (m == -INFINITY && t > -INFINITY);
+                bool waited = i == 0;
+                if (__any_sync(0xffffffffu, moves || (i > 0 && new_e != e_v))) {
+                    const float to = moves ? t : m;
+                    const float f = m == -INFINITY ? 0.f : exp2_fast(m - to);
+                    const float fo = m == -INFINITY ? 0.f : exp2_fast(0.5f * (m - to + (float)(e_v - new_e)));
+                    m = to;
+                    l *= f;
+                    if (i > 0) {
+                        wait(&o_done[tile], done - 1);
+                        waited = true;
+                        tc_fence_after();
+                        for (int d = 0; d < pad; d += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(t_o + d, o);
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fo * fo);
+                            tmem_st32(t_o + d, o);
+                        }
+                        tmem_st_wait();
+                        tc_fence_before();
+                    }
+                }
+                e_v = new_e;
+                const float off = m == -INFINITY ? 0.f : -m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                uint32_t p[32];
+                if constexpr (TWO) {
+                    uint32_t lo[32];
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        const float x = exp2_fast(fmaf(s[2 * k], c, off)), y = exp2_fast(fmaf(s[2 * k + 1], c, off));
+                        sum[k % 2 * 2] += x; sum[k % 2 * 2 + 1] += y;
+                        p[k] = halves(x, y);
+                        const float2 b = unhalves(p[k]);
+                        lo[k] = halves(x - b.x, y - b.y);
+                    }
+                    if (!waited) wait(&o_done[tile], done - 1);
+                    tmem_st32(t_p, p);
+                    tmem_st32(t_p + 32, lo);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        const float x = exp2_fast(fmaf(s[2 * k], c, off)), y = exp2_fast(fmaf(s[2 * k + 1], c, off));
+                        sum[k % 2 * 2] += x; sum[k % 2 * 2 + 1] += y;
+                        p[k] = halves(x, y);
+                    }
+                    if (!waited) wait(&o_done[tile], done - 1);
+                    tmem_st32(t_p, p);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (of.no_number[0] | of.no_number[1])     // (rare) a row that sees such a token is none
+                    for (int k = 0; k < 64; ++k)
+                        if ((of.no_number[k / 32] >> (k % 32) & 1) && pos0 + k >= lo_pos && pos0 + k <= pos) l = __uint_as_float(0x7fc00000u);
+                tmem_st_wait();
+                tc_fence_before();
+                arrive(&p_full[tile]);
+            }
+            wait(&o_done[tile], done - 1);
+            tc_fence_after();
+            const int e = e_v + 9;                         // numbers are O 2^e / l
+            const float back = power_of_two(e / 2), back2 = power_of_two(e - e / 2);
+            auto put_row = [&](int d, const float (&o)[8], float f) {      // eight numbers as they lie in the tile
+                T* const y = (T*)a.y + out_row * a.ldy + (long)out_head * a.dv + d;
+                const float u[4] = {o[0] * f, o[2] * f, o[4] * f, o[6] * f}, v[4] = {o[1] * f, o[3] * f, o[5] * f, o[7] * f};
+                put_four(y, a.dv - d, a.wide_y, u);
+                put_four(y + 4, a.dv - d - 4, a.wide_y, v);
+            };
+            auto inverse = [&](float mm, float ll) {
+                if (a.sink && mm != -INFINITY) ll += exp2_fast(-mm);
+                return *dead_s ? __uint_as_float(0x7fc00000u) : mm == -INFINITY && ll == 0.f ? 0.f : __fdiv_rn(1.f, ll);
+            };
+            const bool whole = g.p0 == g.lo && g.p1 == g.hi;
+            const int places = COLS, at = tile * kTile + r;
+            const int rec = places * (2 + pad);
+            float* const to = a.parts + ((size_t)cta * 2 + (g.p0 == g.lo ? 1 : 0)) * rec;
+            const float inv = whole ? inverse(m, l) : 1.f;
+            for (int d = 0; d < pad; d += 32) {
+                uint32_t o[32];
+                tmem_ld32(t_o + d, o);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(o[8 * k + j]) * back * back2;
+                    if (whole) { if (valid) put_row(d + 8 * k, v, inv); }
+                    else {
+                        *reinterpret_cast<float4*>(to + 2 * places + ((d / 4 + 2 * k) * places + at) * 4) = make_float4(v[0], v[1], v[2], v[3]);
+                        *reinterpret_cast<float4*>(to + 2 * places + ((d / 4 + 2 * k + 1) * places + at) * 4) = make_float4(v[4], v[5], v[6], v[7]);
+                    }
+                }
+            }
+            tc_fence_before();
+            if (whole) return;
+            // ---- the unit is shared: who arrives last joins the parts, in the order of CTAs
+            to[at] = m;
+            to[places + at] = *dead_s ? __uint_as_float(0x7fc00000u) : l;
+            __threadfence();
+            group_barrier(1 + tile);
+            const long long unit_hi = unit_lo + (g.hi - g.lo);
+            const int c0 = (int)quotient((unit_lo + 1) * ctas - 1, total), c1 = (int)quotient(unit_hi * ctas - 1, total);
+            if (r == 0) {
+                int32_t* const ticket = a.tickets + kTicketsAt + c0 * 2 + tile;
+                last_s[tile] = atomicAdd(ticket, 1) == c1 - c0;
+                if (last_s[tile]) *ticket = 0;
+            }
+            group_barrier(1 + tile);
+            if (!last_s[tile]) return;
+            __threadfence();
+            auto place_of = [&](int k) { return a.parts + ((size_t)k * 2 + (k == c0 ? 1 : 0)) * rec; };
+            float mm = -INFINITY, ll = 0.f;
+#pragma unroll 4
+            for (int k = c0; k <= c1; ++k) mm = fmaxf(mm, __ldcg(place_of(k) + at));
+#pragma unroll 4
+            for (int k = c0; k <= c1; ++k) {
+                const float pm = __ldcg(place_of(k) + at), pl = __ldcg(place_of(k) + places + at);
+                ll += pl == pl ? pl * (pm == -INFINITY ? 0.f : exp2_fast(pm - mm)) : pl;
+            }
+            const float f = inverse(mm, ll);
+            if (valid)
+                for (int d = 0; d < pad; d += 8) {
+                    float o[8] = {};
+#pragma unroll 4
+                    for (int k = c0; k <= c1; ++k) {
+                        const float* const p = place_of(k);
+                        const float pm = __ldcg(p + at), w = pm == -INFINITY ? 0.f : exp2_fast(pm - mm);
+                        const float4 x = __ldcg(reinterpret_cast<const float4*>(p + 2 * places + (d / 4 * places + at) * 4)), y = __ldcg(reinterpret_cast<const float4*>(p + 2 * places + ((d / 4 + 1) * places + at) * 4));
+                        o[0] = fmaf(x.x, w, o[0]); o[1] = fmaf(x.y, w, o[1]); o[2] = fmaf(x.z, w, o[2]); o[3] = fmaf(x.w, w, o[3]);
+                        o[4] = fmaf(y.x, w, o[4]); o[5] = fmaf(y.y, w, o[5]); o[6] = fmaf(y.z, w, o[6]); o[7] = fmaf(y.w, w, o[7]);
+                    }
+                    put_row(d, o, f);
+                }
+        });
+    } else if (warp < TILES * 4 + 4) {
+        // ---- codes and scales to fp16 tiles
+        const int dt = tid - TILES * kTile, dw = dt / 32;
+        uint32_t pages = 0;
+        walk([&](const Segment& g, long long) {
+            int e_run = -90;
+            for (int p = g.p0; p < g.p1; ++p, ++pages) {
+                const int slot = pages % ring_n, live = min(kPage, g.q.total - p * kPage);      // tokens that have been written
+                const uint8_t* const raw = ring + slot * block;
+                wait(&raw_full[slot], pages / ring_n);
+                const bool absent = absent_s[slot] != 0;
+                // the largest scales
+                uint32_t top_k = 0, top_v = 0, none[2] = {0, 0};
+                if (!absent) {
+                    for (int w = dt; w < (gk + gv) * 32; w += 128) {
+                        const bool keys = w < gk * 32;
+                        const int tok = w % 32 * 2;
+                        const uint32_t u = *reinterpret_cast<const uint32_t*>(raw + (keys ? gk * kPlane : part + gv * kPlane) + (keys ? w : w - gk * 32) * 4);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            uint32_t b = (e ? u >> 16 : u) & 0x7fffu;
+                            if (tok + e >= live) b = 0;
+                            if (b >= 0x7f80u) { if (!keys) none[tok / 32] |= 1u << ((tok + e) % 32); b = 0; }
+                            if (keys) top_k = max(top_k, b); else top_v = max(top_v, b);
+                        }
+                    }
+                }
+                top_k = __reduce_max_sync(0xffffffffu, top_k);
+                top_v = __reduce_max_sync(0xffffffffu, top_v);
+                if (lane == 0) { red_s[dw][0] = (int)top_k; red_s[dw][1] = (int)top_v; }
+                PageInfo& to = info[pages % 4];
+                if (dt == 0) to.no_number[0] = to.no_number[1] = 0;
+                group_barrier(3);
+                if (none[0]) atomicOr(&to.no_number[0], none[0]);
+                if (none[1]) atomicOr(&to.no_number[1], none[1]);
+                const int mk = max(max(red_s[0][0], red_s[1][0]), max(red_s[2][0], red_s[3][0])), mv = max(max(red_s[0][1], red_s[1][1]), max(red_s[2][1], red_s[3][1]));
+                // scales are below 2^e; they become fp16 numbers below 2^15
+                const int e_k = max(-90, min(127, (mk >> 7) - 126));
+                e_run = max(e_run, max(-90, min(127, (mv >> 7) - 126)));
+                if (dt == 0) { to.e_k = e_k; to.e_v = e_run; to.absent = absent; }
+                const int buf = pages % BUFS;
+                auto tile_of = [&](bool keys) {
+                    const int groups = keys ? gk : gv;
+                    const uint8_t* const codes = raw + (keys ? 0 : part);
+                    uint8_t* const out = (keys ? k_sm : v_sm) + buf * Shape::kKv;
+                    const float by = power_of_two(15 - (keys ? e_k : e_run));
+                    for (int x = dt; x < groups * kPage; x += 128) {
+                        const int tok = x % kPage, grp = x / kPage;
+                        uint4 u = make_uint4(0, 0, 0, 0);
+                        float s = 0.f;
+                        if (!absent && tok < live) {
+                            u = *reinterpret_cast<const uint4*>(codes + grp * kPlane + tok * 16);
+                            const uint32_t bits = *reinterpret_cast<const uint16_t*>(codes + groups * kPlane + grp * kScales + tok * 2);
+                            s = __uint_as_float(bits << 16);
+                            if (!keys && (bits & 0x7fffu) >= 0x7f80u) s = 0.f;
+                        }
+                        const __half2 t = __float2half2_rn(s * by), t16 = __float2half2_rn(s * by * 0.0625f), t8 = __float2half2_rn(s * by * -4.76837158203125e-07f);      // -8 2^-24
+                        uint8_t* const row = out + grp / 2 * (kPage * 128) + tok * 128;
+                        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t c[4] = {w[j] & 0x000f000fu, w[j] & 0x00f000f0u, w[j] >> 8 & 0x000f000fu, w[j] >> 8 & 0x00f000f0u};
+                            uint32_t o[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&c[k]), k % 2 ? t16 : t, t8);
+                                o[k] = *reinterpret_cast<const uint32_t*>(&v);
+                            }
+                            *reinterpret_cast<uint4*>(row + ((grp % 2 * 4 + j) ^ (tok & 7)) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                };
+                wait(&k_empty[buf], pages / BUFS + 1);
+                tile_of(true);
+                group_barrier(3);                          // info is complete (and red_s has been read)
+                arrive(&k_full[buf]);
+                arrive(&info_full[pages % 4]);
+                wait(&v_empty[buf], pages / BUFS + 1);
+                tile_of(false);
+                arrive(&v_full[buf]);
+                arrive(&raw_empty[slot]);
+            }
+        });
+    } else if (warp == TILES * 4 + 4) {
+        // ---- products
+        const uint32_t id_s = (1u << 4) | ((uint32_t)(kPage >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+        const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(pad >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);      // B: numbers contiguous
+        uint32_t pages = 0, scores[2] = {0, 0}, outs[2] = {0, 0}, units[2] = {0, 0};
+        bool pending = false, pend_first = false, pend_live[2] = {false, false};
+        uint32_t pend_page = 0;
+        auto values = [&]() {
+            if (!pending) return;
+            pending = false;
+            const int buf = pend_page % BUFS;
+            wait(&v_full[buf], pend_page / BUFS);
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                if (!pend_live[t]) continue;
+                wait(&p_full[t], outs[t]);
+                ++outs[t];
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t v = smem_u32(v_sm) + buf * Shape::kKv;
+#pragma unroll
+                    for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+                        for (int k = 0; k < kPage / 16; ++k)
+                            umma_tmem_a(tmem + t * Shape::kO, tmem + Shape::kP + t * Shape::kPCols + term * 32 + k * 8, values_desc(v + k * 2048), id_o, !(pend_first && term == 0 && k == 0));
+                    umma_commit(&o_done[t]);
+                }
+                __syncwarp();
+            }
+            if (lane == 0) umma_commit(&v_empty[buf]);
+            __syncwarp();
+        };
+        walk([&](const Segment& g, long long) {
+            values();                                      // the unit ahead: its accumulators are read before this one's queries come
+            bool live[2];
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                live[t] = g.tile * COLS + t * kTile < g.cols;
+                if (live[t]) { wait(&q_full[t], units[t]); ++units[t]; }
+            }
+            for (int p = g.p0; p < g.p1; ++p, ++pages) {
+                const int buf = pages % BUFS;
+                wait(&k_full[buf], pages / BUFS);
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    if (!live[t]) continue;
+                    wait(&s_empty[t], scores[t] + 1);
+                    ++scores[t];
+                    tc_fence_after();
+                    if (lane == 0) {
+                        const uint32_t q = smem_u32(q_sm) + t * TERMS * BLOCKS * (kTile * 128), k = smem_u32(k_sm) + buf * Shape::kKv;
+#pragma unroll
+                        for (int term = 0; term < TERMS; ++term)
+                            for (int x = 0; x < 2 * gk; ++x)
+                                umma_bf16(tmem + Shape::kS + t * kPage, make_smem_desc(q + (term * BLOCKS + x / 4) * (kTile * 128) + x % 4 * 32),
+                                          make_smem_desc(k + x / 4 * (kPage * 128) + x % 4 * 32), id_s, !(term == 0 && x == 0));
+                        umma_commit(&s_full[t]);
+                    }
+                    __syncwarp();
+                }
+                if (lane == 0) umma_commit(&k_empty[buf]);
+                __syncwarp();
+                values();
+                pending = true; pend_page = pages; pend_first = p == g.p0;
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) pend_live[t] = live[t];
+            }
+        });
+        values();
+        if (lane == 0) umma_commit(&all_done);
+        __syncwarp();
+    } else {
+        // ---- copies
+        uint32_t pages = 0;
+        walk([&](const Segment& g, long long unit_lo) {
+            for (int p = g.p0; p < g.p1; ++p, ++pages) {
+                const int slot = pages % ring_n;
+                int page = lane == 0 ? a.table[(size_t)g.s * a.width + p] : 0;
+                wait(&raw_empty[slot], pages / ring_n + 1);
+                if (lane == 0 && !*dead_s) {
+                    const bool absent = page < 0 || page >= a.n_pages;
+                    absent_s[slot] = absent;
+                    if (absent) {
+                        if (a.status != nullptr) atomicOr(a.status, kBadPage);
+                        mbar_arrive(&raw_full[slot]);
+                    } else {
+                        mbar_expect_tx(&raw_full[slot], block);
+                        if (a.skip < 0 || unit_lo + (p - g.lo) != a.skip) bulk_copy(smem_u32(ring) + slot * block, a.kv + ((size_t)page * a.kv_heads + g.head) * block, block, &raw_full[slot]);
+                    }
+                    ++copied;
+                }
+                __syncwarp();
+            }
+        });
+    }
+    // ---- nothing may be under way when the CTA ends: products have ended, and after a wait that gave up so have copies
+    if (warp == TILES * 4 + 4) wait(&all_done, 0);
+    __syncthreads();
+    if (*dead_s && warp == TILES * 4 + 5 && lane == 0) {
+        mbar_wait(&all_done, 0, a.wait_ns);
+        for (int i = max(0, copied - ring_n); i < copied; ++i) mbar_wait(&raw_full[i % ring_n], (i / ring_n) & 1, a.wait_ns);
+        if (a.status != nullptr) atomicOr(a.status, STATUS_TIMEOUT);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+template <typename T, int NG>
+int32_t launch(AttendArgs a, uint64_t work, cudaStream_t st) {
+    using Shape = PromptShape<NG, sizeof(T) == 4>;
+    const int block = kv4_block(a.dk, a.dv);
+    // 232448 bytes of shared memory per CTA, less what is declared in the kernel and what alignment to 1024 bytes may cost
+    const int ring_n = std::min(kMaxRing, (232448 - 1024 - 5120 - Shape::kFixed) / block);
+    a.tickets = (int32_t*)work;
+    a.parts = (float*)(work + 4096);
+    const size_t smem = 1024 + Shape::kFixed + (size_t)ring_n * block;
+    LUMI_CUDA(cudaFuncSetAttribute(kv4_prompt_kernel<T, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3((unsigned)std::min(kPromptCtas, sm_count()));
+    cfg.blockDim = dim3(Shape::kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // the launch itself overlaps the kernel in front
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    LUMI_CUDA(cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<T, NG>, a, ring_n));
+    return LUMI_OK;
+}
+
+template <typename T>
+int32_t of_type(const AttendArgs& a, uint64_t work, cudaStream_t st) {
+    const int groups = std::max(kv4_groups(a.dk), kv4_groups(a.dv));
+    if (groups <= 2) return launch<T, 2>(a, work, st);
+    if (groups <= 4) return launch<T, 4>(a, work, st);
+    return launch<T, 8>(a, work, st);
+}
+
+}  // namespace
+
+int32_t launch_kv4_prompt(const AttendArgs& a, bool f32, uint64_t work, cudaStream_t st) { return f32 ? of_type<float>(a, work, st) : of_type<__nv_bfloat16>(a, work, st); }
+
+}  // namespace lumi
