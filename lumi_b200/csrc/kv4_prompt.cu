@@ -6,7 +6,7 @@
 //   copy warp        the page's block into a ring, by one bulk copy
 //   4 dequant warps  codes and scales to (n - 8) s as fp16 tiles of keys and values, times a power of two per page (keys) or per unit so far (values): exact, since a number has 3 + 8
 //                    significant bits, down to 2^-8 of the largest scale, and to 2^-19 of it below
-//   MMA warp         S = Q K^T (128 x 64 per tile), O += P V, P from tensor memory
+//   2 MMA warps      S = Q K^T (128 x 64 per tile), O += P V, P from tensor memory
 //   softmax warps    4 per tile, a thread per column: S from tensor memory, running maximum and sum, P back as fp16; O is scaled in place where the maximum moves by more than 2^8
 //
 // fp32 rows: q and P as two fp16 terms each, their products into the same accumulators (2^-22).  Products and exponentials need about the same time (16 exponentials per SM and clock,
@@ -35,7 +35,7 @@ struct PromptShape {
     static constexpr int kBufs = NG == 8 && TWO ? 1 : 2;   // tiles of keys and of values
     static constexpr int kQ = kTiles * kTerms * kBlocks * kTile * 128, kKv = kBlocks * kPage * 128;
     static constexpr int kFixed = kQ + 2 * kBufs * kKv;
-    static constexpr int kThreads = (kTiles * 4 + 4 + 2) * 32;
+    static constexpr int kThreads = (kTiles * 4 + 4 + kTiles + 1) * 32;
     // tensor memory: O of each tile, S, P
     static constexpr int kO = NG * kGroup, kS = kTiles * kO, kP = kS + kTiles * kPage, kPCols = TWO ? 64 : 32;
 };
@@ -94,11 +94,11 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
     if (tid == 0) {
         for (int i = 0; i < kMaxRing; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&k_full[i], 4); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 4); mbar_init(&v_empty[i], 1);
+            mbar_init(&k_full[i], 4); mbar_init(&k_empty[i], TILES); mbar_init(&v_full[i], 4); mbar_init(&v_empty[i], TILES);
             mbar_init(&q_full[i], 4); mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 4); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1);
         }
         for (int i = 0; i < 4; ++i) mbar_init(&info_full[i], 4);
-        mbar_init(&all_done, 1);
+        mbar_init(&all_done, TILES);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         dead_flag = 0;
     }
@@ -517,23 +517,28 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                 arrive(&raw_empty[slot]);
             }
         });
-    } else if (warp == TILES * 4 + 4) {
-        // ---- products
+    } else if (warp < TILES * 4 + 4 + TILES) {
+        // ---- products: a warp per tile, so that neither waits for the other one's softmax
+        const int t = warp - TILES * 4 - 4;
         const uint32_t id_s = (1u << 4) | ((uint32_t)(kPage >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
         const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(pad >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);      // B: numbers contiguous
-        uint32_t pages = 0, scores[2] = {0, 0}, outs[2] = {0, 0}, units[2] = {0, 0};
-        bool pending = false, pend_first = false, pend_live[2] = {false, false};
-        uint32_t pend_page = 0;
-        auto values = [&]() {
-            if (!pending) return;
-            pending = false;
-            const int buf = pend_page % BUFS;
-            wait(&v_full[buf], pend_page / BUFS);
-#pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-                if (!pend_live[t]) continue;
-                wait(&p_full[t], outs[t]);
-                ++outs[t];
+        const uint32_t q = smem_u32(q_sm) + t * TERMS * BLOCKS * (kTile * 128);
+        uint32_t pages = 0, done = 0, outs = 0, units = 0;
+        walk([&](const Segment& g, long long) {
+            if (g.tile * COLS + t * kTile >= g.cols) {     // not a column of this tile: the buffers are free of it
+                for (int p = g.p0; p < g.p1; ++p, ++pages) {
+                    wait(&k_full[pages % BUFS], pages / BUFS);
+                    if (lane == 0) mbar_arrive(&k_empty[pages % BUFS]);
+                    wait(&v_full[pages % BUFS], pages / BUFS);
+                    if (lane == 0) mbar_arrive(&v_empty[pages % BUFS]);
+                }
+                return;
+            }
+            auto values = [&](uint32_t page, bool first) {
+                const int buf = page % BUFS;
+                wait(&v_full[buf], page / BUFS);
+                wait(&p_full[t], outs);
+                ++outs;
                 tc_fence_after();
                 if (lane == 0) {
                     const uint32_t v = smem_u32(v_sm) + buf * Shape::kKv;
@@ -541,51 +546,35 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                     for (int term = 0; term < TERMS; ++term)
 #pragma unroll
                         for (int k = 0; k < kPage / 16; ++k)
-                            umma_tmem_a(tmem + t * Shape::kO, tmem + Shape::kP + t * Shape::kPCols + term * 32 + k * 8, values_desc(v + k * 2048), id_o, !(pend_first && term == 0 && k == 0));
+                            umma_tmem_a(tmem + t * Shape::kO, tmem + Shape::kP + t * Shape::kPCols + term * 32 + k * 8, values_desc(v + k * 2048), id_o, !(first && term == 0 && k == 0));
                     umma_commit(&o_done[t]);
+                    umma_commit(&v_empty[buf]);
                 }
                 __syncwarp();
-            }
-            if (lane == 0) umma_commit(&v_empty[buf]);
-            __syncwarp();
-        };
-        walk([&](const Segment& g, long long) {
-            values();                                      // the unit ahead: its accumulators are read before this one's queries come
-            bool live[2];
-#pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-                live[t] = g.tile * COLS + t * kTile < g.cols;
-                if (live[t]) { wait(&q_full[t], units[t]); ++units[t]; }
-            }
+            };
+            wait(&q_full[t], units);
+            ++units;
             for (int p = g.p0; p < g.p1; ++p, ++pages) {
                 const int buf = pages % BUFS;
                 wait(&k_full[buf], pages / BUFS);
+                wait(&s_empty[t], done + 1);
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t k = smem_u32(k_sm) + buf * Shape::kKv;
 #pragma unroll
-                for (int t = 0; t < TILES; ++t) {
-                    if (!live[t]) continue;
-                    wait(&s_empty[t], scores[t] + 1);
-                    ++scores[t];
-                    tc_fence_after();
-                    if (lane == 0) {
-                        const uint32_t q = smem_u32(q_sm) + t * TERMS * BLOCKS * (kTile * 128), k = smem_u32(k_sm) + buf * Shape::kKv;
-#pragma unroll
-                        for (int term = 0; term < TERMS; ++term)
-                            for (int x = 0; x < 2 * gk; ++x)
-                                umma_bf16(tmem + Shape::kS + t * kPage, make_smem_desc(q + (term * BLOCKS + x / 4) * (kTile * 128) + x % 4 * 32),
-                                          make_smem_desc(k + x / 4 * (kPage * 128) + x % 4 * 32), id_s, !(term == 0 && x == 0));
-                        umma_commit(&s_full[t]);
-                    }
-                    __syncwarp();
+                    for (int term = 0; term < TERMS; ++term)
+                        for (int x = 0; x < 2 * gk; ++x)
+                            umma_bf16(tmem + Shape::kS + t * kPage, make_smem_desc(q + (term * BLOCKS + x / 4) * (kTile * 128) + x % 4 * 32),
+                                      make_smem_desc(k + x / 4 * (kPage * 128) + x % 4 * 32), id_s, !(term == 0 && x == 0));
+                    umma_commit(&s_full[t]);
+                    umma_commit(&k_empty[buf]);
                 }
-                if (lane == 0) umma_commit(&k_empty[buf]);
                 __syncwarp();
-                values();
-                pending = true; pend_page = pages; pend_first = p == g.p0;
-#pragma unroll
-                for (int t = 0; t < TILES; ++t) pend_live[t] = live[t];
+                if (p > g.p0) values(pages - 1, p - 1 == g.p0);
+                ++done;
             }
+            values(pages - 1, g.p1 - 1 == g.p0);
         });
-        values();
         if (lane == 0) umma_commit(&all_done);
         __syncwarp();
     } else {
@@ -613,9 +602,9 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
         });
     }
     // ---- nothing may be under way when the CTA ends: products have ended, and after a wait that gave up so have copies
-    if (warp == TILES * 4 + 4) wait(&all_done, 0);
+    if (warp >= TILES * 4 + 4) wait(&all_done, 0);
     __syncthreads();
-    if (*dead_s && warp == TILES * 4 + 5 && lane == 0) {
+    if (*dead_s && warp == TILES * 5 + 4 && lane == 0) {
         mbar_wait(&all_done, 0, a.wait_ns);
         for (int i = max(0, copied - ring_n); i < copied; ++i) mbar_wait(&raw_full[i % ring_n], (i / ring_n) & 1, a.wait_ns);
         if (a.status != nullptr) atomicOr(a.status, STATUS_TIMEOUT);
