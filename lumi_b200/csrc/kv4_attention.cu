@@ -52,14 +52,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t u) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(v) : "r"(u));
     return v;
 }
-// two fp32 operations in one
-__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0, float c1) {
-    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
-}
-__device__ __forceinline__ void add2(float& d0, float& d1, float a0, float a1) {
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%0, %1};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(d0), "+f"(d1) : "f"(a0), "f"(a1));
-}
 // Pages that any of its rows sees, and units of `cols` columns.  Nothing of a sequence that is left out, or that is another kernel's.
 __device__ __forceinline__ Sequence step_sequence(const AttendArgs& a, int s, int cols, bool& bad) {
     Sequence q;

@@ -25,6 +25,7 @@ constexpr int kPromptCtas = 160;                           // places for parts
 constexpr int kTicketsAt = 320;                            // behind the step kernel's
 constexpr int kRunPages = 4;                               // a CTA's, at least
 constexpr int kMaxRing = 4;
+constexpr int kInfos = 8;                                  // pages whose exponents are kept: the copies run up to kMaxRing ahead of the values' tiles, these two ahead of the softmax
 
 template <int NG, bool TWO>
 struct PromptShape {
@@ -35,11 +36,29 @@ struct PromptShape {
     static constexpr int kBufs = NG == 8 && TWO ? 1 : 2;   // tiles of keys and of values
     static constexpr int kQ = kTiles * kTerms * kBlocks * kTile * 128, kKv = kBlocks * kPage * 128;
     static constexpr int kFixed = kQ + 2 * kBufs * kKv;
-    static constexpr int kThreads = (kTiles * 4 + 4 + kTiles + 1) * 32;
+    static constexpr int kThreads = (kTiles * 4 + 4 + kTiles + 2) * 32;
     // tensor memory: O of each tile, S, P
     static constexpr int kO = NG * kGroup, kS = kTiles * kO, kP = kS + kTiles * kPage, kPCols = TWO ? 64 : 32;
 };
 
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&r)[64]) {
+#define LUMI_LD32(i)                                                                                                                                            \
+    asm volatile(                                                                                                                                               \
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "                                                                                                               \
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "                                                                               \
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"                                                               \
+        : "=f"(r[i]), "=f"(r[i + 1]), "=f"(r[i + 2]), "=f"(r[i + 3]), "=f"(r[i + 4]), "=f"(r[i + 5]), "=f"(r[i + 6]), "=f"(r[i + 7]), "=f"(r[i + 8]),           \
+          "=f"(r[i + 9]), "=f"(r[i + 10]), "=f"(r[i + 11]), "=f"(r[i + 12]), "=f"(r[i + 13]), "=f"(r[i + 14]), "=f"(r[i + 15]), "=f"(r[i + 16]),                \
+          "=f"(r[i + 17]), "=f"(r[i + 18]), "=f"(r[i + 19]), "=f"(r[i + 20]), "=f"(r[i + 21]), "=f"(r[i + 22]), "=f"(r[i + 23]), "=f"(r[i + 24]),               \
+          "=f"(r[i + 25]), "=f"(r[i + 26]), "=f"(r[i + 27]), "=f"(r[i + 28]), "=f"(r[i + 29]), "=f"(r[i + 30]), "=f"(r[i + 31])                                 \
+        : "r"(taddr + i))
+    LUMI_LD32(0);
+    LUMI_LD32(32);
+#undef LUMI_LD32
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 64; ++i) asm volatile("" : "+f"(r[i]));      // no use ahead of the wait
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -79,10 +98,9 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
     extern __shared__ __align__(1024) uint8_t sm_raw[];
     uint8_t* const sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
     uint8_t *const q_sm = sm, *const k_sm = q_sm + Shape::kQ, *const v_sm = k_sm + BUFS * Shape::kKv, *const ring = v_sm + BUFS * Shape::kKv;
-    __shared__ uint64_t raw_full[kMaxRing], raw_empty[kMaxRing], k_full[2], k_empty[2], v_full[2], v_empty[2], q_full[2], s_full[2], s_empty[2], p_full[2], o_done[2], info_full[4], all_done;
-    __shared__ PageInfo info[4];
+    __shared__ uint64_t raw_full[kMaxRing], raw_empty[kMaxRing], k_full[2], k_empty[2], v_full[2], v_empty[2], q_full[2], s_full[2], s_empty[2], p_full[2], o_done[2], info_full[kInfos], all_done;
+    __shared__ PageInfo info[kInfos];
     __shared__ int absent_s[kMaxRing];
-    __shared__ int red_s[4][2];
     __shared__ uint32_t tmem_slot;
     __shared__ int dead_flag, last_s[2];
     __shared__ long long before[THREADS + 1], warp_pages[THREADS / 32];
@@ -92,12 +110,12 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
     const int gk = kv4_groups(a.dk), gv = kv4_groups(a.dv), part = kv4_part(a.dk), block = kv4_block(a.dk, a.dv), pad = gv * kGroup;
 
     if (tid == 0) {
-        for (int i = 0; i < kMaxRing; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
+        for (int i = 0; i < kMaxRing; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 5); }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&k_full[i], 4); mbar_init(&k_empty[i], TILES); mbar_init(&v_full[i], 4); mbar_init(&v_empty[i], TILES);
             mbar_init(&q_full[i], 4); mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 4); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1);
         }
-        for (int i = 0; i < 4; ++i) mbar_init(&info_full[i], 4);
+        for (int i = 0; i < kInfos; ++i) mbar_init(&info_full[i], 1);
         mbar_init(&all_done, TILES);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         dead_flag = 0;
@@ -212,7 +230,7 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
         }
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (!*dead_s && !mbar_wait(bar, parity & 1, a.wait_ns)) *dead_s = 1;
+        if (!mbar_try_wait(bar, parity & 1) && !*dead_s && !mbar_wait(bar, parity & 1, a.wait_ns)) *dead_s = 1;
         __syncwarp();
     };
     auto arrive = [&](uint64_t* bar) {                     // one of four warps, all of its lanes
@@ -276,22 +294,22 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 arrive(&q_full[tile]);
             }
+            const int first_full = __reduce_max_sync(0xffffffffu, lo_pos), last_full = __reduce_min_sync(0xffffffffu, pos);      // positions that all of the warp's columns see
             float m = -INFINITY, l = 0.f;
             int e_v = 0;
             for (int i = 0; i < n_pages; ++i, ++pages, ++done) {
                 wait(&s_full[tile], done);
-                wait(&info_full[pages % 4], pages / 4);
-                const PageInfo& of = info[pages % 4];
+                wait(&info_full[pages % kInfos], pages / kInfos);
+                const PageInfo& of = info[pages % kInfos];
                 tc_fence_after();
                 float s[64];
-                tmem_ld32(t_s, reinterpret_cast<uint32_t(&)[32]>(s[0]));
-                tmem_ld32(t_s + 32, reinterpret_cast<uint32_t(&)[32]>(s[32]));
+                tmem_ld64(t_s, s);
                 tc_fence_before();
                 arrive(&s_empty[tile]);
                 const int up = of.e_k + 9;
                 const float c = fmaxf(cx * power_of_two(up / 2) * power_of_two(up - up / 2), 1e-37f);
                 const int pos0 = (g.p0 + i) * kPage, new_e = of.e_v;
-                if (__any_sync(0xffffffffu, pos0 < lo_pos || pos0 + kPage - 1 > pos || of.absent)) {
+                if (pos0 < first_full || pos0 + kPage - 1 > last_full || of.absent) {
 #pragma unroll
                     for (int k = 0; k < 64; ++k)
                         if (pos0 + k < lo_pos || pos0 + k > pos || of.absent) s[k] = -INFINITY;
@@ -325,14 +343,17 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                 }
                 e_v = new_e;
                 const float off = m == -INFINITY ? 0.f : -m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};       // (two chains of pairs)
                 uint32_t p[32];
                 if constexpr (TWO) {
                     uint32_t lo[32];
 #pragma unroll
                     for (int k = 0; k < 32; ++k) {
-                        const float x = exp2_fast(fmaf(s[2 * k], c, off)), y = exp2_fast(fmaf(s[2 * k + 1], c, off));
-                        sum[k % 2 * 2] += x; sum[k % 2 * 2 + 1] += y;
+                        float x, y;
+                        fma2(x, y, s[2 * k], s[2 * k + 1], c, c, off, off);
+                        x = exp2_fast(x);
+                        y = exp2_fast(y);
+                        add2(sum[k % 2 * 2], sum[k % 2 * 2 + 1], x, y);
                         p[k] = halves(x, y);
                         const float2 b = unhalves(p[k]);
                         lo[k] = halves(x - b.x, y - b.y);
@@ -343,8 +364,11 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                 } else {
 #pragma unroll
                     for (int k = 0; k < 32; ++k) {
-                        const float x = exp2_fast(fmaf(s[2 * k], c, off)), y = exp2_fast(fmaf(s[2 * k + 1], c, off));
-                        sum[k % 2 * 2] += x; sum[k % 2 * 2 + 1] += y;
+                        float x, y;
+                        fma2(x, y, s[2 * k], s[2 * k + 1], c, c, off, off);
+                        x = exp2_fast(x);
+                        y = exp2_fast(y);
+                        add2(sum[k % 2 * 2], sum[k % 2 * 2 + 1], x, y);
                         p[k] = halves(x, y);
                     }
                     if (!waited) wait(&o_done[tile], done - 1);
@@ -435,51 +459,27 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
         });
     } else if (warp < TILES * 4 + 4) {
         // ---- codes and scales to fp16 tiles
-        const int dt = tid - TILES * kTile, dw = dt / 32;
+        const int dt = tid - TILES * kTile;
         uint32_t pages = 0;
         walk([&](const Segment& g, long long) {
-            int e_run = -90;
             for (int p = g.p0; p < g.p1; ++p, ++pages) {
                 const int slot = pages % ring_n, live = min(kPage, g.q.total - p * kPage);      // tokens that have been written
                 const uint8_t* const raw = ring + slot * block;
                 wait(&raw_full[slot], pages / ring_n);
-                const bool absent = absent_s[slot] != 0;
-                // the largest scales
-                uint32_t top_k = 0, top_v = 0, none[2] = {0, 0};
-                if (!absent) {
-                    for (int w = dt; w < (gk + gv) * 32; w += 128) {
-                        const bool keys = w < gk * 32;
-                        const int tok = w % 32 * 2;
-                        const uint32_t u = *reinterpret_cast<const uint32_t*>(raw + (keys ? gk * kPlane : part + gv * kPlane) + (keys ? w : w - gk * 32) * 4);
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            uint32_t b = (e ? u >> 16 : u) & 0x7fffu;
-                            if (tok + e >= live) b = 0;
-                            if (b >= 0x7f80u) { if (!keys) none[tok / 32] |= 1u << ((tok + e) % 32); b = 0; }
-                            if (keys) top_k = max(top_k, b); else top_v = max(top_v, b);
-                        }
-                    }
-                }
-                top_k = __reduce_max_sync(0xffffffffu, top_k);
-                top_v = __reduce_max_sync(0xffffffffu, top_v);
-                if (lane == 0) { red_s[dw][0] = (int)top_k; red_s[dw][1] = (int)top_v; }
-                PageInfo& to = info[pages % 4];
-                if (dt == 0) to.no_number[0] = to.no_number[1] = 0;
-                group_barrier(3);
-                if (none[0]) atomicOr(&to.no_number[0], none[0]);
-                if (none[1]) atomicOr(&to.no_number[1], none[1]);
-                const int mk = max(max(red_s[0][0], red_s[1][0]), max(red_s[2][0], red_s[3][0])), mv = max(max(red_s[0][1], red_s[1][1]), max(red_s[2][1], red_s[3][1]));
-                // scales are below 2^e; they become fp16 numbers below 2^15
-                const int e_k = max(-90, min(127, (mk >> 7) - 126));
-                e_run = max(e_run, max(-90, min(127, (mv >> 7) - 126)));
-                if (dt == 0) { to.e_k = e_k; to.e_v = e_run; to.absent = absent; }
+                wait(&info_full[pages % kInfos], pages / kInfos);
+                const PageInfo& of = info[pages % kInfos];
+                const int e_k = of.e_k, e_v = of.e_v;
+                const bool absent = of.absent != 0;
                 const int buf = pages % BUFS;
                 auto tile_of = [&](bool keys) {
                     const int groups = keys ? gk : gv;
                     const uint8_t* const codes = raw + (keys ? 0 : part);
                     uint8_t* const out = (keys ? k_sm : v_sm) + buf * Shape::kKv;
-                    const float by = power_of_two(15 - (keys ? e_k : e_run));
-                    for (int x = dt; x < groups * kPage; x += 128) {
+                    const float by = power_of_two(15 - (keys ? e_k : e_v));
+#pragma unroll
+                    for (int i = 0; i < NG / 2; ++i) {
+                        const int x = i * 128 + dt;
+                        if (x >= groups * kPage) break;
                         const int tok = x % kPage, grp = x / kPage;
                         uint4 u = make_uint4(0, 0, 0, 0);
                         float s = 0.f;
@@ -508,9 +508,7 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                 };
                 wait(&k_empty[buf], pages / BUFS + 1);
                 tile_of(true);
-                group_barrier(3);                          // info is complete (and red_s has been read)
                 arrive(&k_full[buf]);
-                arrive(&info_full[pages % 4]);
                 wait(&v_empty[buf], pages / BUFS + 1);
                 tile_of(false);
                 arrive(&v_full[buf]);
@@ -522,7 +520,8 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
         const int t = warp - TILES * 4 - 4;
         const uint32_t id_s = (1u << 4) | ((uint32_t)(kPage >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
         const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(pad >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);      // B: numbers contiguous
-        const uint32_t q = smem_u32(q_sm) + t * TERMS * BLOCKS * (kTile * 128);
+        // descriptors count in 16 bytes: a step of 16 numbers or tokens is an addition
+        const uint64_t q_desc = make_smem_desc(smem_u32(q_sm) + t * TERMS * BLOCKS * (kTile * 128)), k_desc = make_smem_desc(smem_u32(k_sm)), v_desc = values_desc(smem_u32(v_sm));
         uint32_t pages = 0, done = 0, outs = 0, units = 0;
         walk([&](const Segment& g, long long) {
             if (g.tile * COLS + t * kTile >= g.cols) {     // not a column of this tile: the buffers are free of it
@@ -541,12 +540,12 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                 ++outs;
                 tc_fence_after();
                 if (lane == 0) {
-                    const uint32_t v = smem_u32(v_sm) + buf * Shape::kKv;
+                    const uint64_t v = v_desc + buf * (Shape::kKv >> 4);
 #pragma unroll
                     for (int term = 0; term < TERMS; ++term)
 #pragma unroll
                         for (int k = 0; k < kPage / 16; ++k)
-                            umma_tmem_a(tmem + t * Shape::kO, tmem + Shape::kP + t * Shape::kPCols + term * 32 + k * 8, values_desc(v + k * 2048), id_o, !(first && term == 0 && k == 0));
+                            umma_tmem_a(tmem + t * Shape::kO, tmem + Shape::kP + t * Shape::kPCols + term * 32 + k * 8, v + k * (2048 >> 4), id_o, !(first && term == 0 && k == 0));
                     umma_commit(&o_done[t]);
                     umma_commit(&v_empty[buf]);
                 }
@@ -560,12 +559,15 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                 wait(&s_empty[t], done + 1);
                 tc_fence_after();
                 if (lane == 0) {
-                    const uint32_t k = smem_u32(k_sm) + buf * Shape::kKv;
-#pragma unroll
+                    const uint64_t k = k_desc + buf * (Shape::kKv >> 4);
+#pragma unroll 1
                     for (int term = 0; term < TERMS; ++term)
-                        for (int x = 0; x < 2 * gk; ++x)
-                            umma_bf16(tmem + Shape::kS + t * kPage, make_smem_desc(q + (term * BLOCKS + x / 4) * (kTile * 128) + x % 4 * 32),
-                                      make_smem_desc(k + x / 4 * (kPage * 128) + x % 4 * 32), id_s, !(term == 0 && x == 0));
+#pragma unroll 1
+                        for (int x = 0; x < 2 * gk; x += 2) {      // a group of 32 numbers
+                            const uint64_t qd = q_desc + (((term * BLOCKS + x / 4) * (kTile * 128) + x % 4 * 32) >> 4), kd = k + ((x / 4 * (kPage * 128) + x % 4 * 32) >> 4);
+                            umma_bf16(tmem + Shape::kS + t * kPage, qd, kd, id_s, term + x > 0);
+                            umma_bf16(tmem + Shape::kS + t * kPage, qd + 2, kd + 2, id_s, 1u);
+                        }
                     umma_commit(&s_full[t]);
                     umma_commit(&k_empty[buf]);
                 }
@@ -577,6 +579,50 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
         });
         if (lane == 0) umma_commit(&all_done);
         __syncwarp();
+    } else if (warp == TILES * 5 + 4) {
+        // ---- the largest scales of a page, a power of two each: keys' of the page, values' of the unit so far
+        uint32_t pages = 0;
+        walk([&](const Segment& g, long long) {
+            int e_run = -90;
+            for (int p = g.p0; p < g.p1; ++p, ++pages) {
+                const int slot = pages % ring_n, live = min(kPage, g.q.total - p * kPage);      // tokens that have been written
+                const uint8_t* const raw = ring + slot * block;
+                wait(&raw_full[slot], pages / ring_n);
+                const bool absent = absent_s[slot] != 0;
+                uint32_t top[2] = {0, 0}, none[2] = {0, 0};
+                if (!absent)
+#pragma unroll
+                    for (int i = 0; i < NG / 2; ++i) {     // eight tokens' scales of a group
+                        const int x = i * 32 + lane, values = x >= gk * 8, tok = x % 8 * 8;
+                        if (x >= (gk + gv) * 8) break;
+                        const uint4 u = *reinterpret_cast<const uint4*>(raw + (values ? part + gv * kPlane + (x - gk * 8) * 16 : gk * kPlane + x * 16));
+                        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            uint32_t b = (w[k / 2] >> (k % 2 * 16)) & 0x7fffu;
+                            if (tok + k >= live) b = 0;
+                            if (b >= 0x7f80u) { if (values) none[tok / 32] |= 1u << ((tok + k) % 32); b = 0; }
+                            top[values] = max(top[values], b);
+                        }
+                    }
+                top[0] = __reduce_max_sync(0xffffffffu, top[0]);
+                top[1] = __reduce_max_sync(0xffffffffu, top[1]);
+                none[0] = __reduce_or_sync(0xffffffffu, none[0]);
+                none[1] = __reduce_or_sync(0xffffffffu, none[1]);
+                // scales are below 2^e; they become fp16 numbers below 2^15
+                e_run = max(e_run, max(-90, min(127, (int)(top[1] >> 7) - 126)));
+                if (lane == 0) {
+                    PageInfo& to = info[pages % kInfos];
+                    to.e_k = max(-90, min(127, (int)(top[0] >> 7) - 126));
+                    to.e_v = e_run;
+                    to.absent = absent;
+                    to.no_number[0] = none[0]; to.no_number[1] = none[1];
+                    mbar_arrive(&info_full[pages % kInfos]);
+                    mbar_arrive(&raw_empty[slot]);
+                }
+                __syncwarp();
+            }
+        });
     } else {
         // ---- copies
         uint32_t pages = 0;
@@ -602,9 +648,9 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
         });
     }
     // ---- nothing may be under way when the CTA ends: products have ended, and after a wait that gave up so have copies
-    if (warp >= TILES * 4 + 4) wait(&all_done, 0);
+    if (warp >= TILES * 4 + 4 && warp < TILES * 5 + 4) wait(&all_done, 0);
     __syncthreads();
-    if (*dead_s && warp == TILES * 5 + 4 && lane == 0) {
+    if (*dead_s && warp == TILES * 5 + 5 && lane == 0) {
         mbar_wait(&all_done, 0, a.wait_ns);
         for (int i = max(0, copied - ring_n); i < copied; ++i) mbar_wait(&raw_full[i % ring_n], (i / ring_n) & 1, a.wait_ns);
         if (a.status != nullptr) atomicOr(a.status, STATUS_TIMEOUT);
