@@ -7,7 +7,7 @@
 //   4 dequant warps  codes and scales to (n - 8) s as fp16 tiles of keys and values, times a power of two per page (keys) or per unit so far (values): exact, since a number has 3 + 8
 //                    significant bits, down to 2^-8 of the largest scale, and to 2^-19 of it below
 //   2 MMA warps      S = Q K^T (128 x 64 per tile), O += P V, P from tensor memory
-//   softmax warps    4 per tile, a thread per column: S from tensor memory, running maximum and sum, P back as fp16; O is scaled in place where the maximum moves by more than 2^8
+//   softmax warps    8 per tile, two threads per column: S from tensor memory, running maximum and sum, P back as fp16; O is scaled in place where the maximum moves by more than 2^8
 //
 // fp32 rows: q and P as two fp16 terms each, their products into the same accumulators (2^-22).  Products and exponentials need about the same time (16 exponentials per SM and clock,
 // 4096 multiply-adds): 1024 clocks each per page and two tiles at heads of 128.
@@ -25,6 +25,7 @@ constexpr int kPromptCtas = 160;                           // places for parts
 constexpr int kTicketsAt = 320;                            // behind the step kernel's
 constexpr int kRunPages = 4;                               // a CTA's, at least
 constexpr int kMaxRing = 4;
+constexpr int kStatic = 10 * 1024;                         // bytes declared in the kernel, at most
 constexpr int kInfos = 8;                                  // pages whose exponents are kept: the copies run up to kMaxRing ahead of the values' tiles, these two ahead of the softmax
 
 template <int NG, bool TWO>
@@ -36,37 +37,25 @@ struct PromptShape {
     static constexpr int kBufs = NG == 8 && TWO ? 1 : 2;   // tiles of keys and of values
     static constexpr int kQ = kTiles * kTerms * kBlocks * kTile * 128, kKv = kBlocks * kPage * 128;
     static constexpr int kFixed = kQ + 2 * kBufs * kKv;
-    static constexpr int kThreads = (kTiles * 4 + 4 + kTiles + 2) * 32;
+    static constexpr int kThreads = (kTiles * 8 + 4 + kTiles + 2) * 32;
     // tensor memory: O of each tile, S, P
     static constexpr int kO = NG * kGroup, kS = kTiles * kO, kP = kS + kTiles * kPage, kPCols = TWO ? 64 : 32;
 };
 
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&r)[64]) {
-#define LUMI_LD32(i)                                                                                                                                            \
-    asm volatile(                                                                                                                                               \
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "                                                                                                               \
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "                                                                               \
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"                                                               \
-        : "=f"(r[i]), "=f"(r[i + 1]), "=f"(r[i + 2]), "=f"(r[i + 3]), "=f"(r[i + 4]), "=f"(r[i + 5]), "=f"(r[i + 6]), "=f"(r[i + 7]), "=f"(r[i + 8]),           \
-          "=f"(r[i + 9]), "=f"(r[i + 10]), "=f"(r[i + 11]), "=f"(r[i + 12]), "=f"(r[i + 13]), "=f"(r[i + 14]), "=f"(r[i + 15]), "=f"(r[i + 16]),                \
-          "=f"(r[i + 17]), "=f"(r[i + 18]), "=f"(r[i + 19]), "=f"(r[i + 20]), "=f"(r[i + 21]), "=f"(r[i + 22]), "=f"(r[i + 23]), "=f"(r[i + 24]),               \
-          "=f"(r[i + 25]), "=f"(r[i + 26]), "=f"(r[i + 27]), "=f"(r[i + 28]), "=f"(r[i + 29]), "=f"(r[i + 30]), "=f"(r[i + 31])                                 \
-        : "r"(taddr + i))
-    LUMI_LD32(0);
-    LUMI_LD32(32);
-#undef LUMI_LD32
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 64; ++i) asm volatile("" : "+f"(r[i]));      // no use ahead of the wait
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld32f(uint32_t taddr, float (&r)[32]) { tmem_ld32(taddr, reinterpret_cast<uint32_t(&)[32]>(r)); }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-        "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "r"(r[14]), "r"(r[15])
         : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -84,7 +73,13 @@ __device__ __forceinline__ uint64_t values_desc(uint32_t addr) {
     uint64_t d = make_smem_desc(addr) & ~((uint64_t)0x3fff << 16);
     return d | (uint64_t)((kPage * 128) >> 4) << 16;
 }
-__device__ __forceinline__ void group_barrier(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void pair_barrier(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void tile_barrier(int id) { asm volatile("bar.sync %0, 256;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool pair_any(int id, bool v) {      // of two warps
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbar.red.or.pred q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"(id), "r"((uint32_t)v) : "memory");
+    return any != 0;
+}
 
 struct PageInfo { int e_k, e_v, absent; uint32_t no_number[2]; };      // exponents of keys and values; tokens with values that are no numbers
 
@@ -105,6 +100,7 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
     __shared__ int dead_flag, last_s[2];
     __shared__ long long before[THREADS + 1], warp_pages[THREADS / 32];
     __shared__ Cursor start_s;
+    __shared__ float tops_s[2][TILES][kTile];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* const dead_s = &dead_flag;
     const int gk = kv4_groups(a.dk), gv = kv4_groups(a.dv), part = kv4_part(a.dk), block = kv4_block(a.dk, a.dv), pad = gv * kGroup;
@@ -113,7 +109,7 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
         for (int i = 0; i < kMaxRing; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 5); }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&k_full[i], 4); mbar_init(&k_empty[i], TILES); mbar_init(&v_full[i], 4); mbar_init(&v_empty[i], TILES);
-            mbar_init(&q_full[i], 4); mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 4); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1);
+            mbar_init(&q_full[i], 8); mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 8); mbar_init(&p_full[i], 8); mbar_init(&o_done[i], 1);
         }
         for (int i = 0; i < kInfos; ++i) mbar_init(&info_full[i], 1);
         mbar_init(&all_done, TILES);
@@ -239,11 +235,12 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
     };
     int copied = 0;                                        // (copy warp) copies issued
 
-    if (warp < TILES * 4) {
-        // ---- softmax: a thread per column
-        const int tile = warp / 4, r = tid % kTile;
+    if (warp < TILES * 8) {
+        // ---- softmax: two threads per column, each 32 of a page's 64 tokens and half of the column's numbers
+        const int tile = warp / 8, half = warp / 4 % 2, r = tid % kTile, pair = 1 + tile * 4 + warp % 4;
         const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
-        const uint32_t t_o = tmem + tile * Shape::kO + lanes, t_s = tmem + Shape::kS + tile * kPage + lanes, t_p = tmem + Shape::kP + tile * Shape::kPCols + lanes;
+        const uint32_t t_o = tmem + tile * Shape::kO + lanes, t_s = tmem + Shape::kS + tile * kPage + half * 32 + lanes, t_p = tmem + Shape::kP + tile * Shape::kPCols + half * 16 + lanes;
+        const int d_lo = half == 0 ? 0 : (gv + 1) / 2 * kGroup, d_hi = half == 0 ? (gv + 1) / 2 * kGroup : pad;      // numbers of values
         uint32_t pages = 0, done = 0;                      // of the CTA, of this tile
         walk([&](const Segment& g, long long unit_lo) {
             const int col0 = g.tile * COLS + tile * kTile, n_pages = g.p1 - g.p0;
@@ -277,7 +274,7 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                 cx = fminf(fmaxf(__fdiv_rn(fabsf(a.scale) * kLog2e, by), 1e-37f), 3.4e38f);
                 const float f = a.scale < 0.f ? -by : by;
 #pragma unroll 2
-                for (int d = 0; d < gk * kGroup; d += 8) {
+                for (int d = half * 8; d < gk * kGroup; d += 16) {
                     float t[8];
                     eight(d, t);
                     uint32_t hi[4], lo[4];
@@ -295,33 +292,37 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                 arrive(&q_full[tile]);
             }
             const int first_full = __reduce_max_sync(0xffffffffu, lo_pos), last_full = __reduce_min_sync(0xffffffffu, pos);      // positions that all of the warp's columns see
-            float m = -INFINITY, l = 0.f;
+            float m = -INFINITY, l = 0.f;                  // (l: of this thread's tokens)
             int e_v = 0;
             for (int i = 0; i < n_pages; ++i, ++pages, ++done) {
                 wait(&s_full[tile], done);
                 wait(&info_full[pages % kInfos], pages / kInfos);
                 const PageInfo& of = info[pages % kInfos];
                 tc_fence_after();
-                float s[64];
-                tmem_ld64(t_s, s);
+                float s[32];
+                tmem_ld32f(t_s, s);
                 tc_fence_before();
                 arrive(&s_empty[tile]);
                 const int up = of.e_k + 9;
                 const float c = fmaxf(cx * power_of_two(up / 2) * power_of_two(up - up / 2), 1e-37f);
-                const int pos0 = (g.p0 + i) * kPage, new_e = of.e_v;
-                if (pos0 < first_full || pos0 + kPage - 1 > last_full || of.absent) {
+                const int pos0 = (g.p0 + i) * kPage + half * 32, new_e = of.e_v;
+                if (pos0 < first_full || pos0 + 31 > last_full || of.absent) {
 #pragma unroll
-                    for (int k = 0; k < 64; ++k)
+                    for (int k = 0; k < 32; ++k)
                         if (pos0 + k < lo_pos || pos0 + k > pos || of.absent) s[k] = -INFINITY;
                 }
                 float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int k = 4; k < 64; ++k) top[k % 4] = fmaxf(top[k % 4], s[k]);
-                const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+                for (int k = 4; k < 32; ++k) top[k % 4] = fmaxf(top[k % 4], s[k]);
+                float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
                 const bool moves = t > m + 8.f || (m == -INFINITY && t > -INFINITY);
                 bool waited = i == 0;
-                if (__any_sync(0xffffffffu, moves || (i > 0 && new_e != e_v))) {
-                    const float to = moves ? t : m;
+                if (pair_any(pair, moves || (i > 0 && new_e != e_v))) {      // of both halves of 32 columns
+                    tops_s[half][tile][r] = t;
+                    pair_barrier(pair);
+                    t = fmaxf(t, tops_s[1 - half][tile][r]);
+                    const bool both = t > m + 8.f || (m == -INFINITY && t > -INFINITY);
+                    const float to = both ? t : m;
                     const float f = m == -INFINITY ? 0.f : exp2_fast(m - to);
                     const float fo = m == -INFINITY ? 0.f : exp2_fast(0.5f * (m - to + (float)(e_v - new_e)));
                     m = to;
@@ -330,58 +331,52 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                         wait(&o_done[tile], done - 1);
                         waited = true;
                         tc_fence_after();
-                        for (int d = 0; d < pad; d += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(t_o + d, o);
+#pragma unroll 1
+                        for (int d = d_lo; d < d_hi; d += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(t_o + d, o);
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fo * fo);
-                            tmem_st32(t_o + d, o);
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fo * fo);
+                            tmem_st16(t_o + d, o);
                         }
                         tmem_st_wait();
                         tc_fence_before();
                     }
+                    pair_barrier(pair);                    // tops_s has been read
                 }
                 e_v = new_e;
                 const float off = m == -INFINITY ? 0.f : -m;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};       // (two chains of pairs)
-                uint32_t p[32];
-                if constexpr (TWO) {
-                    uint32_t lo[32];
+                uint32_t p[16];
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        float x, y;
-                        fma2(x, y, s[2 * k], s[2 * k + 1], c, c, off, off);
-                        x = exp2_fast(x);
-                        y = exp2_fast(y);
-                        add2(sum[k % 2 * 2], sum[k % 2 * 2 + 1], x, y);
-                        p[k] = halves(x, y);
-                        const float2 b = unhalves(p[k]);
-                        lo[k] = halves(x - b.x, y - b.y);
-                    }
-                    if (!waited) wait(&o_done[tile], done - 1);
-                    tmem_st32(t_p, p);
-                    tmem_st32(t_p + 32, lo);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        float x, y;
-                        fma2(x, y, s[2 * k], s[2 * k + 1], c, c, off, off);
-                        x = exp2_fast(x);
-                        y = exp2_fast(y);
-                        add2(sum[k % 2 * 2], sum[k % 2 * 2 + 1], x, y);
-                        p[k] = halves(x, y);
-                    }
-                    if (!waited) wait(&o_done[tile], done - 1);
-                    tmem_st32(t_p, p);
+                for (int k = 0; k < 16; ++k) {
+                    float &x = s[2 * k], &y = s[2 * k + 1];
+                    fma2(x, y, x, y, c, c, off, off);
+                    x = exp2_fast(x);
+                    y = exp2_fast(y);
+                    add2(sum[k % 2 * 2], sum[k % 2 * 2 + 1], x, y);
+                    p[k] = halves(x, y);
+                    if (TWO) { const float2 b = unhalves(p[k]); x -= b.x; y -= b.y; }
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                if (of.no_number[0] | of.no_number[1])     // (rare) a row that sees such a token is none
-                    for (int k = 0; k < 64; ++k)
-                        if ((of.no_number[k / 32] >> (k % 32) & 1) && pos0 + k >= lo_pos && pos0 + k <= pos) l = __uint_as_float(0x7fc00000u);
+                if (!waited) wait(&o_done[tile], done - 1);
+                tmem_st16(t_p, p);
+                if constexpr (TWO) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) p[k] = halves(s[2 * k], s[2 * k + 1]);
+                    tmem_st16(t_p + 32, p);
+                }
+                if (of.no_number[half])                    // (rare) a row that sees such a token is none
+                    for (int k = 0; k < 32; ++k)
+                        if ((of.no_number[half] >> k & 1) && pos0 + k >= lo_pos && pos0 + k <= pos) l = __uint_as_float(0x7fc00000u);
                 tmem_st_wait();
                 tc_fence_before();
                 arrive(&p_full[tile]);
             }
+            tops_s[half][tile][r] = l;
+            pair_barrier(pair);
+            l += tops_s[1 - half][tile][r];
+            pair_barrier(pair);
             wait(&o_done[tile], done - 1);
             tc_fence_after();
             const int e = e_v + 9;                         // numbers are O 2^e / l
@@ -401,11 +396,12 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
             const int rec = places * (2 + pad);
             float* const to = a.parts + ((size_t)cta * 2 + (g.p0 == g.lo ? 1 : 0)) * rec;
             const float inv = whole ? inverse(m, l) : 1.f;
-            for (int d = 0; d < pad; d += 32) {
-                uint32_t o[32];
-                tmem_ld32(t_o + d, o);
+#pragma unroll 1
+            for (int d = d_lo; d < d_hi; d += 16) {
+                uint32_t o[16];
+                tmem_ld16(t_o + d, o);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
+                for (int k = 0; k < 2; ++k) {
                     float v[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(o[8 * k + j]) * back * back2;
@@ -419,18 +415,20 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
             tc_fence_before();
             if (whole) return;
             // ---- the unit is shared: who arrives last joins the parts, in the order of CTAs
-            to[at] = m;
-            to[places + at] = *dead_s ? __uint_as_float(0x7fc00000u) : l;
+            if (half == 0) {
+                to[at] = m;
+                to[places + at] = *dead_s ? __uint_as_float(0x7fc00000u) : l;
+            }
             __threadfence();
-            group_barrier(1 + tile);
+            tile_barrier(9 + tile);
             const long long unit_hi = unit_lo + (g.hi - g.lo);
             const int c0 = (int)quotient((unit_lo + 1) * ctas - 1, total), c1 = (int)quotient(unit_hi * ctas - 1, total);
-            if (r == 0) {
+            if (r == 0 && half == 0) {
                 int32_t* const ticket = a.tickets + kTicketsAt + c0 * 2 + tile;
                 last_s[tile] = atomicAdd(ticket, 1) == c1 - c0;
                 if (last_s[tile]) *ticket = 0;
             }
-            group_barrier(1 + tile);
+            tile_barrier(9 + tile);
             if (!last_s[tile]) return;
             __threadfence();
             auto place_of = [&](int k) { return a.parts + ((size_t)k * 2 + (k == c0 ? 1 : 0)) * rec; };
@@ -444,9 +442,9 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
             }
             const float f = inverse(mm, ll);
             if (valid)
-                for (int d = 0; d < pad; d += 8) {
+                for (int d = d_lo; d < d_hi; d += 8) {
                     float o[8] = {};
-#pragma unroll 4
+#pragma unroll 2
                     for (int k = c0; k <= c1; ++k) {
                         const float* const p = place_of(k);
                         const float pm = __ldcg(p + at), w = pm == -INFINITY ? 0.f : exp2_fast(pm - mm);
@@ -457,9 +455,9 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                     put_row(d, o, f);
                 }
         });
-    } else if (warp < TILES * 4 + 4) {
+    } else if (warp < TILES * 8 + 4) {
         // ---- codes and scales to fp16 tiles
-        const int dt = tid - TILES * kTile;
+        const int dt = tid - TILES * 2 * kTile;
         uint32_t pages = 0;
         walk([&](const Segment& g, long long) {
             for (int p = g.p0; p < g.p1; ++p, ++pages) {
@@ -476,22 +474,26 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                     const uint8_t* const codes = raw + (keys ? 0 : part);
                     uint8_t* const out = (keys ? k_sm : v_sm) + buf * Shape::kKv;
                     const float by = power_of_two(15 - (keys ? e_k : e_v));
+                    uint4 u[NG / 2];                       // a token's group each
+                    float sc[NG / 2];
 #pragma unroll
                     for (int i = 0; i < NG / 2; ++i) {
-                        const int x = i * 128 + dt;
-                        if (x >= groups * kPage) break;
-                        const int tok = x % kPage, grp = x / kPage;
-                        uint4 u = make_uint4(0, 0, 0, 0);
-                        float s = 0.f;
-                        if (!absent && tok < live) {
-                            u = *reinterpret_cast<const uint4*>(codes + grp * kPlane + tok * 16);
+                        const int x = i * 128 + dt, tok = x % kPage, grp = x / kPage;
+                        u[i] = make_uint4(0, 0, 0, 0);
+                        sc[i] = 0.f;
+                        if (grp < groups && !absent && tok < live) {
+                            u[i] = *reinterpret_cast<const uint4*>(codes + grp * kPlane + tok * 16);
                             const uint32_t bits = *reinterpret_cast<const uint16_t*>(codes + groups * kPlane + grp * kScales + tok * 2);
-                            s = __uint_as_float(bits << 16);
-                            if (!keys && (bits & 0x7fffu) >= 0x7f80u) s = 0.f;
+                            sc[i] = !keys && (bits & 0x7fffu) >= 0x7f80u ? 0.f : __uint_as_float(bits << 16);
                         }
-                        const __half2 t = __float2half2_rn(s * by), t16 = __float2half2_rn(s * by * 0.0625f), t8 = __float2half2_rn(s * by * -4.76837158203125e-07f);      // -8 2^-24
+                    }
+#pragma unroll
+                    for (int i = 0; i < NG / 2; ++i) {
+                        const int x = i * 128 + dt, tok = x % kPage, grp = x / kPage;
+                        const float s = sc[i] * by;
+                        const __half2 t = __float2half2_rn(s), t16 = __float2half2_rn(s * 0.0625f), t8 = __float2half2_rn(s * -4.76837158203125e-07f);      // -8 2^-24
                         uint8_t* const row = out + grp / 2 * (kPage * 128) + tok * 128;
-                        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                        const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const uint32_t c[4] = {w[j] & 0x000f000fu, w[j] & 0x00f000f0u, w[j] >> 8 & 0x000f000fu, w[j] >> 8 & 0x00f000f0u};
@@ -501,7 +503,7 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                                 const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&c[k]), k % 2 ? t16 : t, t8);
                                 o[k] = *reinterpret_cast<const uint32_t*>(&v);
                             }
-                            *reinterpret_cast<uint4*>(row + ((grp % 2 * 4 + j) ^ (tok & 7)) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+                            if (grp < groups) *reinterpret_cast<uint4*>(row + ((grp % 2 * 4 + j) ^ (tok & 7)) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
                         }
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -515,9 +517,9 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                 arrive(&raw_empty[slot]);
             }
         });
-    } else if (warp < TILES * 4 + 4 + TILES) {
+    } else if (warp < TILES * 9 + 4) {
         // ---- products: a warp per tile, so that neither waits for the other one's softmax
-        const int t = warp - TILES * 4 - 4;
+        const int t = warp - TILES * 8 - 4;
         const uint32_t id_s = (1u << 4) | ((uint32_t)(kPage >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
         const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(pad >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);      // B: numbers contiguous
         // descriptors count in 16 bytes: a step of 16 numbers or tokens is an addition
@@ -579,7 +581,7 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
         });
         if (lane == 0) umma_commit(&all_done);
         __syncwarp();
-    } else if (warp == TILES * 5 + 4) {
+    } else if (warp == TILES * 9 + 4) {
         // ---- the largest scales of a page, a power of two each: keys' of the page, values' of the unit so far
         uint32_t pages = 0;
         walk([&](const Segment& g, long long) {
@@ -648,9 +650,9 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
         });
     }
     // ---- nothing may be under way when the CTA ends: products have ended, and after a wait that gave up so have copies
-    if (warp >= TILES * 4 + 4 && warp < TILES * 5 + 4) wait(&all_done, 0);
+    if (warp >= TILES * 8 + 4 && warp < TILES * 9 + 4) wait(&all_done, 0);
     __syncthreads();
-    if (*dead_s && warp == TILES * 5 + 5 && lane == 0) {
+    if (*dead_s && warp == TILES * 9 + 5 && lane == 0) {
         mbar_wait(&all_done, 0, a.wait_ns);
         for (int i = max(0, copied - ring_n); i < copied; ++i) mbar_wait(&raw_full[i % ring_n], (i / ring_n) & 1, a.wait_ns);
         if (a.status != nullptr) atomicOr(a.status, STATUS_TIMEOUT);
@@ -668,7 +670,7 @@ int32_t launch(AttendArgs a, uint64_t work, cudaStream_t st) {
     using Shape = PromptShape<NG, sizeof(T) == 4>;
     const int block = kv4_block(a.dk, a.dv);
     // 232448 bytes of shared memory per CTA, less what is declared in the kernel and what alignment to 1024 bytes may cost
-    const int ring_n = std::min(kMaxRing, (232448 - 1024 - 5120 - Shape::kFixed) / block);
+    const int ring_n = std::min(kMaxRing, (232448 - 1024 - kStatic - Shape::kFixed) / block);
     a.tickets = (int32_t*)work;
     a.parts = (float*)(work + 4096);
     const size_t smem = 1024 + Shape::kFixed + (size_t)ring_n * block;
