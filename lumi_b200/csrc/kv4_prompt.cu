@@ -81,6 +81,21 @@ __device__ __forceinline__ bool pair_any(int id, bool v) {      // of two warps
     return any != 0;
 }
 
+// A wait that asks seldom: the hardware wakes the warp, and idle roles leave the issue slots to the others.
+__device__ __noinline__ void patient_wait(uint64_t* bar, uint32_t parity, uint64_t limit_ns, volatile int* dead) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!*dead) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(20000u) : "memory");
+        if (ok) return;
+        if (globaltimer_ns() - t0 > limit_ns) { *dead = 1; return; }
+    }
+}
+
 struct PageInfo { int e_k, e_v, absent; uint32_t no_number[2]; };      // exponents of keys and values; tokens with values that are no numbers
 
 struct Cursor { int s, head, tile, skip; };                // a unit, and pages of it that are the CTA's ahead
@@ -98,9 +113,9 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
     __shared__ int absent_s[kMaxRing];
     __shared__ uint32_t tmem_slot;
     __shared__ int dead_flag, last_s[2];
-    __shared__ long long before[THREADS + 1], warp_pages[THREADS / 32];
+    __shared__ long long warp_pages[THREADS / 32];
     __shared__ Cursor start_s;
-    __shared__ float tops_s[2][TILES][kTile];
+    __shared__ float tops_s[2][TILES][kTile], factors_s[TILES][kTile];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* const dead_s = &dead_flag;
     const int gk = kv4_groups(a.dk), gv = kv4_groups(a.dv), part = kv4_part(a.dk), block = kv4_block(a.dk, a.dv), pad = gv * kGroup;
@@ -134,25 +149,38 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
         hi = (q.total - q.n + row1) / kPage + 1;
     };
     auto tiles_of = [&](const Sequence& q) { return (q.n * a.group + COLS - 1) / COLS; };
-    // pages of one head; 0: nothing of this kernel's
-    auto head_pages = [&](int s, Sequence& q, bool& bad) {
-        bad = !lengths_of(a, s, q);
-        if (bad || q.n <= 0 || q.n > a.max_new || (long)q.n * a.group <= a.few) return 0ll;
+    auto pages_of = [&](const Sequence& q, int tile) {
+        int lo, hi;
+        unit_pages(q, tile, lo, hi);
+        return hi - lo;
+    };
+    auto has_work = [&](int s, Sequence& q) { return lengths_of(a, s, q) && q.n > 0 && q.n <= a.max_new && (long)q.n * a.group > a.few; };
+    auto warp_sum = [&](long long v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    };
+    // Pages of one head of each lane's sequence (s < 0: none), 0 where there is nothing of this kernel's.  Sequences of many tiles are summed up by the whole warp.
+    auto head_pages = [&](int s) {
+        Sequence q;
         long long sum = 0;
-        for (int t = 0, n = tiles_of(q); t < n; ++t) {
-            int lo, hi;
-            unit_pages(q, t, lo, hi);
-            sum += hi - lo;
+        const bool work = s >= 0 && has_work(s, q);
+        const int tiles = work ? tiles_of(q) : 0;
+        for (int t = 0; t < tiles && tiles <= 8; ++t) sum += pages_of(q, t);
+        for (uint32_t many = __ballot_sync(0xffffffffu, tiles > 8); many != 0; many &= many - 1) {
+            const int lane_of = __ffs(many) - 1;
+            Sequence w;
+            lengths_of(a, __shfl_sync(0xffffffffu, s, lane_of), w);
+            long long part_sum = 0;
+            for (int t = lane, n = tiles_of(w); t < n; t += 32) part_sum += pages_of(w, t);
+            part_sum = warp_sum(part_sum);
+            if (lane == lane_of) sum = part_sum;
         }
         return sum;
     };
-    const int each = (a.nseq + THREADS - 1) / THREADS, s_lo = min(a.nseq, tid * each), s_hi = min(a.nseq, s_lo + each);
+    const int each = (a.nseq + THREADS - 1) / THREADS, s_lo = tid * each;
     long long mine = 0;
-    for (int s = s_lo; s < s_hi; ++s) {
-        Sequence q;
-        bool bad;
-        mine += head_pages(s, q, bad) * a.kv_heads;
-    }
+    for (int k = 0; k < each; ++k) mine += head_pages(s_lo + k < a.nseq ? s_lo + k : -1) * a.kv_heads;
     long long run = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const long long t = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += t; }
@@ -160,36 +188,41 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
     __syncthreads();
     long long ahead = 0, total = 0;
     for (int w = 0; w < THREADS / 32; ++w) { const long long p = warp_pages[w]; if (w < warp) ahead += p; total += p; }
-    before[tid] = ahead + run - mine;
-    if (tid == 0) before[THREADS] = total;
-    __syncthreads();
+    const long long begins = ahead + run - mine;
     const int ctas = (int)min((long long)gridDim.x, quotient(total + kRunPages - 1, kRunPages)), cta = blockIdx.x;
     const bool works = cta < ctas;
     const long long c_lo = works ? quotient(total * cta, ctas) : 0, c_hi = works ? quotient(total * (cta + 1), ctas) : 0;
-    if (works && mine > 0 && before[tid] <= c_lo && c_lo < before[tid] + mine) {      // one thread's sequences hold the CTA's first page
-        long long at = before[tid];
-        for (int s = s_lo; s < s_hi; ++s) {
+    // the warp whose sequences hold the CTA's first page looks for its place
+    const uint32_t holds = __ballot_sync(0xffffffffu, works && mine > 0 && begins <= c_lo && c_lo < begins + mine);
+    if (holds != 0) {
+        const int lane_of = __ffs(holds) - 1;
+        long long at = __shfl_sync(0xffffffffu, begins, lane_of);
+        Cursor c{__shfl_sync(0xffffffffu, s_lo, lane_of), 0, 0, 0};
+        for (int k = 0; k < each; ++k, ++c.s) {
+            long long per = head_pages(lane == 0 && c.s < a.nseq ? c.s : -1);
+            per = __shfl_sync(0xffffffffu, per, 0);
+            if (c_lo >= at + per * a.kv_heads) { at += per * a.kv_heads; continue; }
+            c.head = (int)quotient(c_lo - at, per);
+            long long rel = c_lo - at - c.head * per;
             Sequence q;
-            bool bad;
-            const long long per = head_pages(s, q, bad), n = per * a.kv_heads;
-            if (c_lo < at + n) {
-                long long rel = c_lo - at;
-                Cursor c;
-                c.s = s;
-                c.head = (int)quotient(rel, per);
-                rel -= c.head * per;
-                for (c.tile = 0;; ++c.tile) {
-                    int lo, hi;
-                    unit_pages(q, c.tile, lo, hi);
-                    if (rel < hi - lo) break;
-                    rel -= hi - lo;
+            lengths_of(a, c.s, q);
+            for (int t0 = 0, n = tiles_of(q); t0 < n; t0 += 32) {       // 32 tiles at a time
+                const int here = t0 + lane < n ? pages_of(q, t0 + lane) : 0;
+                long long upto = here;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) { const long long t = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += t; }
+                const uint32_t in = __ballot_sync(0xffffffffu, rel < upto);
+                if (in != 0) {
+                    const int x = __ffs(in) - 1;
+                    c.tile = t0 + x;
+                    c.skip = (int)(rel - (__shfl_sync(0xffffffffu, upto, x) - __shfl_sync(0xffffffffu, here, x)));
+                    break;
                 }
-                c.skip = (int)rel;
-                start_s = c;
-                break;
+                rel -= __shfl_sync(0xffffffffu, upto, 31);
             }
-            at += n;
+            break;
         }
+        if (lane == 0) start_s = c;
     }
     __syncthreads();
 
@@ -217,16 +250,13 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                 if (++c.head == a.kv_heads) {
                     c.head = 0;
                     Sequence q;
-                    do {
-                        ++c.s;                             // (there is one more: pages are left)
-                        if (!lengths_of(a, c.s, q)) continue;
-                    } while (c.s + 1 < a.nseq && !(lengths_of(a, c.s, q) && q.n > 0 && q.n <= a.max_new && (long)q.n * a.group > a.few));
+                    do ++c.s; while (c.s + 1 < a.nseq && !has_work(c.s, q));      // (there is one more: pages are left)
                 }
             }
         }
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (!mbar_try_wait(bar, parity & 1) && !*dead_s && !mbar_wait(bar, parity & 1, a.wait_ns)) *dead_s = 1;
+        if (!mbar_try_wait(bar, parity & 1)) patient_wait(bar, parity & 1, a.wait_ns, dead_s);
         __syncwarp();
     };
     auto arrive = [&](uint64_t* bar) {                     // one of four warps, all of its lanes
@@ -250,47 +280,52 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
             const int pos = g.q.total - g.q.n + row, lo_pos = a.window > 0 ? max(0, pos - a.window + 1) : 0;
             const long out_row = g.q.first + row;
             const int out_head = g.head * a.group + h;
-            // q: times a power of two that brings the column's largest to 2^13 .. 2^14
-            float cx;
+            // q, times a power of two that brings the column's largest to 2^13 .. 2^14: each warp 16 columns of the tile, eight numbers per lane
             {
-                const T* const p = (const T*)a.q + out_row * a.ldq + (long)out_head * a.dk;
-                auto eight = [&](int d, float(&t)[8]) {
-                    const int n = valid ? a.dk - d : 0;
-                    if (a.wide_q) eight_numbers(p + d, n, t);
-                    else {
+                constexpr int PER = NG * 4, AT_ONCE = 4;   // lanes per column; loads under way
+                const int c_lane = lane / PER, d = lane % PER * 8, c0 = warp % 8 * 16;
+#pragma unroll 1
+                for (int i0 = 0; i0 < PER / 2; i0 += AT_ONCE) {
+                    float t[AT_ONCE][8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) t[e] = e < n ? number(p + d + e) : 0.f;
+                    for (int i = 0; i < AT_ONCE; ++i) {
+                        const int c = col0 + c0 + (i0 + i) * (32 / PER) + c_lane, c_row = min(c, g.cols - 1) / a.group, c_head = min(c, g.cols - 1) - c_row * a.group;
+                        const T* const p = (const T*)a.q + (long)(g.q.first + c_row) * a.ldq + (long)(g.head * a.group + c_head) * a.dk + d;
+                        const int n = c < g.cols ? a.dk - d : 0;
+                        if (a.wide_q) eight_numbers(p, n, t[i]);
+                        else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) t[i][e] = e < n ? number(p + e) : 0.f;
+                        }
                     }
-                };
-                uint32_t top = 0;
-#pragma unroll 4
-                for (int d = 0; d < a.dk; d += 8) {
-                    float t[8];
-                    eight(d, t);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(t[e]) & 0x7fffffffu);
-                }
-                const float by = power_of_two(top >= 0x7f800000u || top == 0 ? 0 : min(126, 13 + 127 - (int)(top >> 23)));
-                cx = fminf(fmaxf(__fdiv_rn(fabsf(a.scale) * kLog2e, by), 1e-37f), 3.4e38f);
-                const float f = a.scale < 0.f ? -by : by;
-#pragma unroll 2
-                for (int d = half * 8; d < gk * kGroup; d += 16) {
-                    float t[8];
-                    eight(d, t);
-                    uint32_t hi[4], lo[4];
+                    for (int i = 0; i < AT_ONCE; ++i) {
+                        const int c = c0 + (i0 + i) * (32 / PER) + c_lane;
+                        uint32_t top = 0;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float x = t[2 * e] * f, y = t[2 * e + 1] * f;
-                        hi[e] = halves(x, y);
-                        if (TWO) { const float2 b = unhalves(hi[e]); lo[e] = halves(x - b.x, y - b.y); }
+                        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(t[i][e]) & 0x7fffffffu);
+#pragma unroll
+                        for (int o = 1; o < PER; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        const float by = power_of_two(top >= 0x7f800000u || top == 0 ? 0 : min(126, 13 + 127 - (int)(top >> 23)));
+                        if (lane % PER == 0) factors_s[tile][c] = fminf(fmaxf(__fdiv_rn(fabsf(a.scale) * kLog2e, by), 1e-37f), 3.4e38f);
+                        const float f = a.scale < 0.f ? -by : by;
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = t[i][2 * e] * f, y = t[i][2 * e + 1] * f;
+                            hi[e] = halves(x, y);
+                            if (TWO) { const float2 b = unhalves(hi[e]); lo[e] = halves(x - b.x, y - b.y); }
+                        }
+                        uint8_t* const to = q_sm + ((tile * TERMS) * BLOCKS + d / 64) * (kTile * 128) + c * 128 + ((d / 8 % 8) ^ (c & 7)) * 16;
+                        *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        if (TWO) *reinterpret_cast<uint4*>(to + BLOCKS * (kTile * 128)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
-                    uint8_t* const to = q_sm + ((tile * TERMS) * BLOCKS + d / 64) * (kTile * 128) + r * 128 + ((d / 8 % 8) ^ (r & 7)) * 16;
-                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if (TWO) *reinterpret_cast<uint4*>(to + BLOCKS * (kTile * 128)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 arrive(&q_full[tile]);
+                tile_barrier(9 + tile);
             }
+            const float cx = factors_s[tile][r];
             const int first_full = __reduce_max_sync(0xffffffffu, lo_pos), last_full = __reduce_min_sync(0xffffffffu, pos);      // positions that all of the warp's columns see
             float m = -INFINITY, l = 0.f;                  // (l: of this thread's tokens)
             int e_v = 0;
@@ -629,6 +664,12 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
         // ---- copies
         uint32_t pages = 0;
         walk([&](const Segment& g, long long unit_lo) {
+            // rows of the tile behind this one, on their way into L2
+            if (a.wide_q && (g.tile + 1) * COLS < g.cols) {
+                const int row0 = (g.tile + 1) * COLS / a.group, row1 = (min((g.tile + 2) * COLS, g.cols) - 1) / a.group;
+                const uint32_t bytes = (uint32_t)(a.group * a.dk * sizeof(T));
+                for (int x = row0 + lane; x <= row1; x += 32) l2_prefetch((const T*)a.q + (long)(g.q.first + x) * a.ldq + (long)g.head * a.group * a.dk, bytes);
+            }
             for (int p = g.p0; p < g.p1; ++p, ++pages) {
                 const int slot = pages % ring_n;
                 int page = lane == 0 ? a.table[(size_t)g.s * a.width + p] : 0;
