@@ -25,7 +25,7 @@ struct AttendArgs {
     long ldq, ldy;
     int heads, kv_heads, group, dk, dv, window, sink, nseq, rows, max_new, n_pages, width;
     int few;                                               // columns per head of the cache up to which a sequence is the step kernel's
-    int wide_q, wide_y;                                    // rows and heads lie on boundaries of 16 bytes, of four numbers
+    int wide_q, wide_y, wide_y16;                          // rows and heads of q lie on boundaries of 16 bytes; of y on those of four numbers, of 16 bytes
     int slots, slot_bytes;                                 // of a warp's ring
     int skip;                                              // failure tests: the copy of this page of the line is not issued
     float scale;

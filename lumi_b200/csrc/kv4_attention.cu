@@ -757,6 +757,7 @@ extern "C" int32_t lumi_k_kv4_attention(uint64_t q, int32_t ldq, int32_t dtype, 
     a.window = window; a.sink = sink != 0; a.nseq = nseq; a.rows = rows; a.max_new = max_new; a.n_pages = n_pages; a.width = pages_per_seq; a.scale = scale;
     a.wide_q = (q & 15) == 0 && dk % 8 == 0 && (long)ldq * (f32 ? 4 : 2) % 16 == 0;
     a.wide_y = (y & (f32 ? 15 : 7)) == 0 && dv % 4 == 0 && ldy % 4 == 0;
+    a.wide_y16 = (y & 15) == 0 && dv % (f32 ? 4 : 8) == 0 && ldy % (f32 ? 4 : 8) == 0;
     a.few = kFewColumns; a.wait_ns = kWaitLimitNs; a.skip = -1;
     LUMI_TRY(f32 ? step<float>(a, work, (cudaStream_t)stream) : step<__nv_bfloat16>(a, work, (cudaStream_t)stream));
     return (long)max_new * a.group > a.few ? launch_kv4_prompt(a, f32, work, (cudaStream_t)stream) : LUMI_OK;

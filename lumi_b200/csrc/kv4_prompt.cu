@@ -23,7 +23,8 @@ namespace {
 constexpr int kTile = 128;
 constexpr int kPromptCtas = 160;                           // places for parts
 constexpr int kTicketsAt = 320;                            // behind the step kernel's
-constexpr int kRunPages = 4;                               // a CTA's, at least
+constexpr int kUnitPages = 3;                              // what a unit costs beside its pages: queries, pipeline, results.  On the line it begins with as many places without a page
+constexpr int kRunPages = 8;                               // a CTA's, at least
 constexpr int kMaxRing = 4;
 constexpr int kStatic = 10 * 1024;                         // bytes declared in the kernel, at most
 constexpr int kInfos = 8;                                  // pages whose exponents are kept: the copies run up to kMaxRing ahead of the values' tiles, these two ahead of the softmax
@@ -96,6 +97,54 @@ __device__ __noinline__ void patient_wait(uint64_t* bar, uint32_t parity, uint64
     }
 }
 
+// Eight numbers of a row that has n of them, as memory holds them; and as fp32.
+__device__ __forceinline__ void eight_raw(const float* p, int n, bool wide, uint4 (&w)[2]) {
+    w[0] = w[1] = make_uint4(0, 0, 0, 0);
+    if (wide) {
+        if (n > 0) { w[0] = reinterpret_cast<const uint4*>(p)[0]; w[1] = reinterpret_cast<const uint4*>(p)[1]; }
+    } else {
+        uint32_t u[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = e < n ? __float_as_uint(p[e]) : 0u;
+        w[0] = make_uint4(u[0], u[1], u[2], u[3]);
+        w[1] = make_uint4(u[4], u[5], u[6], u[7]);
+    }
+}
+__device__ __forceinline__ void eight_raw(const __nv_bfloat16* p, int n, bool wide, uint4 (&w)[1]) {
+    w[0] = make_uint4(0, 0, 0, 0);
+    if (wide) {
+        if (n > 0) w[0] = *reinterpret_cast<const uint4*>(p);
+    } else {
+        uint32_t u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            u[e] = (2 * e < n ? (uint32_t)__bfloat16_as_ushort(p[2 * e]) : 0u) | (2 * e + 1 < n ? (uint32_t)__bfloat16_as_ushort(p[2 * e + 1]) << 16 : 0u);
+        w[0] = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+}
+__device__ __forceinline__ void eight_of(const uint4 (&w)[2], float (&t)[8]) {
+    t[0] = __uint_as_float(w[0].x); t[1] = __uint_as_float(w[0].y); t[2] = __uint_as_float(w[0].z); t[3] = __uint_as_float(w[0].w);
+    t[4] = __uint_as_float(w[1].x); t[5] = __uint_as_float(w[1].y); t[6] = __uint_as_float(w[1].z); t[7] = __uint_as_float(w[1].w);
+}
+__device__ __forceinline__ void eight_of(const uint4 (&w)[1], float (&t)[8]) {
+    const uint32_t u[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { t[2 * i] = low_bf16(u[i]); t[2 * i + 1] = high_bf16(u[i]); }
+}
+// 16 bytes of a row of y that has n numbers from here on.
+__device__ __forceinline__ void put_16(float* y, int n, bool wide, uint4 u) {
+    if (wide) { if (n > 0) *reinterpret_cast<uint4*>(y) = u; return; }
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (i < n) y[i] = __uint_as_float(w[i]);
+}
+__device__ __forceinline__ void put_16(__nv_bfloat16* y, int n, bool wide, uint4 u) {
+    if (wide) { if (n > 0) *reinterpret_cast<uint4*>(y) = u; return; }
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) if (i < n) y[i] = __ushort_as_bfloat16((unsigned short)(w[i / 2] >> (i % 2 * 16)));
+}
+
 struct PageInfo { int e_k, e_v, absent; uint32_t no_number[2]; };      // exponents of keys and values; tokens with values that are no numbers
 
 struct Cursor { int s, head, tile, skip; };                // a unit, and pages of it that are the CTA's ahead
@@ -152,7 +201,7 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
     auto pages_of = [&](const Sequence& q, int tile) {
         int lo, hi;
         unit_pages(q, tile, lo, hi);
-        return hi - lo;
+        return hi - lo + kUnitPages;
     };
     auto has_work = [&](int s, Sequence& q) { return lengths_of(a, s, q) && q.n > 0 && q.n <= a.max_new && (long)q.n * a.group > a.few; };
     auto warp_sum = [&](long long v) {
@@ -160,7 +209,7 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         return v;
     };
-    // Pages of one head of each lane's sequence (s < 0: none), 0 where there is nothing of this kernel's.  Sequences of many tiles are summed up by the whole warp.
+    // Places of one head of each lane's sequence (s < 0: none), 0 where there is nothing of this kernel's.  Sequences of many tiles are summed up by the whole warp.
     auto head_pages = [&](int s) {
         Sequence q;
         long long sum = 0;
@@ -238,11 +287,12 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
             g.s = c.s; g.head = c.head; g.tile = c.tile;
             g.cols = g.q.n * a.group;
             unit_pages(g.q, c.tile, g.lo, g.hi);
-            g.p0 = g.lo + c.skip;
-            g.p1 = g.p0 + (int)min(left, (long long)(g.hi - g.p0));
-            body(g, at - c.skip);
-            left -= g.p1 - g.p0;
-            at += g.p1 - g.p0;
+            const int take = (int)min(left, (long long)(g.hi - g.lo + kUnitPages - c.skip));
+            g.p0 = g.lo + max(0, c.skip - kUnitPages);
+            g.p1 = g.lo + max(0, c.skip + take - kUnitPages);
+            if (g.p1 > g.p0) body(g, at - c.skip + kUnitPages);
+            left -= take;
+            at += take;
             if (left <= 0) break;
             c.skip = 0;
             if (++c.tile * COLS >= g.cols) {
@@ -282,28 +332,25 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
             const int out_head = g.head * a.group + h;
             // q, times a power of two that brings the column's largest to 2^13 .. 2^14: each warp 16 columns of the tile, eight numbers per lane
             {
-                constexpr int PER = NG * 4, AT_ONCE = 4;   // lanes per column; loads under way
+                constexpr int PER = NG * 4, AT_ONCE = TWO ? 4 : NG * 2 < 8 ? NG * 2 : 8;      // lanes per column; loads under way
                 const int c_lane = lane / PER, d = lane % PER * 8, c0 = warp % 8 * 16;
 #pragma unroll 1
                 for (int i0 = 0; i0 < PER / 2; i0 += AT_ONCE) {
-                    float t[AT_ONCE][8];
+                    uint4 raw[AT_ONCE][sizeof(T) / 2];
 #pragma unroll
                     for (int i = 0; i < AT_ONCE; ++i) {
                         const int c = col0 + c0 + (i0 + i) * (32 / PER) + c_lane, c_row = min(c, g.cols - 1) / a.group, c_head = min(c, g.cols - 1) - c_row * a.group;
                         const T* const p = (const T*)a.q + (long)(g.q.first + c_row) * a.ldq + (long)(g.head * a.group + c_head) * a.dk + d;
-                        const int n = c < g.cols ? a.dk - d : 0;
-                        if (a.wide_q) eight_numbers(p, n, t[i]);
-                        else {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) t[i][e] = e < n ? number(p + e) : 0.f;
-                        }
+                        eight_raw(p, c < g.cols ? a.dk - d : 0, a.wide_q, raw[i]);
                     }
 #pragma unroll
                     for (int i = 0; i < AT_ONCE; ++i) {
                         const int c = c0 + (i0 + i) * (32 / PER) + c_lane;
+                        float t[8];
+                        eight_of(raw[i], t);
                         uint32_t top = 0;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(t[i][e]) & 0x7fffffffu);
+                        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(t[e]) & 0x7fffffffu);
 #pragma unroll
                         for (int o = 1; o < PER; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
                         const float by = power_of_two(top >= 0x7f800000u || top == 0 ? 0 : min(126, 13 + 127 - (int)(top >> 23)));
@@ -312,7 +359,7 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                         uint32_t hi[4], lo[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float x = t[i][2 * e] * f, y = t[i][2 * e + 1] * f;
+                            const float x = t[2 * e] * f, y = t[2 * e + 1] * f;
                             hi[e] = halves(x, y);
                             if (TWO) { const float2 b = unhalves(hi[e]); lo[e] = halves(x - b.x, y - b.y); }
                         }
@@ -431,6 +478,12 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
             const int rec = places * (2 + pad);
             float* const to = a.parts + ((size_t)cta * 2 + (g.p0 == g.lo ? 1 : 0)) * rec;
             const float inv = whole ? inverse(m, l) : 1.f;
+            // Rows of y by way of the queries' places that this warp alone fills (their products are done): 32 columns, CHUNKS x 16 bytes each
+            constexpr int CHUNKS = NG / 2 * kGroup * (int)sizeof(T) / 16, PIECE = 16 * 128, E = 16 / (int)sizeof(T);
+            auto stage = [&](int c, int chunk) {
+                const int x = (c * CHUNKS + (CHUNKS >= 8 ? chunk ^ (c & 7) : chunk ^ (c >> 1 & 3))) * 16;
+                return q_sm + (tile * TERMS * BLOCKS + x / PIECE) * (kTile * 128) + warp % 8 * PIECE + x % PIECE;
+            };
 #pragma unroll 1
             for (int d = d_lo; d < d_hi; d += 16) {
                 uint32_t o[16];
@@ -440,11 +493,32 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                     float v[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(o[8 * k + j]) * back * back2;
-                    if (whole) { if (valid) put_row(d + 8 * k, v, inv); }
-                    else {
+                    if (whole) {                           // (numbers of a tile lie as 0 4 1 5 2 6 3 7)
+                        const int chunk = (d - d_lo + 8 * k) / E;
+                        if constexpr (TWO) {
+                            *reinterpret_cast<float4*>(stage(lane, chunk)) = make_float4(v[0] * inv, v[2] * inv, v[4] * inv, v[6] * inv);
+                            *reinterpret_cast<float4*>(stage(lane, chunk + 1)) = make_float4(v[1] * inv, v[3] * inv, v[5] * inv, v[7] * inv);
+                        } else {
+                            const __nv_bfloat162 x0 = __floats2bfloat162_rn(v[0] * inv, v[2] * inv), x1 = __floats2bfloat162_rn(v[4] * inv, v[6] * inv);
+                            const __nv_bfloat162 x2 = __floats2bfloat162_rn(v[1] * inv, v[3] * inv), x3 = __floats2bfloat162_rn(v[5] * inv, v[7] * inv);
+                            *reinterpret_cast<uint4*>(stage(lane, chunk)) = make_uint4(*reinterpret_cast<const uint32_t*>(&x0), *reinterpret_cast<const uint32_t*>(&x1),
+                                                                                      *reinterpret_cast<const uint32_t*>(&x2), *reinterpret_cast<const uint32_t*>(&x3));
+                        }
+                    } else {
                         *reinterpret_cast<float4*>(to + 2 * places + ((d / 4 + 2 * k) * places + at) * 4) = make_float4(v[0], v[1], v[2], v[3]);
                         *reinterpret_cast<float4*>(to + 2 * places + ((d / 4 + 2 * k + 1) * places + at) * 4) = make_float4(v[4], v[5], v[6], v[7]);
                     }
+                }
+            }
+            if (whole) {
+                __syncwarp();
+                const unsigned long long mine_at = (unsigned long long)((T*)a.y + out_row * a.ldy + (long)out_head * a.dv) | (valid ? 0 : 1ull << 63);
+#pragma unroll 4
+                for (int i = 0; i < CHUNKS; ++i) {
+                    const int c = (i * 32 + lane) / CHUNKS, chunk = (i * 32 + lane) % CHUNKS, d = d_lo + chunk * E;
+                    const unsigned long long y = __shfl_sync(0xffffffffu, mine_at, c);
+                    const uint4 u = *reinterpret_cast<const uint4*>(stage(c, chunk));
+                    if (y >> 63 == 0 && d < d_hi) put_16((T*)y + d, a.dv - d, a.wide_y16, u);
                 }
             }
             tc_fence_before();
