@@ -156,8 +156,11 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
 }
 
 // ---- rows into the cache, and back ---------------------------------------------------------------------------------
-// A warp takes eight rows and one group of a head, four lanes a row: eight numbers each, one word of codes.  Rows of a prompt are neighbouring tokens of a page, so that a warp's
-// words are 128 bytes in a row and its scales 16.
+// A warp takes one group of a head, of eight rows at a time, four lanes a row: eight numbers each, one word of codes.  Rows of a prompt are neighbouring tokens of a page, so that a
+// warp's words are 128 bytes in a row and its scales 16.  kDeep eights of rows per warp where there are many: their loads are under way together, and what a group's place costs in
+// arithmetic is shared.  Bound by memory: KV4_ROWS_MEASURED
+constexpr int kDeep = 4;
+constexpr int kManyRows = 1024;                            // rows from which on warps take kDeep eights
 struct RowsArgs {
     const void *k, *v;
     void *k_out, *v_out;
@@ -165,22 +168,28 @@ struct RowsArgs {
     uint8_t* kv;
     long ldk, ldv;
     int n_slots, heads, dk, dv, rows;
+    int split;                                             // log2 of the groups that a block of eight warps takes; its warps share rows by the rest
 };
-struct Place { uint8_t* codes; uint8_t* scale; int d, column; bool keys; };
-// item: [head][groups of keys, then of values]
-__device__ __forceinline__ Place place_of(const RowsArgs& a, int slot, int item, int quarter) {
-    const int gk = kv4_groups(a.dk), gv = kv4_groups(a.dv), head = item / (gk + gv), i = item % (gk + gv);
-    const bool keys = i < gk;
-    const int g = keys ? i : i - gk, token = slot % kPage;
-    uint8_t* const part = a.kv + ((size_t)(slot / kPage) * a.heads + head) * kv4_block(a.dk, a.dv) + (keys ? 0 : kv4_part(a.dk));
+// One group of a head: where it lies in a page and in a row.
+struct Place { size_t page_bytes; int codes, scale, d, column; bool keys, any; };
+__device__ __forceinline__ Place place_of(const RowsArgs& a, int quarter) {
+    const int gk = kv4_groups(a.dk), gv = kv4_groups(a.dv), block = kv4_block(a.dk, a.dv);
+    const int item = (blockIdx.y << a.split) + ((threadIdx.x >> 5) & ((1 << a.split) - 1));      // [head][groups of keys, then of values]
+    const int head = item / (gk + gv), i = item - head * (gk + gv);
     Place p;
-    p.codes = part + g * kPlane + token * 16 + quarter * 4;
-    p.scale = part + (keys ? gk : gv) * kPlane + g * kScales + token * 2;
-    p.keys = keys;
-    const int first = g * kGroup + quarter * 8;
-    p.d = (keys ? a.dk : a.dv) - first;                    // numbers that the head has from here on
-    p.column = head * (keys ? a.dk : a.dv) + first;
+    p.any = head < a.heads;
+    p.keys = i < gk;
+    const int g = p.keys ? i : i - gk, part = head * block + (p.keys ? 0 : kv4_part(a.dk)), first = g * kGroup + quarter * 8;
+    p.page_bytes = (size_t)a.heads * block;
+    p.codes = part + g * kPlane + quarter * 4;
+    p.scale = part + (p.keys ? gk : gv) * kPlane + g * kScales;
+    p.d = (p.keys ? a.dk : a.dv) - first;                  // numbers that the head has from here on
+    p.column = head * (p.keys ? a.dk : a.dv) + first;
     return p;
+}
+template <int DEEP>
+__device__ __forceinline__ long first_row(const RowsArgs& a) {
+    return (((long)blockIdx.x << (3 - a.split)) + (threadIdx.x >> (5 + a.split))) * (8 * DEEP) + ((threadIdx.x & 31) >> 2);
 }
 // Where number e of a lane's eight lies in its word, as a shift.
 __device__ __forceinline__ int nibble_shift(bool keys, int e) { return 4 * (keys ? (e >> 1) + 4 * (e & 1) : e); }
@@ -227,53 +236,92 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&t)[8]) {
     }
 }
 
-template <typename T, bool WHOLE>
+template <typename T, bool WHOLE, int DEEP>
 __global__ void __launch_bounds__(256) kv4_append_kernel(RowsArgs a) {
-    const int lane = threadIdx.x & 31, items = a.heads * (kv4_groups(a.dk) + kv4_groups(a.dv));
-    const long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const long row = w / items * 8 + (lane >> 2);
+    const int lane = threadIdx.x & 31;
+    const Place p = place_of(a, lane & 3);
+    const long row0 = first_row<DEEP>(a);
     pdl_release();
     pdl_sync();
-    const int slot = row < a.rows ? a.slot[row] : -1;
-    const bool lives = slot >= 0 && slot < a.n_slots;
-    const Place p = place_of(a, lives ? slot : 0, (int)(w % items), lane & 3);
-    float t[8];
-    load8<T, WHOLE>((p.keys ? (const T*)a.k + row * a.ldk : (const T*)a.v + row * a.ldv) + p.column, lives ? p.d : 0, t);
-    uint32_t m = 0;                                        // absolute values as bits: the largest, and infinities and NaN above all
+    if (!p.any) return;                                    // (the whole warp)
+    const T* const from = p.keys ? (const T*)a.k : (const T*)a.v;
+    const long ld = p.keys ? a.ldk : a.ldv;
+    int slot[DEEP];
+    float t[DEEP][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(t[i]) & 0x7fffffffu);
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    if (!lives) return;
-    const bool numbers = m < 0x7f800000u;
-    const uint32_t up = numbers ? (__float_as_uint(__fdiv_rn(fmaxf(__uint_as_float(m), kLeast), 7.f)) + 0xffffu) & 0xffff0000u : 0x7fc00000u;
-    const float s = __uint_as_float(up);
-    uint32_t word = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int n = numbers ? 8 + __float2int_rn(__fdiv_rn(t[i], s)) : 8;
-        word |= (uint32_t)n << nibble_shift(p.keys, i);
+    for (int k = 0; k < DEEP; ++k) {
+        const long row = row0 + 8 * k;
+        slot[k] = row < a.rows ? a.slot[row] : -1;
+        if (slot[k] >= a.n_slots) slot[k] = -1;
     }
-    *reinterpret_cast<uint32_t*>(p.codes) = word;
-    if ((lane & 3) == 0) *reinterpret_cast<uint16_t*>(p.scale) = (uint16_t)(up >> 16);
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) load8<T, WHOLE>(from + (row0 + 8 * k) * ld + p.column, slot[k] >= 0 ? p.d : 0, t[k]);
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) {
+        uint32_t m = 0;                                    // absolute values as bits: the largest, and infinities and NaN above all
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(t[k][i]) & 0x7fffffffu);
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const bool numbers = m < 0x7f800000u;
+        const uint32_t up = numbers ? (__float_as_uint(__fdiv_rn(fmaxf(__uint_as_float(m), kLeast), 7.f)) + 0xffffu) & 0xffff0000u : 0x7fc00000u;
+        const float s = __uint_as_float(up), inv = __frcp_rn(s);
+        // 8 + rint(t / s) by way of t (1 / s), which is the quotient to 2^-20: the low bits of a sum at 1.5 2^23.  Beside a half, where that might round the other way, the quotient itself.
+        uint32_t word = 0;
+        float off = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x = fmaf(t[k][i], inv, 12582920.f);
+            off = fmaxf(off, fabsf(fmaf(t[k][i], inv, 12582920.f - x)));
+            word |= (__float_as_uint(x) & 15u) << nibble_shift(p.keys, i);
+        }
+        if (!numbers) word = 0x88888888u;
+        else if (off > 0.49999f) {
+            word = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) word |= (uint32_t)(8 + __float2int_rn(__fdiv_rn(t[k][i], s))) << nibble_shift(p.keys, i);
+        }
+        if (slot[k] < 0) continue;
+        uint8_t* const page = a.kv + (size_t)(slot[k] / kPage) * p.page_bytes;
+        *reinterpret_cast<uint32_t*>(page + p.codes + slot[k] % kPage * 16) = word;
+        if ((lane & 3) == 0) *reinterpret_cast<uint16_t*>(page + p.scale + slot[k] % kPage * 2) = (uint16_t)(up >> 16);
+    }
 }
 
-template <typename T, bool WHOLE>
+template <typename T, bool WHOLE, int DEEP>
 __global__ void __launch_bounds__(256) kv4_read_kernel(RowsArgs a) {
-    const int lane = threadIdx.x & 31, items = a.heads * (kv4_groups(a.dk) + kv4_groups(a.dv));
-    const long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const long row = w / items * 8 + (lane >> 2);
+    const int lane = threadIdx.x & 31;
+    const Place p = place_of(a, lane & 3);
+    const long row0 = first_row<DEEP>(a);
     pdl_release();
     pdl_sync();
-    const int slot = row < a.rows ? a.slot[row] : -1;
-    if (slot < 0 || slot >= a.n_slots) return;
-    const Place p = place_of(a, slot, (int)(w % items), lane & 3);
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(p.codes);
-    const float s = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(p.scale) << 16);
-    float t[8];
+    if (!p.any) return;
+    T* const to = p.keys ? (T*)a.k_out : (T*)a.v_out;
+    const long ld = p.keys ? a.ldk : a.ldv;
+    int slot[DEEP];
+    uint32_t word[DEEP], scale[DEEP];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = (float)((int)((word >> nibble_shift(p.keys, i)) & 15u) - 8) * s;
-    store8<T, WHOLE>((p.keys ? (T*)a.k_out + row * a.ldk : (T*)a.v_out + row * a.ldv) + p.column, p.d, t);
+    for (int k = 0; k < DEEP; ++k) {
+        const long row = row0 + 8 * k;
+        slot[k] = row < a.rows ? a.slot[row] : -1;
+        if (slot[k] >= a.n_slots) slot[k] = -1;
+    }
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) {
+        word[k] = scale[k] = 0;
+        if (slot[k] < 0) continue;
+        const uint8_t* const page = a.kv + (size_t)(slot[k] / kPage) * p.page_bytes;
+        word[k] = *reinterpret_cast<const uint32_t*>(page + p.codes + slot[k] % kPage * 16);
+        scale[k] = *reinterpret_cast<const uint16_t*>(page + p.scale + slot[k] % kPage * 2);
+    }
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) {
+        const float s = __uint_as_float(scale[k] << 16);
+        float t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = (__uint_as_float((word[k] >> nibble_shift(p.keys, i) & 15u) | 0x4b000000u) - 8388616.f) * s;      // a code under the exponent of 2^23
+        if (slot[k] >= 0) store8<T, WHOLE>(to + (row0 + 8 * k) * ld + p.column, p.d, t);
+    }
 }
 
 bool whole(uint64_t p, int ld, int d, int dtype) { const int e = dtype == LUMI_DTYPE_F32 ? 4 : 2; return (p & 15) == 0 && (long)ld * e % 16 == 0 && d % 8 == 0; }
@@ -288,17 +336,20 @@ int32_t check_cache(const char* name, uint64_t kv, int n_pages, int kv_heads, in
 bool known(int dtype) { return dtype == LUMI_DTYPE_F32 || dtype == LUMI_DTYPE_BF16; }
 
 template <bool READ>
-int32_t rows_call(const char* name, const RowsArgs& a, int dtype, bool fits, cudaStream_t st) {
-    const long warps = ((long)a.rows + 7) / 8 * a.heads * (kv4_groups(a.dk) + kv4_groups(a.dv));
-    if ((warps + 7) / 8 > 0x7fffffffl) return fail(LUMI_E_UNSUPPORTED, "%s: %d rows of %d heads", name, a.rows, a.heads);
+int32_t rows_call(const char* name, RowsArgs a, int dtype, bool fits, cudaStream_t st) {
+    const int items = a.heads * (kv4_groups(a.dk) + kv4_groups(a.dv)), deep = a.rows >= kManyRows ? kDeep : 1;
+    a.split = items >= 8 ? 3 : items >= 4 ? 2 : 1;         // (there are two groups at least)
+    const long rows_per_block = 8l * deep << (3 - a.split), blocks = ((long)a.rows + rows_per_block - 1) / rows_per_block, across = ((long)items + (1 << a.split) - 1) >> a.split;
+    if (across > 65535) return fail(LUMI_E_UNSUPPORTED, "%s: %d heads of %d and %d numbers", name, a.heads, a.dk, a.dv);
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[1];
-    dependent(cfg, attr, dim3((unsigned)((warps + 7) / 8)), 256, 0, st);
-    auto go = [&](auto t, auto w) {
+    dependent(cfg, attr, dim3((unsigned)blocks, (unsigned)across), 256, 0, st);
+    auto of_depth = [&](auto t, auto w, auto d) {
         using T = decltype(t);
-        if constexpr (READ) return cudaLaunchKernelEx(&cfg, kv4_read_kernel<T, decltype(w)::value>, a);
-        else return cudaLaunchKernelEx(&cfg, kv4_append_kernel<T, decltype(w)::value>, a);
+        if constexpr (READ) return cudaLaunchKernelEx(&cfg, kv4_read_kernel<T, decltype(w)::value, decltype(d)::value>, a);
+        else return cudaLaunchKernelEx(&cfg, kv4_append_kernel<T, decltype(w)::value, decltype(d)::value>, a);
     };
+    auto go = [&](auto t, auto w) { return deep == 1 ? of_depth(t, w, std::integral_constant<int, 1>()) : of_depth(t, w, std::integral_constant<int, kDeep>()); };
     using Yes = std::integral_constant<bool, true>;
     using No = std::integral_constant<bool, false>;
     if (dtype == LUMI_DTYPE_F32) LUMI_CUDA(fits ? go(float(), Yes()) : go(float(), No()));
@@ -358,7 +409,7 @@ extern "C" int32_t lumi_k_kv4_append(uint64_t k, int32_t ldk, uint64_t v, int32_
     LUMI_TRY(check_rows("lumi_k_kv4_append", k, ldk, v, ldv, dtype, slot, kv, n_pages, kv_heads, dk, dv, rows));
     if (rows == 0) return LUMI_OK;
     LUMI_TRY(check_device_memory("lumi_k_kv4_append", {k, v, slot, kv}));
-    const RowsArgs a{(const void*)k, (const void*)v, nullptr, nullptr, (const int32_t*)slot, (uint8_t*)kv, ldk, ldv, n_pages * kPage, kv_heads, dk, dv, rows};
+    const RowsArgs a{(const void*)k, (const void*)v, nullptr, nullptr, (const int32_t*)slot, (uint8_t*)kv, ldk, ldv, n_pages * kPage, kv_heads, dk, dv, rows, 0};
     return rows_call<false>("lumi_k_kv4_append", a, dtype, whole(k, ldk, dk, dtype) && whole(v, ldv, dv, dtype), (cudaStream_t)stream);
 }
 
@@ -367,6 +418,6 @@ extern "C" int32_t lumi_k_kv4_read(uint64_t kv, int32_t n_pages, uint64_t slot, 
     LUMI_TRY(check_rows("lumi_k_kv4_read", k, ldk, v, ldv, dtype, slot, kv, n_pages, kv_heads, dk, dv, rows));
     if (rows == 0) return LUMI_OK;
     LUMI_TRY(check_device_memory("lumi_k_kv4_read", {k, v, slot, kv}));
-    const RowsArgs a{nullptr, nullptr, (void*)k, (void*)v, (const int32_t*)slot, (uint8_t*)kv, ldk, ldv, n_pages * kPage, kv_heads, dk, dv, rows};
+    const RowsArgs a{nullptr, nullptr, (void*)k, (void*)v, (const int32_t*)slot, (uint8_t*)kv, ldk, ldv, n_pages * kPage, kv_heads, dk, dv, rows, 0};
     return rows_call<true>("lumi_k_kv4_read", a, dtype, whole(k, ldk, dk, dtype) && whole(v, ldv, dv, dtype), (cudaStream_t)stream);
 }
