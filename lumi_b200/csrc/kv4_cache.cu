@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
 // warp's words are 128 bytes in a row and its scales 16.  kDeep eights of rows per warp where there are many: their loads are under way together, and what a group's place costs in
 // arithmetic is shared.  Bound by memory: KV4_ROWS_MEASURED
 constexpr int kDeep = 4;
-constexpr int kManyRows = 1024;                            // rows from which on warps take kDeep eights
+constexpr int kManyRows = 4096;                            // rows from which on warps take kDeep eights
 struct RowsArgs {
     const void *k, *v;
     void *k_out, *v_out;
@@ -236,6 +236,12 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&t)[8]) {
     }
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+
 template <typename T, bool WHOLE, int DEEP>
 __global__ void __launch_bounds__(256) kv4_append_kernel(RowsArgs a) {
     const int lane = threadIdx.x & 31;
@@ -258,35 +264,49 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(RowsArgs a) {
     for (int k = 0; k < DEEP; ++k) load8<T, WHOLE>(from + (row0 + 8 * k) * ld + p.column, slot[k] >= 0 ? p.d : 0, t[k]);
 #pragma unroll
     for (int k = 0; k < DEEP; ++k) {
-        uint32_t m = 0;                                    // absolute values as bits: the largest, and infinities and NaN above all
+        float m = fabsf(t[k][0]);                          // the largest; infinities and NaN stay
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(t[k][i]) & 0x7fffffffu);
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const bool numbers = m < 0x7f800000u;
-        const uint32_t up = numbers ? (__float_as_uint(__fdiv_rn(fmaxf(__uint_as_float(m), kLeast), 7.f)) + 0xffffu) & 0xffff0000u : 0x7fc00000u;
+        for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(t[k][i]));
+        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const bool numbers = m < INFINITY;
+        const uint32_t up = numbers ? (__float_as_uint(__fdiv_rn(fmaxf(m, kLeast), 7.f)) + 0xffffu) & 0xffff0000u : 0x7fc00000u;
         const float s = __uint_as_float(up), inv = __frcp_rn(s);
-        // 8 + rint(t / s) by way of t (1 / s), which is the quotient to 2^-20: the low bits of a sum at 1.5 2^23.  Beside a half, where that might round the other way, the quotient itself.
-        uint32_t word = 0;
-        float off = 0.f;
+        // 8 + rint(t / s) by way of t (1 / s), which is the quotient to 2^-20: the low half of a sum at 1.5 2^23.  Beside a half, where that might round the other way, the quotient itself.
+        float x[8], off = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float x = fmaf(t[k][i], inv, 12582920.f);
-            off = fmaxf(off, fabsf(fmaf(t[k][i], inv, 12582920.f - x)));
-            word |= (__float_as_uint(x) & 15u) << nibble_shift(p.keys, i);
+            x[i] = fmaf(t[k][i], inv, 12582920.f);
+            off = fmaxf(off, fabsf(fmaf(t[k][i], inv, 12582920.f - x[i])));
         }
-        if (!numbers) word = 0x88888888u;
-        else if (off > 0.49999f) {
-            word = 0;
+        if (numbers && off > 0.49999f) {
+            if constexpr (sizeof(T) == 2) {
+                // bf16 numbers are often exactly half a step off, and else further from it than a quotient rounds: what is left of t decides, which is exact
 #pragma unroll
-            for (int i = 0; i < 8; ++i) word |= (uint32_t)(8 + __float2int_rn(__fdiv_rn(t[k][i], s))) << nibble_shift(p.keys, i);
+                for (int i = 0; i < 8; ++i) {
+                    const float left = fmaf(12582920.f - x[i], s, t[k][i]), over = fabsf(left) - 0.5f * s;
+                    if (over > 0.f || (over == 0.f && (__float_as_uint(x[i]) & 1u))) x[i] += copysignf(1.f, left);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = 12582920.f + rintf(__fdiv_rn(t[k][i], s));
+            }
         }
+        // two codes side by side in halves, four such pairs four bits apart: numbers 2 i and 2 i + 1 of keys, i and i + 4 of values
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 3; i >= 0; --i)
+            word = word * 16 + (p.keys ? __byte_perm(__float_as_uint(x[2 * i]), __float_as_uint(x[2 * i + 1]), 0x5410) : __byte_perm(__float_as_uint(x[i]), __float_as_uint(x[i + 4]), 0x5410));
+        if (!numbers) word = 0x88888888u;
         if (slot[k] < 0) continue;
         uint8_t* const page = a.kv + (size_t)(slot[k] / kPage) * p.page_bytes;
         *reinterpret_cast<uint32_t*>(page + p.codes + slot[k] % kPage * 16) = word;
         if ((lane & 3) == 0) *reinterpret_cast<uint16_t*>(page + p.scale + slot[k] % kPage * 2) = (uint16_t)(up >> 16);
     }
 }
+
+// The low nibble's code under the exponent of 2^23, less 2^23 + 8, times s.
+__device__ __forceinline__ float code_times(uint32_t w, float s) { return (__uint_as_float((w & 15u) | 0x4b000000u) - 8388616.f) * s; }
 
 template <typename T, bool WHOLE, int DEEP>
 __global__ void __launch_bounds__(256) kv4_read_kernel(RowsArgs a) {
@@ -317,10 +337,24 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(RowsArgs a) {
 #pragma unroll
     for (int k = 0; k < DEEP; ++k) {
         const float s = __uint_as_float(scale[k] << 16);
-        float t[8];
+        if constexpr (WHOLE && sizeof(T) == 4) {
+            // 32 numbers are 128 bytes: each store takes 16 of them per lane side by side, numbers 4 q .. and 16 + 4 q .., whose words neighbours hold
+            const int q = lane & 3, back = (q & 1) * (p.keys ? 8 : 16);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t[i] = (__uint_as_float((word[k] >> nibble_shift(p.keys, i) & 15u) | 0x4b000000u) - 8388616.f) * s;      // a code under the exponent of 2^23
-        if (slot[k] >= 0) store8<T, WHOLE>(to + (row0 + 8 * k) * ld + p.column, p.d, t);
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t w = __shfl_sync(0xffffffffu, word[k], (lane & 28) + 2 * h + (q >> 1)) >> back;
+                float t[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) t[i] = code_times(w >> nibble_shift(p.keys, i), s);
+                const int at = 16 * h + 4 * q - 8 * q;     // from the lane's own first number
+                if (slot[k] >= 0 && at < p.d) *reinterpret_cast<float4*>(to + (row0 + 8 * k) * ld + p.column + at) = make_float4(t[0], t[1], t[2], t[3]);
+            }
+        } else {
+            float t[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = code_times(word[k] >> nibble_shift(p.keys, i), s);
+            if (slot[k] >= 0) store8<T, WHOLE>(to + (row0 + 8 * k) * ld + p.column, p.d, t);
+        }
     }
 }
 
