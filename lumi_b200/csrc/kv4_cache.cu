@@ -29,8 +29,8 @@ void dependent(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, dim3 grid, in
 }
 
 // ---- plan ------------------------------------------------------------------------------------------------------
-// Every CTA takes the prefix sums over all sequences itself (they are few numbers), so that nothing but a barrier has to pass between CTAs: results may lie where the inputs
-// lie, and are written once all CTAs of the cluster have read.  Then each row finds its sequence by bisection in shared memory.
+// Every CTA takes the prefix sums over all sequences itself (they are few numbers), so that nothing has to pass between CTAs: as many run as there are rows for.  Where results lie where
+// inputs lie they are a cluster of eight at most, and a barrier keeps them from being written before all have read (2048 sequences and 57000 rows: PLAN_MEASURED).  Then each row finds its sequence by bisection in shared memory.
 //
 // Free pages are a stack; the pages of requests that end lie on top of it, in the order of sequences, and new pages are taken from the top.  Taken are either pages that came back
 // in this call and all of those, then older ones, or some of those that came back: entries that are read lie below the old count, and entries that are written above.
@@ -50,6 +50,8 @@ __device__ __forceinline__ int last_at_most(const int* a, int n, int v) {      /
     return lo;
 }
 
+// TOGETHER: results lie where inputs lie; the CTAs are a cluster.
+template <bool TOGETHER>
 __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
     extern __shared__ int sm[];
     int* const held = sm;                                  // tokens before
@@ -59,7 +61,6 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
     __shared__ PlanSums warp_sums[kPlanThreads / 32];
     __shared__ int bad_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const bool many = gridDim.x > 1;
     pdl_release();
     if (tid == 0) bad_s = 0;
     pdl_sync();
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
         if (blockIdx.x == 0) a.row_start[a.nseq] = bad ? 0 : (int)total.rows;
     }
     __syncthreads();
-    if (many) {
+    if constexpr (TOGETHER) {
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
@@ -425,16 +426,19 @@ extern "C" int32_t lumi_k_page_plan(uint64_t tokens, uint64_t len, int32_t nseq,
     const PlanArgs a{(const int32_t*)tokens, (const int32_t*)len, (const int32_t*)pool, (int32_t*)page_table, (int32_t*)free_pages, (int32_t*)pool_after, (int32_t*)tokens_after,
                      (int32_t*)row_start, (int32_t*)pos, (int32_t*)slot, nseq, pages_per_seq, n_pages, rows};
     const size_t smem = sizeof(int) * (4 * (size_t)nseq + 3);
-    if (smem > 48 * 1024) LUMI_CUDA(cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    const int ctas = rows > 2 * kPlanThreads ? kPlanCtas : 1;
+    const bool together = pool == pool_after || tokens == tokens_after;
+    const auto kernel = together ? page_plan_kernel<true> : page_plan_kernel<false>;
+    if (smem > 48 * 1024) LUMI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int wanted = std::max(1, (rows + kPlanThreads - 1) / kPlanThreads);
+    const int ctas = together ? (wanted > 2 ? kPlanCtas : 1) : std::min(wanted, sm_count());
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[2];
     dependent(cfg, attr, dim3(ctas), kPlanThreads, smem, (cudaStream_t)stream);
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)ctas;
+    attr[1].val.clusterDim.x = (unsigned)(together ? ctas : 1);
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
-    LUMI_CUDA(cudaLaunchKernelEx(&cfg, page_plan_kernel, a));
+    LUMI_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
     return LUMI_OK;
 }
 
