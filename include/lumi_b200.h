@@ -438,11 +438,20 @@ int32_t lumi_k_kv4_read(uint64_t kv, int32_t n_pages, uint64_t slot, uint64_t k,
  * they were; rows <= 2^24.  max_new: at least the largest number of rows of a sequence; sequences of more are left out.
  * work: at least lumi_k_kv4_attention_work_bytes, zero before its first call; calls that may run at the same time (other streams, other graphs) need areas of their own.
  * status: a device int32 or 0.  Bit 1: a sequence's lengths do not fit its rows or its row of the table (its rows are left as they were), or a page that rows see is not one of the cache's (its tokens are
- * passed over; a row that sees nothing is 0).  Bit 4: a bounded wait on the device gave up; rows that it cost are NaN. */
+ * passed over; a row that sees nothing is 0).  Bit 4: a bounded wait on the device gave up; rows that it cost are NaN.
+ * Keys or values of a token and head that are no numbers make the rows that see the token NaN, in all of the query heads that read that head; rows that do not see it are as without it. */
 int32_t lumi_k_kv4_attention_work_bytes(int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv, int64_t* bytes);
 int32_t lumi_k_kv4_attention(uint64_t q, int32_t ldq, int32_t dtype, uint64_t kv, int32_t n_pages, uint64_t page_table, int32_t pages_per_seq, uint64_t row_start, uint64_t tokens,
                              uint64_t y, int32_t ldy, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv, int32_t window, float scale, int32_t sink, int32_t nseq, int32_t rows,
                              int32_t max_new, uint64_t work, uint64_t work_bytes, uint64_t status, uint64_t stream);
+
+/* Failure-path test hook of that call: waits limited to wait_limit_ns, and the copy of page skip_page (-1: none) never arrives, counted along the pages of all units of work: sequence after
+ * sequence, tile of columns and head after head; of sequences of more than 32 columns (rows times query heads of a cache's head) apart, every unit beginning with three places without a page.
+ * status: a zeroed device int32.  Returns LUMI_E_TIMEOUT when a wait gave up; the kernels have then returned cleanly and further calls work.  Synchronises the default stream. */
+int32_t lumi_debug_kv4_attention_wait_timeout(uint64_t q, int32_t ldq, int32_t dtype, uint64_t kv, int32_t n_pages, uint64_t page_table, int32_t pages_per_seq, uint64_t row_start,
+                                              uint64_t tokens, uint64_t y, int32_t ldy, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv, int32_t window, float scale, int32_t sink,
+                                              int32_t nseq, int32_t rows, int32_t max_new, uint64_t work, uint64_t work_bytes, uint64_t status, uint64_t wait_limit_ns,
+                                              int32_t skip_page);
 
 /* The norms around a block, with its gate and residual scale: x[r] += scale * gate[r] * (o[r] / sqrt(mean(o[r]^2) + eps) * w_post) (rounded to x's type), then
  * y[r] = x[r] / sqrt(mean(x[r]^2) + eps) * w_pre of the rounded row.  w_post = 0: o as it is; gate = 0: none, else of o's type, ldg = 0: one row of gates for all rows; y = 0: x alone.

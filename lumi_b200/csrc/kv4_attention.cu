@@ -332,8 +332,7 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                     }
         }
         // the largest scale of values: a lane looks at eight of them
-        int e_top;
-        {
+        auto top_scale = [&]() {
             uint32_t top = 0;
             const uint4* const sv = reinterpret_cast<const uint4*>(slot + part + gv * kPlane);
 #pragma unroll
@@ -342,14 +341,41 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                 if (at < gv * 8) {
                     const uint4 u = sv[at];
                     const __nv_bfloat162* const b = reinterpret_cast<const __nv_bfloat162*>(&u);
-                    const __nv_bfloat162 x = __hmax2(__hmax2(b[0], b[1]), __hmax2(b[2], b[3]));
+                    const __nv_bfloat162 x = __hmax2_nan(__hmax2_nan(b[0], b[1]), __hmax2_nan(b[2], b[3]));
                     const uint32_t bits = *reinterpret_cast<const uint32_t*>(&x);
-                    const uint32_t b0 = bits & 0x7fffu, b1 = bits >> 16 & 0x7fffu;
-                    top = max(top, max(b0 < 0x7f80u ? b0 : 0u, b1 < 0x7f80u ? b1 : 0u));      // what is no number has no size
+                    top = max(top, max(bits & 0x7fffu, bits >> 16 & 0x7fffu));
                 }
             }
-            e_top = min(127, (int)(top >> 7) - 126);       // the largest is below 2^e
+            return top;
+        };
+        uint32_t top_bits = top_scale();
+        if (__any_sync(0xffffffffu, top_bits >= 0x7f80u)) {
+            // (rare) tokens with values that are no numbers: a column that sees one is none, and the others do not meet them
+            uint16_t* const sv = reinterpret_cast<uint16_t*>(slot + part + gv * kPlane);
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {
+                bool none = false;                         // token half * 32 + lane
+#pragma unroll 1
+                for (int g = 0; g < gv; ++g) {
+                    uint16_t& b = sv[g * kPage + half * 32 + lane];
+                    if ((b & 0x7fffu) >= 0x7f80u) { b = 0; none = true; }
+                }
+#pragma unroll 1
+                for (uint32_t at = __ballot_sync(0xffffffffu, none); at != 0; at &= at - 1) {
+                    const int pos = pos0 + half * 32 + __ffs(at) - 1;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (pos >= lo_pos[nt][e] && pos <= hi_pos[nt][e]) l[nt][e] = __uint_as_float(0x7fc00000u);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            top_bits = top_scale();
         }
+        const int e_top = min(127, (int)(top_bits >> 7) - 126);      // the largest is below 2^e
+        const uint32_t vals = pinned(smem_u32(slot) + part);
         // weights are relative to the running maximum, which moves where it would have to by more than 2^8, and to 2^(e_v - 7)
         bool moves = e_top > e_v;
         float top[NT][2];
@@ -408,10 +434,10 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 if (g >= gv) break;
-                if (g % 2 == 0) pair_scales(base + part + gv * kPlane, g, gv, h, sc);
+                if (g % 2 == 0) pair_scales(vals + gv * kPlane, g, gv, h, sc);
                 const uint32_t eights = i8 == g ? 0x00080008u : 0u;
                 uint32_t w[4];
-                ldmatrix4_trans(base + part + g * kPlane + lane * 16 + h * 512, w);
+                ldmatrix4_trans(vals + g * kPlane + lane * 16 + h * 512, w);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const uint32_t r0 = w[2 * k], r1 = w[2 * k + 1], u0 = r0 >> 8, u1 = r1 >> 8;
@@ -732,24 +758,26 @@ extern "C" int32_t lumi_k_kv4_attention_work_bytes(int32_t heads, int32_t kv_hea
     return LUMI_OK;
 }
 
-extern "C" int32_t lumi_k_kv4_attention(uint64_t q, int32_t ldq, int32_t dtype, uint64_t kv, int32_t n_pages, uint64_t page_table, int32_t pages_per_seq, uint64_t row_start,
-                                        uint64_t tokens, uint64_t y, int32_t ldy, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv, int32_t window, float scale, int32_t sink,
-                                        int32_t nseq, int32_t rows, int32_t max_new, uint64_t work, uint64_t work_bytes, uint64_t status, uint64_t stream) {
+namespace {
+
+int32_t check_and_run(const char* what, uint64_t q, int32_t ldq, int32_t dtype, uint64_t kv, int32_t n_pages, uint64_t page_table, int32_t pages_per_seq, uint64_t row_start,
+                      uint64_t tokens, uint64_t y, int32_t ldy, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv, int32_t window, float scale, int32_t sink, int32_t nseq,
+                      int32_t rows, int32_t max_new, uint64_t work, uint64_t work_bytes, uint64_t status, uint64_t wait_ns, int32_t skip, cudaStream_t st) {
     const bool f32 = dtype == LUMI_DTYPE_F32;
     if (!q || !kv || !page_table || !row_start || !tokens || !y || !work || (!f32 && dtype != LUMI_DTYPE_BF16) || n_pages <= 0 || pages_per_seq <= 0 || heads <= 0 || kv_heads <= 0 ||
         heads % kv_heads || dk <= 0 || dv <= 0 || window < 0 || !(scale >= -3.4e38f && scale <= 3.4e38f) || nseq < 0 || rows < 0 || max_new < 0 || ldq < (long)heads * dk ||
         ldy < (long)heads * dv)
-        return fail(LUMI_E_INVALID, "bad argument to lumi_k_kv4_attention");
+        return fail(LUMI_E_INVALID, "bad argument to %s", what);
     if ((kv & 15) || (work & 15) || ((page_table | row_start | tokens | status) & 3) || ((q | y) & (f32 ? 3 : 1)))
-        return fail(LUMI_E_INVALID, "lumi_k_kv4_attention: cache and work area have to begin on 16-byte boundaries, numbers on their own");
+        return fail(LUMI_E_INVALID, "%s: cache and work area have to begin on 16-byte boundaries, numbers on their own", what);
     if (dk > kMaxHead || dv > kMaxHead || n_pages > kMaxPages || pages_per_seq > kMaxPages || heads > 65535 || rows > kMaxRows)
-        return fail(LUMI_E_UNSUPPORTED, "lumi_k_kv4_attention: heads of %d and %d numbers (at most %d), %d heads, %d pages (at most %d), %d rows (at most %d)", dk, dv, kMaxHead,
-                    heads, n_pages, kMaxPages, rows, kMaxRows);
+        return fail(LUMI_E_UNSUPPORTED, "%s: heads of %d and %d numbers (at most %d), %d heads, %d pages (at most %d), %d rows (at most %d)", what, dk, dv, kMaxHead, heads, n_pages,
+                    kMaxPages, rows, kMaxRows);
     int64_t need = 0;
     LUMI_TRY(lumi_k_kv4_attention_work_bytes(heads, kv_heads, dk, dv, &need));
-    if (work_bytes < (uint64_t)need) return fail(LUMI_E_INVALID, "lumi_k_kv4_attention: a work area of %lld bytes, %lld are needed", (long long)work_bytes, (long long)need);
+    if (work_bytes < (uint64_t)need) return fail(LUMI_E_INVALID, "%s: a work area of %lld bytes, %lld are needed", what, (long long)work_bytes, (long long)need);
     if (nseq == 0 || rows == 0 || max_new == 0) return LUMI_OK;
-    LUMI_TRY(check_device_memory("lumi_k_kv4_attention", {q, kv, page_table, row_start, tokens, y, work, status}));
+    LUMI_TRY(check_device_memory(what, {q, kv, page_table, row_start, tokens, y, work, status}));
     AttendArgs a{};
     a.q = (const void*)q; a.y = (void*)y; a.kv = (const uint8_t*)kv;
     a.table = (const int32_t*)page_table; a.row_start = (const int32_t*)row_start; a.tokens = (const int32_t*)tokens; a.status = (int32_t*)status;
@@ -758,7 +786,28 @@ extern "C" int32_t lumi_k_kv4_attention(uint64_t q, int32_t ldq, int32_t dtype, 
     a.wide_q = (q & 15) == 0 && dk % 8 == 0 && (long)ldq * (f32 ? 4 : 2) % 16 == 0;
     a.wide_y = (y & (f32 ? 15 : 7)) == 0 && dv % 4 == 0 && ldy % 4 == 0;
     a.wide_y16 = (y & 15) == 0 && dv % (f32 ? 4 : 8) == 0 && ldy % (f32 ? 4 : 8) == 0;
-    a.few = kFewColumns; a.wait_ns = kWaitLimitNs; a.skip = -1;
-    LUMI_TRY(f32 ? step<float>(a, work, (cudaStream_t)stream) : step<__nv_bfloat16>(a, work, (cudaStream_t)stream));
-    return (long)max_new * a.group > a.few ? launch_kv4_prompt(a, f32, work, (cudaStream_t)stream) : LUMI_OK;
+    a.few = kFewColumns; a.wait_ns = wait_ns; a.skip = skip;
+    LUMI_TRY(f32 ? step<float>(a, work, st) : step<__nv_bfloat16>(a, work, st));
+    return (long)max_new * a.group > a.few ? launch_kv4_prompt(a, f32, work, st) : LUMI_OK;
+}
+
+}  // namespace
+
+extern "C" int32_t lumi_k_kv4_attention(uint64_t q, int32_t ldq, int32_t dtype, uint64_t kv, int32_t n_pages, uint64_t page_table, int32_t pages_per_seq, uint64_t row_start,
+                                        uint64_t tokens, uint64_t y, int32_t ldy, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv, int32_t window, float scale, int32_t sink,
+                                        int32_t nseq, int32_t rows, int32_t max_new, uint64_t work, uint64_t work_bytes, uint64_t status, uint64_t stream) {
+    return check_and_run("lumi_k_kv4_attention", q, ldq, dtype, kv, n_pages, page_table, pages_per_seq, row_start, tokens, y, ldy, heads, kv_heads, dk, dv, window, scale, sink, nseq, rows,
+                         max_new, work, work_bytes, status, kWaitLimitNs, -1, (cudaStream_t)stream);
+}
+
+extern "C" int32_t lumi_debug_kv4_attention_wait_timeout(uint64_t q, int32_t ldq, int32_t dtype, uint64_t kv, int32_t n_pages, uint64_t page_table, int32_t pages_per_seq,
+                                                         uint64_t row_start, uint64_t tokens, uint64_t y, int32_t ldy, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv,
+                                                         int32_t window, float scale, int32_t sink, int32_t nseq, int32_t rows, int32_t max_new, uint64_t work, uint64_t work_bytes,
+                                                         uint64_t status, uint64_t wait_limit_ns, int32_t skip_page) {
+    if (!status || !wait_limit_ns) return fail(LUMI_E_INVALID, "bad argument to lumi_debug_kv4_attention_wait_timeout");
+    LUMI_TRY(check_and_run("lumi_debug_kv4_attention_wait_timeout", q, ldq, dtype, kv, n_pages, page_table, pages_per_seq, row_start, tokens, y, ldy, heads, kv_heads, dk, dv, window, scale,
+                           sink, nseq, rows, max_new, work, work_bytes, status, wait_limit_ns, skip_page, nullptr));
+    int32_t word = 0;
+    LUMI_CUDA(cudaMemcpy(&word, (const void*)status, sizeof(word), cudaMemcpyDeviceToHost));
+    return (word & STATUS_TIMEOUT) ? fail(LUMI_E_TIMEOUT, "a bounded wait of the attention ran out") : LUMI_OK;
 }

@@ -194,6 +194,33 @@ def test_keys_that_are_no_numbers(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group,new", [(1, 1), (4, 1), (2, 3), (1, 12), (8, 4), (1, 90), (4, 40)])
+def test_values_that_are_no_numbers(group, new, dtype):
+    """A NaN or an infinity in the values of a token and head makes the rows that see the token NaN, of that head alone; the other rows of the same call are as without it."""
+    window, held, d = 100, 300, 64
+    for spot in (held - window - 5, held - window, held - window + new // 2, held - 3, held + new // 2):
+        b = Batch([held, 70], [new, 1], 2 * group, 2, d, d, dtype, seed=spot)
+        v = torch.ones(1, 2 * d, device="cuda")
+        v[0, 3] = float("nan") if spot % 2 else float("inf")
+        at = torch.tensor([b.slots[0][spot]], device="cuda", dtype=torch.int32)
+        k = torch.zeros(1, 2 * d, device="cuda")
+        put = lambda: ok(lumi_b200.lib().lumi_k_kv4_append(k.data_ptr(), 2 * d, v.data_ptr(), 2 * d, 0, at.data_ptr(), b.kv.data_ptr(), b.n_pages, 2, d, d, 1, torch.cuda.current_stream().cuda_stream))
+        put()
+        ok(b.launch(window=window))
+        torch.cuda.synchronize()
+        got = b.y[:b.rows, :2 * group * d].clone().view(b.rows, 2, group * d)
+        v.fill_(1.0)                                                     # (the same token with numbers)
+        put()
+        b.check(window=window)
+        whole = b.y[:b.rows, :2 * group * d].view(b.rows, 2, group * d)
+        for row in range(b.rows):
+            sees = row < new and held + row - window < spot <= held + row
+            assert torch.isnan(got[row, 0]).all() if sees else torch.isfinite(got[row, 0]).all()
+            close = lambda x, y: (x.float() - y.float()).abs().max() <= 2.0 ** (-6 if dtype == BF16 else -14)
+            assert close(got[row, 1], whole[row, 1]) and (sees or close(got[row, 0], whole[row, 0]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_queries_that_are_no_numbers(dtype):
     for new in (1, 70):
         b = Batch([100], [new], 2, 1, 64, 64, dtype)
