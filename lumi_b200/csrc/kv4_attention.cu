@@ -25,6 +25,9 @@ constexpr int kMaxCtas = 296;                              // of the step kernel
 // Fewer pages than these for each CTA are taken by fewer CTAs (us of one sequence of 4000 tokens and four heads of 64, and of 8 x 1000 and eight of 128): 4 pages 16.8, 19.7; 6 16.5, 19.6;
 // 8 15.1, 16.7; 12 18.0, 20.3.
 constexpr int kCtaPages = 8;
+// What a unit's beginning and end (queries in, results out) cost, in pages: where units are many, each begins with so many places without a page on the line that is split.  us of 256 sequences
+// of 32 to 1024 visible tokens, 16 fp32 heads of 80 each, and of 64 of 90 to 8192, 8 bf16 heads of 128: none 150, 75; one 112, 63; two 113, 60; three 116, 59.
+constexpr int kUnitCost = 1;
 constexpr int kFewColumns = 32;                            // of a sequence, that the step kernel still takes
 
 // Matrix loads may be moved as the arithmetic around them allows; what orders them is their address, which comes from pinned() behind what they have to wait for.
@@ -86,13 +89,13 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
     constexpr int W = Shape::kWarps, COLS = Shape::kCols, THREADS = W * 32, NT = MODE == 1 ? 2 : 1;
     constexpr bool TWO = MODE == 2;                        // two terms of q and of the weights
     extern __shared__ __align__(128) uint8_t sm[];
-    __shared__ long long before[THREADS + 1];                   // pages of the sequences ahead of each thread's
+    __shared__ long long before[THREADS + 1], units_before[THREADS + 1];      // pages and units of the sequences ahead of each thread's
     __shared__ uint64_t full[W][4];
-    __shared__ long long warp_pages[W];
+    __shared__ long long warp_pages[W], warp_units[W];
     __shared__ Open heads_s[W], tails_s[W];                // units that began ahead of a warp's run and end in it; that its run ends with and that it does not hold whole
     __shared__ int lost_s, n_open_s;
     __shared__ int4 opens_s[2 * W], shared_s[2];
-    __shared__ long long line_s[3 + W];                    // pages of the line, the CTA's first and its end, runs' first ones: not kept in registers over the pages
+    __shared__ long long line_s[3 + W];                    // places of the line, the CTA's first page and its end, runs' first ones: not kept in registers over the pages
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i8 = lane >> 2, j4 = lane & 3;
     uint8_t* const ring = sm + (size_t)warp * a.slots * a.slot_bytes;
     const int gk = kv4_groups(a.dk), gv = kv4_groups(a.dv), part = kv4_part(a.dk), block = kv4_block(a.dk, a.dv);
@@ -107,35 +110,69 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
 
     // ---- the line of pages: each thread sums up a run of sequences
     const int each = (a.nseq + THREADS - 1) / THREADS, s_lo = min(a.nseq, tid * each), s_hi = min(a.nseq, s_lo + each);
-    long long mine = 0;
+    long long mine = 0, my_units = 0;
     bool any_bad = false;
     for (int s = s_lo; s < s_hi; ++s) {
         bool bad;
         const Sequence q = step_sequence(a, s, COLS, bad);
         any_bad |= bad;
         mine += (long long)q.pages * q.units;
+        my_units += q.units;
     }
     if (any_bad && blockIdx.x == 0 && a.status != nullptr) atomicOr(a.status, kBadPage);
-    long long run = mine;
+    long long run = mine, run_units = my_units;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const long long t = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += t; }
-    if (lane == 31) warp_pages[warp] = run;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, run, o), u = __shfl_up_sync(0xffffffffu, run_units, o);
+        if (lane >= o) { run += t; run_units += u; }
+    }
+    if (lane == 31) { warp_pages[warp] = run; warp_units[warp] = run_units; }
     __syncthreads();
-    long long ahead = 0, total = 0;
+    long long ahead = 0, total = 0, units_ahead = 0, units = 0;
 #pragma unroll
-    for (int w = 0; w < W; ++w) { const long long p = warp_pages[w]; if (w < warp) ahead += p; total += p; }
+    for (int w = 0; w < W; ++w) {
+        const long long p = warp_pages[w], u = warp_units[w];
+        if (w < warp) { ahead += p; units_ahead += u; }
+        total += p;
+        units += u;
+    }
     before[tid] = ahead + run - mine;
-    if (tid == THREADS - 1) before[THREADS] = total;
+    units_before[tid] = units_ahead + run_units - my_units;
+    if (tid == THREADS - 1) { before[THREADS] = total; units_before[THREADS] = units; }
     __syncthreads();
-    // CTAs that get work: some pages each.  CTA c takes the pages from c total / ctas on.
+    // CTAs that get work: some pages each.  Where units are many, each begins with places without a page on the line that is split, so that short ones are not taken for cheap ones.
     const int ctas = (int)min((long long)gridDim.x, quotient(total + kCtaPages - 1, kCtaPages)), cta = blockIdx.x;
     if (cta >= ctas) return;
-    const long long c_lo = quotient(total * cta, ctas), c_hi = quotient(total * (cta + 1), ctas);
+    const int extra = units > ctas ? kUnitCost : 0;
+    const long long places = total + units * extra;
+    const long long c_lo = quotient(places * cta, ctas), c_hi = quotient(places * (cta + 1), ctas);
     const int runs = (int)min((long long)W, c_hi - c_lo);    // runs that are not empty come first
     auto warp_from = [&](int w) { return c_lo + quotient((c_hi - c_lo) * min(w, runs), runs); };
-    const int run_n = (int)(warp_from(warp + 1) - warp_from(warp));
-    if (lane == 0) line_s[3 + warp] = warp_from(warp);
-    if (tid == 0) { line_s[0] = total; line_s[1] = c_lo; line_s[2] = c_hi; }
+    // the first page at or behind a place
+    auto page_at = [&](long long x) {
+        int lo = 0, hi = THREADS;
+        while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (before[mid] + extra * units_before[mid] <= x) lo = mid; else hi = mid; }
+        long long at = before[lo], rel = x - at - extra * units_before[lo];
+        for (int s = lo * each; s < min(a.nseq, (lo + 1) * each); ++s) {
+            bool bad;
+            const Sequence q = step_sequence(a, s, COLS, bad);
+            const int per = q.pages + extra;
+            if (rel < (long long)per * q.units) {
+                const long long unit = quotient(rel, per);
+                return at + unit * q.pages + max(0, (int)(rel - unit * per) - extra);
+            }
+            rel -= (long long)per * q.units;
+            at += (long long)q.pages * q.units;
+        }
+        return at;
+    };
+    long long edge_of = lane == 0 ? warp_from(warp) : lane == 1 ? warp_from(warp + 1) : lane == 2 ? c_lo : c_hi;
+    if (extra != 0 && lane < 4) edge_of = page_at(edge_of);
+    __syncwarp();
+    const int run_n = (int)(__shfl_sync(0xffffffffu, edge_of, 1) - __shfl_sync(0xffffffffu, edge_of, 0));
+    if (lane == 0) line_s[3 + warp] = edge_of;
+    if (warp == 0 && lane == 2) { line_s[0] = places; line_s[1] = edge_of; }
+    if (warp == 0 && lane == 3) line_s[2] = edge_of;
     __syncwarp();
     volatile const long long* const x_lo_s = line_s + 3 + warp;
 
@@ -627,8 +664,7 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
     }
     __syncthreads();
     const int n_open = n_open_s, items = COLS * pad / 4;
-    const long long all_pages = line_s[0], cta_lo = line_s[1], cta_hi = line_s[2];
-    const int sharers = (int)min((long long)gridDim.x, quotient(all_pages + kCtaPages - 1, kCtaPages));
+    const long long all_places = line_s[0], cta_lo = line_s[1], cta_hi = line_s[2];
     auto open_unit = [&](int k) { const int4 o = opens_s[k]; return o.y < o.x ? heads_s[o.z] : tails_s[o.x]; };
     auto put_numbers = [&](const Open& u, int col, int d, float4 v, float m, float sum) {      // sums over all of the unit
         Sequence q;
@@ -677,7 +713,15 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
     __syncthreads();
     if (tid < 2 && shared[tid]) {
         const Open u = ends[tid];
-        const int c0 = (int)quotient((u.lo + 1) * sharers - 1, all_pages), c1 = (int)quotient(u.hi * sharers - 1, all_pages);
+        const int sharers = (int)min((long long)gridDim.x, quotient(before[THREADS] + kCtaPages - 1, kCtaPages));
+        long long ahead_of = 0;                            // places without a page ahead of the unit's first page
+        if (units_before[THREADS] > sharers) {
+            const int t = u.s / each;
+            ahead_of = units_before[t] + u.unit + 1;
+            for (int s = t * each; s < u.s; ++s) { bool bad; ahead_of += step_sequence(a, s, COLS, bad).units; }
+            ahead_of *= kUnitCost;
+        }
+        const int c0 = (int)quotient((u.lo + ahead_of + 1) * sharers - 1, all_places), c1 = (int)quotient((u.hi + ahead_of) * sharers - 1, all_places);
         const bool last = atomicAdd(a.tickets + c0, 1) == c1 - c0;
         if (last) a.tickets[c0] = 0;
         shared_s[tid] = make_int4(c0, c1, last, 0);
@@ -712,7 +756,7 @@ int32_t launch_step(AttendArgs a, uint64_t work, cudaStream_t st) {
     const int rec = part_floats(Shape::kCols, a.dv) * 4;
     a.slot_bytes = (std::max(kv4_block(a.dk, a.dv), rec) + 127) / 128 * 128;
     // 232448 bytes of shared memory per CTA, less what is declared in the kernel
-    a.slots = std::min(4, (int)((232448 - 1024 - W * 512) / (W * a.slot_bytes)));
+    a.slots = std::min(4, (int)((232448 - 1024 - W * 704) / (W * a.slot_bytes)));
     a.tickets = (int32_t*)work;
     a.parts = (float*)(work + 4096);
     const size_t smem = (size_t)W * a.slots * a.slot_bytes;
