@@ -70,10 +70,10 @@ __device__ __forceinline__ Sequence step_sequence(const AttendArgs& a, int s, in
 }
 
 // ---- few rows per sequence --------------------------------------------------------------------------------------
-// MODE 0: up to 8 columns of bf16 rows; 1: up to 16; 2: up to 8 columns of fp32 rows, as two terms.
+// MODE 0: up to 8 columns of bf16 rows; 1: up to 16; 2: up to 8 columns of fp32 rows, as two terms; 3: up to 4, whose second terms are the other columns of the same products.
 template <int NG, int MODE>
 struct StepShape {
-    static constexpr int kCols = MODE == 1 ? 16 : 8;
+    static constexpr int kCols = MODE == 1 ? 16 : MODE == 3 ? 4 : 8;
     // registers: accumulators of values 4 NG per eight columns and number block, of their offsets, scores, q
     static constexpr int kWarps = NG == 8 ? 6 : MODE == 1 ? (NG == 4 ? 8 : 12) : (NG == 4 ? 12 : 16);
 };
@@ -87,7 +87,7 @@ template <typename T, int NG, int MODE>
 __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_kernel(const AttendArgs a) {
     using Shape = StepShape<NG, MODE>;
     constexpr int W = Shape::kWarps, COLS = Shape::kCols, THREADS = W * 32, NT = MODE == 1 ? 2 : 1;
-    constexpr bool TWO = MODE == 2;                        // two terms of q and of the weights
+    constexpr bool TWO = MODE == 2, PAIRED = MODE == 3;    // two terms of q and of the weights: products of their own; columns c and 4 + c
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ long long before[THREADS + 1], units_before[THREADS + 1];      // pages and units of the sequences ahead of each thread's
     __shared__ uint64_t full[W][4];
@@ -215,13 +215,14 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
     int first_full = 0, last_full = 0;                     // positions that every column sees
     bool dead = false;                                     // a wait gave up
     const float sign = a.scale < 0.f ? -1.f : 1.f;
+    const float second = j4 >= 2 ? -1.f : 0.f;             // (PAIRED) the lane's columns are second terms
 
     auto begin_unit = [&](const Sequence& q, int unit) {
         const int cols = q.n * a.group, tile = unit / a.kv_heads, head = unit - tile * a.kv_heads, col0 = tile * COLS;
         first_full = 0; last_full = 0x7fffffff;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int col = col0 + nt * 8 + i8, row = min(col, cols - 1) / a.group, h = min(col, cols - 1) - row * a.group;
+            const int col = col0 + nt * 8 + (PAIRED ? i8 & 3 : i8), row = min(col, cols - 1) / a.group, h = min(col, cols - 1) - row * a.group;
             const T* const p = (const T*)a.q + (long)(q.first + row) * a.ldq + (long)(head * a.group + h) * a.dk + j4 * 8;
             float raw[NG][8];                              // numbers 8 j .. 8 j + 7 of each group of column i
 #pragma unroll
@@ -264,6 +265,10 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                     auto& to = Q[nt][2 * g + step];
                     to[0] = halves(v0, v1);
                     to[1] = halves(v2, v3);
+                    if (PAIRED) {
+                        const float2 h0 = unhalves(to[0]), h1 = unhalves(to[1]);
+                        if (i8 >= 4) { to[0] = halves(v0 - h0.x, v1 - h0.y); to[1] = halves(v2 - h1.x, v3 - h1.y); }
+                    }
                     if constexpr (TWO) {
                         const float2 h0 = unhalves(to[0]), h1 = unhalves(to[1]);
                         to[2] = halves(v0 - h0.x, v1 - h0.y);
@@ -356,6 +361,12 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                     }
                 }
             }
+        }
+        if constexpr (PAIRED) {                            // both terms' scores, in lanes of both
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) S[0][t][e] += __shfl_xor_sync(0xffffffffu, S[0][t][e], 2);
         }
         if (edge) {
 #pragma unroll
@@ -483,7 +494,12 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                     for (int nt = 0; nt < NT; ++nt) {
                         const float(&x)[2] = S[nt][4 * h + 2 * k], (&y)[2] = S[nt][4 * h + 2 * k + 1];
                         const float v0 = x[0] * s0, v1 = x[1] * s0, v2 = y[0] * s1, v3 = y[1] * s1;
-                        const uint32_t p0 = halves(v0, v1), p1 = halves(v2, v3);
+                        uint32_t p0 = halves(v0, v1), p1 = halves(v2, v3);
+                        if constexpr (PAIRED) {
+                            const float2 h0 = unhalves(p0), h1 = unhalves(p1);
+                            p0 = halves(fmaf(h0.x, second, v0), fmaf(h0.y, second, v1));
+                            p1 = halves(fmaf(h1.x, second, v2), fmaf(h1.y, second, v3));
+                        }
 #pragma unroll
                         for (int term = 0; term < (TWO ? 2 : 1); ++term) {
                             uint32_t b0 = p0, b1 = p1;
@@ -537,6 +553,17 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
         lengths_of(a, s, q);
         const int cols = q.n * a.group, tile = unit / a.kv_heads, head = unit - tile * a.kv_heads;
         const float by = power_of_two(e_v / 2), by2 = power_of_two(e_v - e_v / 2);          // back from 2^(7 - e_v)
+        if constexpr (PAIRED) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int t = 0; t < 2 * NG; ++t) {
+                    O[0][t][e] += __shfl_xor_sync(0xffffffffu, O[0][t][e], 2);
+                    O[0][t][2 + e] += __shfl_xor_sync(0xffffffffu, O[0][t][2 + e], 2);
+                }
+                OFF[0][0][e] += __shfl_xor_sync(0xffffffffu, OFF[0][0][e], 2);
+            }
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -546,7 +573,8 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                 if (dead) sum = __uint_as_float(0x7fc00000u);
                 const float f = to != nullptr ? 1.f : m[nt][e] == -INFINITY && sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
                 const int c8 = nt * 8 + 2 * j4 + e, col = tile * COLS + c8, row = col / a.group, h = col - row * a.group;
-                if (to != nullptr && i8 == 0) { to[c8] = m[nt][e]; to[COLS + c8] = sum; }
+                const bool puts = !PAIRED || j4 < 2;       // (all lanes take part in the shuffles)
+                if (to != nullptr && i8 == 0 && puts) { to[c8] = m[nt][e]; to[COLS + c8] = sum; }
                 T* const y = (T*)a.y + (long)(q.first + row) * a.ldy + (long)(head * a.group + h) * a.dv;
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
@@ -556,8 +584,8 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
 #pragma unroll
                     for (int t = 0; t < 4; ++t) v[t] = number_at(nt, g, t, e, off) * 131072.f * by * by2 * f;
                     const int d = g * kGroup + 4 * i8;
-                    if (to != nullptr) *reinterpret_cast<float4*>(to + 2 * COLS + c8 * pad + d) = make_float4(v[0], v[1], v[2], v[3]);
-                    else if (col < cols) put_four(y + d, a.dv - d, a.wide_y, v);
+                    if (to != nullptr && puts) *reinterpret_cast<float4*>(to + 2 * COLS + c8 * pad + d) = make_float4(v[0], v[1], v[2], v[3]);
+                    if (to == nullptr && puts && col < cols) put_four(y + d, a.dv - d, a.wide_y, v);
                 }
             }
     };
@@ -780,9 +808,10 @@ template <typename T>
 int32_t step(const AttendArgs& a, uint64_t work, cudaStream_t st) {
     const int groups = std::max(kv4_groups(a.dk), kv4_groups(a.dv));
     if constexpr (sizeof(T) == 4) {
-        if (groups <= 2) return launch_step<T, 2, 2>(a, work, st);
-        if (groups <= 4) return launch_step<T, 4, 2>(a, work, st);
-        return launch_step<T, 8, 2>(a, work, st);
+        const bool many = (long)a.group * a.max_new > 4;
+        if (groups <= 2) return many ? launch_step<T, 2, 2>(a, work, st) : launch_step<T, 2, 3>(a, work, st);
+        if (groups <= 4) return many ? launch_step<T, 4, 2>(a, work, st) : launch_step<T, 4, 3>(a, work, st);
+        return many ? launch_step<T, 8, 2>(a, work, st) : launch_step<T, 8, 3>(a, work, st);
     } else {
         const bool many = (long)a.group * a.max_new > 8;
         if (groups <= 2) return many ? launch_step<T, 2, 1>(a, work, st) : launch_step<T, 2, 0>(a, work, st);
