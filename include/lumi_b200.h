@@ -446,7 +446,7 @@ int32_t lumi_k_kv4_attention(uint64_t q, int32_t ldq, int32_t dtype, uint64_t kv
                              int32_t max_new, uint64_t work, uint64_t work_bytes, uint64_t status, uint64_t stream);
 
 /* Failure-path test hook of that call: waits limited to wait_limit_ns, and the copy of page skip_page (-1: none) never arrives, counted along the pages of all units of work: sequence after
- * sequence, tile of columns and head after head; of sequences of more than 32 columns (rows times query heads of a cache's head) apart, every unit beginning with three places without a page.
+ * sequence, tile of columns and head after head; of sequences of more than 48 columns (rows times query heads of a cache's head) apart, every unit beginning with three places without a page.
  * status: a zeroed device int32.  Returns LUMI_E_TIMEOUT when a wait gave up; the kernels have then returned cleanly and further calls work.  Synchronises the default stream. */
 int32_t lumi_debug_kv4_attention_wait_timeout(uint64_t q, int32_t ldq, int32_t dtype, uint64_t kv, int32_t n_pages, uint64_t page_table, int32_t pages_per_seq, uint64_t row_start,
                                               uint64_t tokens, uint64_t y, int32_t ldy, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv, int32_t window, float scale, int32_t sink,

@@ -28,7 +28,9 @@ constexpr int kCtaPages = 8;
 // What a unit's beginning and end (queries in, results out) cost, in pages: where units are many, each begins with so many places without a page on the line that is split.  us of 256 sequences
 // of 32 to 1024 visible tokens, 16 fp32 heads of 80 each, and of 64 of 90 to 8192, 8 bf16 heads of 128: none 150, 75; one 112, 63; two 113, 60; three 116, 59.
 constexpr int kUnitCost = 1;
-constexpr int kFewColumns = 32;                            // of a sequence, that the step kernel still takes
+// Columns of a sequence up to which this kernel takes it, the one of prompts beyond.  us here and there, of 16 sequences of 4000 tokens and eight heads of 128 (bf16; fp32), and of 64 of 500 and
+// four of 64 (bf16): 32 columns 86, 115; 106, 156; 32, 47.  48 columns 118, 117; 143, 158; 39, 48.  64 columns 146, 117; 187, 158; 49, 53.
+constexpr int kFewColumns = 48;
 
 // Matrix loads may be moved as the arithmetic around them allows; what orders them is their address, which comes from pinned() behind what they have to wait for.
 __device__ __forceinline__ uint32_t pinned(uint32_t a) {

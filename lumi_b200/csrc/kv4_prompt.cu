@@ -24,7 +24,7 @@ constexpr int kTile = 128;
 constexpr int kPromptCtas = 160;                           // places for parts
 constexpr int kTicketsAt = 320;                            // behind the step kernel's
 constexpr int kUnitPages = 3;                              // what a unit costs beside its pages: queries, pipeline, results.  On the line it begins with as many places without a page
-constexpr int kRunPages = 8;                               // a CTA's, at least
+constexpr int kRunPages = 4;                               // a CTA's places, at least: a unit's beginning and a page (64 rows behind 400 tokens, eight heads of 128: 46 us; 8 places 58)
 constexpr int kMaxRing = 4;
 constexpr int kStatic = 10 * 1024;                         // bytes declared in the kernel, at most
 constexpr int kInfos = 8;                                  // pages whose exponents are kept: the copies run up to kMaxRing ahead of the values' tiles, these two ahead of the softmax
@@ -463,12 +463,6 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
             tc_fence_after();
             const int e = e_v + 9;                         // numbers are O 2^e / l
             const float back = power_of_two(e / 2), back2 = power_of_two(e - e / 2);
-            auto put_row = [&](int d, const float (&o)[8], float f) {      // eight numbers as they lie in the tile
-                T* const y = (T*)a.y + out_row * a.ldy + (long)out_head * a.dv + d;
-                const float u[4] = {o[0] * f, o[2] * f, o[4] * f, o[6] * f}, v[4] = {o[1] * f, o[3] * f, o[5] * f, o[7] * f};
-                put_four(y, a.dv - d, a.wide_y, u);
-                put_four(y + 4, a.dv - d - 4, a.wide_y, v);
-            };
             auto inverse = [&](float mm, float ll) {
                 if (a.sink && mm != -INFINITY) ll += exp2_fast(-mm);
                 return *dead_s ? __uint_as_float(0x7fc00000u) : mm == -INFINITY && ll == 0.f ? 0.f : __fdiv_rn(1.f, ll);
@@ -541,28 +535,34 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
             if (!last_s[tile]) return;
             __threadfence();
             auto place_of = [&](int k) { return a.parts + ((size_t)k * 2 + (k == c0 ? 1 : 0)) * rec; };
+            // a thread per column, eight numbers at a time, or several where the tile has few columns
+            const int here = min(kTile, g.cols - col0), ways = 2 * kTile / here, x = half * kTile + r, way = x / here, c = x - way * here, from = tile * kTile + c;
+            if (way >= ways) return;
             float mm = -INFINITY, ll = 0.f;
-#pragma unroll 4
-            for (int k = c0; k <= c1; ++k) mm = fmaxf(mm, __ldcg(place_of(k) + at));
+#pragma unroll 8
+            for (int k = c0; k <= c1; ++k) mm = fmaxf(mm, __ldcg(place_of(k) + from));
 #pragma unroll 4
             for (int k = c0; k <= c1; ++k) {
-                const float pm = __ldcg(place_of(k) + at), pl = __ldcg(place_of(k) + places + at);
+                const float pm = __ldcg(place_of(k) + from), pl = __ldcg(place_of(k) + places + from);
                 ll += pl == pl ? pl * (pm == -INFINITY ? 0.f : exp2_fast(pm - mm)) : pl;
             }
             const float f = inverse(mm, ll);
-            if (valid)
-                for (int d = d_lo; d < d_hi; d += 8) {
-                    float o[8] = {};
-#pragma unroll 2
-                    for (int k = c0; k <= c1; ++k) {
-                        const float* const p = place_of(k);
-                        const float pm = __ldcg(p + at), w = pm == -INFINITY ? 0.f : exp2_fast(pm - mm);
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(p + 2 * places + (d / 4 * places + at) * 4)), y = __ldcg(reinterpret_cast<const float4*>(p + 2 * places + ((d / 4 + 1) * places + at) * 4));
-                        o[0] = fmaf(x.x, w, o[0]); o[1] = fmaf(x.y, w, o[1]); o[2] = fmaf(x.z, w, o[2]); o[3] = fmaf(x.w, w, o[3]);
-                        o[4] = fmaf(y.x, w, o[4]); o[5] = fmaf(y.y, w, o[5]); o[6] = fmaf(y.z, w, o[6]); o[7] = fmaf(y.w, w, o[7]);
-                    }
-                    put_row(d, o, f);
+            const int c_row = (col0 + c) / a.group, c_head = col0 + c - c_row * a.group;
+            T* const y = (T*)a.y + (long)(g.q.first + c_row) * a.ldy + (long)(g.head * a.group + c_head) * a.dv;
+            for (int d = way * 8; d < pad; d += ways * 8) {
+                float o[8] = {};
+#pragma unroll 4
+                for (int k = c0; k <= c1; ++k) {
+                    const float* const p = place_of(k);
+                    const float pm = __ldcg(p + from), w = pm == -INFINITY ? 0.f : exp2_fast(pm - mm);
+                    const float4 u = __ldcg(reinterpret_cast<const float4*>(p + 2 * places + (d / 4 * places + from) * 4)), v = __ldcg(reinterpret_cast<const float4*>(p + 2 * places + ((d / 4 + 1) * places + from) * 4));
+                    o[0] = fmaf(u.x, w, o[0]); o[1] = fmaf(u.y, w, o[1]); o[2] = fmaf(u.z, w, o[2]); o[3] = fmaf(u.w, w, o[3]);
+                    o[4] = fmaf(v.x, w, o[4]); o[5] = fmaf(v.y, w, o[5]); o[6] = fmaf(v.z, w, o[6]); o[7] = fmaf(v.w, w, o[7]);
                 }
+                const float lo[4] = {o[0] * f, o[2] * f, o[4] * f, o[6] * f}, hi[4] = {o[1] * f, o[3] * f, o[5] * f, o[7] * f};      // as they lie in the tile
+                put_four(y + d, a.dv - d, a.wide_y, lo);
+                put_four(y + d + 4, a.dv - d - 4, a.wide_y, hi);
+            }
         });
     } else if (warp < TILES * 8 + 4) {
         // ---- codes and scales to fp16 tiles
