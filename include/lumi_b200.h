@@ -399,7 +399,7 @@ int32_t lumi_debug_gemm_i8_wait_timeout(uint64_t a, int32_t lda, uint64_t a_scal
  * 492-556).  All pointers are memory of the current device.  Nothing is allocated; calls may be captured into graphs.  With no rows (or sequences) a call does nothing, but checks
  * its arguments all the same.
  *
- * A token's keys (dk numbers per head) and values (dv) lie in groups of 32, the last one possibly shorter.  A group t has the scale s = m / 7 rounded up to bf16, m = max(max |t|,
+ * A token's keys (dk numbers per head) and values (dv) lie in groups of 32, the last one possibly shorter.  A group t has the scale s = m (1 / 7) (an fp32 product with 1 / 7 in fp32) rounded up to bf16, m = max(max |t|,
  * 2^-100), and codes n = 8 + rint(t / s) (fp32 quotient, ties to even; 1 .. 15) in 4 bits: t is about (n - 8) s, off by s / 2 at most.  A group that holds an infinity or a NaN gets
  * codes 8 and s = NaN.  A page has a block per head, 16-byte aligned:
  *   keys' codes [group][token][16 bytes], keys' scales [group][token] bf16, values' codes, values' scales (groups of dk, then of dv).

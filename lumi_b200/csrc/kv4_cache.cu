@@ -1,6 +1,6 @@
 // A paged cache of keys and values in 4 bits: page tables and slots from the lengths of requests, rows into the cache, rows back.
 //
-// A group of up to 32 numbers t of a token and head has the scale s = m / 7 rounded up to bf16, m = max(max |t|, 2^-100), and codes n = 8 + rint(t / s) in 1 .. 15.  Rounding the scale up
+// A group of up to 32 numbers t of a token and head has the scale s = m (1 / 7) (an fp32 product with 1 / 7 in fp32) rounded up to bf16, m = max(max |t|, 2^-100), and codes n = 8 + rint(t / s) in 1 .. 15.  Rounding the scale up
 // keeps |t / s| <= 7, so nothing is cut off and t is off by s / 2 at most.  (n - 8) s has 3 + 8 significant bits: exact in fp32 and, scaled, in fp16.  A group that holds an infinity
 // or a NaN gets codes 8 and s = NaN.
 #include "device_args.h"
@@ -160,6 +160,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
 // A warp takes one group of a head, of eight rows at a time, four lanes a row: eight numbers each, one word of codes.  Rows of a prompt are neighbouring tokens of a page, so that a
 // warp's words are 128 bytes in a row and its scales 16.  kDeep eights of rows per warp where there are many: their loads are under way together, and what a group's place costs in
 // arithmetic is shared.  Bound by memory: KV4_ROWS_MEASURED
+constexpr float kSeventh = 0.14285715f;                    // 1 / 7 rounded to fp32, which is above it: numbers of a group are at most 7 steps
 constexpr int kDeep = 4;
 constexpr int kManyRows = 4096;                            // rows from which on warps take kDeep eights
 struct RowsArgs {
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(RowsArgs a) {
         m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
         const bool numbers = m < INFINITY;
-        const uint32_t up = numbers ? (__float_as_uint(__fdiv_rn(fmaxf(m, kLeast), 7.f)) + 0xffffu) & 0xffff0000u : 0x7fc00000u;
+        const uint32_t up = numbers ? (__float_as_uint(__fmul_rn(fmaxf(m, kLeast), kSeventh)) + 0xffffu) & 0xffff0000u : 0x7fc00000u;
         const float s = __uint_as_float(up), inv = __frcp_rn(s);
         // 8 + rint(t / s) by way of t (1 / s), which is the quotient to 2^-20: the low half of a sum at 1.5 2^23.  Beside a half, where that might round the other way, the quotient itself.
         float x[8], off = 0.f;

@@ -27,7 +27,7 @@ def quantise(t):
         part = t[..., g * GROUP:(g + 1) * GROUP]
         good = np.isfinite(part).all(-1)
         m = np.maximum(np.where(good, np.abs(part).max(-1), 1), np.float32(2.0 ** -100)).astype(np.float32)
-        s = bf16_up((m / np.float32(7)).astype(np.float32))
+        s = bf16_up(m * (np.float32(1) / np.float32(7)))
         with np.errstate(invalid="ignore"):
             n = 8 + np.rint((part / s[..., None]).astype(np.float32))
         codes[..., g * GROUP:(g + 1) * GROUP] = np.where(good[..., None], n, 8)
