@@ -51,6 +51,13 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
 __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     mma16(d, a0, a1, a2, a3, b0, b1, d[0], d[1], d[2], d[3]);
 }
+// Two codes n 2^-24 (or 16 n 2^-24) as (n - 8) of them: exact in halves.
+__device__ __forceinline__ uint32_t plus(uint32_t x, uint32_t c) {
+    const __half2 h = __hadd2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&c));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t less_eight(uint32_t x) { return plus(x, 0x80088008u); }
+__device__ __forceinline__ uint32_t less_128(uint32_t x) { return plus(x, 0x80808080u); }
 // An 8 x 8 matrix of 16-bit numbers, one row per four lanes, two numbers each, transposed.
 __device__ __forceinline__ uint32_t transposed(uint32_t u) {
     uint32_t v;
@@ -208,7 +215,6 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
 
     // ---- state of the unit at hand.  Lane 4 i + j: columns 2 j and 2 j + 1 of each eight, tokens i of each eight, numbers 4 i .. 4 i + 3 of each group.
     float O[NT][2 * NG][4], m[NT][2], l[NT][2];
-    float OFF[NT][TWO ? NG : 2][2];                        // 8 sum p s: bf16 rows: row g of the accumulator is group g; fp32 rows: the lane's tokens' part
     uint32_t Q[NT][2 * NG][TWO ? 4 : 2];                   // q as B, first and second term
     float QC[NT][NG][2];                                   // -8 sum q of each group: what the scores' accumulators start at
     float cx[NT][2];                                       // factor from accumulators to scores in units of log2
@@ -290,8 +296,6 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
             }
 #pragma unroll
             for (int t = 0; t < 2 * NG; ++t) O[nt][t][0] = O[nt][t][1] = O[nt][t][2] = O[nt][t][3] = 0.f;
-#pragma unroll
-            for (int g = 0; g < (TWO ? NG : 2); ++g) OFF[nt][g][0] = OFF[nt][g][1] = 0.f;
         }
         e_v = -90;
     };
@@ -460,8 +464,6 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                     const float f0 = top[nt][0], f1 = top[nt][1];
 #pragma unroll
                     for (int t = 0; t < 2 * NG; ++t) { O[nt][t][0] *= f0; O[nt][t][1] *= f1; O[nt][t][2] *= f0; O[nt][t][3] *= f1; }
-#pragma unroll
-                    for (int g = 0; g < (TWO ? NG : 2); ++g) { OFF[nt][g][0] *= f0; OFF[nt][g][1] *= f1; }
                     l[nt][0] *= f0; l[nt][1] *= f1;
                 }
         }
@@ -485,12 +487,13 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
             for (int g = 0; g < NG; ++g) {
                 if (g >= gv) break;
                 if (g % 2 == 0) pair_scales(vals + gv * kPlane, g, gv, h, sc);
-                const uint32_t eights = i8 == g ? 0x00080008u : 0u;
                 uint32_t w[4];
                 ldmatrix4_trans(vals + g * kPlane + lane * 16 + h * 512, w);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const uint32_t r0 = w[2 * k], r1 = w[2 * k + 1], u0 = r0 >> 8, u1 = r1 >> 8;
+                    const uint32_t a0 = less_eight(r0 & 0x000f000fu), a1 = less_128(r0 & 0x00f000f0u), a2 = less_eight(r1 & 0x000f000fu), a3 = less_128(r1 & 0x00f000f0u);
+                    const uint32_t a4 = less_eight(u0 & 0x000f000fu), a5 = less_128(u0 & 0x00f000f0u), a6 = less_eight(u1 & 0x000f000fu), a7 = less_128(u1 & 0x00f000f0u);
                     const float s0 = g % 2 ? high_bf16(sc[2 * k]) : low_bf16(sc[2 * k]), s1 = g % 2 ? high_bf16(sc[2 * k + 1]) : low_bf16(sc[2 * k + 1]);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
@@ -512,17 +515,8 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                             }
                             b0 = transposed(b0);
                             b1 = transposed(b1);
-                            mma16(O[nt][2 * g], r0 & 0x000f000fu, r0 & 0x00f000f0u, r1 & 0x000f000fu, r1 & 0x00f000f0u, b0, b1);
-                            mma16(O[nt][2 * g + 1], u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, b0, b1);
-                            if constexpr (!TWO) {
-                                float t[4] = {OFF[nt][0][0], OFF[nt][0][1], OFF[nt][1][0], OFF[nt][1][1]};
-                                mma16(t, eights, 0u, eights, 0u, b0, b1);
-                                OFF[nt][0][0] = t[0]; OFF[nt][0][1] = t[1]; OFF[nt][1][0] = t[2]; OFF[nt][1][1] = t[3];
-                            }
-                        }
-                        if constexpr (TWO) {
-                            add2(OFF[nt][g][0], OFF[nt][g][1], v0, v1);
-                            add2(OFF[nt][g][0], OFF[nt][g][1], v2, v3);
+                            mma16(O[nt][2 * g], a0, a1, a2, a3, b0, b1);
+                            mma16(O[nt][2 * g + 1], a4, a5, a6, a7, b0, b1);
                         }
                     }
                 }
@@ -533,8 +527,6 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int t = 0; t < 2 * NG; ++t) asm volatile("" : "+f"(O[nt][t][0]), "+f"(O[nt][t][1]), "+f"(O[nt][t][2]), "+f"(O[nt][t][3]) : : "memory");
-#pragma unroll
-            for (int g = 0; g < (TWO ? NG : 2); ++g) asm volatile("" : "+f"(OFF[nt][g][0]), "+f"(OFF[nt][g][1]) : : "memory");
         }
     };
 
@@ -544,11 +536,7 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
         v += __shfl_xor_sync(0xffffffffu, v, 8);
         return v + __shfl_xor_sync(0xffffffffu, v, 16);
     };
-    auto offset_of = [&](int nt, int g, int e) {
-        if constexpr (TWO) return over_tokens(OFF[nt][g][e]) * 4.76837158203125e-07f;      // 8 2^-24
-        else return __shfl_sync(0xffffffffu, OFF[nt][0][e], g * 4 + j4);
-    };
-    auto number_at = [&](int nt, int g, int t, int e, float off) { return O[nt][2 * g + (t >> 1)][(t & 1) * 2 + e] * ((t & 1) ? 0.0625f : 1.f) - off; };
+    auto number_at = [&](int nt, int g, int t, int e) { return O[nt][2 * g + (t >> 1)][(t & 1) * 2 + e] * ((t & 1) ? 0.0625f : 1.f); };
     // to == nullptr: the whole unit was this warp's, rows of y; else a part of it
     auto leave_unit = [&](int s, int unit, float* to) {
         Sequence q;
@@ -563,7 +551,6 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
                     O[0][t][e] += __shfl_xor_sync(0xffffffffu, O[0][t][e], 2);
                     O[0][t][2 + e] += __shfl_xor_sync(0xffffffffu, O[0][t][2 + e], 2);
                 }
-                OFF[0][0][e] += __shfl_xor_sync(0xffffffffu, OFF[0][0][e], 2);
             }
         }
 #pragma unroll
@@ -581,10 +568,9 @@ __global__ void __launch_bounds__(StepShape<NG, MODE>::kWarps * 32, 1) kv4_step_
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     if (g >= gv) break;
-                    const float off = offset_of(nt, g, e);
                     float v[4];
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) v[t] = number_at(nt, g, t, e, off) * 131072.f * by * by2 * f;
+                    for (int t = 0; t < 4; ++t) v[t] = number_at(nt, g, t, e) * 131072.f * by * by2 * f;
                     const int d = g * kGroup + 4 * i8;
                     if (to != nullptr && puts) *reinterpret_cast<float4*>(to + 2 * COLS + c8 * pad + d) = make_float4(v[0], v[1], v[2], v[3]);
                     if (to == nullptr && puts && col < cols) put_four(y + d, a.dv - d, a.wide_y, v);
