@@ -672,11 +672,11 @@ __global__ void __launch_bounds__(PromptShape<NG, sizeof(T) == 4>::kThreads, 1) 
                 if (lane == 0) {
                     const uint64_t k = k_desc + buf * (Shape::kKv >> 4);
 #pragma unroll 1
-                    for (int term = 0; term < TERMS; ++term)
+                    for (int term = TERMS - 1; term >= 0; --term)      // (second terms first: sums are cut off, not rounded, and less so while they are small)
 #pragma unroll 1
                         for (int x = 0; x < 2 * gk; x += 2) {      // a group of 32 numbers
                             const uint64_t qd = q_desc + (((term * BLOCKS + x / 4) * (kTile * 128) + x % 4 * 32) >> 4), kd = k + ((x / 4 * (kPage * 128) + x % 4 * 32) >> 4);
-                            umma_bf16(tmem + Shape::kS + t * kPage, qd, kd, id_s, term + x > 0);
+                            umma_bf16(tmem + Shape::kS + t * kPage, qd, kd, id_s, term < TERMS - 1 || x > 0);
                             umma_bf16(tmem + Shape::kS + t * kPage, qd + 2, kd + 2, id_s, 1u);
                         }
                     umma_commit(&s_full[t]);
