@@ -399,13 +399,13 @@ int32_t lumi_debug_gemm_i8_wait_timeout(uint64_t a, int32_t lda, uint64_t a_scal
  * 492-556).  All pointers are memory of the current device.  Nothing is allocated; calls may be captured into graphs.  With no rows (or sequences) a call does nothing, but checks
  * its arguments all the same.
  *
- * A token's keys (dk numbers per head) and values (dv) lie in groups of 32, the last one possibly shorter.  A group t has the scale s = m (1 / 7) (an fp32 product with 1 / 7 in fp32) rounded up to bf16, m = max(max |t|,
- * 2^-100), and codes n = 8 + rint(t / s) (fp32 quotient, ties to even; 1 .. 15) in 4 bits: t is about (n - 8) s, off by s / 2 at most.  A group that holds an infinity or a NaN gets
+ * A token's keys (dk numbers per head) and values (dv) lie in groups of 32, the last one possibly shorter.  A group t has the scale s = m (1 / 7) (an fp32 product with 1 / 7 in fp32)
+ * rounded up to bf16, m = max(max |t|, 2^-100), and codes n = 8 + rint(t / s) (fp32 quotient, ties to even; 1 .. 15) in 4 bits: t is about (n - 8) s, off by s / 2 at most.  A group that holds an infinity or a NaN gets
  * codes 8 and s = NaN.  A page has a block per head, 16-byte aligned:
  *   keys' codes [group][token][16 bytes], keys' scales [group][token] bf16, values' codes, values' scales (groups of dk, then of dv).
  * Of a group's 16 bytes, number i of the values is nibble i (low nibbles first); of the keys, four 32-bit words hold eight numbers each, number e of a word as nibble e / 2 + 4 (e % 2).
  * Nibbles behind a head's last number are written as 8 and not looked at.
- * The token at place t of page p has slot 64 p + t.  dk, dv <= 256; n_pages < 2^25 (LUMI_E_UNSUPPORTED beyond). */
+ * The token at place t of page p has slot 64 p + t.  dk, dv <= 256; n_pages < 2^25; heads <= 65535, and groups of all heads of keys and values together <= 524280 (LUMI_E_UNSUPPORTED beyond). */
 
 /* Bytes of one page: kv_heads blocks of (ceil(dk / 32) + ceil(dv / 32)) * 1152. */
 int32_t lumi_k_kv4_page_bytes(int32_t kv_heads, int32_t dk, int32_t dv, int64_t* bytes);

@@ -1,17 +1,20 @@
 // Attention over a paged cache in 4 bits: y = softmax(scale q K^T) V for the rows of sequences of different lengths, with an optional sliding window and an optional sink (one more
 // score, 0, without a value).  Row i of a sequence's n new rows stands at position tokens - n + i and sees the positions up to its own.
 //
-// kv4_step_kernel (few rows per sequence): the work is a line of pages, unit after unit; a unit is a sequence's head of the cache with up to 8 or 16 columns, a column being a row and a query
+// kv4_step_kernel (few rows per sequence): the work is a line of pages, unit after unit; a unit is a sequence's head of the cache with up to 4, 8 or 16 columns, a column being a row and a query
 // head that reads that cache head.  CTAs, and within them warps, take equal runs of that line, whatever the lengths.  A page's block comes by one bulk copy into the warp's ring, and a warp
 // needs no other one until its run ends: then the parts of a unit are joined, first within the CTA, then by the CTA that arrives last.
 //
-// Scores: columns are the rows of A (fp16, times a power of two per column), keys are B: codes n as subnormals n 2^-24 straight from the words (an AND each), those of a word's second
-// pair as n 2^-20 against q / 16.  The accumulator starts at -8 sum q, so that it ends with sum q (n - 8); a fp32 multiply-add per score and group brings the scale in.  Nothing is
-// rounded but q: as two fp16 terms of fp32 rows, whole of bf16 rows.
-// Values: codes are A (numbers of a head in its rows, tokens along K, which the transposing matrix load gives), softmax weights times the group's scale are B.  These products are kept
-// in fp16's range by 2^7 / (largest scale so far), and 8 sum p s is taken off at the end (one more MMA with a constant A).  fp32 rows: two fp16 terms of p s; bf16 rows: one (2^-12).
+// Products are m16n8k16 of warps: tokens (scores) and numbers of a head (values) in the rows of A, straight from the words of codes, columns in B.  A page of 64 tokens has too few columns
+// per cache head to fill a tcgen05 tile's 128 rows, and its codes would have to go to shared memory once more.
+// Scores S^T = K q: q times a power of two per column as fp16; codes of keys of bf16 rows as subnormals n 2^-24 (an AND), those of a word's second pair as 16 n 2^-24 against q / 16; the
+// accumulator starts at -8 sum q.  A fp32 multiply-add per score and group brings the scale in.  fp32 rows: two fp16 terms of q, codes as n - 8.
+// Values O^T = V^T P: codes less 8 in A (the transposing matrix load gives them), softmax weights times the group's scale in B, kept in fp16's range by 2^7 / (largest scale so far).
+// fp32 rows: two fp16 terms of p s, in products of their own or, up to four columns, in the other four columns; bf16 rows: one term (2^-12 of a weight, beside 2^-9 of y).
 //
-// Bound by memory on paper (18 bytes per 32 numbers), and close to the issue rate in fact: a page of 128 + 128 numbers is 9216 bytes and about 850 warp instructions.
+// Bound by memory on paper (18 bytes per 32 numbers), by the issue of instructions in fact (a page of 128 + 128 numbers is 9216 bytes and about 850 warp instructions), and for short lines by
+// latency: a page alone takes 10 us, launch, first instructions, copies and joins.  8 sequences of 32000 tokens, 64 / 8 bf16 heads of 128: 83 us, 3.6 TB/s; of 128000: 260 us, 4.6 TB/s;
+// 64 sequences of 90 to 8192 tokens, 32 / 8 heads of 128: 60 us; 256 sequences in windows of 1024, 16 fp32 heads of 80: 106 us; one of 4000 tokens, 16 / 4 fp32 heads of 64: 14.7 us.
 #include "device_args.h"
 #include "kv4.cuh"
 #include "rows.cuh"
@@ -822,7 +825,9 @@ using namespace lumi;
 
 extern "C" int32_t lumi_k_kv4_attention_work_bytes(int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv, int64_t* bytes) {
     if (!bytes || kv_heads <= 0 || heads <= 0 || heads % kv_heads || dk <= 0 || dv <= 0) return fail(LUMI_E_INVALID, "bad argument to lumi_k_kv4_attention_work_bytes");
-    *bytes = 64 << 20;
+    if (dk > kMaxHead || dv > kMaxHead || heads > 65535)
+        return fail(LUMI_E_UNSUPPORTED, "lumi_k_kv4_attention_work_bytes: %d heads of %d and %d numbers (at most %d)", heads, dk, dv, kMaxHead);
+    *bytes = 64 << 20;                                     // of both kernels' parts at their largest: 320 of 256 columns and 130 numbers
     return LUMI_OK;
 }
 

@@ -220,6 +220,17 @@ def test_values_that_are_no_numbers(group, new, dtype):
             assert close(got[row, 1], whole[row, 1]) and (sees or close(got[row, 0], whole[row, 0]))
 
 
+@pytest.mark.parametrize("held,new,heads,d", [(31, 1, 16, 64), (4000, 1, 16, 64), (4000, 2, 4, 128), (1000, 1, 32, 256), (9000, 1, 4, 80), (1000, 40, 16, 64), (300, 300, 8, 128)])
+def test_fp32_rows_keep_their_precision(held, new, heads, d):
+    """The whole result's error: two fp16 terms of q and of weights (2^-22 each), scores of up to 2^4 in units of log2 in fp32 (2^-20), exponentials (2^-21), and sums of up to 2^5 products of the
+    tensor cores, which cut off (2^-19 of a score or a result): 2^-18 of the result, whose numbers are sums that cancel about as much as the errors do."""
+    b = Batch([held], [new], heads, 4, d, d, F32, seed=held + new)
+    b.check()
+    want = b.sequence(0)[0]
+    got = b.y[:new, :heads * d].double().cpu().numpy().reshape(want.shape)
+    assert np.linalg.norm(got - want) <= 2.0 ** -18 * np.linalg.norm(want)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_queries_that_are_no_numbers(dtype):
     for new in (1, 70):

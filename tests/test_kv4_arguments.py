@@ -70,6 +70,25 @@ def test_attention_refuses(k, want):
     assert attention(**k) == want
 
 
+def test_the_hook_refuses_what_the_call_does():
+    base = dict(q=P, ldq=256, dtype=0, kv=P, n_pages=4, table=P, width=4, row_start=P, tokens=P, y=P, ldy=256, heads=4, kv_heads=2, dk=64, dv=64, window=0, scale=0.125, sink=0, nseq=1, rows=4,
+                max_new=1, work=P, work_bytes=1 << 30, status=P, wait_ns=1000, skip=-1)
+    for k, want in ((dict(status=0), INVALID), (dict(wait_ns=0), INVALID), (dict(q=0), INVALID), (dict(heads=3), INVALID), (dict(dk=257, ldq=2000), UNSUPPORTED)):
+        assert call("lumi_debug_kv4_attention_wait_timeout", base, k) == want
+
+
+def test_work_areas():
+    n = C.c_int64()
+    get = lambda *a: lumi_b200.lib().lumi_k_kv4_attention_work_bytes(*a, C.byref(n))
+    assert get(64, 8, 128, 128) == 0 and n.value >= 320 * 256 * (2 + 128) * 4 + 4096
+    assert get(0, 1, 64, 64) == INVALID and get(3, 2, 64, 64) == INVALID and get(4, 2, 0, 64) == INVALID and lumi_b200.lib().lumi_k_kv4_attention_work_bytes(4, 2, 64, 64, None) == INVALID
+    assert get(4, 2, 257, 64) == UNSUPPORTED and get(4, 2, 64, 300) == UNSUPPORTED and get(65536, 1, 64, 64) == UNSUPPORTED
+
+
+def test_more_groups_than_a_launch_takes():
+    assert append(kv_heads=65535, dk=256, dv=256, ldk=1 << 24, ldv=1 << 24) == UNSUPPORTED and append(kv_heads=65535, dk=128, dv=128, ldk=1 << 24, ldv=1 << 24) == 0
+
+
 @pytest.mark.parametrize("k,want", [
     (dict(x=0), INVALID), (dict(o=0), INVALID), (dict(w_pre=0), INVALID), (dict(x_dtype=2), INVALID), (dict(o_dtype=-1), INVALID), (dict(y_dtype=3), INVALID), (dict(rows=-1), INVALID),
     (dict(width=0), INVALID), (dict(ldx=60), INVALID), (dict(ldo=60), INVALID), (dict(ldg=60), INVALID), (dict(ldy=60), INVALID), (dict(ldx=66), INVALID), (dict(ldx=68, x_dtype=1), INVALID),
