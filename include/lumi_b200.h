@@ -435,7 +435,8 @@ int32_t lumi_k_kv4_read(uint64_t kv, int32_t n_pages, uint64_t slot, uint64_t k,
  * row_start[s + 1] - 1 and holds tokens[s] tokens with them: row i of its n rows stands at position tokens[s] - n + i and sees the `window` positions that end with its own (0: all).
  * sink: the softmax has one more score, 0, without a value.  heads a multiple of kv_heads; head h reads the cache's head h / (heads / kv_heads).
  * q [rows][ldq], y [rows][ldy]: dtype LUMI_DTYPE_*, any alignment of theirs; fp32 rows are good to about 2^-20, bf16 rows to their own rounding.  rows behind row_start[nseq] are left as
- * they were; rows <= 2^24.  max_new: at least the largest number of rows of a sequence; sequences of more are left out.
+ * they were; rows <= 2^24, and min(rows, max_new) heads / kv_heads <= 2^30 (LUMI_E_UNSUPPORTED beyond).  max_new: at least the largest number of rows of a sequence; sequences of more are left
+ * out.  y overlaps nothing.
  * work: at least lumi_k_kv4_attention_work_bytes, zero before its first call; calls that may run at the same time (other streams, other graphs) need areas of their own.
  * status: a device int32 or 0.  Bit 1: a sequence's lengths do not fit its rows or its row of the table (its rows are left as they were), or a page that rows see is not one of the cache's (its tokens are
  * passed over; a row that sees nothing is 0).  Bit 4: a bounded wait on the device gave up; rows that it cost are NaN.

@@ -846,6 +846,8 @@ int32_t check_and_run(const char* what, uint64_t q, int32_t ldq, int32_t dtype, 
     if (dk > kMaxHead || dv > kMaxHead || n_pages > kMaxPages || pages_per_seq > kMaxPages || heads > 65535 || rows > kMaxRows)
         return fail(LUMI_E_UNSUPPORTED, "%s: heads of %d and %d numbers (at most %d), %d heads, %d pages (at most %d), %d rows (at most %d)", what, dk, dv, kMaxHead, heads, n_pages,
                     kMaxPages, rows, kMaxRows);
+    if ((long)std::min(rows, max_new) * (heads / kv_heads) > 1 << 30)      // columns of a sequence are 32-bit numbers
+        return fail(LUMI_E_UNSUPPORTED, "%s: %d rows of %d heads on %d", what, std::min(rows, max_new), heads, kv_heads);
     int64_t need = 0;
     LUMI_TRY(lumi_k_kv4_attention_work_bytes(heads, kv_heads, dk, dv, &need));
     if (work_bytes < (uint64_t)need) return fail(LUMI_E_INVALID, "%s: a work area of %lld bytes, %lld are needed", what, (long long)work_bytes, (long long)need);

@@ -65,7 +65,8 @@ def test_calls_without_rows_do_nothing():
     (dict(dv=0), INVALID), (dict(window=-1), INVALID), (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID), (dict(nseq=-1), INVALID), (dict(rows=-1), INVALID),
     (dict(max_new=-1), INVALID), (dict(ldq=255), INVALID), (dict(ldy=255), INVALID), (dict(kv=P + 8), INVALID), (dict(work=P + 8), INVALID), (dict(table=P + 2), INVALID),
     (dict(tokens=P + 1), INVALID), (dict(status=P + 2), INVALID), (dict(q=P + 2), INVALID), (dict(y=P + 1, dtype=1), INVALID), (dict(work_bytes=1024), INVALID),
-    (dict(dk=257, ldq=2000), UNSUPPORTED), (dict(dv=257, ldy=2000), UNSUPPORTED), (dict(n_pages=1 << 25), UNSUPPORTED), (dict(rows=(1 << 24) + 1), UNSUPPORTED)])
+    (dict(dk=257, ldq=2000), UNSUPPORTED), (dict(dv=257, ldy=2000), UNSUPPORTED), (dict(n_pages=1 << 25), UNSUPPORTED), (dict(rows=(1 << 24) + 1), UNSUPPORTED),
+    (dict(rows=1 << 24, max_new=1 << 24, heads=128, kv_heads=1, dk=1, dv=1), UNSUPPORTED), (dict(heads=65536, kv_heads=1, dk=1, dv=1, ldq=65536, ldy=65536), UNSUPPORTED)])
 def test_attention_refuses(k, want):
     assert attention(**k) == want
 
